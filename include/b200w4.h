@@ -476,6 +476,52 @@ int b2w4_rope_tables(float* cos_host, float* sin_host, int positions, int first_
 int b2w4_embed_rows(b2w4_ctx* ctx, const void* table_fp16_dev, const int32_t* ids_dev, int rows,
                     int dim, float* out_dev, int ldo);
 
+/* ---- a paged key-value cache -----------------------------------------------------------
+ * For programs that serve several sequences: keys and values lie in pages of a pool that the
+ * sequences share, and one call works on a batch of them.  No counterpart in the reference,
+ * which keeps one contiguous cache per session (kernels/attention.cpp:1043-1057).
+ * k_dev, v_dev: [pages][kv_heads][page_size][dim] each, numbers of `type`; a contiguous cache
+ * [kv_head][capacity][dim] is the one-page case.  dim 64, 128, 192 or 256; any page_size. */
+enum { B2W4_F32 = 0, B2W4_F16 = 1, B2W4_BF16 = 2 };
+typedef struct b2w4_paged_cache {
+    void *k_dev, *v_dev;
+    int type, pages, kv_heads, page_size, dim;
+} b2w4_paged_cache;
+/* The sequences of a call.  Sequence i has slot slots_dev[i] (NULL: slot i): row `slot` of
+ * tables_dev [slots][table_len] lists its pages, lengths_dev[slot] counts its tokens, THIS
+ * call's rows among them.  Its rows are starts_dev[i] .. starts_dev[i + 1] - 1 (starts_dev NULL:
+ * row i alone), its last tokens in order: row r has position length - (starts_dev[i + 1] - r).
+ * A row whose position is negative has no token (an idle slot: length 0); rows behind the last
+ * sequence are left as they were.  max_new and max_length bound a sequence's rows and tokens;
+ * they choose kernels and sizes.
+ * The arrays are device memory, read when the call runs, so a captured call can be replayed as
+ * they change.  What they say is bounded on the device: a slot, row count, length or page that
+ * the call does not have is left out and b2w4_sync answers B2W4_E_INVALID. */
+typedef struct b2w4_paged_batch {
+    const int32_t *tables_dev, *lengths_dev, *slots_dev, *starts_dev;
+    int slots, table_len, sequences, rows, max_new, max_length;
+} b2w4_paged_batch;
+/* b2w4_qkv_prepare for the batch: Q and K of the merged rows get the per-head RMSNorm (weights
+ * may be NULL) and the rotary embedding of their position (cos / sin [max_length][dim / 2]), with
+ * the same operations; Q lands in q_out [rows][ldq], K and V, rounded to the cache's type, in
+ * their pages.  Rows without a token: zeros in q_out.  A slot is named once in a call. */
+int b2w4_paged_prepare(b2w4_ctx* ctx, const b2w4_paged_cache* cache,
+                       const b2w4_paged_batch* batch, const float* qkv_dev, int ld, int heads,
+                       const float* q_weight_dev, const float* k_weight_dev, float eps,
+                       const float* cos_dev, const float* sin_dev, float* q_out_dev, int ldq);
+/* Attention of the batch's rows over their sequences' pages; everything but the cache is fp32,
+ * and so are the results to rounding, whatever the cache's type.  The token at position p sees
+ * key j if j <= p and, with a window > 0, j > p - window or j < sinks (the first `sinks` tokens
+ * stay visible).  A key whose probability is zero in 32 bits contributes nothing, whatever its
+ * value row holds.  Rows without a token: zeros.  q, out: 16-byte aligned rows [heads * dim]
+ * that do not overlap.  work_dev: b2w4_paged_attention_work bytes, 16-byte aligned, which no
+ * other call uses at the same time; what it holds between calls does not matter. */
+size_t b2w4_paged_attention_work(const b2w4_ctx* ctx, int heads, int dim);
+int b2w4_paged_attention(b2w4_ctx* ctx, const b2w4_paged_cache* cache,
+                         const b2w4_paged_batch* batch, const float* q_dev, int ldq, int heads,
+                         float scale, int window, int sinks, float* out_dev, int ldo,
+                         void* work_dev, size_t work_bytes);
+
 /* Launch counter: how many of this library's kernels have been launched on the
  * context since creation (for benchmark bookkeeping). */
 uint64_t b2w4_kernel_launches(const b2w4_ctx* ctx);

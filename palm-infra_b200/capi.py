@@ -35,6 +35,7 @@ SYMBOLS = [
     "b2w4_attention", "b2w4_embed_rows", "b2w4_copy_rows", "b2w4_advance",
     "b2w4_qkv_prepare", "b2w4_rope_tables", "b2w4_step_matmul", "b2w4_attention_step",
     "b2w4_matmul_norm", "b2w4_matmul_swiglu",
+    "b2w4_paged_prepare", "b2w4_paged_attention", "b2w4_paged_attention_work",
     "b2w4_kernel_launches",
 ]
 
@@ -58,6 +59,59 @@ class ChainShard(C.Structure):
     """b2w4_chain_shard: which columns of the full row this rank's shard of an op holds, and
     (optionally) every rank's plain fp32 row as mapped into this process."""
     _fields_ = [("n_offset", C.c_int), ("n_full", C.c_int), ("y_peers", C.c_void_p * 8)]
+
+
+F32, F16, BF16 = 0, 1, 2  # numbers of a paged cache
+
+
+class PagedCache(C.Structure):
+    """b2w4_paged_cache: the pools of keys and values, torch tensors [pages, kv_heads, page_size,
+    dim] of one type (float32, float16 or bfloat16)."""
+    _fields_ = [("k_dev", C.c_void_p), ("v_dev", C.c_void_p), ("type", C.c_int),
+                ("pages", C.c_int), ("kv_heads", C.c_int), ("page_size", C.c_int),
+                ("dim", C.c_int)]
+
+    def __init__(self, k, v):
+        types = {"torch.float32": F32, "torch.float16": F16, "torch.bfloat16": BF16}
+        if str(k.dtype) not in types or k.dtype != v.dtype or k.shape != v.shape or \
+                k.dim() != 4 or not (k.is_contiguous() and v.is_contiguous()):
+            raise ValueError("k and v: contiguous [pages, kv_heads, page_size, dim] of one type "
+                             "(float32, float16 or bfloat16)")
+        pages, kv_heads, page_size, dim = k.shape
+        super().__init__(k.data_ptr(), v.data_ptr(), types[str(k.dtype)], pages, kv_heads,
+                         page_size, dim)
+        self.keep = (k, v)
+
+
+def _int32(name, t, dims):
+    if str(t.dtype) != "torch.int32" or t.dim() != dims or not t.is_contiguous():
+        raise ValueError(f"{name}: a contiguous int32 tensor of {dims} dimension(s)")
+    return t.data_ptr()
+
+
+class PagedBatch(C.Structure):
+    """b2w4_paged_batch: the sequences of a call, int32 tensors.  tables [slots, table_len],
+    lengths [slots] (the call's rows counted), slots [sequences] (None: sequence i is slot i),
+    starts [sequences + 1] (None: one row per sequence)."""
+    _fields_ = [("tables_dev", C.c_void_p), ("lengths_dev", C.c_void_p),
+                ("slots_dev", C.c_void_p), ("starts_dev", C.c_void_p), ("slots", C.c_int),
+                ("table_len", C.c_int), ("sequences", C.c_int), ("rows", C.c_int),
+                ("max_new", C.c_int), ("max_length", C.c_int)]
+
+    def __init__(self, tables, lengths, max_length, slots=None, starts=None, rows=None, max_new=1):
+        n = tables.shape[0] if slots is None else slots.shape[0]
+        if starts is not None:
+            if slots is not None and starts.shape[0] != n + 1:
+                raise ValueError("starts has one entry more than slots")
+            n = starts.shape[0] - 1
+        super().__init__(_int32("tables", tables, 2), _int32("lengths", lengths, 1),
+                         None if slots is None else _int32("slots", slots, 1),
+                         None if starts is None else _int32("starts", starts, 1),
+                         tables.shape[0], tables.shape[1], n, n if rows is None else rows,
+                         max_new, max_length)
+        if lengths.shape[0] != tables.shape[0]:
+            raise ValueError("a length for every slot")
+        self.keep = (tables, lengths, slots, starts)
 
 
 class B200W4Error(RuntimeError):
@@ -143,6 +197,13 @@ def lib():
                                           f_p, f_p, f_p, i, fl]
         L.b2w4_embed_rows.argtypes = [vp, vp, vp, i, i, f_p, i]
         L.b2w4_copy_rows.argtypes = [vp, f_p, i, f_p, i, i, i]
+        cache_p, batch_p, size = C.POINTER(PagedCache), C.POINTER(PagedBatch), C.c_size_t
+        L.b2w4_paged_prepare.argtypes = [vp, cache_p, batch_p, f_p, i, i, f_p, f_p, fl, f_p, f_p,
+                                         f_p, i]
+        L.b2w4_paged_attention_work.argtypes = [vp, i, i]
+        L.b2w4_paged_attention_work.restype = size
+        L.b2w4_paged_attention.argtypes = [vp, cache_p, batch_p, f_p, i, i, fl, i, i, f_p, i, vp,
+                                           size]
         L.b2w4_kernel_launches.argtypes = [vp]
         L.b2w4_kernel_launches.restype = C.c_uint64
         _lib = L
@@ -506,6 +567,28 @@ class Context:
         rows, dim = out.shape
         self._check(lib().b2w4_embed_rows(self.handle, _dptr(table_fp16), _dptr(ids), rows, dim,
                                           _dptr(out), out.stride(0)))
+
+    # -- a paged key-value cache
+    def paged_prepare(self, cache, batch, qkv, heads, q_weight, k_weight, eps, cos, sin, q_out):
+        """Merged qkv rows -> normalised + rotated Q in q_out, K and V in their pages."""
+        rc = lib().b2w4_paged_prepare(self.handle, C.byref(cache), C.byref(batch), _dptr(qkv),
+                                      qkv.stride(0), heads, _dptr(q_weight), _dptr(k_weight), eps,
+                                      _dptr(cos), _dptr(sin), _dptr(q_out), q_out.stride(0))
+        if rc != 0:
+            self._check(rc)
+
+    def paged_attention_work(self, heads, dim):
+        """Bytes of the work area (a uint8 CUDA tensor) of paged_attention."""
+        return int(lib().b2w4_paged_attention_work(self.handle, heads, dim))
+
+    def paged_attention(self, cache, batch, q, heads, out, scale, work, window=0, sinks=0):
+        """Attention of the batch's rows q [rows, heads * dim] over their pages.  window > 0: the
+        last `window` keys of a token and the sequence's first `sinks`."""
+        rc = lib().b2w4_paged_attention(self.handle, C.byref(cache), C.byref(batch), _dptr(q),
+                                        q.stride(0), heads, scale, window, sinks, _dptr(out),
+                                        out.stride(0), _dptr(work), work.numel())
+        if rc != 0:
+            self._check(rc)
 
     # -- MoE
     def moe_forward(self, hidden, router_fp16, top_k, intermediate, gate_up, down, out,

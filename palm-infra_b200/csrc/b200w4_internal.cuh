@@ -95,6 +95,22 @@ inline bool b2w4_overlap(const void* a, size_t a_bytes, const void* b, size_t b_
                              cudaGetErrorString(e__));                            \
     } while (0)
 
+// Makes the context's device current for a call, and the caller's again behind it.
+struct b2w4_device_guard {
+    int before = -1;
+    explicit b2w4_device_guard(const b2w4_ctx* ctx) {
+        int now = -1;
+        if (cudaGetDevice(&now) == cudaSuccess && now != ctx->device &&
+            cudaSetDevice(ctx->device) == cudaSuccess)
+            before = now;
+    }
+    ~b2w4_device_guard() {
+        if (before >= 0)
+            cudaSetDevice(before);
+    }
+    b2w4_device_guard(const b2w4_device_guard&) = delete;
+};
+
 // The opt-in to more than 48 KB of dynamic shared memory is an attribute of a kernel PER
 // DEVICE: a cache of what has been configured is indexed by the context's device.
 constexpr int kMaxDevices = 64;
@@ -344,6 +360,11 @@ __device__ __forceinline__ uint4 b2w4_ldg_stream(const uint4* p) {
 // before the host's stream synchronise returns.
 __device__ __forceinline__ void b2w4_report_timeout(int* status) {
     *reinterpret_cast<volatile int*>(status) = B2W4_E_TIMEOUT;
+}
+
+// What a kernel found wrong in the device data that it was given, to the same word.
+__device__ __forceinline__ void b2w4_report(int* status, int code) {
+    *reinterpret_cast<volatile int*>(status) = code;
 }
 
 __device__ __forceinline__ void b2w4_pdl_wait() {

@@ -174,14 +174,18 @@ int b2w4_ctx_set_moe_rule(b2w4_ctx* ctx, int act_rule) {
 }
 
 // Drains the stream and reads the status word a kernel sets when one of its bounded waits
-// gave up; clears it so that the context stays usable.
+// gave up, or when its device data name a page, slot or row that is not there; clears it so that the context stays usable.
 static int drain_and_check(b2w4_ctx* ctx) {
     B2W4_CUDA(ctx, cudaStreamSynchronize(ctx->stream));
     const int status = *reinterpret_cast<volatile int*>(ctx->status_host);
     if (status != 0) {
         *reinterpret_cast<volatile int*>(ctx->status_host) = 0;
         cudaMemset(ctx->flag_dev + 2, 0, sizeof(int));  // the persistent kernel's abort word
-        return b2w4_fail(ctx, status, "a device-side wait ran out of iterations");
+        return b2w4_fail(ctx, status,
+                         status == B2W4_E_INVALID ? "a page, slot, row or count that a call's device "
+                                                    "arrays named is outside of what the call has"
+                         : status == B2W4_E_NOMEM ? "a pool ran out of pages"
+                                                  : "a device-side wait ran out of iterations");
     }
     return B2W4_OK;
 }

@@ -1,0 +1,318 @@
+// Paged key-value cache: the step between the qkv matmul and attention (Q/K norm, rotary
+// embedding, append to the pages), and attention over the pages.
+#include "paged.cuh"
+
+#include <climits>
+
+namespace {
+
+using paged::Args;
+using paged::Sequence;
+using paged::Window;
+
+constexpr int kWarps = 8;
+
+// The sequence that row `row` of the call belongs to: the last one that begins at or before it;
+// -1 where the row lies before the first sequence or behind the last.
+__device__ __forceinline__ int sequence_of(const Args& a, int row) {
+    if (!a.starts)
+        return row < a.sequences ? row : -1;
+    int lo = 0, hi = a.sequences;  // starts[lo] <= row < starts[hi], if the row has a sequence
+    if (row < a.starts[0] || row >= a.starts[a.sequences])
+        return -1;
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (a.starts[mid] <= row)
+            lo = mid;
+        else
+            hi = mid;
+    }
+    return lo;
+}
+
+// Whether sequence i's slot is that of an earlier sequence too (whole warp).
+__device__ __forceinline__ bool slot_again(const Args& a, int i) {
+    if (!a.slots_of)
+        return false;
+    const int mine = a.slots_of[i];
+    bool again = false;
+    for (int j = threadIdx.x & 31; j < i; j += 32)
+        again |= a.slots_of[j] == mine;
+    return __any_sync(0xffffffffu, again);
+}
+
+struct Prepare {
+    const float *qkv, *q_weight, *k_weight, *cosv, *sinv;
+    float* q_out;
+    float eps;
+    int ld, ldq, heads;
+};
+
+// One warp per (row, head) of the merged rows.  The arithmetic is that of b2w4_qkv_prepare,
+// operation for operation; keys and values are rounded to the cache's type as they are stored.
+template <typename T, int DIM>
+__global__ void __launch_bounds__(32 * kWarps)
+paged_prepare_kernel(const Args a, const Prepare p) {
+    b2w4_pdl_chain_entry();
+    constexpr int kPer = DIM / 32, kHi = kPer / 2;  // v[i] pairs with v[i + kHi]
+    const unsigned slots = p.heads + 2 * a.kv_heads;
+    const unsigned at = blockIdx.x * kWarps + (threadIdx.x >> 5);
+    const int lane = threadIdx.x & 31;
+    const int row = (int)(at / slots), slot = (int)(at - row * slots);
+    if (row >= a.rows)
+        return;
+    const int i = sequence_of(a, row);
+    if (i < 0)
+        return;
+    bool bad = false;
+    const Sequence s = paged::sequence(a, i, &bad);
+    if (bad)
+        b2w4_report(a.status, B2W4_E_INVALID);
+    const int in = row - s.first;
+    const int pos = s.length - s.count + in;
+    const bool query = slot < p.heads, key = !query && slot < p.heads + a.kv_heads;
+    float* q = p.q_out + (size_t)row * p.ldq + slot * DIM;
+    if (in >= s.count || pos < 0) {
+        if (query) {
+#pragma unroll
+            for (int d = 0; d < DIM; d += 32)
+                q[lane + d] = 0.f;
+        }
+        return;
+    }
+    const float* x = p.qkv + (size_t)row * p.ld + slot * DIM;
+    float v[kPer];
+#pragma unroll
+    for (int d = 0; d < kPer; ++d)
+        v[d] = x[lane + 32 * d];
+    T* dst = nullptr;
+    if (!query) {
+        const int r = slot_again(a, i)
+                          ? -1
+                          : paged::cache_row(a, s.table, pos,
+                                             slot - p.heads - (key ? 0 : a.kv_heads));
+        if (r < 0) {
+            b2w4_report(a.status, B2W4_E_INVALID);
+            return;
+        }
+        dst = static_cast<T*>(key ? a.k : a.v) + (size_t)r * DIM;
+        if (!key) {
+#pragma unroll
+            for (int d = 0; d < kPer; ++d)
+                dst[lane + 32 * d] = paged::stored<T>(v[d]);
+            return;
+        }
+    }
+    const float* w = query ? p.q_weight : p.k_weight;
+    if (w) {
+        float ss = 0.f;
+#pragma unroll
+        for (int d = 0; d < kPer; ++d)
+            ss = __fadd_rn(ss, __fmul_rn(v[d], v[d]));
+        ss = paged::warp_sum(ss);
+        const float r = __fdiv_rn(1.f, sqrtf(__fadd_rn(__fdiv_rn(ss, (float)DIM), p.eps)));
+#pragma unroll
+        for (int d = 0; d < kPer; ++d)
+            v[d] = __fmul_rn(__fmul_rn(v[d], r), w[lane + 32 * d]);
+    }
+    const float* cosv = p.cosv + (size_t)pos * (DIM / 2);
+    const float* sinv = p.sinv + (size_t)pos * (DIM / 2);
+#pragma unroll
+    for (int d = 0; d < kHi; ++d) {
+        const int j = lane + 32 * d;
+        const float c = cosv[j], sn = sinv[j];
+        const float lo = __fsub_rn(__fmul_rn(v[d], c), __fmul_rn(v[d + kHi], sn));
+        const float hi = __fadd_rn(__fmul_rn(v[d], sn), __fmul_rn(v[d + kHi], c));
+        if (query) {
+            q[j] = lo;
+            q[j + DIM / 2] = hi;
+        } else {
+            dst[j] = paged::stored<T>(lo);
+            dst[j + DIM / 2] = paged::stored<T>(hi);
+        }
+    }
+}
+
+struct Attend {
+    const float* q;
+    float* out;
+    float scale;
+    Window window;
+    int ldq, ldo, heads;
+};
+
+// One warp per (row, head), key by key.
+template <typename T, int DIM>
+__global__ void __launch_bounds__(32 * kWarps)
+paged_rows_kernel(const Args a, const Attend p) {
+    b2w4_pdl_chain_entry();
+    const unsigned at = blockIdx.x * kWarps + (threadIdx.x >> 5);
+    const int row = (int)(at / p.heads), head = (int)(at - row * p.heads);
+    if (row >= a.rows)
+        return;
+    const int i = sequence_of(a, row);
+    if (i < 0)
+        return;
+    bool bad = false;
+    const Sequence s = paged::sequence(a, i, &bad);
+    if (bad)
+        b2w4_report(a.status, B2W4_E_INVALID);
+    const int in = row - s.first;
+    const int pos = in < s.count ? s.length - s.count + in : -1;
+    paged::attend_row<T, DIM>(a, s, p.q + (size_t)row * p.ldq + head * DIM, pos,
+                              head / (p.heads / a.kv_heads), p.scale, p.window,
+                              p.out + (size_t)row * p.ldo + head * DIM);
+}
+
+bool misaligned(const void* p, int ld = 0) {
+    return (reinterpret_cast<uintptr_t>(p) & 15) || (ld & 3);
+}
+
+// Calls f with a null pointer of the cache's type and its head size.
+template <typename F>
+int by_type(int type, int dim, F f) {
+    auto by_dim = [&](auto* t) {
+        switch (dim) {
+        case 64: return f(t, std::integral_constant<int, 64>());
+        case 128: return f(t, std::integral_constant<int, 128>());
+        case 192: return f(t, std::integral_constant<int, 192>());
+        default: return f(t, std::integral_constant<int, 256>());
+        }
+    };
+    switch (type) {
+    case B2W4_F16: return by_dim(static_cast<__half*>(nullptr));
+    case B2W4_BF16: return by_dim(static_cast<__nv_bfloat16*>(nullptr));
+    default: return by_dim(static_cast<float*>(nullptr));
+    }
+}
+
+Args args_of(b2w4_ctx* ctx, const b2w4_paged_cache& c, const b2w4_paged_batch& b) {
+    return {c.k_dev,   c.v_dev,  b.tables_dev, b.lengths_dev, b.slots_dev,
+            b.starts_dev, c.pages, c.kv_heads,   c.page_size,   b.slots,
+            b.table_len, b.sequences, b.rows,    b.max_length,  ctx->status_dev};
+}
+
+}  // namespace
+
+// What a cache and a batch must be, whatever is done with them; the text of what is wrong, or
+// NULL.  Host only, for the entry points and for checks without a device.
+extern "C" const char* b2w4_paged_refusal(const b2w4_paged_cache* c, const b2w4_paged_batch* b,
+                                          int heads) {
+    if (!c || !b)
+        return "no cache or no batch";
+    if (!c->k_dev || !c->v_dev || misaligned(c->k_dev) || misaligned(c->v_dev))
+        return "the pools must be 16-byte aligned device memory";
+    if (c->type != B2W4_F32 && c->type != B2W4_F16 && c->type != B2W4_BF16)
+        return "the cache's type is fp32, fp16 or bf16";
+    if (c->dim <= 0 || c->dim > 256 || c->dim % 64)
+        return "heads of 64, 128, 192 or 256 numbers";
+    if (c->pages <= 0 || c->kv_heads <= 0 || c->page_size <= 0 ||
+        (double)c->pages * c->kv_heads * c->page_size > INT_MAX)
+        return "pages, kv_heads and page_size must be positive, with fewer than 2^31 rows";
+    if (heads <= 0 || heads % c->kv_heads || (double)heads * c->dim > INT_MAX / 4)
+        return "heads must be a multiple of kv_heads";
+    if (!b->tables_dev || !b->lengths_dev || b->slots <= 0 || b->table_len <= 0 ||
+        b->sequences <= 0 || b->max_length <= 0 || b->max_new <= 0)
+        return "tables, lengths, slots, table_len, sequences, max_new and max_length are wanted";
+    if (!b->slots_dev && b->sequences > b->slots)
+        return "more sequences than slots";
+    if (b->rows <= 0 || (!b->starts_dev && b->rows != b->sequences))
+        return "without starts every sequence has one row";
+    if ((double)b->rows * heads > INT_MAX / 64)
+        return "too many rows";
+    return nullptr;
+}
+
+// Where token j of a sequence lies, by the kernels' own arithmetic: for checks without a device
+// (every pointer of the batch is host memory).  The row of the pools, -1 for a page that is not
+// theirs, -2 where the sequence is not one of the batch's or has no such token; length, first
+// and count as the kernels bound them.
+extern "C" int b2w4_paged_row(const b2w4_paged_cache* c, const b2w4_paged_batch* b, int i, int j,
+                              int h, int* length, int* first, int* count) {
+    const Args a = {c->k_dev,   c->v_dev,  b->tables_dev, b->lengths_dev, b->slots_dev,
+                    b->starts_dev, c->pages, c->kv_heads,   c->page_size,   b->slots,
+                    b->table_len, b->sequences, b->rows,    b->max_length,  nullptr};
+    bool bad = false;
+    const Sequence s = paged::sequence(a, i, &bad);
+    *length = s.length;
+    *first = s.first;
+    *count = s.count;
+    if (bad || j < 0 || j >= s.length)
+        return -2;
+    return paged::cache_row(a, s.table, j, h);
+}
+
+extern "C" {
+
+int b2w4_paged_prepare(b2w4_ctx* ctx, const b2w4_paged_cache* cache,
+                       const b2w4_paged_batch* batch, const float* qkv_dev, int ld, int heads,
+                       const float* q_weight_dev, const float* k_weight_dev, float eps,
+                       const float* cos_dev, const float* sin_dev, float* q_out_dev, int ldq) {
+    if (!ctx)
+        return B2W4_E_INVALID;
+    if (const char* why = b2w4_paged_refusal(cache, batch, heads))
+        return b2w4_fail(ctx, B2W4_E_INVALID, "paged_prepare: %s", why);
+    const int slots = heads + 2 * cache->kv_heads;
+    if (!qkv_dev || !cos_dev || !sin_dev || !q_out_dev || ld < slots * cache->dim ||
+        ldq < heads * cache->dim || (double)batch->rows * slots > INT_MAX - 2 * kWarps)
+        return b2w4_fail(ctx, B2W4_E_INVALID, "paged_prepare: bad rows (ld %d, ldq %d)", ld, ldq);
+    if (b2w4_overlap(q_out_dev, sizeof(float) * ((size_t)(batch->rows - 1) * ldq +
+                                                 heads * cache->dim),
+                     qkv_dev, sizeof(float) * ((size_t)(batch->rows - 1) * ld +
+                                               slots * cache->dim)))
+        return b2w4_fail(ctx, B2W4_E_INVALID, "paged_prepare: q_out lies over qkv");
+    const b2w4_device_guard device(ctx);
+    const Args a = args_of(ctx, *cache, *batch);
+    const Prepare p = {qkv_dev, q_weight_dev, k_weight_dev, cos_dev, sin_dev,
+                       q_out_dev, eps, ld, ldq, heads};
+    const unsigned blocks = ((unsigned)batch->rows * slots + kWarps - 1) / kWarps;
+    return by_type(cache->type, cache->dim, [&](auto* t, auto dim) {
+        using T = std::remove_pointer_t<decltype(t)>;
+        B2W4_CUDA(ctx, b2w4_launch_chained(ctx->pdl, paged_prepare_kernel<T, dim()>, dim3(blocks),
+                                           dim3(32 * kWarps), 0, ctx->stream, a, p));
+        ctx->launches++;
+        return (int)B2W4_OK;
+    });
+}
+
+size_t b2w4_paged_attention_work(const b2w4_ctx* ctx, int heads, int dim) {
+    return ctx && heads > 0 && dim > 0 ? 256 : 0;
+}
+
+int b2w4_paged_attention(b2w4_ctx* ctx, const b2w4_paged_cache* cache,
+                         const b2w4_paged_batch* batch, const float* q_dev, int ldq, int heads,
+                         float scale, int window, int sinks, float* out_dev, int ldo,
+                         void* work_dev, size_t work_bytes) {
+    if (!ctx)
+        return B2W4_E_INVALID;
+    if (const char* why = b2w4_paged_refusal(cache, batch, heads))
+        return b2w4_fail(ctx, B2W4_E_INVALID, "paged_attention: %s", why);
+    const int width = heads * cache->dim;
+    if (!q_dev || !out_dev || ldq < width || ldo < width || misaligned(q_dev, ldq) ||
+        misaligned(out_dev, ldo))
+        return b2w4_fail(ctx, B2W4_E_INVALID,
+                         "paged_attention: q and out are 16-byte aligned rows of %d numbers",
+                         width);
+    if (window < 0 || sinks < 0)
+        return b2w4_fail(ctx, B2W4_E_INVALID, "paged_attention: a negative window or sinks");
+    const size_t span = sizeof(float) * (size_t)(batch->rows - 1);
+    if (b2w4_overlap(q_dev, span * ldq + sizeof(float) * width, out_dev,
+                     span * ldo + sizeof(float) * width))
+        return b2w4_fail(ctx, B2W4_E_INVALID, "paged_attention: out lies over q");
+    if (!work_dev || misaligned(work_dev) ||
+        work_bytes < b2w4_paged_attention_work(ctx, heads, cache->dim))
+        return b2w4_fail(ctx, B2W4_E_INVALID, "paged_attention: the work area is too small");
+    const b2w4_device_guard device(ctx);
+    const Args a = args_of(ctx, *cache, *batch);
+    const Attend p = {q_dev, out_dev, scale, {window, sinks}, ldq, ldo, heads};
+    const unsigned blocks = ((unsigned)batch->rows * heads + kWarps - 1) / kWarps;
+    return by_type(cache->type, cache->dim, [&](auto* t, auto dim) {
+        using T = std::remove_pointer_t<decltype(t)>;
+        B2W4_CUDA(ctx, b2w4_launch_chained(ctx->pdl, paged_rows_kernel<T, dim()>, dim3(blocks),
+                                           dim3(32 * kWarps), 0, ctx->stream, a, p));
+        ctx->launches++;
+        return (int)B2W4_OK;
+    });
+}
+
+}  // extern "C"

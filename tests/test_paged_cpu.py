@@ -1,0 +1,144 @@
+"""The paged cache's entry points without a device: what they refuse, how the descriptors lie in
+memory, and where the kernels' own arithmetic looks for a token, bad device data included."""
+import ctypes as C
+
+import numpy as np
+import pytest
+
+from __graft_entry__ import load_package
+
+pkg = load_package()
+capi = pkg.capi
+ALIGNED = 1 << 20  # an address that nothing dereferences
+
+
+def cache(**kw):
+    c = capi.PagedCache.__new__(capi.PagedCache)
+    C.Structure.__init__(c, **{**dict(k_dev=ALIGNED, v_dev=2 * ALIGNED, type=capi.BF16, pages=10,
+                                      kv_heads=2, page_size=16, dim=128), **kw})
+    return c
+
+
+def batch(**kw):
+    b = capi.PagedBatch.__new__(capi.PagedBatch)
+    C.Structure.__init__(b, **{**dict(tables_dev=ALIGNED, lengths_dev=ALIGNED, slots_dev=None,
+                                      starts_dev=None, slots=3, table_len=4, sequences=3, rows=3,
+                                      max_new=1, max_length=64), **kw})
+    return b
+
+
+def refusal(c, b, heads=8):
+    fn = capi.lib().b2w4_paged_refusal
+    fn.restype = C.c_char_p
+    fn.argtypes = [C.c_void_p, C.c_void_p, C.c_int]
+    r = fn(C.addressof(c) if c else None, C.addressof(b) if b else None, heads)
+    return r.decode() if r else None
+
+
+def test_descriptors_lie_as_the_header_says():
+    assert C.sizeof(capi.PagedCache) == 40 and capi.PagedCache.type.offset == 16
+    assert C.sizeof(capi.PagedBatch) == 56 and capi.PagedBatch.slots.offset == 32
+
+
+def test_good_descriptors_pass():
+    assert refusal(cache(), batch()) is None
+    for dim in (64, 128, 192, 256):
+        for kind in (capi.F32, capi.F16, capi.BF16):
+            assert refusal(cache(dim=dim, type=kind, page_size=1), batch()) is None
+    assert refusal(cache(), batch(starts_dev=ALIGNED, rows=77, max_new=70)) is None
+    assert refusal(cache(), batch(slots_dev=ALIGNED, sequences=5, rows=5)) is None
+
+
+@pytest.mark.parametrize("c,b,heads", [
+    (None, batch(), 8), (cache(), None, 8),
+    (cache(k_dev=None), batch(), 8), (cache(v_dev=ALIGNED + 8), batch(), 8),
+    (cache(type=3), batch(), 8), (cache(type=-1), batch(), 8),
+    (cache(dim=0), batch(), 8), (cache(dim=80), batch(), 8), (cache(dim=320), batch(), 8),
+    (cache(pages=0), batch(), 8), (cache(page_size=0), batch(), 8),
+    (cache(kv_heads=0), batch(), 8), (cache(pages=1 << 28, page_size=1 << 10), batch(), 8),
+    (cache(), batch(), 0), (cache(), batch(), 7), (cache(), batch(), -2),
+    (cache(), batch(tables_dev=None), 8), (cache(), batch(lengths_dev=None), 8),
+    (cache(), batch(slots=0), 8), (cache(), batch(table_len=0), 8),
+    (cache(), batch(sequences=0), 8), (cache(), batch(max_length=0), 8),
+    (cache(), batch(max_new=0), 8), (cache(), batch(sequences=4, rows=4), 8),
+    (cache(), batch(rows=4), 8), (cache(), batch(rows=0, starts_dev=ALIGNED), 8),
+    (cache(), batch(rows=1 << 30, starts_dev=ALIGNED), 8)])
+def test_bad_descriptors_are_refused(c, b, heads):
+    assert refusal(c, b, heads)
+
+
+def test_null_contexts_are_rejected():
+    lib = capi.lib()
+    assert lib.b2w4_paged_prepare(None, None, None, None, 0, 1, None, None, 1e-6, None, None,
+                                  None, 0) == -1
+    assert lib.b2w4_paged_attention(None, None, None, None, 0, 1, 1.0, 0, 0, None, 0, None, 0) == -1
+    assert lib.b2w4_paged_attention_work(None, 8, 128) == 0
+
+
+def place(c, tables, lengths, i, j, h, slots=None, starts=None, **kw):
+    tables = np.ascontiguousarray(tables, dtype=np.int32)
+    arrays = [tables, np.array(lengths, dtype=np.int32)]
+    fields = dict(tables_dev=arrays[0].ctypes.data, lengths_dev=arrays[1].ctypes.data,
+                  slots=tables.shape[0], table_len=tables.shape[1], sequences=tables.shape[0],
+                  rows=tables.shape[0], max_length=1 << 30)
+    for name, v in (("slots_dev", slots), ("starts_dev", starts)):
+        if v is not None:
+            arrays.append(np.array(v, dtype=np.int32))
+            fields[name] = arrays[-1].ctypes.data
+    b = batch(**{**fields, **kw})
+    out = [C.c_int() for _ in range(3)]
+    row = capi.lib().b2w4_paged_row(C.byref(c), C.byref(b), i, j, h, *[C.byref(o) for o in out])
+    return (row,) + tuple(o.value for o in out)
+
+
+def test_tokens_lie_in_their_pages():
+    tables = [[4, 0, 9], [5, 6, 7]]
+    c = cache(page_size=5)
+    for j in range(13):
+        for h in range(2):
+            page = tables[0][j // 5]
+            assert place(c, tables, [13, 15], 0, j, h)[0] == (page * 2 + h) * 5 + j % 5
+    assert place(c, tables, [13, 15], 0, 13, 0)[0] == -2
+    assert place(c, tables, [13, 15], 1, 14, 1)[0] == (7 * 2 + 1) * 5 + 4
+    assert place(c, tables, [13, 15], 0, 14, 1, slots=[1, 0])[0] == (7 * 2 + 1) * 5 + 4
+
+
+def test_bad_device_data_stay_inside_the_arrays():
+    c = cache(page_size=5)
+    for page in (-1, 10, 1 << 30, -(1 << 31)):
+        assert place(c, [[4, page, 9]], [13], 0, 7, 1)[0] == -1
+        assert place(c, [[4, page, 9]], [13], 0, 4, 1)[0] == (4 * 2 + 1) * 5 + 4
+    # lengths beyond the table, beyond max_length, negative
+    assert place(c, [[4, 0, 9]], [16], 0, 0, 0)[:2] == (-2, 15)
+    assert place(c, [[4, 0, 9]], [14], 0, 0, 0, max_length=12)[:2] == (-2, 12)
+    assert place(c, [[4, 0, 9]], [-3], 0, 0, 0)[:2] == (-2, 0)
+    # slots and rows that are not there
+    assert place(c, [[4, 0, 9]], [13], 0, 0, 0, slots=[1])[:2] == (-2, 0)
+    assert place(c, [[4, 0, 9]], [13], 0, 0, 0, slots=[-1])[:2] == (-2, 0)
+    for starts in ([0, 99], [-1, 1], [3, 1], [2, 1 << 31 - 1]):
+        got = place(c, [[4, 0, 9]], [13], 0, 0, 0, starts=starts, rows=8)
+        assert got[0] == -2 and got[2:] == (0, 0)
+    assert place(c, [[4, 0, 9]], [13], 0, 0, 0, starts=[2, 8], rows=8)[2:] == (2, 6)
+
+
+def test_tensors_of_the_wrong_kind_are_refused():
+    import torch
+    k = torch.zeros(4, 2, 16, 64)
+    with pytest.raises(ValueError):
+        capi.PagedCache(k, k.half())
+    with pytest.raises(ValueError):
+        capi.PagedCache(k, k[:2])
+    with pytest.raises(ValueError):
+        capi.PagedCache(k.transpose(1, 2), k.transpose(1, 2))
+    with pytest.raises(ValueError):
+        capi.PagedCache(k.double(), k.double())
+    tables, lengths = torch.zeros(3, 4, dtype=torch.int32), torch.zeros(3, dtype=torch.int32)
+    capi.PagedBatch(tables, lengths, 64)
+    with pytest.raises(ValueError):
+        capi.PagedBatch(tables.long(), lengths, 64)
+    with pytest.raises(ValueError):
+        capi.PagedBatch(tables, lengths[:2], 64)
+    with pytest.raises(ValueError):
+        capi.PagedBatch(tables.t(), lengths, 64)
+    with pytest.raises(ValueError):
+        capi.PagedBatch(tables, lengths, 64, slots=lengths, starts=lengths)

@@ -1,0 +1,343 @@
+"""The paged cache on the GPU against 64 bits: the step that fills the pages, attention of single
+tokens and of runs, windows and sinks, every type and head size, ragged batches, pages of any
+size, what is masked holding NaN, strides, slots, replays, and device data that are wrong."""
+import math
+
+import pytest
+import torch
+
+import paged_reference as ref
+from __graft_entry__ import load_package
+
+pkg = load_package()
+capi = pkg.capi
+pytestmark = pytest.mark.gpu
+F32, F16, BF16 = torch.float32, torch.float16, torch.bfloat16
+
+
+@pytest.fixture(scope="module")
+def ctx():
+    c = capi.Context(0)
+    yield c
+    c.close()
+
+
+def gen(seed):
+    return torch.Generator().manual_seed(seed)
+
+
+def starts_of(news):
+    s = [0]
+    for n in news:
+        s.append(s[-1] + n)
+    return s
+
+
+def run(ctx, case, seed, q=None, change=None, window=0, sinks=0, pad=0, fill=math.nan,
+        check=True, norm=True):
+    """case: lengths, news (None: one row each, no starts), page, heads, kv, dim, dtype, slots."""
+    g = gen(seed)
+    lengths, news = case["lengths"], case.get("news")
+    heads, kv, dim, dtype = case["heads"], case["kv"], case["dim"], case["dtype"]
+    slots = case.get("slots")
+    k, v, tables, held = ref.make_pool(lengths, case["page"], kv, dim, dtype, g, slots, fill=fill)
+    used = list(range(len(lengths))) if slots is None else slots
+    starts = starts_of(news or [1] * len(lengths))
+    rows = starts[-1] + pad
+    q = torch.randn(rows, heads * dim, generator=g) if q is None else q
+    if change:
+        change(q, k, v, tables, held)
+    scale = dim ** -0.5
+    want, bound = ref.attention(q[:starts[-1]], k, v, tables, held, case["page"], starts, used,
+                                heads, scale, window, sinks)
+    cache = capi.PagedCache(k.cuda(), v.cuda())
+    ints = lambda x: torch.tensor(x, dtype=torch.int32, device="cuda")  # noqa: E731
+    if slots is None and not news:  # idle slots behind the sequences
+        tables, held = tables[:len(lengths)], held[:len(lengths)]
+    batch = capi.PagedBatch(tables.cuda(), held.cuda(), case.get("max_length", max(lengths) or 1),
+                            slots=None if slots is None and not news else ints(used),
+                            starts=ints(starts) if news else None, rows=rows if news else None,
+                            max_new=max(news) if news else 1)
+    width = heads * dim
+    qd = torch.full((rows, width + 8), 7.0, device="cuda")[:, :width]
+    qd.copy_(q)
+    out = torch.full((rows, width + 4), -3.0, device="cuda")
+    work = torch.empty(ctx.paged_attention_work(heads, dim), dtype=torch.uint8, device="cuda")
+    work.fill_(0xff)
+    torch.cuda.synchronize()
+    ctx.paged_attention(cache, batch, qd, heads, out[:, :width], scale, work, window=window,
+                        sinks=sinks)
+    ctx.sync()
+    got = out.cpu()
+    assert (got[:, width:] == -3.0).all(), "wrote beside its rows"
+    assert (got[starts[-1]:] == -3.0).all(), "wrote behind the last sequence"
+    got = got[:starts[-1], :width]
+    if check:
+        off = (got.double() - want).abs()
+        assert torch.isfinite(got).all()
+        assert (off <= bound).all(), float((off / bound).max())
+        assert not norm or ref.norm_error(got, want) <= 2e-6
+    return got, want, bound, (cache, batch, qd, out, work, width)
+
+
+TYPES = [F32, F16, BF16]
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("heads,kv,dim", [(8, 2, 128), (4, 4, 64), (16, 1, 128), (40, 2, 64),
+                                          (7, 1, 192), (6, 2, 256)])
+@pytest.mark.parametrize("page,lengths", [(16, [1, 0, 16, 17, 129, 300]), (5, [64, 63, 0, 65]),
+                                          (1, [40]), (400, [333, 399])])
+def test_single_tokens(ctx, dtype, heads, kv, dim, page, lengths):
+    run(ctx, dict(lengths=lengths, page=page, heads=heads, kv=kv, dim=dim, dtype=dtype), 1)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("window,sinks", [(1, 0), (64, 0), (100, 4), (33, 70), (5000, 3), (0, 9),
+                                          (200, 199)])
+def test_single_tokens_under_a_window(ctx, dtype, window, sinks):
+    run(ctx, dict(lengths=[1, 64, 0, 130, 777, 301], page=24, heads=8, kv=2, dim=128, dtype=dtype),
+        2, window=window, sinks=sinks)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("heads,kv,dim", [(8, 2, 128), (16, 2, 64), (5, 1, 128), (3, 3, 64),
+                                          (4, 2, 192), (4, 2, 256), (66, 1, 64)])
+@pytest.mark.parametrize("window,sinks", [(0, 0), (40, 3)])
+def test_runs(ctx, dtype, heads, kv, dim, window, sinks):
+    run(ctx, dict(lengths=[150, 33, 0, 64, 201], news=[150, 1, 0, 31, 70], page=16, heads=heads,
+                  kv=kv, dim=dim, dtype=dtype), 3, window=window, sinks=sinks, pad=3)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("window,sinks", [(1, 0), (7, 200), (64, 0), (128, 64), (129, 1),
+                                          (100000, 0)])
+@pytest.mark.parametrize("page", [7, 64, 128])
+def test_runs_under_a_window(ctx, dtype, window, sinks, page):
+    run(ctx, dict(lengths=[400, 257], news=[130, 257], page=page, heads=4, kv=1, dim=128,
+                  dtype=dtype), 4, window=window, sinks=sinks)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_long_single_token_in_an_order_of_pages(ctx, dtype):
+    run(ctx, dict(lengths=[20011, 5, 9000], page=32, heads=8, kv=2, dim=64, dtype=dtype), 5)
+
+
+@pytest.mark.parametrize("news", [None, [9, 1, 30]])
+def test_slots_of_a_larger_table(ctx, news):
+    run(ctx, dict(lengths=[100, 7, 55], news=news, slots=[5, 0, 3], page=16, heads=8, kv=2,
+                  dim=128, dtype=BF16), 6)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("news", [None, [90, 41]])
+def test_extreme_scores_and_values(ctx, dtype, news):
+    """Scores of hundreds (in 32 bits off by some 1e-5, so their probabilities too: the bound takes
+    that in), values of one sign, a key that all others vanish beside."""
+    def change(q, k, v, tables, held):
+        q.mul_(40.0)
+        v.abs_()
+        k[tables[0, 0], :, 3] *= 8
+    run(ctx, dict(lengths=[90, 300], news=news, page=16, heads=8, kv=2, dim=128, dtype=dtype), 7,
+        change=change, norm=False)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("news", [None, [64, 130]])
+def test_a_later_token_that_holds_nan_changes_no_earlier_row(ctx, dtype, news):
+    """The last token's key and value are NaN and infinite: only its own row may know."""
+    case = dict(lengths=[64, 200], news=news, page=16, heads=8, kv=2, dim=128, dtype=dtype)
+
+    def spoil(q, k, v, tables, held):
+        for s, n in enumerate((64, 200)):
+            row = tables[s, (n - 1) // 16]
+            k[row, :, (n - 1) % 16, ::2] = math.nan
+            v[row, :, (n - 1) % 16] = math.inf
+    got, want, bound, _ = run(ctx, case, 8, change=spoil, check=False)
+    last = [0, 1] if not news else [63, 193]
+    mine = torch.ones(got.shape[0], dtype=torch.bool)
+    mine[last] = False
+    assert torch.isnan(got[last]).all()
+    assert ((got.double() - want).abs() <= bound)[mine].all()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("news", [None, [70]])
+def test_keys_of_minus_infinity_take_no_part(ctx, dtype, news):
+    """A key whose score is -inf (or the type's lowest value) has probability zero, and its value
+    row, infinite here, contributes nothing."""
+    case = dict(lengths=[100], news=news, page=16, heads=4, kv=1, dim=128, dtype=dtype)
+    low = torch.finfo(dtype).min
+    q = torch.rand(70 if news else 1, 4 * 128, generator=gen(3)) + 0.5
+
+    def change(q, k, v, tables, held):
+        for j, x in ((5, -math.inf), (17, low / 2)):
+            page = tables[0, j // 16]
+            k[page, :, j % 16] = x
+            v[page, :, j % 16] = math.inf
+    got, _, _, _ = run(ctx, case, 9, q=q, change=change, check=False)
+
+    def drop(q, k, v, tables, held):  # what is left: value zero with probability zero
+        for j in (5, 17):
+            page = tables[0, j // 16]
+            k[page, :, j % 16] = -1e4
+            v[page, :, j % 16] = 0.0
+    _, want, bound, _ = run(ctx, case, 9, q=q, change=drop, check=False)
+    assert ((got.double() - want).abs() <= bound).all()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("news", [None, [130, 20, 77]])
+def test_the_same_bits_again_and_replayed(ctx, dtype, news):
+    case = dict(lengths=[2000, 20, 800], news=news, page=16, heads=8, kv=2, dim=128, dtype=dtype)
+    got, _, _, (cache, batch, q, out, work, width) = run(ctx, case, 10, window=500, sinks=4)
+    side, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    call = lambda: ctx.paged_attention(cache, batch, q, 8, out[:, :width], 128 ** -0.5, work,  # noqa: E731
+                                       window=500, sinks=4)
+    with torch.cuda.stream(side):
+        ctx.set_stream(side.cuda_stream)
+        with torch.cuda.graph(graph, stream=side):
+            call()
+    ctx.set_stream(torch.cuda.current_stream().cuda_stream)
+    for _ in range(3):
+        out.fill_(9.0)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out[:got.shape[0], :width].cpu(), got)
+    # shorter sequences through the same graph: lengths are read when it runs
+    batch.keep[1].copy_(torch.tensor([130, 0, 77] + [0] * (batch.slots - 3), dtype=torch.int32))
+    graph.replay()
+    torch.cuda.synchronize()
+    short = out[:, :width].clone()
+    call()
+    ctx.sync()
+    assert torch.equal(out[:, :width], short)
+    assert (short[130:150] if news else short[1]).abs().max() == 0  # no token, no key
+    ctx.set_stream(0)
+
+
+@pytest.mark.parametrize("news", [None, [40, 30]])
+def test_wrong_device_data_are_reported_and_left_out(ctx, news):
+    """Pages that the pool has not: their keys are left out; the context stays usable."""
+    case = dict(lengths=[64, 30], news=news, page=16, heads=4, kv=2, dim=128, dtype=BF16)
+    got, _, _, (cache, batch, q, out, work, width) = run(ctx, case, 11)
+    batch.keep[0][0, 1] = 1 << 20
+    torch.cuda.synchronize()
+    ctx.paged_attention(cache, batch, q, 4, out[:, :width], 128 ** -0.5, work)
+    with pytest.raises(capi.B200W4Error, match="outside of what the call has"):
+        ctx.sync()
+    again = out[:got.shape[0], :width].cpu()
+    first = 1 if news is None else 40
+    assert torch.equal(again[first:], got[first:])  # the other sequence
+    assert torch.isfinite(again).all() and not torch.equal(again, got)
+    run(ctx, case, 11)
+
+
+def test_refusals(ctx):
+    case = dict(lengths=[64, 30], page=16, heads=4, kv=2, dim=128, dtype=BF16)
+    _, _, _, (cache, batch, q, out, work, width) = run(ctx, case, 12)
+    o = out[:, :width]
+    call = lambda **kw: ctx.paged_attention(**{**dict(cache=cache, batch=batch, q=q, heads=4,  # noqa: E731
+                                                      out=o, scale=1.0, work=work), **kw})
+    launches = ctx.launches
+    for bad in (dict(heads=3), dict(window=-1), dict(sinks=-1), dict(work=work[:16]),
+                dict(work=work[8:]), dict(q=o), dict(q=q[:, 1:]), dict(out=out[:, 1:]),
+                dict(out=q), dict(q=q[:, :8].contiguous())):
+        with pytest.raises(capi.B200W4Error):
+            call(**bad)
+    qkv = torch.zeros(2, 8 * 128, device="cuda")
+    table = torch.zeros(64, 64, device="cuda")
+    for bad in (dict(qkv=qkv[:, :-1].contiguous()), dict(q_out=qkv[:, :512]), dict(heads=5)):
+        with pytest.raises(capi.B200W4Error):
+            ctx.paged_prepare(**{**dict(cache=cache, batch=batch, qkv=qkv, heads=4, q_weight=None,
+                                        k_weight=None, eps=1e-6, cos=table, sin=table, q_out=o),
+                                 **bad})
+    assert ctx.launches == launches
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("heads,kv,dim", [(8, 2, 128), (4, 4, 64), (2, 1, 192), (5, 1, 256)])
+@pytest.mark.parametrize("news,slots", [(None, None), ([5, 0, 33, 1], None), ([5, 3, 33, 1],
+                                                                             [4, 0, 2, 1])])
+@pytest.mark.parametrize("weights", [True, False])
+def test_prepare(ctx, dtype, heads, kv, dim, news, slots, weights):
+    """Norm (dim products, a mean, a root, a quotient: dim / 2 + 8 roundings at most matter) and
+    rotation (three roundings) in 32 bits, then half a step of the cache's type."""
+    g = gen(13)
+    lengths, page = [40, 0, 33, 17] if not slots else [40, 3, 33, 17], 8
+    k, v, tables, held = ref.make_pool(lengths, page, kv, dim, dtype, g, slots)
+    used = list(range(4)) if slots is None else slots
+    starts = starts_of(news or [1] * 4)
+    rows = starts[-1]
+    qkv = torch.randn(rows, (heads + 2 * kv) * dim, generator=g) * 3
+    qw = torch.randn(dim, generator=g) * 0.1 + 1 if weights else None
+    kw = torch.randn(dim, generator=g) * 0.1 + 1 if weights else None
+    angle = torch.rand(40, dim // 2, generator=g) * 6.28
+    cos, sin = angle.cos(), angle.sin()
+    q, new = ref.prepare(qkv, held, starts, used, heads, kv, dim, qw, kw, 1e-6, cos, sin)
+    ints = lambda x: torch.tensor(x, dtype=torch.int32, device="cuda")  # noqa: E731
+    cache = capi.PagedCache(k.cuda(), v.cuda())
+    if news is None:
+        tables, held = tables[:4], held[:4]
+    batch = capi.PagedBatch(tables.cuda(), held.cuda(), 40,
+                            slots=None if news is None else ints(used),
+                            starts=ints(starts) if news else None, rows=rows if news else None,
+                            max_new=max(news) if news else 1)
+    dev = lambda t: None if t is None else t.cuda()  # noqa: E731
+    wide = torch.zeros(rows, qkv.shape[1] + 3, device="cuda")
+    wide[:, :-3] = qkv.cuda()
+    q_out = torch.full((rows, heads * dim), 5.0, device="cuda")
+    ctx.paged_prepare(cache, batch, wide[:, :-3], heads, dev(qw), dev(kw), 1e-6, cos.cuda(),
+                      sin.cuda(), q_out)
+    ctx.sync()
+    eps = 2.0 ** -24
+    pair = lambda x: torch.cat([x[..., dim // 2:], x[..., :dim // 2]], -1)  # noqa: E731
+    size = lambda x: (x.abs() + pair(x).abs()) * 2  # noqa: E731
+    slack = (dim / 2 + 11) * eps
+    assert ((q_out.cpu().double().view(q.shape) - q).abs() <= size(q) * slack).all()
+    for want_k, want_v in [(k.clone(), v.clone())]:
+        for s, (p, nk, nv) in zip(used, new):
+            ids = tables[s][p // page].long()
+            got = cache.keep[0].cpu()[ids, :, p % page].double()
+            tiny = 2.0 ** -24 if dtype == F16 else 0.0  # below fp16's normal numbers
+            limit = size(nk) * slack * 2 + nk.abs() * (ref.EPS[dtype] if dtype != F32 else 0) + tiny
+            assert ((got - nk).abs() <= limit).all()
+            want_k[ids, :, p % page] = cache.keep[0].cpu()[ids, :, p % page]
+            want_v[ids, :, p % page] = nv.float().to(dtype)
+        assert torch.equal(cache.keep[0].cpu(), want_k)  # nothing else was written
+        assert torch.equal(cache.keep[1].cpu(), want_v)
+
+
+def test_prepare_takes_the_bits_of_the_contiguous_form(ctx):
+    """One sequence in one page that is the whole cache: b2w4_qkv_prepare's bits."""
+    g = gen(14)
+    qkv = torch.randn(9, 12 * 128, generator=g).cuda()
+    w = (torch.randn(128, generator=g) * 0.1 + 1).cuda()
+    cos, sin = (torch.from_numpy(t).cuda() for t in capi.rope_tables(64, 0, 128, 1e6))
+    q0, k0, v0 = (torch.zeros(n, 128, device="cuda") for n in (9 * 8, 2 * 64, 2 * 64))
+    ctx.qkv_prepare(qkv, 9, 8, 2, 128, w, w, 1e-6, cos, sin, 20, q0, k0, v0, 64)
+    cache = capi.PagedCache(torch.zeros(1, 2, 64, 128, device="cuda"),
+                            torch.zeros(1, 2, 64, 128, device="cuda"))
+    ints = lambda x: torch.tensor(x, dtype=torch.int32, device="cuda")  # noqa: E731
+    batch = capi.PagedBatch(ints([[0]]), ints([29]), 64, starts=ints([0, 9]), rows=9, max_new=9)
+    q1 = torch.zeros(9, 8 * 128, device="cuda")
+    ctx.paged_prepare(cache, batch, qkv, 8, w, w, 1e-6, cos, sin, q1)
+    ctx.sync()
+    assert torch.equal(q0.view(9, -1), q1)
+    assert torch.equal(k0.view(1, 2, 64, 128), cache.keep[0])
+    assert torch.equal(v0.view(1, 2, 64, 128), cache.keep[1])
+
+
+def test_a_slot_named_twice_is_reported(ctx):
+    cache = capi.PagedCache(torch.zeros(2, 1, 8, 64, device="cuda"),
+                            torch.zeros(2, 1, 8, 64, device="cuda"))
+    ints = lambda x: torch.tensor(x, dtype=torch.int32, device="cuda")  # noqa: E731
+    batch = capi.PagedBatch(ints([[0], [1]]), ints([3, 3]), 8, slots=ints([1, 1]))
+    qkv = torch.ones(2, 3 * 64, device="cuda")
+    qkv[1] = 2.0
+    table = torch.zeros(8, 32, device="cuda")
+    ctx.paged_prepare(cache, batch, qkv, 1, None, None, 1e-6, table, table,
+                      torch.zeros(2, 64, device="cuda"))
+    with pytest.raises(capi.B200W4Error, match="outside of what the call has"):
+        ctx.sync()
+    assert (cache.keep[1][1, 0, 2] == 1.0).all() and cache.keep[1].sum() == 64
