@@ -522,6 +522,47 @@ int b2w4_paged_attention(b2w4_ctx* ctx, const b2w4_paged_cache* cache,
                          float scale, int window, int sinks, float* out_dev, int ldo,
                          void* work_dev, size_t work_bytes);
 
+/* The pages of a pool, kept on the device: refs_dev [pages] counts the tables that hold a page
+ * (0: free), tables_dev [slots][table_len] and lengths_dev [slots] are the sequences', as in
+ * b2w4_paged_batch.  All zero is an empty pool of empty slots.  Free pages are handed out lowest
+ * first, so a call's result follows from the state and its arguments alone; entries of a table
+ * behind a sequence's pages mean nothing.  None of the calls waits for the host or allocates, and
+ * all can be captured.  Work that a call refuses on the device (a slot, page or length that is not
+ * there, a slot named twice, a pool without enough pages) is left undone item by item, and
+ * b2w4_sync answers B2W4_E_INVALID or B2W4_E_NOMEM. */
+typedef struct b2w4_page_pool {
+    int32_t *refs_dev, *tables_dev, *lengths_dev;
+    int pages, page_size, slots, table_len;
+} b2w4_page_pool;
+/* What lies in the pages: count planes [pages][page_bytes], for instance the keys and the values
+ * of every layer.  `planes` is a host array of device pointers, read during the call; page_bytes
+ * a multiple of 16. */
+typedef struct b2w4_page_planes {
+    void* const* planes;
+    int count, pages;
+    size_t page_bytes;
+} b2w4_page_planes;
+/* lengths[slots_dev[i]] += counts_dev[i] for i < n <= 1024 (slots_dev NULL: slot i; counts_dev
+ * NULL: one each), with the pages that takes, in the order of the list; a sequence gets all that
+ * it needs or stays as it was. */
+int b2w4_pages_extend(b2w4_ctx* ctx, const b2w4_page_pool* pool, const int32_t* slots_dev,
+                      const int32_t* counts_dev, int n);
+/* children_dev[i], an empty slot, becomes a copy of parents_dev[i] as that was before the call,
+ * i < n <= 1024: full pages are shared, a last page that is not full is copied in every plane. */
+int b2w4_pages_fork(b2w4_ctx* ctx, const b2w4_page_pool* pool, const b2w4_page_planes* planes,
+                    const int32_t* parents_dev, const int32_t* children_dev, int n);
+/* The slots give their pages back and are empty; a slot that is empty stays so. */
+int b2w4_pages_free(b2w4_ctx* ctx, const b2w4_page_pool* pool, const int32_t* slots_dev, int n);
+/* Moves the pages in use to the front of the pool: with u of them in use, the ones at or beyond u
+ * go to the free ones below, in order, in every plane and table; u goes to used_dev (optional).
+ * work_dev: int32 [pages]. */
+int b2w4_pages_compact(b2w4_ctx* ctx, const b2w4_page_pool* pool, const b2w4_page_planes* planes,
+                       int32_t* work_dev, int32_t* used_dev);
+/* Page src_dev[i] of every plane to page dst_dev[i], i < n.  No page is a destination twice, or a
+ * destination and another's source. */
+int b2w4_pages_copy(b2w4_ctx* ctx, const b2w4_page_planes* planes, const int32_t* src_dev,
+                    const int32_t* dst_dev, int n);
+
 /* Launch counter: how many of this library's kernels have been launched on the
  * context since creation (for benchmark bookkeeping). */
 uint64_t b2w4_kernel_launches(const b2w4_ctx* ctx);

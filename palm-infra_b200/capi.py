@@ -36,6 +36,8 @@ SYMBOLS = [
     "b2w4_qkv_prepare", "b2w4_rope_tables", "b2w4_step_matmul", "b2w4_attention_step",
     "b2w4_matmul_norm", "b2w4_matmul_swiglu",
     "b2w4_paged_prepare", "b2w4_paged_attention", "b2w4_paged_attention_work",
+    "b2w4_pages_extend", "b2w4_pages_fork", "b2w4_pages_free", "b2w4_pages_compact",
+    "b2w4_pages_copy",
     "b2w4_kernel_launches",
 ]
 
@@ -112,6 +114,38 @@ class PagedBatch(C.Structure):
         if lengths.shape[0] != tables.shape[0]:
             raise ValueError("a length for every slot")
         self.keep = (tables, lengths, slots, starts)
+
+
+class PagePool(C.Structure):
+    """b2w4_page_pool: the bookkeeping of a pool's pages, int32 tensors.  refs [pages], tables
+    [slots, table_len], lengths [slots]; all zero is an empty pool."""
+    _fields_ = [("refs_dev", C.c_void_p), ("tables_dev", C.c_void_p), ("lengths_dev", C.c_void_p),
+                ("pages", C.c_int), ("page_size", C.c_int), ("slots", C.c_int),
+                ("table_len", C.c_int)]
+
+    def __init__(self, refs, tables, lengths, page_size):
+        super().__init__(_int32("refs", refs, 1), _int32("tables", tables, 2),
+                         _int32("lengths", lengths, 1), refs.shape[0], page_size, *tables.shape)
+        if lengths.shape[0] != tables.shape[0]:
+            raise ValueError("a length for every slot")
+        self.keep = (refs, tables, lengths)
+
+
+class PagePlanes(C.Structure):
+    """b2w4_page_planes: what lies in the pages, contiguous tensors [pages, ...] of one size."""
+    _fields_ = [("planes", C.POINTER(C.c_void_p)), ("count", C.c_int), ("pages", C.c_int),
+                ("page_bytes", C.c_size_t)]
+
+    def __init__(self, tensors):
+        tensors = list(tensors)
+        pages = tensors[0].shape[0]
+        size = tensors[0][0].numel() * tensors[0].element_size()
+        if any(t.shape[0] != pages or t[0].numel() * t.element_size() != size or
+               not t.is_contiguous() for t in tensors):
+            raise ValueError("planes: contiguous tensors of the same pages")
+        array = (C.c_void_p * len(tensors))(*[t.data_ptr() for t in tensors])
+        super().__init__(C.cast(array, C.POINTER(C.c_void_p)), len(tensors), pages, size)
+        self.keep = (array, tensors)
 
 
 class B200W4Error(RuntimeError):
@@ -204,6 +238,12 @@ def lib():
         L.b2w4_paged_attention_work.restype = size
         L.b2w4_paged_attention.argtypes = [vp, cache_p, batch_p, f_p, i, i, fl, i, i, f_p, i, vp,
                                            size]
+        pool_p, planes_p = C.POINTER(PagePool), C.POINTER(PagePlanes)
+        L.b2w4_pages_extend.argtypes = [vp, pool_p, vp, vp, i]
+        L.b2w4_pages_fork.argtypes = [vp, pool_p, planes_p, vp, vp, i]
+        L.b2w4_pages_free.argtypes = [vp, pool_p, vp, i]
+        L.b2w4_pages_compact.argtypes = [vp, pool_p, planes_p, vp, vp]
+        L.b2w4_pages_copy.argtypes = [vp, planes_p, vp, vp, i]
         L.b2w4_kernel_launches.argtypes = [vp]
         L.b2w4_kernel_launches.restype = C.c_uint64
         _lib = L
@@ -589,6 +629,45 @@ class Context:
                                         out.stride(0), _dptr(work), work.numel())
         if rc != 0:
             self._check(rc)
+
+    def pages_extend(self, pool, slots=None, counts=None):
+        """lengths[slots[i]] += counts[i] (None: every slot, one each), with the pages it takes."""
+        if slots is not None and counts is not None and slots.shape != counts.shape:
+            raise ValueError("a count for every slot")
+        given = counts if slots is None else slots
+        n = pool.slots if given is None else given.shape[0]
+        self._check(lib().b2w4_pages_extend(
+            self.handle, C.byref(pool), None if slots is None else _int32("slots", slots, 1),
+            None if counts is None else _int32("counts", counts, 1), n))
+
+    def pages_fork(self, pool, planes, parents, children):
+        """children[i], an empty slot, becomes a copy of parents[i]."""
+        if parents.shape != children.shape:
+            raise ValueError("a child for every parent")
+        self._check(lib().b2w4_pages_fork(self.handle, C.byref(pool), C.byref(planes),
+                                          _int32("parents", parents, 1),
+                                          _int32("children", children, 1), parents.shape[0]))
+
+    def pages_free(self, pool, slots=None):
+        """The slots (None: all) give their pages back."""
+        self._check(lib().b2w4_pages_free(
+            self.handle, C.byref(pool), None if slots is None else _int32("slots", slots, 1),
+            pool.slots if slots is None else slots.shape[0]))
+
+    def pages_compact(self, pool, planes, work, used=None):
+        """The pages in use move to the front; work: int32 [pages]; used: int32 [1], their count."""
+        if work.numel() < pool.pages:
+            raise ValueError("work: an entry for every page")
+        self._check(lib().b2w4_pages_compact(
+            self.handle, C.byref(pool), C.byref(planes), _int32("work", work, 1),
+            None if used is None else _int32("used", used, 1)))
+
+    def pages_copy(self, planes, src, dst):
+        """Page src[i] -> dst[i] of every plane."""
+        if src.shape != dst.shape:
+            raise ValueError("a destination for every source")
+        self._check(lib().b2w4_pages_copy(self.handle, C.byref(planes), _int32("src", src, 1),
+                                          _int32("dst", dst, 1), src.shape[0]))
 
     # -- MoE
     def moe_forward(self, hidden, router_fp16, top_k, intermediate, gate_up, down, out,

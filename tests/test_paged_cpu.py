@@ -142,3 +142,55 @@ def test_tensors_of_the_wrong_kind_are_refused():
         capi.PagedBatch(tables.t(), lengths, 64)
     with pytest.raises(ValueError):
         capi.PagedBatch(tables, lengths, 64, slots=lengths, starts=lengths)
+
+
+def pages_refusal(pool, planes, wants_pool=1, wants_planes=1):
+    fn = capi.lib().b2w4_pages_refusal
+    fn.restype = C.c_char_p
+    fn.argtypes = [C.c_void_p, C.c_void_p, C.c_int, C.c_int]
+    r = fn(C.addressof(pool) if pool else None, C.addressof(planes) if planes else None,
+           wants_pool, wants_planes)
+    return r.decode() if r else None
+
+
+def pool(**kw):
+    p = capi.PagePool.__new__(capi.PagePool)
+    C.Structure.__init__(p, **{**dict(refs_dev=ALIGNED, tables_dev=ALIGNED, lengths_dev=ALIGNED,
+                                      pages=9, page_size=4, slots=2, table_len=3), **kw})
+    return p
+
+
+def planes(at=(ALIGNED, 2 * ALIGNED), **kw):
+    p = capi.PagePlanes.__new__(capi.PagePlanes)
+    array = (C.c_void_p * max(1, len(at)))(*at)
+    C.Structure.__init__(p, **{**dict(planes=C.cast(array, C.POINTER(C.c_void_p)), count=len(at),
+                                      pages=9, page_bytes=48), **kw})
+    p.keep = array
+    return p
+
+
+def test_good_pools_pass():
+    assert pages_refusal(pool(), planes()) is None
+    assert pages_refusal(None, planes(pages=4), 0, 1) is None
+    assert pages_refusal(pool(), None, 1, 0) is None
+    assert C.sizeof(capi.PagePool) == 40 and C.sizeof(capi.PagePlanes) == 24
+
+
+@pytest.mark.parametrize("p,pl", [
+    (None, planes()), (pool(), None), (pool(refs_dev=None), planes()),
+    (pool(tables_dev=None), planes()), (pool(lengths_dev=None), planes()),
+    (pool(pages=0), planes()), (pool(page_size=0), planes()), (pool(slots=0), planes()),
+    (pool(table_len=0), planes()), (pool(pages=8), planes()), (pool(), planes(at=())),
+    (pool(), planes(page_bytes=0)), (pool(), planes(page_bytes=40)),
+    (pool(), planes(at=(ALIGNED, ALIGNED + 8))), (pool(), planes(at=(ALIGNED, None)))])
+def test_bad_pools_are_refused(p, pl):
+    assert pages_refusal(p, pl)
+
+
+def test_pages_calls_reject_null_contexts():
+    lib = capi.lib()
+    assert lib.b2w4_pages_extend(None, None, None, None, 1) == -1
+    assert lib.b2w4_pages_fork(None, None, None, None, None, 1) == -1
+    assert lib.b2w4_pages_free(None, None, None, 1) == -1
+    assert lib.b2w4_pages_compact(None, None, None, None, None) == -1
+    assert lib.b2w4_pages_copy(None, None, None, None, 1) == -1
