@@ -563,6 +563,20 @@ int b2w4_pages_compact(b2w4_ctx* ctx, const b2w4_page_pool* pool, const b2w4_pag
 int b2w4_pages_copy(b2w4_ctx* ctx, const b2w4_page_planes* planes, const int32_t* src_dev,
                     const int32_t* dst_dev, int n);
 
+/* ---- log probabilities -------------------------------------------------------------------
+ * What a step answers beside the greedy token (b2w4_matmul_argmax), from logits fp32 [rows][ld]:
+ * logprob_dev [rows] = log softmax of targets_dev[row] (a negative target: 0; both or neither),
+ * entropy_dev [rows] of the distribution, and the `top` (0 to 32) most likely tokens in
+ * top_indices_dev / top_values_dev [rows][top] with their log probabilities, larger first, the
+ * lower index among equals.  Any output may be NULL.  A logit of -inf rules its token out
+ * (probability 0, log probability -inf).  A row with a NaN or a +inf, or of -inf alone, has no
+ * distribution: its floating outputs are NaN (a NaN token comes last among the top).  A target
+ * at or beyond vocab: NaN, and b2w4_sync answers B2W4_E_INVALID.  One pass over the logits; no
+ * counterpart in the reference, whose sampler works on the host (engine/sampler.cpp:31-77). */
+int b2w4_logprobs(b2w4_ctx* ctx, const float* logits_dev, int ld, int rows, int vocab,
+                  const int32_t* targets_dev, float* logprob_dev, float* entropy_dev, int top,
+                  float* top_values_dev, int32_t* top_indices_dev);
+
 /* Launch counter: how many of this library's kernels have been launched on the
  * context since creation (for benchmark bookkeeping). */
 uint64_t b2w4_kernel_launches(const b2w4_ctx* ctx);

@@ -37,7 +37,7 @@ SYMBOLS = [
     "b2w4_matmul_norm", "b2w4_matmul_swiglu",
     "b2w4_paged_prepare", "b2w4_paged_attention", "b2w4_paged_attention_work",
     "b2w4_pages_extend", "b2w4_pages_fork", "b2w4_pages_free", "b2w4_pages_compact",
-    "b2w4_pages_copy",
+    "b2w4_pages_copy", "b2w4_logprobs",
     "b2w4_kernel_launches",
 ]
 
@@ -244,6 +244,7 @@ def lib():
         L.b2w4_pages_free.argtypes = [vp, pool_p, vp, i]
         L.b2w4_pages_compact.argtypes = [vp, pool_p, planes_p, vp, vp]
         L.b2w4_pages_copy.argtypes = [vp, planes_p, vp, vp, i]
+        L.b2w4_logprobs.argtypes = [vp, f_p, i, i, i, vp, f_p, f_p, i, f_p, vp]
         L.b2w4_kernel_launches.argtypes = [vp]
         L.b2w4_kernel_launches.restype = C.c_uint64
         _lib = L
@@ -668,6 +669,29 @@ class Context:
             raise ValueError("a destination for every source")
         self._check(lib().b2w4_pages_copy(self.handle, C.byref(planes), _int32("src", src, 1),
                                           _int32("dst", dst, 1), src.shape[0]))
+
+    def logprobs(self, logits, targets=None, logprob=None, entropy=None, top_values=None,
+                 top_indices=None):
+        """Of logits [rows, vocab]: log probabilities of targets (int32 [rows]; negative: none),
+        entropies, and the most likely tokens (top_values float32, top_indices int32, both
+        contiguous [rows, top])."""
+        rows, vocab = logits.shape
+        best = top_values if top_values is not None else top_indices
+        top = 0 if best is None else best.shape[1]
+        shapes = ((targets, "int32", (rows,)), (logprob, "float32", (rows,)),
+                  (entropy, "float32", (rows,)), (top_values, "float32", (rows, top)),
+                  (top_indices, "int32", (rows, top)))
+        for t, kind, shape in shapes:
+            if t is not None and (tuple(t.shape) != shape or str(t.dtype) != "torch." + kind or
+                                  not t.is_contiguous()):
+                raise ValueError(f"logprobs: a contiguous {kind} tensor {shape} is wanted")
+        if logits.stride(1) != 1 and vocab > 1:
+            raise ValueError("logprobs: a row's logits lie one after the other")
+        rc = lib().b2w4_logprobs(self.handle, _dptr(logits), max(logits.stride(0), vocab), rows,
+                                 vocab, _dptr(targets), _dptr(logprob), _dptr(entropy), top,
+                                 _dptr(top_values), _dptr(top_indices))
+        if rc != 0:
+            self._check(rc)
 
     # -- MoE
     def moe_forward(self, hidden, router_fp16, top_k, intermediate, gate_up, down, out,
