@@ -491,8 +491,8 @@ typedef struct b2w4_paged_cache {
  * tables_dev [slots][table_len] lists its pages, lengths_dev[slot] counts its tokens, THIS
  * call's rows among them.  Its rows are starts_dev[i] .. starts_dev[i + 1] - 1 (starts_dev NULL:
  * row i alone), its last tokens in order: row r has position length - (starts_dev[i + 1] - r).
- * A row whose position is negative has no token (an idle slot: length 0); rows behind the last
- * sequence are left as they were.  max_new and max_length bound a sequence's rows and tokens;
+ * A row whose position is negative has no token (an empty slot, or -1 for a slot, which names
+ * none); rows behind the last sequence are left as they were.  max_new and max_length bound a sequence's rows and tokens;
  * they choose kernels and sizes.
  * The arrays are device memory, read when the call runs, so a captured call can be replayed as
  * they change.  What they say is bounded on the device: a slot, row count, length or page that
@@ -527,7 +527,7 @@ int b2w4_paged_attention(b2w4_ctx* ctx, const b2w4_paged_cache* cache,
  * b2w4_paged_batch.  All zero is an empty pool of empty slots.  Free pages are handed out lowest
  * first, so a call's result follows from the state and its arguments alone; entries of a table
  * behind a sequence's pages mean nothing.  None of the calls waits for the host or allocates, and
- * all can be captured.  Work that a call refuses on the device (a slot, page or length that is not
+ * all can be captured.  A slot of -1 names none: its item does nothing.  Work that a call refuses on the device (a slot, page or length that is not
  * there, a slot named twice, a pool without enough pages) is left undone item by item, and
  * b2w4_sync answers B2W4_E_INVALID or B2W4_E_NOMEM. */
 typedef struct b2w4_page_pool {
@@ -544,9 +544,10 @@ typedef struct b2w4_page_planes {
 } b2w4_page_planes;
 /* lengths[slots_dev[i]] += counts_dev[i] for i < n <= 1024 (slots_dev NULL: slot i; counts_dev
  * NULL: one each), with the pages that takes, in the order of the list; a sequence gets all that
- * it needs or stays as it was. */
+ * it needs or stays as it was.  granted_dev [n] (optional, not slots_dev): the slots that got it,
+ * -1 for the others -- the slots of the call's b2w4_paged_batch. */
 int b2w4_pages_extend(b2w4_ctx* ctx, const b2w4_page_pool* pool, const int32_t* slots_dev,
-                      const int32_t* counts_dev, int n);
+                      const int32_t* counts_dev, int n, int32_t* granted_dev);
 /* children_dev[i], an empty slot, becomes a copy of parents_dev[i] as that was before the call,
  * i < n <= 1024: full pages are shared, a last page that is not full is copied in every plane. */
 int b2w4_pages_fork(b2w4_ctx* ctx, const b2w4_page_pool* pool, const b2w4_page_planes* planes,

@@ -239,7 +239,7 @@ def lib():
         L.b2w4_paged_attention.argtypes = [vp, cache_p, batch_p, f_p, i, i, fl, i, i, f_p, i, vp,
                                            size]
         pool_p, planes_p = C.POINTER(PagePool), C.POINTER(PagePlanes)
-        L.b2w4_pages_extend.argtypes = [vp, pool_p, vp, vp, i]
+        L.b2w4_pages_extend.argtypes = [vp, pool_p, vp, vp, i, vp]
         L.b2w4_pages_fork.argtypes = [vp, pool_p, planes_p, vp, vp, i]
         L.b2w4_pages_free.argtypes = [vp, pool_p, vp, i]
         L.b2w4_pages_compact.argtypes = [vp, pool_p, planes_p, vp, vp]
@@ -631,15 +631,19 @@ class Context:
         if rc != 0:
             self._check(rc)
 
-    def pages_extend(self, pool, slots=None, counts=None):
-        """lengths[slots[i]] += counts[i] (None: every slot, one each), with the pages it takes."""
+    def pages_extend(self, pool, slots=None, counts=None, granted=None):
+        """lengths[slots[i]] += counts[i] (None: every slot, one each), with the pages it takes;
+        granted[i]: the slot if it got them, else -1."""
         if slots is not None and counts is not None and slots.shape != counts.shape:
             raise ValueError("a count for every slot")
         given = counts if slots is None else slots
         n = pool.slots if given is None else given.shape[0]
+        if granted is not None and granted.shape[0] < n:
+            raise ValueError("granted: an entry for every slot")
         self._check(lib().b2w4_pages_extend(
             self.handle, C.byref(pool), None if slots is None else _int32("slots", slots, 1),
-            None if counts is None else _int32("counts", counts, 1), n))
+            None if counts is None else _int32("counts", counts, 1), n,
+            None if granted is None else _int32("granted", granted, 1)))
 
     def pages_fork(self, pool, planes, parents, children):
         """children[i], an empty slot, becomes a copy of parents[i]."""

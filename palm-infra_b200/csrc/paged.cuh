@@ -34,7 +34,7 @@ inline __host__ __device__ Sequence sequence(const Args& a, int i, bool* bad) {
     Sequence s;
     int slot = a.slots_of ? a.slots_of[i] : i;
     if (slot < 0 || slot >= a.slots) {
-        *bad = true;
+        *bad |= slot != -1;  // that names no slot
         slot = 0;
         s.length = 0;
     } else {

@@ -94,7 +94,7 @@ __device__ int free_pages(const Pool& p, int want, int* s_part, F take) {
 // out in the order of the list, to a sequence all that it needs or none.
 __global__ void __launch_bounds__(kMostItems)
 pages_extend_kernel(const Pool p, const int32_t* __restrict__ slots,
-                    const int32_t* __restrict__ counts, int n) {
+                    const int32_t* __restrict__ counts, int n, int32_t* __restrict__ granted) {
     b2w4_pdl_chain_entry();
     __shared__ int s_part[32], s_slot[kMostItems], s_off[kMostItems + 1], s_first[kMostItems];
     const int i = threadIdx.x;
@@ -113,7 +113,7 @@ pages_extend_kernel(const Pool p, const int32_t* __restrict__ slots,
         if (good)
             need = pages_of(p, length + count) - pages_of(p, length);
     }
-    if (i < n && !good)
+    if (i < n && !good && slot != -1)
         bad(p);
     int total;
     const int off = scan<kMostItems>(need, s_part, &total);
@@ -136,9 +136,12 @@ pages_extend_kernel(const Pool p, const int32_t* __restrict__ slots,
             p.tables[(size_t)s_slot[lo] * p.table_len + s_first[lo] + rank - s_off[lo]] = page;
             p.refs[page] = 1;
         });
+    const bool fits = good && (need == 0 || off + need <= have);
+    if (granted && i < n)
+        granted[i] = fits ? slot : -1;
     if (!good)
         return;
-    if (need > 0 && off + need > have) {  // back with what it got
+    if (!fits) {  // back with what it got
         const int32_t* row = p.tables + (size_t)slot * p.table_len + s_first[i];
         for (int r = off; r < have; ++r)
             p.refs[row[r - off]] = 0;
@@ -223,7 +226,7 @@ struct ForkPlan {
             child[i] = children[i];
         }
         __syncthreads();
-        unsigned wrong = 0, need = 0;  // a bit per item
+        unsigned wrong = 0, quiet = 0, need = 0;  // a bit per item
 #pragma unroll
         for (int e = 0; e < kEach; ++e) {
             const int i = first + e;
@@ -240,6 +243,7 @@ struct ForkPlan {
             }
             length[i] = good ? len : 0;
             wrong |= (unsigned)!good << e;
+            quiet |= (unsigned)(parent[i] == -1 || child[i] == -1) << e;
             need |= (unsigned)(good && len % p.page_size != 0) << e;
         }
         int total;  // the barriers of the sum: every thread has compared the children
@@ -257,7 +261,7 @@ struct ForkPlan {
             rank += wants;
             if ((wrong >> e & 1) || (wants && !gets)) {
                 child[i] = -1;
-                if (report)
+                if (report && !(quiet >> e & 1))
                     b2w4_report(p.status, wants ? B2W4_E_NOMEM : B2W4_E_INVALID);
             }
         }
@@ -327,7 +331,7 @@ pages_free_kernel(const Pool p, const int32_t* __restrict__ slots) {
     __shared__ int s_length;
     const int slot = slots ? slots[blockIdx.x] : (int)blockIdx.x;
     if ((unsigned)slot >= (unsigned)p.slots) {
-        if (threadIdx.x == 0)
+        if (threadIdx.x == 0 && slot != -1)
             bad(p);
         return;
     }
@@ -505,7 +509,7 @@ extern "C" const char* b2w4_pages_refusal(const b2w4_page_pool* p, const b2w4_pa
 extern "C" {
 
 int b2w4_pages_extend(b2w4_ctx* ctx, const b2w4_page_pool* pool, const int32_t* slots_dev,
-                      const int32_t* counts_dev, int n) {
+                      const int32_t* counts_dev, int n, int32_t* granted_dev) {
     if (!ctx)
         return B2W4_E_INVALID;
     if (const char* why = b2w4_pages_refusal(pool, nullptr, 1, 0))
@@ -516,7 +520,7 @@ int b2w4_pages_extend(b2w4_ctx* ctx, const b2w4_page_pool* pool, const int32_t* 
     const b2w4_device_guard device(ctx);
     B2W4_CUDA(ctx, b2w4_launch_chained(ctx->pdl, pages_extend_kernel, dim3(1), dim3(kMostItems), 0,
                                        ctx->stream, pool_of(ctx, *pool), slots_dev, counts_dev,
-                                       n));
+                                       n, granted_dev));
     ctx->launches++;
     return B2W4_OK;
 }

@@ -132,8 +132,7 @@ class DenseDecoder:
                 **{k: ctx.upload_weight(w[k], *sh[k]) for k in sh},
                 **{k: dev(w[k]) for k in ("ln1", "ln2", "q_norm", "k_norm")},
                 **({"router": dev(w["router"].view(np.int16))} if cfg.experts else {}),
-                "k_cache": torch.zeros((cfg.kv_heads, capacity, cfg.head_dim), device=device),
-                "v_cache": torch.zeros((cfg.kv_heads, capacity, cfg.head_dim), device=device)})
+                **self._layer_cache()})
         self.final_norm = dev(weights["final_norm"])
         self.embed = dev(weights["embed"].view(np.int16))
         self.lm_head = ctx.upload_weight(weights["lm_head"], cfg.vocab, cfg.hidden)
@@ -145,6 +144,11 @@ class DenseDecoder:
         self.history = torch.zeros((capacity,), dtype=torch.int32, device=device)
         self.step_graph = None
         self._buf = {}
+
+    def _layer_cache(self):
+        shape = (self.cfg.kv_heads, self.capacity, self.cfg.head_dim)
+        return {"k_cache": self.torch.zeros(shape, device=self.device),
+                "v_cache": self.torch.zeros(shape, device=self.device)}
 
     def _b(self, name, rows, cols):
         key = (name, rows, cols)
@@ -336,6 +340,234 @@ class DenseDecoder:
             for k in ("qkv", "o", "gate_up", "down"):
                 L[k].free()
         self.lm_head.free()
+
+
+class PagedDecoder(DenseDecoder):
+    """The decoder for several sequences at a time, whose keys and values lie in pages of a common
+    pool: prompts of any lengths go in together, a step gives every running sequence a token,
+    sequences are forked (full pages shared), stopped, resumed and dropped, and the pool is
+    compacted.  Nothing of a step waits for the host -- pages are handed out on the device -- so
+    one captured step serves every mix of sequences.
+
+    cache_type: torch.float32, float16 or bfloat16.  window, sinks: as b2w4_paged_attention's; a
+    window bounds what a step reads, not the pages that a sequence keeps.
+
+    The matmuls of one row (a decoder of one slot, a prompt of one token) take the rule per 128
+    values, those of several rows `multi_row_rule`."""
+
+    def __init__(self, ctx, cfg, weights, slots, pages, page_size=32, max_length=None,
+                 cache_type=None, window=0, sinks=0, multi_row_rule=capi.ACT_G32):
+        import torch
+        if cfg.head_dim % 64 or cfg.head_dim > 256:
+            raise ValueError("a paged decoder takes heads of 64, 128, 192 or 256 numbers")
+        self.pages, self.page_size, self.slots = pages, page_size, slots
+        self.cache_type = cache_type or torch.float32
+        self.window, self.sinks = window, sinks
+        max_length = max_length or pages * page_size
+        super().__init__(ctx, cfg, weights, max_length, multi_row_rule=multi_row_rule)
+        zeros = lambda *shape: torch.zeros(shape, dtype=torch.int32, device="cuda")
+        table_len = -(-max_length // page_size)
+        self.pool = capi.PagePool(zeros(pages), zeros(slots, table_len), zeros(slots), page_size)
+        self.refs, self.tables, self.lengths = self.pool.keep
+        for L in self.layers:
+            L["cache"] = capi.PagedCache(L["k_cache"], L["v_cache"])
+        self.planes = capi.PagePlanes([L[k] for L in self.layers for k in ("k_cache", "v_cache")])
+        self.compact_work, self.used = zeros(pages), zeros(1)
+        self.token = zeros(slots)               # the next token of every slot
+        self.running = torch.full((slots,), -1, dtype=torch.int32, device="cuda")
+        # A step's rows are always the slots, so what its context holds for them keeps its place
+        # while the prompts' context grows: a captured step stays valid.
+        self.step_ctx = capi.Context(ctx.device)
+        self.work = {c: torch.empty(ctx.paged_attention_work(cfg.heads, cfg.head_dim),
+                                    dtype=torch.uint8, device="cuda")
+                     for c in (self.ctx, self.step_ctx)}
+        # A step's sequences: the running ones that got a page where they needed one.  The others
+        # keep their token and their place.
+        self.granted, self.next = zeros(slots), zeros(slots)
+        self.step_batch = capi.PagedBatch(self.tables, self.lengths, max_length,
+                                          slots=self.granted)
+
+    def _layer_cache(self):
+        shape = (self.pages, self.cfg.kv_heads, self.page_size, self.cfg.head_dim)
+        return {k: self.torch.zeros(shape, dtype=self.cache_type, device=self.device)
+                for k in ("k_cache", "v_cache")}
+
+    def _ints(self, values):
+        return self.torch.tensor(list(values), dtype=self.torch.int32, device="cuda")
+
+    def _rows(self, c, ids, batch, rows):
+        """The normalised hidden rows of `rows` tokens ahead of the lm_head."""
+        cfg = self.cfg
+        H, D, inter = cfg.hidden, cfg.head_dim, cfg.intermediate
+        rule = capi.ACT_G128 if rows == 1 else self.multi_row_rule
+        x, h = self._b("x", rows, H), self._b("h", rows, H)
+        qkv = self._b("qkv", rows, cfg.q_dim + 2 * cfg.kv_dim)
+        q, attn = self._b("q", rows, cfg.q_dim), self._b("attn", rows, cfg.q_dim)
+        o, dn = self._b("o", rows, H), self._b("dn", rows, H)
+        # rows behind the last sequence do not exist: every row here has one, if an idle one
+        c.embed_rows(self.embed, ids, x)
+        c.rms_norm(x, self.layers[0]["ln1"], cfg.eps, h)
+        for li, L in enumerate(self.layers):
+            c.matmul(L["qkv"], h, qkv, rule=rule)
+            c.paged_prepare(L["cache"], batch, qkv, cfg.heads, L["q_norm"], L["k_norm"], cfg.eps,
+                            self.cos, self.sin, q)
+            c.paged_attention(L["cache"], batch, q, cfg.heads, attn, D ** -0.5, self.work[c],
+                              window=self.window, sinks=self.sinks)
+            c.matmul(L["o"], attn, o, rule=rule)
+            if cfg.experts:
+                c.add_rms_norm(x, o, L["ln2"], cfg.eps, h)
+                c.moe_forward(h, L["router"], cfg.top_k, inter, L["gate_up"], L["down"], dn)
+            elif rows > 8:  # norm and SwiGLU made by the matmuls' quantisers
+                gu = self._b("gu", rows, 2 * inter)
+                c.matmul_norm(L["gate_up"], x, o, L["ln2"], cfg.eps, gu, rule=rule)
+                c.matmul_swiglu(L["down"], gu, dn, rule=rule)
+            else:
+                gu, act = self._b("gu", rows, 2 * inter), self._b("act", rows, inter)
+                c.add_rms_norm(x, o, L["ln2"], cfg.eps, h)
+                c.matmul(L["gate_up"], h, gu, rule=rule)
+                c.swiglu(gu, act)
+                c.matmul(L["down"], act, dn, rule=rule)
+            nxt = self.layers[li + 1]["ln1"] if li + 1 < len(self.layers) else self.final_norm
+            c.add_rms_norm(x, dn, nxt, cfg.eps, h)
+        return h
+
+    def _greedy(self, c, h, tokens):
+        for first in range(0, h.shape[0], 8):
+            c.matmul_argmax(self.lm_head, h[first:first + 8], tokens[first:first + 8])
+
+    def _check_slots(self, slots):
+        if len(set(slots)) != len(slots) or not all(0 <= s < self.slots for s in slots):
+            raise ValueError(f"slots {slots}: different ones of {self.slots} are wanted")
+
+    def _prompts(self, prompts, slots):
+        """Extends the slots by their prompts and runs those; (hidden rows, starts)."""
+        self._check_slots(slots)
+        counts = [len(p) for p in prompts]
+        if len(counts) != len(slots) or min(counts, default=0) < 1:
+            raise ValueError("a prompt of at least one token for every slot")
+        starts = np.concatenate([[0], np.cumsum(counts)]).tolist()
+        ids = self._ints(t for p in prompts for t in p)
+        where = self._ints(slots)
+        self.ctx.pages_extend(self.pool, where, self._ints(counts))
+        # the pool may have refused: nothing runs on a sequence that is not there
+        self.ctx.sync()
+        batch = capi.PagedBatch(self.tables, self.lengths, self.capacity, slots=where,
+                                starts=self._ints(starts), rows=starts[-1], max_new=max(counts))
+        return self._rows(self.ctx, ids, batch, starts[-1]), starts
+
+    def add(self, prompts, slots):
+        """Runs prompts into slots (empty ones, or behind what is there) and starts them."""
+        h, starts = self._prompts(prompts, slots)
+        last = self._ints(s - 1 for s in starts[1:])
+        rows = h.index_select(0, last)
+        tokens = self.torch.empty(len(slots), dtype=self.torch.int32, device="cuda")
+        self._greedy(self.ctx, rows, tokens)
+        where = self._ints(slots).long()
+        self.token.index_copy_(0, where, tokens)
+        self.running.index_copy_(0, where, self._ints(slots))
+
+    def score(self, ids, slot, top=0):
+        """Runs ids into an empty slot that then stops; of each token after the first the log
+        probability, the entropy of its distribution and, with top, the most likely tokens and
+        their log probabilities (tensors of len(ids) - 1 rows)."""
+        torch = self.torch
+        if len(ids) < 2:
+            raise ValueError("two tokens or more")
+        h, _ = self._prompts([ids], [slot])
+        n = len(ids) - 1
+        targets = self._ints(ids[1:])
+        out = {"logprob": torch.empty(n, device="cuda"), "entropy": torch.empty(n, device="cuda")}
+        if top:
+            out["top_values"] = torch.empty((n, top), device="cuda")
+            out["top_indices"] = torch.empty((n, top), dtype=torch.int32, device="cuda")
+        step = 256  # rows of logits at a time
+        for first in range(0, n, step):
+            rows = min(step, n - first)
+            logits = self._b("logits", rows, self.cfg.vocab)
+            self.ctx.matmul(self.lm_head, h[first:first + rows], logits, rule=capi.ACT_G128)
+            self.ctx.logprobs(logits, targets[first:first + rows],
+                              **{k: v[first:first + rows] for k, v in out.items()})
+        self.stop([slot])
+        return out
+
+    def stop(self, slots):
+        """The slots keep what they have and take no part in steps."""
+        self._check_slots(slots)
+        self.running.index_fill_(0, self._ints(slots).long(), -1)
+
+    def drop(self, slots):
+        """The slots give their pages back."""
+        self.stop(slots)
+        self.ctx.pages_free(self.pool, self._ints(slots))
+
+    def fork(self, parent, children):
+        """The children, empty slots, go on from where the parent is."""
+        self._check_slots([parent] + list(children))
+        where = self._ints(children)
+        self.ctx.pages_fork(self.pool, self.planes, self._ints([parent] * len(children)), where)
+        self.ctx.sync()
+        self.token.index_copy_(0, where.long(), self.token[parent].expand(len(children)))
+        self.running.index_copy_(0, where.long(), where)
+
+    def compact(self):
+        """Moves the pages in use to the front of the pool; returns how many they are."""
+        self.ctx.pages_compact(self.pool, self.planes, self.compact_work, self.used)
+        self.ctx.sync()
+        return int(self.used.item())
+
+    def _step(self):
+        c = self.step_ctx
+        c.pages_extend(self.pool, self.running, granted=self.granted)
+        h = self._rows(c, self.token, self.step_batch, self.slots)
+        self._greedy(c, h, self.next)
+        self.torch.where(self.granted >= 0, self.next, self.token, out=self.token)
+
+    def step(self, replay=False):
+        """Every running slot's token goes in and its next one comes out, in self.token.
+        replay: by one captured graph."""
+        torch = self.torch
+        if not replay:
+            self.step_ctx.set_stream(torch.cuda.current_stream().cuda_stream)
+            return self._step()
+        if self.step_graph is None:
+            # the kernels' first use outside the capture, with no slot running
+            running = self.running.clone()
+            self.running.fill_(-1)
+            self.step_ctx.set_stream(torch.cuda.current_stream().cuda_stream)
+            self._step()
+            self.step_ctx.sync()
+            self.running.copy_(running)
+            torch.cuda.synchronize()
+            graph, side = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+            with torch.cuda.stream(side):
+                self.step_ctx.set_stream(side.cuda_stream)
+                with torch.cuda.graph(graph, stream=side):
+                    self._step()
+            self.step_graph = graph
+        self.step_graph.replay()
+
+    def sync(self):
+        """Waits for the device; raises where the pool ran out of pages."""
+        self.ctx.sync()
+        self.torch.cuda.synchronize()
+        self.step_ctx.sync()
+
+    def generate(self, prompts, steps, replay=False):
+        """Greedy tokens of each prompt, in slots 0, 1, ..: [prompts][steps]."""
+        slots = list(range(len(prompts)))
+        self.drop(list(range(self.slots)))
+        self.add(prompts, slots)
+        out = [self.token[:len(prompts)].clone()]
+        for _ in range(steps - 1):
+            self.step(replay)
+            out.append(self.token[:len(prompts)].clone())
+        self.sync()
+        return self.torch.stack(out, 1).tolist()
+
+    def free(self):
+        super().free()
+        self.step_graph = None
+        self.step_ctx.close()
 
 
 class TensorParallelDecoder(DenseDecoder):

@@ -189,7 +189,7 @@ def test_bad_pools_are_refused(p, pl):
 
 def test_pages_calls_reject_null_contexts():
     lib = capi.lib()
-    assert lib.b2w4_pages_extend(None, None, None, None, 1) == -1
+    assert lib.b2w4_pages_extend(None, None, None, None, 1, None) == -1
     assert lib.b2w4_pages_fork(None, None, None, None, None, 1) == -1
     assert lib.b2w4_pages_free(None, None, None, 1) == -1
     assert lib.b2w4_pages_compact(None, None, None, None, None) == -1

@@ -40,6 +40,8 @@ class Model:
         """What of it cannot be done: the codes."""
         wrong, seen, free, full = set(), set(), self.free_pages(), False
         for s, c in zip(slots, counts):
+            if s == -1:
+                continue
             if not 0 <= s < self.slots or s in seen or c < 0 or \
                     self.length[s] + c > self.table_len * self.page:
                 seen.add(s)
@@ -62,6 +64,9 @@ class Model:
         wrong, seen, free, copies = set(), set(), self.free_pages(), []
         before = list(self.length)
         for p, c in zip(parents, children):
+            if -1 in (p, c):
+                seen.add(c)
+                continue
             if not (0 <= p < self.slots and 0 <= c < self.slots) or c in seen or before[c] != 0:
                 seen.add(c)
                 wrong.add("outside")
@@ -86,6 +91,8 @@ class Model:
     def free(self, slots):
         wrong = set()
         for s in slots:
+            if s == -1:
+                continue
             if not 0 <= s < self.slots:
                 wrong.add("outside")
                 continue
@@ -160,18 +167,27 @@ def test_random_histories(ctx, pages, page, slots, table_len, page_bytes, seed):
                       for _ in some]
             if rng.random() < 0.2:
                 some[-1] = rng.choice([-1, slots, some[0]])
-            d.ctx.pages_extend(d.pool, ints(some), ints(counts))
+            granted = ints([-9] * (len(some) + 1))
+            before = list(m.length)
+            d.ctx.pages_extend(d.pool, ints(some), ints(counts), granted)
             wrong = m.extend(some, counts)
+            for i, (s, c) in enumerate(zip(some, counts)):
+                if s in some[:i] or not 0 <= s < slots:
+                    assert granted[i] == -1
+                elif c:
+                    assert granted[i] == (s if m.length[s] != before[s] else -1)
+            assert granted[-1] == -9
         elif what == "fork":
             parents = [rng.randrange(slots) for _ in range(rng.randint(1, slots))]
-            children = [rng.randrange(slots) for _ in parents]
+            children = [rng.randrange(-1, slots) for _ in parents]
+            parents[0] = rng.choice([parents[0], -1])
             d.ctx.pages_fork(d.pool, d.planes, ints(parents), ints(children))
             wrong, copies = m.fork(parents, children)
             d.copied(copies)
         elif what == "free":
             some = [rng.randrange(slots) for _ in range(rng.randint(1, slots // 2))]
             if rng.random() < 0.2:
-                some.append(slots)
+                some.append(rng.choice([slots, -1]))
             d.ctx.pages_free(d.pool, ints(some))
             wrong = m.free(some)
         else:
