@@ -1,12 +1,13 @@
 // Paged key-value cache: the step between the qkv matmul and attention (Q/K norm, rotary
 // embedding, append to the pages), and attention over the pages.
-#include "paged.cuh"
+#include "paged_kernels.cuh"
 
 #include <climits>
 
 namespace {
 
 using paged::Args;
+using paged::Attend;
 using paged::Sequence;
 using paged::Window;
 
@@ -132,14 +133,6 @@ paged_prepare_kernel(const Args a, const Prepare p) {
         }
     }
 }
-
-struct Attend {
-    const float* q;
-    float* out;
-    float scale;
-    Window window;
-    int ldq, ldo, heads;
-};
 
 // One warp per (row, head), key by key.
 template <typename T, int DIM>
@@ -276,7 +269,7 @@ int b2w4_paged_prepare(b2w4_ctx* ctx, const b2w4_paged_cache* cache,
 }
 
 size_t b2w4_paged_attention_work(const b2w4_ctx* ctx, int heads, int dim) {
-    return ctx && heads > 0 && dim > 0 ? 256 : 0;
+    return ctx && heads > 0 && dim > 0 ? b2w4_paged_split_work(ctx->sm_count, dim) : 0;
 }
 
 int b2w4_paged_attention(b2w4_ctx* ctx, const b2w4_paged_cache* cache,
@@ -305,6 +298,8 @@ int b2w4_paged_attention(b2w4_ctx* ctx, const b2w4_paged_cache* cache,
     const b2w4_device_guard device(ctx);
     const Args a = args_of(ctx, *cache, *batch);
     const Attend p = {q_dev, out_dev, scale, {window, sinks}, ldq, ldo, heads};
+    if (batch->max_new == 1 && b2w4_paged_split_takes(cache->dim))
+        return b2w4_launch_paged_split(ctx, cache->type, cache->dim, a, p, work_dev);
     const unsigned blocks = ((unsigned)batch->rows * heads + kWarps - 1) / kWarps;
     return by_type(cache->type, cache->dim, [&](auto* t, auto dim) {
         using T = std::remove_pointer_t<decltype(t)>;

@@ -1,0 +1,682 @@
+// Attention of one new token per sequence over a paged cache, split over the cache's length and
+// joined.
+//
+// For the heads of a kv head, with the keys of a part of the cache: m = max s_j, l = sum
+// exp(s_j - m), o = sum exp(s_j - m) v_j; parts join by scaling with exp(m_part - m).
+//
+// What bounds it: the bytes of the cache.  So the keys that the batch sees, in blocks of 16, lie
+// in one line over sequences, kv heads and sets of 16 heads, of which every warp of the chip takes
+// an equal share, whatever the lengths: one long sequence fills the chip as well as many short
+// ones.  A warp streams its blocks through a cp.async ring of its own and meets no other warp.  A
+// part of the cache that began or ended inside another warp's share goes to the work area; a
+// second launch joins those.
+//
+// Products are mma.sync m16n8k16, the heads as the rows: with 16 heads a key costs 8192
+// multiply-adds, more than the fp32 pipe has in the time that the key's bytes take.  Every operand
+// of 32 bits is a sum of pieces of the cache's 16-bit type, products small ones first, sums in 32
+// bits: three bf16 pieces (24 bits) beside a bf16 cache; two fp16 pieces (22 bits) of the row's
+// query or probabilities times a power of two beside an fp16 cache, which loses below 2^-22 of the
+// row's largest; three pieces of both sides beside an fp32 cache, six products of the nine.  A sum
+// in the tensor core truncates, so an output's sum over a block of keys starts from zero and is
+// added to the running one with one rounding.
+//
+// What pieces cannot hold -- infinities, NaN, results that are not finite -- is done key by key in
+// 32 bits (paged::attend_row), which has the rule for values of probability zero.
+#include "paged_kernels.cuh"
+
+#include <climits>
+
+namespace {
+
+using paged::Args;
+using paged::Attend;
+using paged::Sequence;
+
+constexpr int kKeys = 16;  // of a block
+constexpr int kSet = 16;   // heads of a set: rows of the products
+
+template <typename T>
+struct Pieces {  // of a query or probability, and of a key or value
+    static constexpr int kQ = 3, kK = 1;
+};
+template <>
+struct Pieces<__half> {
+    static constexpr int kQ = 2, kK = 1;
+};
+template <>
+struct Pieces<float> {
+    static constexpr int kQ = 3, kK = 3;
+};
+
+template <typename T, int DIM>
+struct Ring {
+    static constexpr int kRow = DIM * sizeof(T);       // bytes
+    static constexpr int kHalf = kKeys * kRow;          // keys; the values behind them
+    static constexpr int kSlot = 2 * kHalf;
+    static constexpr int kSlots = kSlot > 8192 ? 2 : kSlot > 4096 ? 3 : 5;
+    static constexpr int kWarps = kSlot > 8192 ? 7 : 8;
+    static constexpr int kBytes = kWarps * kSlots * kSlot;
+};
+
+// The line of blocks: how many a warp takes, and where sequences begin in it.
+struct Line {
+    int total, share;
+};
+// The least share: below that, parts cost more than they save.
+constexpr int kLeastShare = 4;
+
+// Keys that the one token of a sequence sees: [0, low) and [from, length).
+struct Seen {
+    int low, from, count;
+};
+__device__ __forceinline__ Seen seen_by(const Sequence& s, const paged::Window& w) {
+    Seen v = {0, 0, 0};
+    if (s.count != 1 || s.length <= 0)
+        return v;
+    v.from = w.from(s.length - 1);
+    v.low = min(w.sinks, v.from);
+    v.count = v.low + s.length - v.from;
+    return v;
+}
+__device__ __forceinline__ int blocks_of(const Args& a, const paged::Window& w, int i, bool report) {
+    bool bad = false;
+    const Sequence s = paged::sequence(a, i, &bad);
+    if (report && (bad || s.count > 1))
+        b2w4_report(a.status, B2W4_E_INVALID);
+    return (seen_by(s, w).count + kKeys - 1) / kKeys;
+}
+
+// Whole warp.  Blocks of all sequences; every tile (kv head and set of heads) of a sequence has as
+// many.
+__device__ Line line_of(const Args& a, const paged::Window& w, int tiles, int warps, bool report) {
+    int sum = 0;
+    for (int i = threadIdx.x & 31; i < a.sequences; i += 32)
+        sum += blocks_of(a, w, i, report);
+    sum = __reduce_add_sync(0xffffffffu, sum) * tiles;
+    return {sum, max(kLeastShare, (sum + warps - 1) / warps)};
+}
+
+// Whole warp.  The sequence whose blocks hold block `at` of the line, and where they begin.
+__device__ int find(const Args& a, const paged::Window& w, int tiles, int at, int* begin) {
+    const int lane = threadIdx.x & 31;
+    int before = 0;
+    for (int base = 0; base < a.sequences; base += 32) {
+        const int n = base + lane < a.sequences ? blocks_of(a, w, base + lane, false) * tiles : 0;
+        int x = n;
+#pragma unroll
+        for (int off = 1; off < 32; off <<= 1) {
+            const int y = __shfl_up_sync(0xffffffffu, x, off);
+            if (lane >= off)
+                x += y;
+        }
+        const unsigned past = __ballot_sync(0xffffffffu, before + x > at);
+        if (past) {
+            const int l = __ffs(past) - 1;
+            *begin = before + __shfl_sync(0xffffffffu, x - n, l);
+            return base + l;
+        }
+        before += __shfl_sync(0xffffffffu, x, 31);
+    }
+    *begin = before;
+    return a.sequences;
+}
+
+// A part: m and l of its 16 rows, then their outputs.
+template <int DIM>
+struct Part {
+    static constexpr int kFloats = 2 * kSet + kSet * DIM;
+};
+
+__device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool there) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src),
+                 "r"(there ? 16 : 0)
+                 : "memory");
+}
+template <int N>
+__device__ __forceinline__ void cp_wait() {
+    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ void ldmatrix(uint32_t (&r)[4], uint32_t at) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(at));
+}
+__device__ __forceinline__ void ldmatrix_trans(uint32_t (&r)[4], uint32_t at) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(at));
+}
+__device__ __forceinline__ float4 lds128(uint32_t at) {
+    float4 v;
+    asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];"
+                 : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+                 : "r"(at));
+    return v;
+}
+// bf16 products except beside an fp16 cache
+template <typename T>
+__device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0,
+                                    uint32_t b1) {
+    if constexpr (std::is_same_v<T, __half>)
+        asm volatile(
+            "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, "
+            "%7}, {%8, %9}, {%0, %1, %2, %3};"
+            : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+            : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+    else
+        asm volatile(
+            "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, "
+            "%7}, {%8, %9}, {%0, %1, %2, %3};"
+            : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+            : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+// The next piece of two numbers, lo in the low half; they keep what is left (exact).
+template <typename T>
+__device__ __forceinline__ uint32_t take_piece(float& lo, float& hi) {
+    uint32_t p;
+    if constexpr (std::is_same_v<T, __half>) {
+        asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(p) : "f"(hi), "f"(lo));
+        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&p));
+        lo = __fsub_rn(lo, f.x);
+        hi = __fsub_rn(hi, f.y);
+    } else {
+        asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(p) : "f"(hi), "f"(lo));
+        lo = __fsub_rn(lo, __uint_as_float(p << 16));
+        hi = __fsub_rn(hi, __uint_as_float(p & 0xffff0000u));
+    }
+    return p;
+}
+__device__ __forceinline__ float exp2_neg(float x) {
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+
+constexpr float kHalfScale = 1024.f;  // of probabilities beside an fp16 cache
+
+template <typename T, int DIM>
+__global__ void __launch_bounds__(Ring<T, DIM>::kWarps * 32, 1)
+paged_split_kernel(const Args a, const Attend p, float* __restrict__ parts) {
+    using R = Ring<T, DIM>;
+    constexpr int kQ = Pieces<T>::kQ, kK = Pieces<T>::kK, kSteps = DIM / 16, kTiles = DIM / 8;
+    constexpr bool kWide = sizeof(T) == 4;  // an fp32 cache
+    extern __shared__ __align__(1024) uint8_t smem[];
+    b2w4_pdl_chain_entry();
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int r = lane >> 2, t = lane & 3;  // row of the products' operands, column pair
+    const int group = p.heads / a.kv_heads, sets = (group + kSet - 1) / kSet;
+    const int tiles = a.kv_heads * sets;
+    const int warps = gridDim.x * R::kWarps, me = blockIdx.x * R::kWarps + warp;
+    const Line line = line_of(a, p.window, tiles, warps, me == 0);
+    int at = min(line.total, me * line.share);
+    const int end = min(line.total, at + line.share);
+    if (at >= end)
+        return;
+    int begin;
+    int seq = find(a, p.window, tiles, at, &begin);
+    const uint32_t ring = (uint32_t)__cvta_generic_to_shared(smem) + warp * R::kSlots * R::kSlot;
+    const int first = at;
+
+    while (at < end) {
+        bool bad = false;
+        const Sequence s = paged::sequence(a, seq, &bad);
+        const Seen seen = seen_by(s, p.window);
+        const int blocks = (seen.count + kKeys - 1) / kKeys;
+        if (blocks == 0) {
+            ++seq;
+            continue;
+        }
+        // the tile, and the share's blocks of it
+        const int tile = (at - begin) / blocks;
+        const int b0 = at - begin - tile * blocks, b1 = min(blocks, b0 + end - at);
+        const int kvh = tile / sets, head0 = kvh * group + (tile - kvh * sets) * kSet;
+        const int heads = min(kSet, (kvh + 1) * group - head0);
+
+        // ---- the heads' queries as operands ------------------------------------------
+        uint32_t q[kQ][kSteps][4];
+        float unscale[2] = {1.f, 1.f};
+        {
+            const float* row = p.q + (size_t)s.first * p.ldq + (size_t)head0 * DIM;
+            float x[kSteps][8];
+#pragma unroll
+            for (int k = 0; k < kSteps; ++k)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const bool in = r + 8 * h < heads;
+                    const float* src = row + (r + 8 * h) * DIM + 16 * k;
+                    if (kWide) {  // column pairs 2t and 2t + 8 hold features 4t .. 4t + 3
+                        const float4 v = in ? *reinterpret_cast<const float4*>(src + 4 * t)
+                                            : make_float4(0.f, 0.f, 0.f, 0.f);
+                        x[k][4 * h] = v.x;
+                        x[k][4 * h + 1] = v.y;
+                        x[k][4 * h + 2] = v.z;
+                        x[k][4 * h + 3] = v.w;
+                    } else {
+                        const float2 z = make_float2(0.f, 0.f);
+                        const float2 v = in ? *reinterpret_cast<const float2*>(src + 2 * t) : z;
+                        const float2 w = in ? *reinterpret_cast<const float2*>(src + 2 * t + 8) : z;
+                        x[k][4 * h] = v.x;
+                        x[k][4 * h + 1] = v.y;
+                        x[k][4 * h + 2] = w.x;
+                        x[k][4 * h + 3] = w.y;
+                    }
+                }
+            if constexpr (std::is_same_v<T, __half>) {  // the row's largest to [2^10, 2^11)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    float top = 0.f;
+#pragma unroll
+                    for (int k = 0; k < kSteps; ++k)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            top = fmaxf(top, fabsf(x[k][4 * h + e]));
+                    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+                    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+                    int e = (int)(__float_as_uint(top) >> 23) - 127;
+                    e = top == 0.f ? 10 : min(max(e, -100), 120);
+                    const float up = __uint_as_float((unsigned)(127 + 10 - e) << 23);
+                    unscale[h] = __uint_as_float((unsigned)(127 - 10 + e) << 23);
+#pragma unroll
+                    for (int k = 0; k < kSteps; ++k)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+                            x[k][4 * h + i] = __fmul_rn(x[k][4 * h + i], up);
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < kQ; ++i)
+#pragma unroll
+                for (int k = 0; k < kSteps; ++k) {
+                    q[i][k][0] = take_piece<T>(x[k][0], x[k][1]);
+                    q[i][k][1] = take_piece<T>(x[k][4], x[k][5]);
+                    q[i][k][2] = take_piece<T>(x[k][2], x[k][3]);
+                    q[i][k][3] = take_piece<T>(x[k][6], x[k][7]);
+                }
+        }
+
+        // ---- the stream of blocks ----------------------------------------------------
+        // Lane j < 16 knows where key j of a block lies; -1: no such key.
+        auto row_of = [&](int b) {
+            const int i = b * kKeys + (lane & 15);
+            if (b >= b1 || i >= seen.count)
+                return -1;
+            const int j = i < seen.low ? i : i - seen.low + seen.from;
+            const int row = paged::cache_row(a, s.table, j, kvh);
+            if (row < 0)
+                b2w4_report(a.status, B2W4_E_INVALID);
+            return row;
+        };
+        constexpr int kChunks = R::kRow / 16, kRows = kChunks >= 32 ? 1 : 32 / kChunks;
+        auto swizzled = [&](int key, int chunk, bool values) {
+            const int x = kWide ? (values ? key & 6 : (key & 1) << 2) : key & 7;
+            return (uint32_t)(key * R::kRow + ((chunk ^ x) << 4));
+        };
+        auto fetch = [&](int slot, int row) {
+            const uint32_t dst = ring + slot * R::kSlot;
+#pragma unroll
+            for (int i = 0; i < kKeys / kRows; ++i) {
+                const int key = i * kRows + (kRows > 1 ? lane / kChunks : 0);
+                const int from = __shfl_sync(0xffffffffu, row, key);
+                const size_t off = (size_t)max(from, 0) * R::kRow;
+#pragma unroll
+                for (int c = lane % kChunks; c < kChunks; c += 32) {
+                    cp16(dst + swizzled(key, c, false),
+                         static_cast<const uint8_t*>(a.k) + off + c * 16, from >= 0);
+                    cp16(dst + R::kHalf + swizzled(key, c, true),
+                         static_cast<const uint8_t*>(a.v) + off + c * 16, from >= 0);
+                }
+            }
+            asm volatile("cp.async.commit_group;" ::: "memory");
+            return __ballot_sync(0xffffffffu, row >= 0) & 0xffffu;
+        };
+        unsigned there[R::kSlots];  // of the slots' keys, those that exist
+#pragma unroll
+        for (int i = 0; i < R::kSlots - 1; ++i)
+            there[i] = fetch(i, row_of(b0 + i));
+        int next_row = row_of(b0 + R::kSlots - 1);
+
+        float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+        float o[kTiles][4];
+#pragma unroll
+        for (int i = 0; i < kTiles; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                o[i][e] = 0.f;
+        const float factor[2] = {__fmul_rn(__fmul_rn(p.scale, 1.4426950408889634f), unscale[0]),
+                                 __fmul_rn(__fmul_rn(p.scale, 1.4426950408889634f), unscale[1])};
+
+        auto block = [&](int slot, unsigned keys) {
+            const uint32_t ks = ring + slot * R::kSlot, vs = ks + R::kHalf;
+            float sc[2][4] = {};
+#pragma unroll
+            for (int k = 0; k < kSteps; ++k) {
+                if constexpr (kWide) {
+#pragma unroll
+                    for (int n = 0; n < 2; ++n) {
+                        const float4 f = lds128(ks + swizzled(n * 8 + r, 4 * k + t, false));
+                        float v[4] = {f.x, f.y, f.z, f.w};
+                        uint32_t b[kK][2];
+#pragma unroll
+                        for (int i = 0; i < kK; ++i) {
+                            b[i][0] = take_piece<T>(v[0], v[1]);
+                            b[i][1] = take_piece<T>(v[2], v[3]);
+                        }
+                        mma<T>(sc[n], q[2][k], b[0][0], b[0][1]);
+                        mma<T>(sc[n], q[0][k], b[2][0], b[2][1]);
+                        mma<T>(sc[n], q[1][k], b[1][0], b[1][1]);
+                        mma<T>(sc[n], q[1][k], b[0][0], b[0][1]);
+                        mma<T>(sc[n], q[0][k], b[1][0], b[1][1]);
+                        mma<T>(sc[n], q[0][k], b[0][0], b[0][1]);
+                    }
+                } else {
+                    // matrices: keys 0-7 and 8-15, features 0-7 and 8-15 of the step
+                    uint32_t b[4];
+                    ldmatrix(b, ks + swizzled((lane & 7) + (lane >> 4) * 8,
+                                              2 * k + ((lane >> 3) & 1), false));
+#pragma unroll
+                    for (int i = kQ - 1; i >= 0; --i) {
+                        mma<T>(sc[0], q[i][k], b[0], b[1]);
+                        mma<T>(sc[1], q[i][k], b[2], b[3]);
+                    }
+                }
+            }
+            float alpha[2], pr[2][4];
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                float top = m[h];
+#pragma unroll
+                for (int n = 0; n < 2; ++n)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        float& x = sc[n][2 * h + e];
+                        x = __fmul_rn(x, factor[h]);
+                        if (!(keys >> (8 * n + 2 * t + e) & 1))
+                            x = -INFINITY;
+                        top = fmaxf(top, x);
+                    }
+                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+                const float base = top == -INFINITY ? 0.f : top;
+                alpha[h] = exp2_neg(__fsub_rn(m[h], base));
+                m[h] = top;
+                float sum = 0.f;
+#pragma unroll
+                for (int n = 0; n < 2; ++n)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        const float v = exp2_neg(__fsub_rn(sc[n][2 * h + e], base));
+                        sum = __fadd_rn(sum, v);
+                        pr[n][2 * h + e] =
+                            std::is_same_v<T, __half> ? __fmul_rn(v, kHalfScale) : v;
+                    }
+                l[h] = __fmaf_rn(l[h], alpha[h], sum);
+            }
+            uint32_t pp[kQ][4];
+#pragma unroll
+            for (int i = 0; i < kQ; ++i) {
+                pp[i][0] = take_piece<T>(pr[0][0], pr[0][1]);
+                pp[i][1] = take_piece<T>(pr[0][2], pr[0][3]);
+                pp[i][2] = take_piece<T>(pr[1][0], pr[1][1]);
+                pp[i][3] = take_piece<T>(pr[1][2], pr[1][3]);
+            }
+            auto add = [&](int n, const float (&x)[4]) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    o[n][e] = __fmaf_rn(o[n][e], alpha[e >> 1], x[e]);
+            };
+            if constexpr (kWide) {
+                // a group of 32 features: lane's four of each of its keys, one per tile
+#pragma unroll
+                for (int j = 0; j < DIM / 32; ++j) {
+                    float v[4][4];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const float4 f =
+                            lds128(vs + swizzled(2 * t + (e & 1) + (e >> 1) * 8, 8 * j + r, true));
+                        v[e][0] = f.x;
+                        v[e][1] = f.y;
+                        v[e][2] = f.z;
+                        v[e][3] = f.w;
+                    }
+#pragma unroll
+                    for (int n = 0; n < 4; ++n) {
+                        float x[4] = {};
+                        uint32_t b[kK][2];
+#pragma unroll
+                        for (int i = 0; i < kK; ++i) {
+                            b[i][0] = take_piece<T>(v[0][n], v[1][n]);
+                            b[i][1] = take_piece<T>(v[2][n], v[3][n]);
+                        }
+                        mma<T>(x, pp[2], b[0][0], b[0][1]);
+                        mma<T>(x, pp[0], b[2][0], b[2][1]);
+                        mma<T>(x, pp[1], b[1][0], b[1][1]);
+                        mma<T>(x, pp[1], b[0][0], b[0][1]);
+                        mma<T>(x, pp[0], b[1][0], b[1][1]);
+                        mma<T>(x, pp[0], b[0][0], b[0][1]);
+                        add(4 * j + n, x);
+                    }
+                }
+            } else {
+#pragma unroll
+                for (int n = 0; n < kTiles; n += 2) {
+                    // keys 0-7 and 8-15, features 8n .. 8n + 7 and the next eight
+                    uint32_t b[4];
+                    ldmatrix_trans(b, vs + swizzled((lane & 7) + ((lane >> 3) & 1) * 8,
+                                                    n + (lane >> 4), true));
+                    float x[4] = {}, y[4] = {};
+#pragma unroll
+                    for (int i = kQ - 1; i >= 0; --i) {
+                        mma<T>(x, pp[i], b[0], b[1]);
+                        mma<T>(y, pp[i], b[2], b[3]);
+                    }
+                    add(n, x);
+                    add(n + 1, y);
+                }
+            }
+        };
+
+        for (int b = b0; b < b1; b += R::kSlots) {
+#pragma unroll
+            for (int u = 0; u < R::kSlots; ++u) {
+                if (b + u >= b1)
+                    break;
+                cp_wait<R::kSlots - 2>();
+                __syncwarp();
+                // the slot that the block before has left
+                constexpr int kLast = R::kSlots - 1;
+                const int into = (u + kLast) % R::kSlots;
+                there[into] = fetch(into, next_row);
+                next_row = row_of(b + u + R::kSlots);
+                block(u, there[u]);
+                __syncwarp();
+            }
+        }
+        cp_wait<0>();
+        __syncwarp();
+
+        // ---- the part, or the result -------------------------------------------------
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            l[h] = __fadd_rn(l[h], __shfl_xor_sync(0xffffffffu, l[h], 1));
+            l[h] = __fadd_rn(l[h], __shfl_xor_sync(0xffffffffu, l[h], 2));
+        }
+        const bool whole = b0 == 0 && b1 == blocks;
+        constexpr float kDown = std::is_same_v<T, __half> ? 1.f / kHalfScale : 1.f;
+        float* part = parts + ((size_t)2 * me + (at != first)) * Part<DIM>::kFloats;
+        bool odd = false;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const int row = r + 8 * h;
+            if (row >= heads)
+                continue;
+            float* dst = whole ? p.out + (size_t)s.first * p.ldo + (size_t)(head0 + row) * DIM
+                               : part + 2 * kSet + row * DIM;
+            if (!whole && t == 0) {
+                part[row] = m[h];
+                part[kSet + row] = l[h];
+            }
+            auto final = [&](float x) {
+                x = __fmul_rn(x, kDown);
+                if (!whole)
+                    return x;
+                x = __fdiv_rn(x, l[h]);
+                odd |= paged::odd_result<T>(x);
+                return x;
+            };
+            if constexpr (kWide) {
+#pragma unroll
+                for (int j = 0; j < DIM / 32; ++j)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e)
+                        *reinterpret_cast<float4*>(dst + 32 * j + 8 * t + 4 * e) =
+                            make_float4(final(o[4 * j][2 * h + e]), final(o[4 * j + 1][2 * h + e]),
+                                        final(o[4 * j + 2][2 * h + e]),
+                                        final(o[4 * j + 3][2 * h + e]));
+            } else {
+#pragma unroll
+                for (int n = 0; n < kTiles; ++n)
+                    *reinterpret_cast<float2*>(dst + 8 * n + 2 * t) =
+                        make_float2(final(o[n][2 * h]), final(o[n][2 * h + 1]));
+            }
+        }
+        __syncwarp();
+        if (__any_sync(0xffffffffu, odd)) {
+            for (int h = 0; h < heads; ++h)
+                paged::attend_row<T, DIM>(a, s, p.q + (size_t)s.first * p.ldq +
+                                                    (size_t)(head0 + h) * DIM,
+                                          s.length - 1, kvh, p.scale, p.window,
+                                          p.out + (size_t)s.first * p.ldo +
+                                              (size_t)(head0 + h) * DIM);
+        }
+        at += b1 - b0;
+        if (at - begin == blocks * tiles) {
+            begin = at;
+            ++seq;
+        }
+    }
+}
+
+// Joins what several warps' shares hold of a tile; rows without a key.  A block per sequence and
+// head: warps take the parts in turn, then the block joins the warps' sums.
+constexpr int kJoinWarps = 8;
+template <typename T, int DIM>
+__global__ void __launch_bounds__(kJoinWarps * 32)
+paged_join_kernel(const Args a, const Attend p, const float* __restrict__ parts, int warps) {
+    b2w4_pdl_chain_entry();
+    constexpr int kOwn = DIM / 32;
+    __shared__ float s_o[kJoinWarps][DIM];
+    __shared__ float s_m[kJoinWarps], s_l[kJoinWarps];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int seq = blockIdx.x / p.heads, head = blockIdx.x - seq * p.heads;
+    const int group = p.heads / a.kv_heads, sets = (group + kSet - 1) / kSet;
+    const int tiles = a.kv_heads * sets;
+    bool bad = false;
+    const Sequence s = paged::sequence(a, seq, &bad);
+    if (s.count != 1)
+        return;
+    const Seen seen = seen_by(s, p.window);
+    float* out = p.out + (size_t)s.first * p.ldo + (size_t)head * DIM;
+    if (seen.count == 0) {
+        if (threadIdx.x < DIM)
+            out[threadIdx.x] = 0.f;
+        return;
+    }
+    const Line line = line_of(a, p.window, tiles, warps, false);
+    int before = 0;
+    for (int i = lane; i < seq; i += 32)
+        before += blocks_of(a, p.window, i, false);
+    before = __reduce_add_sync(0xffffffffu, before) * tiles;
+    const int blocks = (seen.count + kKeys - 1) / kKeys;
+    const int kvh = head / group, in = head - kvh * group, row = in % kSet;
+    const int begin = before + (kvh * sets + in / kSet) * blocks;
+    const int w0 = begin / line.share, w1 = (begin + blocks - 1) / line.share;
+    if (w0 == w1)
+        return;  // one warp had all of it
+    float m = -INFINITY, l = 0.f, o[kOwn];
+#pragma unroll
+    for (int i = 0; i < kOwn; ++i)
+        o[i] = 0.f;
+    for (int w = w0 + warp; w <= w1; w += kJoinWarps) {
+        const bool second = w == w0 && begin != w0 * line.share;
+        const float* part = parts + ((size_t)2 * w + second) * Part<DIM>::kFloats;
+        const float pm = part[row], pl = part[kSet + row];
+        float x[kOwn];
+#pragma unroll
+        for (int i = 0; i < kOwn; ++i)
+            x[i] = part[2 * kSet + row * DIM + lane + 32 * i];
+        const float top = fmaxf(m, pm), base = top == -INFINITY ? 0.f : top;
+        const float ea = exp2_neg(__fsub_rn(m, base)), eb = exp2_neg(__fsub_rn(pm, base));
+        m = top;
+        l = __fmaf_rn(l, ea, __fmul_rn(pl, eb));
+#pragma unroll
+        for (int i = 0; i < kOwn; ++i)
+            o[i] = __fmaf_rn(o[i], ea, __fmul_rn(x[i], eb));
+    }
+    if (lane == 0) {
+        s_m[warp] = m;
+        s_l[warp] = l;
+    }
+#pragma unroll
+    for (int i = 0; i < kOwn; ++i)
+        s_o[warp][lane + 32 * i] = o[i];
+    __syncthreads();
+    float top = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < kJoinWarps; ++w)
+        top = fmaxf(top, s_m[w]);
+    const float base = top == -INFINITY ? 0.f : top;
+    float total = 0.f, x = 0.f;
+    const int d = threadIdx.x;
+#pragma unroll
+    for (int w = 0; w < kJoinWarps; ++w) {
+        const float e = exp2_neg(__fsub_rn(s_m[w], base));
+        total = __fmaf_rn(s_l[w], e, total);
+        if (d < DIM)
+            x = __fmaf_rn(s_o[w][d], e, x);
+    }
+    x = __fdiv_rn(x, total);
+    if (d < DIM)
+        out[d] = x;
+    if (__syncthreads_or(d < DIM && paged::odd_result<T>(x)) && warp == 0)
+        paged::attend_row<T, DIM>(a, s, p.q + (size_t)s.first * p.ldq + (size_t)head * DIM,
+                                  s.length - 1, kvh, p.scale, p.window, out);
+}
+
+template <typename T, int DIM>
+int launch(b2w4_ctx* ctx, const Args& a, const Attend& p, void* work) {
+    using R = Ring<T, DIM>;
+    static b2w4_smem_optin cfg;
+    auto kern = paged_split_kernel<T, DIM>;
+    B2W4_CUDA(ctx, b2w4_opt_in_smem(ctx, kern, R::kBytes, cfg));
+    const int blocks = ctx->sm_count;
+    float* parts = static_cast<float*>(work);
+    B2W4_CUDA(ctx, b2w4_launch_chained(ctx->pdl, kern, dim3(blocks), dim3(R::kWarps * 32),
+                                       R::kBytes, ctx->stream, a, p, parts));
+    ctx->launches++;
+    B2W4_CUDA(ctx, b2w4_launch_chained(ctx->pdl, paged_join_kernel<T, DIM>,
+                                       dim3((unsigned)a.sequences * p.heads),
+                                       dim3(kJoinWarps * 32), 0, ctx->stream, a, p,
+                                       static_cast<const float*>(parts), blocks * R::kWarps));
+    ctx->launches++;
+    return B2W4_OK;
+}
+
+}  // namespace
+
+// Two parts of every warp.
+size_t b2w4_paged_split_work(int sm_count, int dim) {
+    return sizeof(float) * 2 * (2 * kSet + kSet * (size_t)dim) * 8 * sm_count;
+}
+
+bool b2w4_paged_split_takes(int dim) { return dim <= 128; }
+
+int b2w4_launch_paged_split(b2w4_ctx* ctx, int type, int dim, const Args& a, const Attend& p,
+                            void* work) {
+    if (dim == 64)
+        return type == B2W4_F16    ? launch<__half, 64>(ctx, a, p, work)
+               : type == B2W4_BF16 ? launch<__nv_bfloat16, 64>(ctx, a, p, work)
+                                   : launch<float, 64>(ctx, a, p, work);
+    return type == B2W4_F16    ? launch<__half, 128>(ctx, a, p, work)
+           : type == B2W4_BF16 ? launch<__nv_bfloat16, 128>(ctx, a, p, work)
+                               : launch<float, 128>(ctx, a, p, work);
+}
