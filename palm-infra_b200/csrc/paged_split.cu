@@ -56,6 +56,7 @@ struct Ring {
     static constexpr int kSlots = kSlot > 8192 ? 2 : kSlot > 4096 ? 3 : 5;
     static constexpr int kWarps = kSlot > 8192 ? 7 : 8;
     static constexpr int kBytes = kWarps * kSlots * kSlot;
+    static_assert(kWarps <= 8, "the work area");
 };
 
 // The line of blocks: how many a warp takes, and where sequences begin in it.
@@ -63,7 +64,7 @@ struct Line {
     int total, share;
 };
 // The least share: below that, parts cost more than they save.
-constexpr int kLeastShare = 4;
+constexpr int kLeastShare = 1;
 
 // Keys that the one token of a sequence sees: [0, low) and [from, length).
 struct Seen {
@@ -126,6 +127,17 @@ template <int DIM>
 struct Part {
     static constexpr int kFloats = 2 * kSet + kSet * DIM;
 };
+// Whose part it is: the tile's sequence, its heads, and the warps that have parts of it, the
+// first's in its second place if `second`.  count 0: no part.
+struct Owner {
+    int seq, head0, count, w0, w1, second, pad[2];
+};
+// The work area: two parts of every warp, and their owners.
+constexpr int kMostWarps = 8;
+template <int DIM>
+__host__ __device__ size_t owners_at(int warps) {
+    return sizeof(float) * 2 * Part<DIM>::kFloats * (size_t)warps;
+}
 
 __device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool there) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src),
@@ -158,14 +170,12 @@ template <typename T>
 __device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0,
                                     uint32_t b1) {
     if constexpr (std::is_same_v<T, __half>)
-        asm volatile(
-            "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, "
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, "
             "%7}, {%8, %9}, {%0, %1, %2, %3};"
             : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
             : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
     else
-        asm volatile(
-            "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, "
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, "
             "%7}, {%8, %9}, {%0, %1, %2, %3};"
             : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
             : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
@@ -196,7 +206,8 @@ constexpr float kHalfScale = 1024.f;  // of probabilities beside an fp16 cache
 
 template <typename T, int DIM>
 __global__ void __launch_bounds__(Ring<T, DIM>::kWarps * 32, 1)
-paged_split_kernel(const Args a, const Attend p, float* __restrict__ parts) {
+paged_split_kernel(const Args a, const Attend p, float* __restrict__ parts,
+                   Owner* __restrict__ owners) {
     using R = Ring<T, DIM>;
     constexpr int kQ = Pieces<T>::kQ, kK = Pieces<T>::kK, kSteps = DIM / 16, kTiles = DIM / 8;
     constexpr bool kWide = sizeof(T) == 4;  // an fp32 cache
@@ -206,12 +217,23 @@ paged_split_kernel(const Args a, const Attend p, float* __restrict__ parts) {
     const int r = lane >> 2, t = lane & 3;  // row of the products' operands, column pair
     const int group = p.heads / a.kv_heads, sets = (group + kSet - 1) / kSet;
     const int tiles = a.kv_heads * sets;
-    const int warps = gridDim.x * R::kWarps, me = blockIdx.x * R::kWarps + warp;
+    const int warps = gridDim.x * R::kWarps;
+    const int me = warp * gridDim.x + blockIdx.x;  // few shares: a multiprocessor each
     const Line line = line_of(a, p.window, tiles, warps, me == 0);
     int at = min(line.total, me * line.share);
     const int end = min(line.total, at + line.share);
+    if (lane < 2)
+        owners[2 * me + lane].count = 0;
+    for (int i = me; i < a.sequences; i += warps) {  // sequences that see no key
+        bool bad = false;
+        const Sequence s = paged::sequence(a, i, &bad);
+        if (s.count == 1 && seen_by(s, p.window).count == 0)
+            for (int d = lane; d < p.heads * DIM; d += 32)
+                p.out[(size_t)s.first * p.ldo + d] = 0.f;
+    }
     if (at >= end)
         return;
+    __syncwarp();
     int begin;
     int seq = find(a, p.window, tiles, at, &begin);
     const uint32_t ring = (uint32_t)__cvta_generic_to_shared(smem) + warp * R::kSlots * R::kSlot;
@@ -329,7 +351,8 @@ paged_split_kernel(const Args a, const Attend p, float* __restrict__ parts) {
             asm volatile("cp.async.commit_group;" ::: "memory");
             return __ballot_sync(0xffffffffu, row >= 0) & 0xffffu;
         };
-        unsigned there[R::kSlots];  // of the slots' keys, those that exist
+        // of the keys of the blocks on their way, those that exist: the next block's first
+        unsigned there[R::kSlots - 1];
 #pragma unroll
         for (int i = 0; i < R::kSlots - 1; ++i)
             there[i] = fetch(i, row_of(b0 + i));
@@ -347,7 +370,8 @@ paged_split_kernel(const Args a, const Attend p, float* __restrict__ parts) {
 
         auto block = [&](int slot, unsigned keys) {
             const uint32_t ks = ring + slot * R::kSlot, vs = ks + R::kHalf;
-            float sc[2][4] = {};
+            // a sum for each size of products: six chains instead of two
+            float by[kQ][2][4] = {};
 #pragma unroll
             for (int k = 0; k < kSteps; ++k) {
                 if constexpr (kWide) {
@@ -361,12 +385,12 @@ paged_split_kernel(const Args a, const Attend p, float* __restrict__ parts) {
                             b[i][0] = take_piece<T>(v[0], v[1]);
                             b[i][1] = take_piece<T>(v[2], v[3]);
                         }
-                        mma<T>(sc[n], q[2][k], b[0][0], b[0][1]);
-                        mma<T>(sc[n], q[0][k], b[2][0], b[2][1]);
-                        mma<T>(sc[n], q[1][k], b[1][0], b[1][1]);
-                        mma<T>(sc[n], q[1][k], b[0][0], b[0][1]);
-                        mma<T>(sc[n], q[0][k], b[1][0], b[1][1]);
-                        mma<T>(sc[n], q[0][k], b[0][0], b[0][1]);
+                        mma<T>(by[2][n], q[2][k], b[0][0], b[0][1]);
+                        mma<T>(by[1][n], q[1][k], b[0][0], b[0][1]);
+                        mma<T>(by[0][n], q[0][k], b[0][0], b[0][1]);
+                        mma<T>(by[2][n], q[1][k], b[1][0], b[1][1]);
+                        mma<T>(by[1][n], q[0][k], b[1][0], b[1][1]);
+                        mma<T>(by[2][n], q[0][k], b[2][0], b[2][1]);
                     }
                 } else {
                     // matrices: keys 0-7 and 8-15, features 0-7 and 8-15 of the step
@@ -375,12 +399,21 @@ paged_split_kernel(const Args a, const Attend p, float* __restrict__ parts) {
                                               2 * k + ((lane >> 3) & 1), false));
 #pragma unroll
                     for (int i = kQ - 1; i >= 0; --i) {
-                        mma<T>(sc[0], q[i][k], b[0], b[1]);
-                        mma<T>(sc[1], q[i][k], b[2], b[3]);
+                        mma<T>(by[i][0], q[i][k], b[0], b[1]);
+                        mma<T>(by[i][1], q[i][k], b[2], b[3]);
                     }
                 }
             }
-            float alpha[2], pr[2][4];
+            float alpha[2], pr[2][4], sc[2][4];
+#pragma unroll
+            for (int n = 0; n < 2; ++n)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    sc[n][e] = by[kQ - 1][n][e];
+#pragma unroll
+                    for (int i = kQ - 2; i >= 0; --i)
+                        sc[n][e] = __fadd_rn(sc[n][e], by[i][n][e]);
+                }
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
                 float top = m[h];
@@ -438,58 +471,64 @@ paged_split_kernel(const Args a, const Attend p, float* __restrict__ parts) {
                         v[e][2] = f.z;
                         v[e][3] = f.w;
                     }
+                    float x[4][4] = {};
+                    uint32_t b[4][kK][2];
 #pragma unroll
-                    for (int n = 0; n < 4; ++n) {
-                        float x[4] = {};
-                        uint32_t b[kK][2];
+                    for (int n = 0; n < 4; ++n)
 #pragma unroll
                         for (int i = 0; i < kK; ++i) {
-                            b[i][0] = take_piece<T>(v[0][n], v[1][n]);
-                            b[i][1] = take_piece<T>(v[2][n], v[3][n]);
+                            b[n][i][0] = take_piece<T>(v[0][n], v[1][n]);
+                            b[n][i][1] = take_piece<T>(v[2][n], v[3][n]);
                         }
-                        mma<T>(x, pp[2], b[0][0], b[0][1]);
-                        mma<T>(x, pp[0], b[2][0], b[2][1]);
-                        mma<T>(x, pp[1], b[1][0], b[1][1]);
-                        mma<T>(x, pp[1], b[0][0], b[0][1]);
-                        mma<T>(x, pp[0], b[1][0], b[1][1]);
-                        mma<T>(x, pp[0], b[0][0], b[0][1]);
-                        add(4 * j + n, x);
-                    }
+                    constexpr int kPa[6] = {2, 0, 1, 1, 0, 0}, kPb[6] = {0, 2, 1, 0, 1, 0};
+#pragma unroll
+                    for (int i = 0; i < 6; ++i)
+#pragma unroll
+                        for (int n = 0; n < 4; ++n)
+                            mma<T>(x[n], pp[kPa[i]], b[n][kPb[i]][0], b[n][kPb[i]][1]);
+#pragma unroll
+                    for (int n = 0; n < 4; ++n)
+                        add(4 * j + n, x[n]);
                 }
             } else {
 #pragma unroll
-                for (int n = 0; n < kTiles; n += 2) {
+                for (int n = 0; n < kTiles; n += 4) {
                     // keys 0-7 and 8-15, features 8n .. 8n + 7 and the next eight
-                    uint32_t b[4];
-                    ldmatrix_trans(b, vs + swizzled((lane & 7) + ((lane >> 3) & 1) * 8,
-                                                    n + (lane >> 4), true));
-                    float x[4] = {}, y[4] = {};
+                    uint32_t b[2][4];
 #pragma unroll
-                    for (int i = kQ - 1; i >= 0; --i) {
-                        mma<T>(x, pp[i], b[0], b[1]);
-                        mma<T>(y, pp[i], b[2], b[3]);
-                    }
-                    add(n, x);
-                    add(n + 1, y);
+                    for (int j = 0; j < 2; ++j)
+                        ldmatrix_trans(b[j], vs + swizzled((lane & 7) + ((lane >> 3) & 1) * 8,
+                                                           n + 2 * j + (lane >> 4), true));
+                    float x[4][4] = {};
+#pragma unroll
+                    for (int i = kQ - 1; i >= 0; --i)
+#pragma unroll
+                        for (int j = 0; j < 4; ++j)
+                            mma<T>(x[j], pp[i], b[j >> 1][(j & 1) * 2], b[j >> 1][(j & 1) * 2 + 1]);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+                        add(n + j, x[j]);
                 }
             }
         };
 
-        for (int b = b0; b < b1; b += R::kSlots) {
+        // One copy of the body: unrolled over the slots, its code came from beyond the
+        // instruction cache.
+        int slot = 0, into = R::kSlots - 1;
+#pragma unroll 1
+        for (int b = b0; b < b1; ++b) {
+            cp_wait<R::kSlots - 2>();
+            __syncwarp();
+            const unsigned keys = there[0];
 #pragma unroll
-            for (int u = 0; u < R::kSlots; ++u) {
-                if (b + u >= b1)
-                    break;
-                cp_wait<R::kSlots - 2>();
-                __syncwarp();
-                // the slot that the block before has left
-                constexpr int kLast = R::kSlots - 1;
-                const int into = (u + kLast) % R::kSlots;
-                there[into] = fetch(into, next_row);
-                next_row = row_of(b + u + R::kSlots);
-                block(u, there[u]);
-                __syncwarp();
-            }
+            for (int i = 0; i + 1 < R::kSlots - 1; ++i)
+                there[i] = there[i + 1];
+            there[R::kSlots - 2] = fetch(into, next_row);  // the slot that the block before left
+            next_row = row_of(b + R::kSlots);
+            block(slot, keys);
+            __syncwarp();
+            into = slot;
+            slot = slot + 1 == R::kSlots ? 0 : slot + 1;
         }
         cp_wait<0>();
         __syncwarp();
@@ -503,6 +542,12 @@ paged_split_kernel(const Args a, const Attend p, float* __restrict__ parts) {
         const bool whole = b0 == 0 && b1 == blocks;
         constexpr float kDown = std::is_same_v<T, __half> ? 1.f / kHalfScale : 1.f;
         float* part = parts + ((size_t)2 * me + (at != first)) * Part<DIM>::kFloats;
+        if (!whole && lane == 0) {
+            const int from = begin + tile * blocks, w0 = from / line.share;
+            owners[2 * me + (at != first)] = {seq, head0, heads, w0,
+                                              (from + blocks - 1) / line.share,
+                                              from != w0 * line.share, {}};
+        }
         bool odd = false;
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
@@ -556,90 +601,97 @@ paged_split_kernel(const Args a, const Attend p, float* __restrict__ parts) {
     }
 }
 
-// Joins what several warps' shares hold of a tile; rows without a key.  A block per sequence and
-// head: warps take the parts in turn, then the block joins the warps' sums.
+// Joins what several warps' shares hold of a tile.  Block w has the parts of warp w: with the
+// other blocks that have parts of the same tile it shares out the tile's heads, to warps where
+// there are few parts, else to blocks whose warps take the parts in turn.
 constexpr int kJoinWarps = 8;
 template <typename T, int DIM>
 __global__ void __launch_bounds__(kJoinWarps * 32)
-paged_join_kernel(const Args a, const Attend p, const float* __restrict__ parts, int warps) {
+paged_join_kernel(const Args a, const Attend p, const float* __restrict__ parts,
+                  const Owner* __restrict__ owners) {
     b2w4_pdl_chain_entry();
     constexpr int kOwn = DIM / 32;
     __shared__ float s_o[kJoinWarps][DIM];
     __shared__ float s_m[kJoinWarps], s_l[kJoinWarps];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int seq = blockIdx.x / p.heads, head = blockIdx.x - seq * p.heads;
-    const int group = p.heads / a.kv_heads, sets = (group + kSet - 1) / kSet;
-    const int tiles = a.kv_heads * sets;
-    bool bad = false;
-    const Sequence s = paged::sequence(a, seq, &bad);
-    if (s.count != 1)
-        return;
-    const Seen seen = seen_by(s, p.window);
-    float* out = p.out + (size_t)s.first * p.ldo + (size_t)head * DIM;
-    if (seen.count == 0) {
-        if (threadIdx.x < DIM)
-            out[threadIdx.x] = 0.f;
-        return;
+#pragma unroll 1
+    for (int side = 0; side < 2; ++side) {
+        const Owner t = owners[2 * blockIdx.x + side];
+        if (t.count == 0)
+            continue;
+        const int n = t.w1 - t.w0 + 1, mine = blockIdx.x - t.w0;
+        const bool few = n <= kJoinWarps;
+        const int step = few ? kJoinWarps * n : n;
+        for (int row = few ? mine * kJoinWarps + warp : mine; row < t.count; row += step) {
+            float m = -INFINITY, l = 0.f, o[kOwn];
+#pragma unroll
+            for (int i = 0; i < kOwn; ++i)
+                o[i] = 0.f;
+#pragma unroll 4
+            for (int w = t.w0 + (few ? 0 : warp); w <= t.w1; w += few ? 1 : kJoinWarps) {
+                const float* part =
+                    parts + ((size_t)2 * w + (w == t.w0 && t.second)) * Part<DIM>::kFloats;
+                const float pm = part[row], pl = part[kSet + row];
+                float x[kOwn];
+#pragma unroll
+                for (int i = 0; i < kOwn; ++i)
+                    x[i] = part[2 * kSet + row * DIM + lane + 32 * i];
+                const float top = fmaxf(m, pm), base = top == -INFINITY ? 0.f : top;
+                const float ea = exp2_neg(__fsub_rn(m, base)), eb = exp2_neg(__fsub_rn(pm, base));
+                m = top;
+                l = __fmaf_rn(l, ea, __fmul_rn(pl, eb));
+#pragma unroll
+                for (int i = 0; i < kOwn; ++i)
+                    o[i] = __fmaf_rn(o[i], ea, __fmul_rn(x[i], eb));
+            }
+            if (!few) {
+                __syncthreads();  // of the row before
+                if (lane == 0) {
+                    s_m[warp] = m;
+                    s_l[warp] = l;
+                }
+#pragma unroll
+                for (int i = 0; i < kOwn; ++i)
+                    s_o[warp][lane + 32 * i] = o[i];
+                __syncthreads();
+                if (warp != 0)
+                    continue;
+                m = -INFINITY;
+#pragma unroll
+                for (int w = 0; w < kJoinWarps; ++w)
+                    m = fmaxf(m, s_m[w]);
+                const float base = m == -INFINITY ? 0.f : m;
+                l = 0.f;
+#pragma unroll
+                for (int i = 0; i < kOwn; ++i)
+                    o[i] = 0.f;
+#pragma unroll
+                for (int w = 0; w < kJoinWarps; ++w) {
+                    const float e = exp2_neg(__fsub_rn(s_m[w], base));
+                    l = __fmaf_rn(s_l[w], e, l);
+#pragma unroll
+                    for (int i = 0; i < kOwn; ++i)
+                        o[i] = __fmaf_rn(s_o[w][lane + 32 * i], e, o[i]);
+                }
+            }
+            bool bad = false, odd = false;
+            const Sequence s = paged::sequence(a, t.seq, &bad);
+            const int head = t.head0 + row;
+            float* out = p.out + (size_t)s.first * p.ldo + (size_t)head * DIM;
+#pragma unroll
+            for (int i = 0; i < kOwn; ++i) {
+                const float x = __fdiv_rn(o[i], l);
+                odd |= paged::odd_result<T>(x);
+                out[lane + 32 * i] = x;
+            }
+            __syncwarp();
+            if (__any_sync(0xffffffffu, odd))
+                paged::attend_row<T, DIM>(a, s, p.q + (size_t)s.first * p.ldq + (size_t)head * DIM,
+                                          s.length - 1, head / (p.heads / a.kv_heads), p.scale,
+                                          p.window, out);
+        }
+        __syncthreads();
     }
-    const Line line = line_of(a, p.window, tiles, warps, false);
-    int before = 0;
-    for (int i = lane; i < seq; i += 32)
-        before += blocks_of(a, p.window, i, false);
-    before = __reduce_add_sync(0xffffffffu, before) * tiles;
-    const int blocks = (seen.count + kKeys - 1) / kKeys;
-    const int kvh = head / group, in = head - kvh * group, row = in % kSet;
-    const int begin = before + (kvh * sets + in / kSet) * blocks;
-    const int w0 = begin / line.share, w1 = (begin + blocks - 1) / line.share;
-    if (w0 == w1)
-        return;  // one warp had all of it
-    float m = -INFINITY, l = 0.f, o[kOwn];
-#pragma unroll
-    for (int i = 0; i < kOwn; ++i)
-        o[i] = 0.f;
-    for (int w = w0 + warp; w <= w1; w += kJoinWarps) {
-        const bool second = w == w0 && begin != w0 * line.share;
-        const float* part = parts + ((size_t)2 * w + second) * Part<DIM>::kFloats;
-        const float pm = part[row], pl = part[kSet + row];
-        float x[kOwn];
-#pragma unroll
-        for (int i = 0; i < kOwn; ++i)
-            x[i] = part[2 * kSet + row * DIM + lane + 32 * i];
-        const float top = fmaxf(m, pm), base = top == -INFINITY ? 0.f : top;
-        const float ea = exp2_neg(__fsub_rn(m, base)), eb = exp2_neg(__fsub_rn(pm, base));
-        m = top;
-        l = __fmaf_rn(l, ea, __fmul_rn(pl, eb));
-#pragma unroll
-        for (int i = 0; i < kOwn; ++i)
-            o[i] = __fmaf_rn(o[i], ea, __fmul_rn(x[i], eb));
-    }
-    if (lane == 0) {
-        s_m[warp] = m;
-        s_l[warp] = l;
-    }
-#pragma unroll
-    for (int i = 0; i < kOwn; ++i)
-        s_o[warp][lane + 32 * i] = o[i];
-    __syncthreads();
-    float top = -INFINITY;
-#pragma unroll
-    for (int w = 0; w < kJoinWarps; ++w)
-        top = fmaxf(top, s_m[w]);
-    const float base = top == -INFINITY ? 0.f : top;
-    float total = 0.f, x = 0.f;
-    const int d = threadIdx.x;
-#pragma unroll
-    for (int w = 0; w < kJoinWarps; ++w) {
-        const float e = exp2_neg(__fsub_rn(s_m[w], base));
-        total = __fmaf_rn(s_l[w], e, total);
-        if (d < DIM)
-            x = __fmaf_rn(s_o[w][d], e, x);
-    }
-    x = __fdiv_rn(x, total);
-    if (d < DIM)
-        out[d] = x;
-    if (__syncthreads_or(d < DIM && paged::odd_result<T>(x)) && warp == 0)
-        paged::attend_row<T, DIM>(a, s, p.q + (size_t)s.first * p.ldq + (size_t)head * DIM,
-                                  s.length - 1, kvh, p.scale, p.window, out);
 }
 
 template <typename T, int DIM>
@@ -650,22 +702,24 @@ int launch(b2w4_ctx* ctx, const Args& a, const Attend& p, void* work) {
     B2W4_CUDA(ctx, b2w4_opt_in_smem(ctx, kern, R::kBytes, cfg));
     const int blocks = ctx->sm_count;
     float* parts = static_cast<float*>(work);
+    Owner* owners = reinterpret_cast<Owner*>(static_cast<uint8_t*>(work) +
+                                             owners_at<DIM>(blocks * R::kWarps));
     B2W4_CUDA(ctx, b2w4_launch_chained(ctx->pdl, kern, dim3(blocks), dim3(R::kWarps * 32),
-                                       R::kBytes, ctx->stream, a, p, parts));
+                                       R::kBytes, ctx->stream, a, p, parts, owners));
     ctx->launches++;
     B2W4_CUDA(ctx, b2w4_launch_chained(ctx->pdl, paged_join_kernel<T, DIM>,
-                                       dim3((unsigned)a.sequences * p.heads),
-                                       dim3(kJoinWarps * 32), 0, ctx->stream, a, p,
-                                       static_cast<const float*>(parts), blocks * R::kWarps));
+                                       dim3(blocks * R::kWarps), dim3(kJoinWarps * 32), 0,
+                                       ctx->stream, a, p, static_cast<const float*>(parts),
+                                       static_cast<const Owner*>(owners)));
     ctx->launches++;
     return B2W4_OK;
 }
 
 }  // namespace
 
-// Two parts of every warp.
 size_t b2w4_paged_split_work(int sm_count, int dim) {
-    return sizeof(float) * 2 * (2 * kSet + kSet * (size_t)dim) * 8 * sm_count;
+    const size_t warps = (size_t)kMostWarps * sm_count;
+    return (dim <= 64 ? owners_at<64>(warps) : owners_at<128>(warps)) + 2 * warps * sizeof(Owner);
 }
 
 bool b2w4_paged_split_takes(int dim) { return dim <= 128; }
