@@ -300,6 +300,9 @@ int b2w4_paged_attention(b2w4_ctx* ctx, const b2w4_paged_cache* cache,
     const Attend p = {q_dev, out_dev, scale, {window, sinks}, ldq, ldo, heads};
     if (batch->max_new == 1 && b2w4_paged_split_takes(cache->dim))
         return b2w4_launch_paged_split(ctx, cache->type, cache->dim, a, p, work_dev);
+    if (batch->max_new > 1 &&
+        b2w4_paged_runs_takes(cache->dim, heads, cache->kv_heads, batch->rows, batch->sequences))
+        return b2w4_launch_paged_runs(ctx, cache->type, cache->dim, a, p);
     const unsigned blocks = ((unsigned)batch->rows * heads + kWarps - 1) / kWarps;
     return by_type(cache->type, cache->dim, [&](auto* t, auto dim) {
         using T = std::remove_pointer_t<decltype(t)>;

@@ -25,6 +25,11 @@ __device__ __forceinline__ bool odd_result(float x) {
 
 }  // namespace paged
 
+// Runs of rows (paged_runs.cu): heads of 64 or 128 numbers.
+bool b2w4_paged_runs_takes(int dim, int heads, int kv_heads, int rows, int sequences);
+int b2w4_launch_paged_runs(b2w4_ctx* ctx, int type, int dim, const paged::Args& a,
+                           const paged::Attend& p);
+
 // One row per sequence (paged_split.cu): heads of 64 or 128 numbers.
 bool b2w4_paged_split_takes(int dim);
 size_t b2w4_paged_split_work(int sm_count, int dim);

@@ -1,0 +1,767 @@
+// Attention of runs of new tokens (prompts, chunks of prompts, several sequences at once) over a
+// paged cache, on tcgen05.mma kind::f16.
+//
+// A block takes 128 rows -- the heads of one kv head for consecutive tokens of a sequence --
+// against blocks of kKeys keys with a running softmax in 32 bits (base 2): m the running maximum,
+// p = 2^(s - m), o = o 2^(m_old - m) + p V.  The keys that any of its rows sees, the first ones
+// that stay visible and those from the first row's window on, are taken as one list; what a row
+// does not see of them is masked.
+//
+// Operands of 32 bits are sums of pieces of the cache's 16-bit type, as in paged_split.cu: three
+// bf16 pieces of queries and probabilities beside a bf16 cache, two fp16 pieces of a row's queries
+// times a power of two beside an fp16 cache, three pieces of both sides, six products, beside an
+// fp32 cache; small products first.  Sums in tensor memory truncate, so those of an output are of
+// one block of keys, and the running output is in registers, one rounding per block.
+//
+// What bounds it: the MMAs, which the pieces multiply: 128 rows x 128 keys x 128 features in three
+// pieces are 48 MMAs of 66 cycles, about 3200 cycles; a softmax takes about 2000 beside them.
+//
+// Roles: eight warps of rows, two threads to a row; a warp that issues the scores' MMAs, a block
+// ahead, and one for P V; the rest bring keys and values.  Both lie in shared memory as they lie in
+// the cache, a key's features in 128-byte rows: the keys are the scores' B operand with features
+// running fastest, the values P V's with them running slowest, so neither is transposed.  Rows
+// come one by one with their pages' addresses, so a page may end anywhere.
+//
+// A row whose result is not finite is done again key by key (paged::attend_row): a key that it does
+// not see, or that has no probability, may hold anything.  Every wait is bounded.
+#include "paged_kernels.cuh"
+#include "tcgen05_ops.cuh"
+
+namespace {
+
+using paged::Args;
+using paged::Attend;
+using paged::Sequence;
+
+constexpr int kRows = 128;
+constexpr int kRowWarps = 8, kScoreWarp = 8, kOutWarp = 9, kLoadWarp0 = 10;
+
+template <typename T, int DIM>
+struct Cfg {
+    static constexpr bool kWide = sizeof(T) == 4;
+    static constexpr int kKeys = kWide ? 64 : 128;
+    static constexpr int kK = kWide ? 3 : 1;                             // pieces of a key
+    static constexpr int kQ = std::is_same_v<T, __half> ? 2 : 3;         // of a query
+    static constexpr int kQTmem = kWide ? 2 : 0;                         // in tensor memory
+    static constexpr int kLoadWarps = kWide ? 14 : 4;
+    static constexpr int kThreads = kWide ? 768 : 512;  // warpgroups
+    static_assert((kLoadWarp0 + kLoadWarps) * 32 <= kThreads);
+    static constexpr int kRegsStart = kWide ? 80 : 128;
+    static constexpr int kRegsRows = kWide ? 128 : 200, kRegsOther = 56;
+    static_assert(2 * kRegsRows + (kThreads / 128 - 2) * kRegsOther <= kThreads / 128 * kRegsStart,
+                  "registers of the block");
+    // A piece of a block of keys or values: 64 features' rows of 128 bytes, then the next 64's.
+    static constexpr int kPart = kKeys * 128, kPiece = kPart * (DIM / 64);
+    static constexpr int kBuf = kK * kPiece;
+    static constexpr int kQPart = kRows * 128, kQPiece = kQPart * (DIM / 64);
+    static constexpr int kKs = 0, kVs = 2 * kBuf, kQs = 4 * kBuf;
+    static constexpr int kMax = kQs + (kQ - kQTmem) * kQPiece;  // float [2 parities][2 halves][kRows]
+    static constexpr int kBar = kMax + 4 * kRows * 4;
+    static constexpr int kTotal = kBar + 512;
+    static_assert(kTotal <= 227 * 1024, "shared memory");
+    // tensor memory, columns
+    static constexpr int kTq = 0, kTs = kTq + kQTmem * DIM / 2, kTp = kTs + kKeys;
+    static constexpr int kTo = kTp + kQ * kKeys / 2;
+    static_assert(kTo + DIM <= 512, "tensor memory");
+};
+
+// fp32 accumulate, M = 128, N = n; type 0: fp16, 1: bf16; b_slow: B's columns run fastest
+__host__ __device__ constexpr uint32_t idesc(int type, int n, bool b_slow) {
+    return (1u << 4) | ((uint32_t)type << 7) | ((uint32_t)type << 10) | ((uint32_t)b_slow << 16) |
+           ((uint32_t)(n >> 3) << 17) | ((uint32_t)(kRows >> 4) << 24);
+}
+// B with its columns (features) fastest, 128-byte swizzle: 64 columns of eight k rows are an atom
+// of 1024 bytes; `next` bytes to the next 64 columns, 1024 to the next eight rows
+__device__ __forceinline__ uint64_t desc_slow(uint32_t at, uint32_t next) {
+    return (uint64_t)((at & 0x3FFFF) >> 4) | (uint64_t)(next >> 4) << 16 |
+           (uint64_t)(1024 >> 4) << 32 | (uint64_t)1 << 46 | (uint64_t)2 << 61;
+}
+__device__ __forceinline__ void umma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t id,
+                                        uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+        ::"r"(d), "r"(a), "l"(b), "r"(id), "r"(accumulate)
+        : "memory");
+}
+__device__ __forceinline__ void umma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t id,
+                                        uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+        ::"r"(d), "l"(a), "l"(b), "r"(id), "r"(accumulate)
+        : "memory");
+}
+#define B2W4_W8(r, o) "=r"(r[o]), "=r"(r[o + 1]), "=r"(r[o + 2]), "=r"(r[o + 3]),            \
+                      "=r"(r[o + 4]), "=r"(r[o + 5]), "=r"(r[o + 6]), "=r"(r[o + 7])
+#define B2W4_RW8(r, o) "+r"(r[o]), "+r"(r[o + 1]), "+r"(r[o + 2]), "+r"(r[o + 3]),           \
+                       "+r"(r[o + 4]), "+r"(r[o + 5]), "+r"(r[o + 6]), "+r"(r[o + 7])
+#define B2W4_R8(r, o) "r"(r[o]), "r"(r[o + 1]), "r"(r[o + 2]), "r"(r[o + 3]), "r"(r[o + 4]), \
+                      "r"(r[o + 5]), "r"(r[o + 6]), "r"(r[o + 7])
+__device__ __forceinline__ void tmem_ld16(uint32_t at, uint32_t (&r)[16]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, "
+        "%11, %12, %13, %14, %15}, [%16];"
+        : B2W4_W8(r, 0), B2W4_W8(r, 8)
+        : "r"(at)
+        : "memory");
+}
+__device__ __forceinline__ void tmem_ld_wait(uint32_t (&a)[16], uint32_t (&b)[16]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : B2W4_RW8(a, 0), B2W4_RW8(a, 8), B2W4_RW8(b, 0), B2W4_RW8(b, 8)
+                 :
+                 : "memory");
+}
+__device__ __forceinline__ void tmem_st16(uint32_t at, const uint32_t (&r)[16]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, "
+        "%10, %11, %12, %13, %14, %15};" ::B2W4_R8(r, 0),
+        B2W4_R8(r, 8), "r"(at)
+        : "memory");
+}
+__device__ __forceinline__ void tmem_st_wait() {
+    asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+    uint64_t d;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+// The next piece of two numbers, low half = lo; they keep what is left (exact).
+template <typename T>
+__device__ __forceinline__ uint32_t take_piece(uint64_t& v) {
+    float lo, hi;
+    b2w4_unpack2(v, lo, hi);
+    uint32_t p;
+    if constexpr (std::is_same_v<T, __half>) {
+        asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(p) : "f"(hi), "f"(lo));
+        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&p));
+        v = b2w4_sub2(v, b2w4_pack2(f.x, f.y));
+    } else {
+        asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(p) : "f"(hi), "f"(lo));
+        v = b2w4_sub2(v, b2w4_pack2(__uint_as_float(p << 16), __uint_as_float(p & 0xffff0000u)));
+    }
+    return p;
+}
+__device__ __forceinline__ float exp2_neg(float x) {
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+__device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool there) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src),
+                 "r"(there ? 16 : 0)
+                 : "memory");
+}
+// row, chunk of 16 bytes -> bytes in 128-byte rows: 8-row atoms, chunks swizzled with the row
+__device__ __forceinline__ uint32_t place(int row, int chunk) {
+    return (uint32_t)((row >> 3) * 1024 + (row & 7) * 128 + ((chunk ^ (row & 7)) << 4));
+}
+
+constexpr float kHalfScale = 1024.f;  // of probabilities beside an fp16 cache
+
+// Whole warp.  Tile `at` of the call's, counted from the last sequence's last tile; false: there is
+// none.  t0: its first token of the sequence's rows.
+__device__ bool find_tile(const Args& a, int tq, int at, int* seq, int* t0) {
+    const int lane = threadIdx.x & 31;
+    for (int base = a.sequences; base > 0; base -= 32) {
+        const int i = base - 1 - lane;
+        int n = 0;
+        if (i >= 0) {
+            bool bad = false;
+            n = (paged::sequence(a, i, &bad).count + tq - 1) / tq;
+            if (bad)
+                b2w4_report(a.status, B2W4_E_INVALID);
+        }
+        int x = n;
+#pragma unroll
+        for (int off = 1; off < 32; off <<= 1) {
+            const int y = __shfl_up_sync(0xffffffffu, x, off);
+            if (lane >= off)
+                x += y;
+        }
+        const unsigned past = __ballot_sync(0xffffffffu, x > at);
+        if (past) {
+            const int l = __ffs(past) - 1;
+            *seq = base - 1 - l;
+            *t0 = (__shfl_sync(0xffffffffu, x, l) - 1 - at) * tq;
+            return true;
+        }
+        at -= __shfl_sync(0xffffffffu, x, 31);
+    }
+    return false;
+}
+
+template <typename T, int DIM>
+__global__ void __launch_bounds__(Cfg<T, DIM>::kThreads, 1)
+paged_runs_kernel(const Args a, const Attend p, int tq) {
+    using C = Cfg<T, DIM>;
+    constexpr int kKeys = C::kKeys, kType = std::is_same_v<T, __half> ? 0 : 1;
+    extern __shared__ __align__(1024) uint8_t smem[];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::kBar);
+    uint64_t* q_full = bars;        // the queries' pieces
+    uint64_t* s_full = bars + 1;    // scores of a block complete
+    uint64_t* s_free = bars + 2;    // ... and in registers
+    uint64_t* p_full = bars + 3;    // probabilities' pieces in tensor memory
+    uint64_t* o_full = bars + 4;    // P V of a block complete (and P read)
+    uint64_t* o_free = bars + 5;    // ... and in registers
+    uint64_t* drained = bars + 6;   // [2] every MMA retired
+    uint64_t* k_full = bars + 8;    // [2]
+    uint64_t* k_free = bars + 10;   // [2]
+    uint64_t* v_full = bars + 12;   // [2]
+    uint64_t* v_free = bars + 14;   // [2]
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 16);
+    volatile int* s_abort = reinterpret_cast<volatile int*>(tmem_slot + 1);
+    volatile int* s_tile = reinterpret_cast<volatile int*>(tmem_slot + 2);  // sequence, token
+    uint32_t* s_odd = tmem_slot + 4;  // [4] rows to be done again
+    float* s_max = reinterpret_cast<float*>(smem + C::kMax);
+
+    b2w4_pdl_launch_dependents();
+    if (threadIdx.x == 0) {
+        mbar_init(q_full, kRowWarps);
+        mbar_init(s_full, 1);
+        mbar_init(s_free, kRowWarps);
+        mbar_init(p_full, kRowWarps);
+        mbar_init(o_full, 1);
+        mbar_init(o_free, kRowWarps);
+        for (int b = 0; b < 2; ++b) {
+            mbar_init(&drained[b], 1);
+            mbar_init(&k_full[b], C::kLoadWarps);
+            mbar_init(&k_free[b], 1);
+            mbar_init(&v_full[b], C::kLoadWarps);
+            mbar_init(&v_free[b], 1);
+        }
+        *s_abort = 0;
+        for (int i = 0; i < 4; ++i)
+            s_odd[i] = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    b2w4_pdl_wait();
+    if (warp == kOutWarp) {
+        int seq = -1, t0 = 0;
+        if (!find_tile(a, tq, blockIdx.y, &seq, &t0))
+            seq = -1;
+        if (lane == 0) {
+            s_tile[0] = seq;
+            s_tile[1] = t0;
+        }
+    }
+    __syncthreads();
+    const int seq = s_tile[0], t0 = s_tile[1];
+    if (seq < 0)
+        return;
+    if (warp == kScoreWarp) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;"
+                     ::"r"(smem_u32(tmem_slot)), "r"(512)
+                     : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    const uint32_t tmem = *tmem_slot;
+    auto fail = [&]() {
+        *s_abort = 1;
+        b2w4_report_timeout(a.status);
+    };
+    auto wait = [&](uint64_t* bar, uint32_t parity) {
+        return mbar_try_wait(bar, parity) || (!*s_abort && mbar_wait(bar, parity));
+    };
+    auto warp_wait = [&](uint64_t* bar, uint32_t parity) {
+        return __all_sync(0xffffffffu, wait(bar, parity)) != 0;
+    };
+    auto warp_arrive = [&](uint64_t* bar) {
+        __syncwarp();
+        if (lane == 0)
+            mbar_arrive(bar);
+    };
+
+    bool bad = false;
+    const Sequence s = paged::sequence(a, seq, &bad);
+    const int kvh = blockIdx.x, rep = p.heads / a.kv_heads;
+    const int p0 = s.length - s.count + t0;                 // position of the tile's first token
+    const int p1 = s.length - s.count + min(t0 + tq, s.count) - 1;  // and of its last
+    // the keys that the tile's rows see: [0, low) and [from, p1], as one list
+    const int from = p.window.from(max(p0, 0)), low = min(p.window.sinks, from);
+    const int count = p1 < 0 ? 0 : low + p1 + 1 - from;
+    const int steps = (count + kKeys - 1) / kKeys;
+    auto row_offset = [&](int r, int ld) {
+        return (size_t)(s.first + t0 + r / rep) * ld + (size_t)(kvh * rep + r % rep) * DIM;
+    };
+    auto row_exists = [&](int r) { return r < tq * rep && t0 + r / rep < s.count; };
+
+    if (warp < kRowWarps) {
+        // ================================== rows =====================================
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(C::kRegsRows));
+        const int quarter = warp & 3, half = warp >> 2;
+        const int row = quarter * 32 + lane;
+        const bool exists = row_exists(row);
+        const int pos = exists ? p0 + row / rep : -1;
+        const uint32_t lane_addr = tmem + ((uint32_t)(quarter * 32) << 16);
+        auto pair_sync = [&]() { asm volatile("bar.sync %0, 64;" ::"r"(3 + quarter) : "memory"); };
+        // both threads' larger value, through the words of a parity
+        auto pair_max = [&](float v, int parity) {
+            float* mx = s_max + parity * 2 * kRows;
+            mx[half * kRows + row] = v;
+            pair_sync();
+            return fmaxf(v, mx[(1 - half) * kRows + row]);
+        };
+        float factor = __fmul_rn(p.scale, 1.4426950408889634f);
+        if (steps > 0) {
+            const float4* src =
+                reinterpret_cast<const float4*>(p.q + (exists ? row_offset(row, p.ldq) : 0));
+            const float4 zero = make_float4(0.f, 0.f, 0.f, 0.f);
+            float up = 1.f;
+            if constexpr (std::is_same_v<T, __half>) {  // the row's largest to [2^10, 2^11)
+                float top = 0.f;
+                if (exists)
+                    for (int c = half * (DIM / 8); c < (half + 1) * (DIM / 8); ++c) {
+                        const float4 f = src[c];
+                        top = fmaxf(fmaxf(fmaxf(top, fabsf(f.x)), fmaxf(fabsf(f.y), fabsf(f.z))),
+                                    fabsf(f.w));
+                    }
+                top = pair_max(top, 1);
+                int e = (int)(__float_as_uint(top) >> 23) - 127;
+                e = top == 0.f ? 10 : min(max(e, -100), 120);
+                up = __uint_as_float((unsigned)(127 + 10 - e) << 23);
+                factor = __fmul_rn(factor, __uint_as_float((unsigned)(127 - 10 + e) << 23));
+            }
+#pragma unroll 1
+            for (int c = half * (DIM / 2); c < (half + 1) * (DIM / 2); c += 32) {
+                uint64_t v[16];
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    float4 f = exists ? src[c / 4 + i] : zero;
+                    if constexpr (std::is_same_v<T, __half>)
+                        f = make_float4(__fmul_rn(f.x, up), __fmul_rn(f.y, up), __fmul_rn(f.z, up),
+                                        __fmul_rn(f.w, up));
+                    v[2 * i] = b2w4_pack2(f.x, f.y);
+                    v[2 * i + 1] = b2w4_pack2(f.z, f.w);
+                }
+#pragma unroll
+                for (int i = 0; i < C::kQ; ++i) {
+                    uint32_t r[16];
+#pragma unroll
+                    for (int e = 0; e < 16; ++e)
+                        r[e] = take_piece<T>(v[e]);
+                    if (i < C::kQTmem) {
+                        tmem_st16(lane_addr + C::kTq + i * (DIM / 2) + c / 2, r);
+                    } else {
+                        uint8_t* to = smem + C::kQs + (i - C::kQTmem) * C::kQPiece +
+                                      c / 64 * C::kQPart;
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            *reinterpret_cast<uint4*>(to + place(row, c % 64 / 8 + e)) =
+                                make_uint4(r[4 * e], r[4 * e + 1], r[4 * e + 2], r[4 * e + 3]);
+                    }
+                }
+            }
+            tmem_st_wait();
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+            warp_arrive(q_full);
+        }
+        float m = -INFINITY, l = 0.f, alpha = 1.f;
+        constexpr int kOwn = DIM / 2, kMine = kKeys / 2;  // the thread's features and keys
+        uint64_t acc[kOwn / 2];
+#pragma unroll
+        for (int i = 0; i < kOwn / 2; ++i)
+            acc[i] = 0ull;
+        bool live = true;  // no way out of the loop: the two threads of a row meet once a step
+        auto await = [&](uint64_t* bar, uint32_t parity) {
+            if (live && !warp_wait(bar, parity)) {
+                live = false;
+                fail();
+            }
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        };
+        auto take_output = [&]() {
+            const uint64_t al = b2w4_pack2(alpha, alpha);
+#pragma unroll
+            for (int c = 0; c < kOwn; c += 32) {
+                uint32_t r0[16], r1[16];
+                tmem_ld16(lane_addr + C::kTo + half * kOwn + c, r0);
+                tmem_ld16(lane_addr + C::kTo + half * kOwn + c + 16, r1);
+                tmem_ld_wait(r0, r1);
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    const uint32_t* r = i < 8 ? r0 : r1;
+                    acc[c / 2 + i] = b2w4_fma2(acc[c / 2 + i], al,
+                                               b2w4_pack2(__uint_as_float(r[2 * (i & 7)]),
+                                                          __uint_as_float(r[2 * (i & 7) + 1])));
+                }
+            }
+            asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+            warp_arrive(o_free);
+        };
+        // of the list, the row sees [0, sinks) and [lo, hi)
+        const int hi = pos < 0 ? 0 : pos - from + low + 1;
+        const int lo = p.window.from(max(pos, 0)) - from + low;
+        for (int j = 0; j < steps; ++j) {
+            await(s_full, j & 1);
+            uint64_t sc[kMine / 2];
+#pragma unroll
+            for (int h = 0; h < kMine; h += 32) {
+                uint32_t r0[16], r1[16];
+                tmem_ld16(lane_addr + C::kTs + half * kMine + h, r0);
+                tmem_ld16(lane_addr + C::kTs + half * kMine + h + 16, r1);
+                tmem_ld_wait(r0, r1);
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    const uint32_t* r = i < 8 ? r0 : r1;
+                    sc[h / 2 + i] =
+                        b2w4_mul2(b2w4_pack2(__uint_as_float(r[2 * (i & 7)]),
+                                             __uint_as_float(r[2 * (i & 7) + 1])),
+                                  b2w4_pack2(factor, factor));
+                }
+            }
+            asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+            warp_arrive(s_free);
+            const int first = j * kKeys + half * kMine;  // the thread's first key of the list
+            if (first + kMine > hi || (first < lo && first + kMine > p.window.sinks)) {
+#pragma unroll
+                for (int i = 0; i < kMine / 2; ++i) {
+                    float x, y;
+                    b2w4_unpack2(sc[i], x, y);
+                    auto sees = [&](int k) { return k < hi && (k >= lo || k < p.window.sinks); };
+                    sc[i] = b2w4_pack2(sees(first + 2 * i) ? x : -INFINITY,
+                                       sees(first + 2 * i + 1) ? y : -INFINITY);
+                }
+            }
+            float top = m;
+#pragma unroll
+            for (int i = 0; i < kMine / 2; ++i) {
+                float x, y;
+                b2w4_unpack2(sc[i], x, y);
+                top = fmaxf(fmaxf(top, x), y);
+            }
+            top = pair_max(top, j & 1);
+            const float base = top == -INFINITY ? 0.f : top;
+#pragma unroll
+            for (int i = 0; i < kMine / 2; ++i) {
+                float x, y;
+                b2w4_unpack2(sc[i], x, y);
+                sc[i] = b2w4_pack2(exp2_neg(__fsub_rn(x, base)), exp2_neg(__fsub_rn(y, base)));
+            }
+            uint64_t sum[4] = {sc[0], sc[1], sc[2], sc[3]};
+#pragma unroll
+            for (int i = 4; i < kMine / 2; ++i)
+                sum[i & 3] = add2(sum[i & 3], sc[i]);
+            sum[0] = add2(add2(sum[0], sum[1]), add2(sum[2], sum[3]));
+            float sum0, sum1;
+            b2w4_unpack2(sum[0], sum0, sum1);
+            const float next_alpha = exp2_neg(__fsub_rn(m, base));
+            m = top;
+            l = __fmaf_rn(l, next_alpha, __fadd_rn(sum0, sum1));
+            if constexpr (std::is_same_v<T, __half>) {
+#pragma unroll
+                for (int i = 0; i < kMine / 2; ++i)
+                    sc[i] = b2w4_mul2(sc[i], b2w4_pack2(kHalfScale, kHalfScale));
+            }
+            // the product before has read the probabilities
+            if (j) {
+                await(o_full, (j - 1) & 1);
+                take_output();
+            }
+            alpha = next_alpha;
+#pragma unroll
+            for (int i = 0; i < C::kQ; ++i)
+#pragma unroll
+                for (int h = 0; h < kMine / 2; h += 16) {
+                    uint32_t r[16];
+#pragma unroll
+                    for (int e = 0; e < 16; ++e)
+                        r[e] = take_piece<T>(sc[h + e]);
+                    tmem_st16(lane_addr + C::kTp + i * (kKeys / 2) + half * (kMine / 2) + h, r);
+                }
+            tmem_st_wait();
+            asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+            warp_arrive(p_full);
+        }
+        if (steps > 0) {
+            await(o_full, (steps - 1) & 1);
+            take_output();
+        }
+        // the other thread's part of the sum (the other parity's words: they may still be read)
+        float* mx = s_max + (steps & 1) * 2 * kRows;
+        mx[half * kRows + row] = l;
+        pair_sync();
+        const float total = __fadd_rn(mx[row], mx[kRows + row]);
+        const float down = std::is_same_v<T, __half> ? 1.f / kHalfScale : 1.f;
+        bool odd = false;
+#pragma unroll
+        for (int i = 0; i < kOwn / 2; ++i) {
+            float x, y;
+            b2w4_unpack2(acc[i], x, y);
+            x = pos < 0 ? 0.f : __fdiv_rn(__fmul_rn(x, down), total);
+            y = pos < 0 ? 0.f : __fdiv_rn(__fmul_rn(y, down), total);
+            odd |= paged::odd_result<T>(x) || paged::odd_result<T>(y);
+            acc[i] = b2w4_pack2(x, y);
+        }
+        if (exists && !*s_abort) {
+            ulonglong2* dst =
+                reinterpret_cast<ulonglong2*>(p.out + row_offset(row, p.ldo) + half * kOwn);
+#pragma unroll
+            for (int i = 0; i < kOwn / 4; ++i)
+                dst[i] = make_ulonglong2(acc[2 * i], acc[2 * i + 1]);
+        }
+        const unsigned again = __ballot_sync(0xffffffffu, exists && odd);
+        if (lane == 0 && again)
+            atomicOr(&s_odd[quarter], again);
+    } else {
+      asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::kRegsOther));
+      if (warp == kScoreWarp) {
+        // ============================ MMA issue: scores ==============================
+        if (lane == 0) {
+            const uint64_t k_desc0 = umma_desc_k_sw128(smem_u32(smem + C::kKs));
+            const uint64_t q_desc = umma_desc_k_sw128(smem_u32(smem + C::kQs));
+            constexpr uint32_t id = idesc(kType, kKeys, false);
+            bool ok = steps == 0 || wait(q_full, 0);
+            for (int j = 0; j < steps && ok; ++j) {
+                ok = wait(&k_full[j & 1], (j >> 1) & 1) && (j == 0 || wait(s_free, (j - 1) & 1));
+                if (!ok)
+                    break;
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                const uint64_t d = k_desc0 + (uint64_t)((j & 1) * (C::kBuf >> 4));
+                bool more = false;
+                // sizes of products, the smallest first: pieces i of Q and size - i of K
+#pragma unroll
+                for (int size = C::kQ - 1; size >= 0; --size)
+#pragma unroll
+                    for (int i = size; i >= 0; --i) {
+                        if (size - i >= C::kK)
+                            continue;
+#pragma unroll
+                        for (int k = 0; k < DIM / 16; ++k) {
+                            const uint64_t kd =
+                                d + (uint64_t)(((size - i) * C::kPiece + k / 4 * C::kPart +
+                                                k % 4 * 32) >> 4);
+                            if (i < C::kQTmem)
+                                umma_ts(tmem + C::kTs, tmem + C::kTq + i * (DIM / 2) + k * 8, kd,
+                                        id, more);
+                            else
+                                umma_ss(tmem + C::kTs,
+                                        q_desc + (uint64_t)(((i - C::kQTmem) * C::kQPiece +
+                                                             k / 4 * C::kQPart + k % 4 * 32) >> 4),
+                                        kd, id, more);
+                            more = true;
+                        }
+                    }
+                umma_commit(s_full);
+                umma_commit(&k_free[j & 1]);
+            }
+            if (!ok)
+                fail();
+            umma_commit(&drained[0]);
+            if (!mbar_wait(&drained[0], 0))
+                fail();
+        }
+      } else if (warp == kOutWarp) {
+        // ============================== MMA issue: P V ===============================
+        if (lane == 0) {
+            const uint64_t v_desc0 = desc_slow(smem_u32(smem + C::kVs), C::kPart);
+            constexpr uint32_t id = idesc(kType, DIM, true);
+            bool ok = true;
+            for (int j = 0; j < steps; ++j) {
+                ok = wait(&v_full[j & 1], (j >> 1) & 1) &&
+                     (j == 0 || wait(o_free, (j - 1) & 1)) && wait(p_full, j & 1);
+                if (!ok)
+                    break;
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                const uint64_t d = v_desc0 + (uint64_t)((j & 1) * (C::kBuf >> 4));
+                bool more = false;
+#pragma unroll
+                for (int size = C::kQ - 1; size >= 0; --size)
+#pragma unroll
+                    for (int i = size; i >= 0; --i) {
+                        if (size - i >= C::kK)
+                            continue;
+#pragma unroll
+                        for (int k = 0; k < kKeys / 16; ++k) {
+                            umma_ts(tmem + C::kTo, tmem + C::kTp + i * (kKeys / 2) + k * 8,
+                                    d + (uint64_t)(((size - i) * C::kPiece + k * 2048) >> 4), id,
+                                    more);
+                            more = true;
+                        }
+                    }
+                umma_commit(o_full);
+                umma_commit(&v_free[j & 1]);
+            }
+            if (!ok)
+                fail();
+            umma_commit(&drained[1]);
+            if (!mbar_wait(&drained[1], 0))
+                fail();
+        }
+      } else {
+        // ============================== keys and values ==============================
+        // Where key i of the list lies; -1: it does not exist.  One whose page is not the pool's
+        // is left out, which a masked row cannot be: the tile's rows are done again.
+        auto row_of = [&](int i) {
+            if (i >= count)
+                return -1;
+            const int row = paged::cache_row(a, s.table, i < low ? i : i - low + from, kvh);
+            if (row < 0) {
+                b2w4_report(a.status, B2W4_E_INVALID);
+                for (int q = 0; q < 4; ++q)
+                    atomicOr(&s_odd[q], 0xffffffffu);
+            }
+            return row;
+        };
+        auto full = [&](uint64_t* bar) {  // make it visible to the tensor core
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            warp_arrive(bar);
+        };
+        const int w0 = warp - kLoadWarp0;
+        constexpr int kChunks = DIM / 8, kPer = 32 / kChunks;  // of eight features; rows at a time
+        const int c = lane % kChunks, sub = lane / kChunks;
+        bool ok = true;
+        auto free = [&](uint64_t* bars2, int j) {
+            if (j >= 2 && !warp_wait(&bars2[j & 1], ((j >> 1) - 1) & 1)) {
+                ok = false;
+                fail();
+            }
+            return ok;
+        };
+        if constexpr (C::kWide) {
+            // a warp has every kLoadWarps-th set of kPer rows of a block
+            constexpr int kSets = kKeys / kPer, kMine = (kSets + C::kLoadWarps - 1) / C::kLoadWarps;
+            int rows[kMine];
+            auto look = [&](int j) {
+#pragma unroll
+                for (int u = 0; u < kMine; ++u) {
+                    const int set = w0 + u * C::kLoadWarps;
+                    rows[u] = set < kSets ? row_of(j * kKeys + set * kPer + sub) : -1;
+                }
+            };
+            auto bring = [&](const float* pool, uint8_t* to) {
+                ulonglong2 f[kMine][2];
+#pragma unroll
+                for (int u = 0; u < kMine; ++u)
+#pragma unroll
+                    for (int h = 0; h < 2; ++h)
+                        f[u][h] = rows[u] >= 0 ? reinterpret_cast<const ulonglong2*>(
+                                                     pool + (size_t)rows[u] * DIM + c * 8)[h]
+                                               : make_ulonglong2(0ull, 0ull);
+#pragma unroll
+                for (int u = 0; u < kMine; ++u) {
+                    const int set = w0 + u * C::kLoadWarps;
+                    if (set >= kSets)
+                        break;
+                    uint64_t x[4] = {f[u][0].x, f[u][0].y, f[u][1].x, f[u][1].y};
+                    uint8_t* dst = to + (c >> 3) * C::kPart + place(set * kPer + sub, c & 7);
+#pragma unroll
+                    for (int i = 0; i < C::kK; ++i) {
+                        uint4 o;
+                        o.x = take_piece<T>(x[0]);
+                        o.y = take_piece<T>(x[1]);
+                        o.z = take_piece<T>(x[2]);
+                        o.w = take_piece<T>(x[3]);
+                        *reinterpret_cast<uint4*>(dst + i * C::kPiece) = o;
+                    }
+                }
+            };
+            look(0);
+            for (int j = 0; j < steps && free(k_free, j); ++j) {
+                bring(static_cast<const float*>(a.k), smem + C::kKs + (j & 1) * C::kBuf);
+                full(&k_full[j & 1]);
+                if (!free(v_free, j))
+                    break;
+                bring(static_cast<const float*>(a.v), smem + C::kVs + (j & 1) * C::kBuf);
+                look(j + 1);
+                full(&v_full[j & 1]);
+            }
+        } else if (w0 < C::kLoadWarps) {
+            // a warp has 32 keys of a block, a lane knows where one of them lies
+            static_assert(C::kWide || C::kLoadWarps * 32 == kKeys);
+            auto bring = [&](const void* pool, uint8_t* to, int row) {
+#pragma unroll
+                for (int i = 0; i < 32 / kPer; ++i) {
+                    const int in = i * kPer + sub;
+                    const int r = __shfl_sync(0xffffffffu, row, in);
+                    cp16(smem_u32(to + (c >> 3) * C::kPart + place(w0 * 32 + in, c & 7)),
+                         static_cast<const T*>(pool) + (size_t)max(r, 0) * DIM + c * 8, r >= 0);
+                }
+                asm volatile("cp.async.commit_group;" ::: "memory");
+            };
+            int row = row_of(w0 * 32 + lane), done = 0;
+            for (int j = 0; j < steps; ++j) {
+                // the block before is handed on as it arrives, ahead of a wait for a free place
+                if (j) {
+                    asm volatile("cp.async.wait_group 1;" ::: "memory");
+                    full(&k_full[(j - 1) & 1]);
+                }
+                if (!free(k_free, j))
+                    break;
+                bring(a.k, smem + C::kKs + (j & 1) * C::kBuf, row);
+                if (j) {
+                    asm volatile("cp.async.wait_group 1;" ::: "memory");
+                    full(&v_full[(j - 1) & 1]);
+                }
+                if (!free(v_free, j))
+                    break;
+                const int now = row;
+                row = row_of((j + 1) * kKeys + w0 * 32 + lane);
+                bring(a.v, smem + C::kVs + (j & 1) * C::kBuf, now);
+                done = j + 1;
+            }
+            if (ok && done) {
+                asm volatile("cp.async.wait_group 1;" ::: "memory");
+                full(&k_full[(done - 1) & 1]);
+                asm volatile("cp.async.wait_group 0;" ::: "memory");
+                full(&v_full[(done - 1) & 1]);
+            }
+            asm volatile("cp.async.wait_group 0;" ::: "memory");
+        }
+      }
+    }
+
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    if (warp == kScoreWarp) {
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;"
+                     ::"r"(tmem), "r"(512)
+                     : "memory");
+    }
+    if (warp < kRowWarps && !*s_abort)
+        for (int r = warp; r < kRows; r += kRowWarps)
+            if ((s_odd[r >> 5] >> (r & 31) & 1) && row_exists(r))
+                paged::attend_row<T, DIM>(a, s, p.q + row_offset(r, p.ldq), p0 + r / rep, kvh,
+                                          p.scale, p.window, p.out + row_offset(r, p.ldo));
+}
+
+template <typename T, int DIM>
+int launch(b2w4_ctx* ctx, const Args& a, const Attend& p) {
+    using C = Cfg<T, DIM>;
+    static b2w4_smem_optin cfg;
+    auto kern = paged_runs_kernel<T, DIM>;
+    const int tq = kRows / (p.heads / a.kv_heads);
+    // a sequence's last tile may be short: one more for each
+    const unsigned tiles = (unsigned)(a.rows / tq + a.sequences);
+    B2W4_CUDA(ctx, b2w4_opt_in_smem(ctx, kern, C::kTotal, cfg));
+    B2W4_CUDA(ctx, b2w4_launch_chained(ctx->pdl, kern, dim3(a.kv_heads, tiles), dim3(C::kThreads),
+                                       C::kTotal, ctx->stream, a, p, tq));
+    ctx->launches++;
+    return B2W4_OK;
+}
+
+}  // namespace
+
+bool b2w4_paged_runs_takes(int dim, int heads, int kv_heads, int rows, int sequences) {
+    const int rep = heads / kv_heads;
+    return dim <= 128 && rep <= kRows && rows / (kRows / rep) + sequences <= 65535;
+}
+
+int b2w4_launch_paged_runs(b2w4_ctx* ctx, int type, int dim, const Args& a, const Attend& p) {
+    if (dim == 64)
+        return type == B2W4_F16    ? launch<__half, 64>(ctx, a, p)
+               : type == B2W4_BF16 ? launch<__nv_bfloat16, 64>(ctx, a, p)
+                                   : launch<float, 64>(ctx, a, p);
+    return type == B2W4_F16    ? launch<__half, 128>(ctx, a, p)
+           : type == B2W4_BF16 ? launch<__nv_bfloat16, 128>(ctx, a, p)
+                               : launch<float, 128>(ctx, a, p);
+}
