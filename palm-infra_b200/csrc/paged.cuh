@@ -18,7 +18,25 @@ struct Args {
     int pages, kv_heads, page_size;
     int slots, table_len, sequences, rows, max_length;
     int* status;
+    // x / page_size for 0 <= x < 2^31 (Granlund and Montgomery, Division by invariant integers
+    // using multiplication, 1994): t = x multiplier >> 32, (t + (x - t >> shift1)) >> shift2
+    uint32_t multiplier;
+    int shift1, shift2;
 };
+inline void set_division(Args& a) {
+    int l = 0;
+    while (l < 31 && (1u << l) < (uint32_t)a.page_size)
+        ++l;
+    a.multiplier = (uint32_t)((((uint64_t)1 << 32) * (((uint64_t)1 << l) - a.page_size)) /
+                                  a.page_size +
+                              1);
+    a.shift1 = l < 1 ? l : 1;
+    a.shift2 = l < 1 ? 0 : l - 1;
+}
+inline __host__ __device__ int page_of(const Args& a, int x) {
+    const uint32_t t = (uint32_t)(((uint64_t)a.multiplier * (uint32_t)x) >> 32);
+    return (int)((t + (((uint32_t)x - t) >> a.shift1)) >> a.shift2);
+}
 
 // A sequence of the batch: its table, its tokens, its first row of the call and how many.
 struct Sequence {
@@ -62,7 +80,7 @@ inline __host__ __device__ Sequence sequence(const Args& a, int i, bool* bad) {
 // Row of the pools (of dim numbers) where token j of a sequence lies, kv head h; -1: its page is
 // not one of the pool's.  A device holds fewer than 2^31 rows of 64 numbers or more.
 inline __host__ __device__ int cache_row(const Args& a, const int32_t* table, int j, int h) {
-    const int n = j / a.page_size;
+    const int n = page_of(a, j);
     const int page = table[n];
     if ((unsigned)page >= (unsigned)a.pages)
         return -1;

@@ -180,9 +180,12 @@ int by_type(int type, int dim, F f) {
 }
 
 Args args_of(b2w4_ctx* ctx, const b2w4_paged_cache& c, const b2w4_paged_batch& b) {
-    return {c.k_dev,   c.v_dev,  b.tables_dev, b.lengths_dev, b.slots_dev,
-            b.starts_dev, c.pages, c.kv_heads,   c.page_size,   b.slots,
-            b.table_len, b.sequences, b.rows,    b.max_length,  ctx->status_dev};
+    Args a = {c.k_dev,   c.v_dev,  b.tables_dev, b.lengths_dev, b.slots_dev,
+              b.starts_dev, c.pages, c.kv_heads,   c.page_size,   b.slots,
+              b.table_len, b.sequences, b.rows,    b.max_length,
+              ctx ? ctx->status_dev : nullptr, 0,  0, 0};
+    paged::set_division(a);
+    return a;
 }
 
 }  // namespace
@@ -222,9 +225,7 @@ extern "C" const char* b2w4_paged_refusal(const b2w4_paged_cache* c, const b2w4_
 // and count as the kernels bound them.
 extern "C" int b2w4_paged_row(const b2w4_paged_cache* c, const b2w4_paged_batch* b, int i, int j,
                               int h, int* length, int* first, int* count) {
-    const Args a = {c->k_dev,   c->v_dev,  b->tables_dev, b->lengths_dev, b->slots_dev,
-                    b->starts_dev, c->pages, c->kv_heads,   c->page_size,   b->slots,
-                    b->table_len, b->sequences, b->rows,    b->max_length,  nullptr};
+    const Args a = args_of(nullptr, *c, *b);
     bool bad = false;
     const Sequence s = paged::sequence(a, i, &bad);
     *length = s.length;

@@ -16,7 +16,7 @@
 // What bounds it: the MMAs, which the pieces multiply: 128 rows x 128 keys x 128 features in three
 // pieces are 48 MMAs of 66 cycles, about 3200 cycles; a softmax takes about 2000 beside them.
 //
-// Roles: eight warps of rows, two threads to a row; a warp that issues the scores' MMAs, a block
+// Roles: warps of rows, four threads to a row (two beside an fp32 cache); a warp that issues the scores' MMAs, a block
 // ahead, and one for P V; the rest bring keys and values.  Both lie in shared memory as they lie in
 // the cache, a key's features in 128-byte rows: the keys are the scores' B operand with features
 // running fastest, the values P V's with them running slowest, so neither is transposed.  Rows
@@ -34,7 +34,6 @@ using paged::Attend;
 using paged::Sequence;
 
 constexpr int kRows = 128;
-constexpr int kRowWarps = 8, kScoreWarp = 8, kOutWarp = 9, kLoadWarp0 = 10;
 
 template <typename T, int DIM>
 struct Cfg {
@@ -42,21 +41,27 @@ struct Cfg {
     static constexpr int kKeys = kWide ? 64 : 128;
     static constexpr int kK = kWide ? 3 : 1;                             // pieces of a key
     static constexpr int kQ = std::is_same_v<T, __half> ? 2 : 3;         // of a query
-    static constexpr int kQTmem = kWide ? 2 : 0;                         // in tensor memory
-    static constexpr int kLoadWarps = kWide ? 14 : 4;
-    static constexpr int kThreads = kWide ? 768 : 512;  // warpgroups
-    static_assert((kLoadWarp0 + kLoadWarps) * 32 <= kThreads);
-    static constexpr int kRegsStart = kWide ? 80 : 128;
-    static constexpr int kRegsRows = kWide ? 128 : 200, kRegsOther = 56;
-    static_assert(2 * kRegsRows + (kThreads / 128 - 2) * kRegsOther <= kThreads / 128 * kRegsStart,
+    // of them in tensor memory: an MMA whose operands both come from shared memory takes twice as
+    // long (its A is 128 bytes a cycle's worth of the port)
+    static constexpr int kQTmem = kWide ? 2 : kQ == 3 && DIM > 64 ? 1 : kQ;
+    static constexpr int kParts = kWide ? 2 : 4;  // threads to a row
+    static constexpr int kRowWarps = 4 * kParts, kMmaWarp = kRowWarps;
+    // for the keys, and as many for the values
+    static constexpr int kLoadWarp0 = kRowWarps + 1, kLoadWarps = kWide ? 7 : 1;
+    static constexpr int kThreads = (kLoadWarp0 + 2 * kLoadWarps + 1) * 32;  // one is idle
+    static_assert(kThreads % 128 == 0, "warpgroups");
+    static constexpr int kRegsStart = kWide ? 80 : 96;
+    static constexpr int kRegsRows = kWide ? 128 : 104, kRegsOther = kWide ? 56 : 64;
+    static_assert(kParts * kRegsRows + (kThreads / 128 - kParts) * kRegsOther <=
+                      kThreads / 128 * kRegsStart,
                   "registers of the block");
     // A piece of a block of keys or values: 64 features' rows of 128 bytes, then the next 64's.
     static constexpr int kPart = kKeys * 128, kPiece = kPart * (DIM / 64);
     static constexpr int kBuf = kK * kPiece;
     static constexpr int kQPart = kRows * 128, kQPiece = kQPart * (DIM / 64);
     static constexpr int kKs = 0, kVs = 2 * kBuf, kQs = 4 * kBuf;
-    static constexpr int kMax = kQs + (kQ - kQTmem) * kQPiece;  // float [2 parities][2 halves][kRows]
-    static constexpr int kBar = kMax + 4 * kRows * 4;
+    static constexpr int kMax = kQs + (kQ - kQTmem) * kQPiece;  // float [2 parities][kParts][kRows]
+    static constexpr int kBar = kMax + 2 * kParts * kRows * 4;
     static constexpr int kTotal = kBar + 512;
     static_assert(kTotal <= 227 * 1024, "shared memory");
     // tensor memory, columns
@@ -108,17 +113,15 @@ __device__ __forceinline__ void tmem_ld16(uint32_t at, uint32_t (&r)[16]) {
         : "r"(at)
         : "memory");
 }
-__device__ __forceinline__ void tmem_ld_wait(uint32_t (&a)[16], uint32_t (&b)[16]) {
-    asm volatile("tcgen05.wait::ld.sync.aligned;"
-                 : B2W4_RW8(a, 0), B2W4_RW8(a, 8), B2W4_RW8(b, 0), B2W4_RW8(b, 8)
-                 :
-                 : "memory");
+// the wait that makes columns readable, and waits for none that is used later
+__device__ __forceinline__ void tmem_ld_wait(uint32_t (&a)[16]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;" : B2W4_RW8(a, 0), B2W4_RW8(a, 8) : : "memory");
 }
-__device__ __forceinline__ void tmem_st16(uint32_t at, const uint32_t (&r)[16]) {
+__device__ __forceinline__ void tmem_st8(uint32_t at, const uint32_t (&r)[8]) {
     asm volatile(
-        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, "
-        "%10, %11, %12, %13, %14, %15};" ::B2W4_R8(r, 0),
-        B2W4_R8(r, 8), "r"(at)
+        "tcgen05.st.sync.aligned.32x32b.x8.b32 [%8], {%0, %1, %2, %3, %4, %5, %6, %7};" ::B2W4_R8(
+            r, 0),
+        "r"(at)
         : "memory");
 }
 __device__ __forceinline__ void tmem_st_wait() {
@@ -129,18 +132,23 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
     asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
     return d;
 }
-// The next piece of two numbers, low half = lo; they keep what is left (exact).
+// The next piece of two numbers, low half = lo; they keep what is left (exact), but not behind the
+// last piece.
 template <typename T>
-__device__ __forceinline__ uint32_t take_piece(uint64_t& v) {
+__device__ __forceinline__ uint32_t take_piece(uint64_t& v, bool last = false) {
     float lo, hi;
     b2w4_unpack2(v, lo, hi);
     uint32_t p;
     if constexpr (std::is_same_v<T, __half>) {
         asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(p) : "f"(hi), "f"(lo));
+        if (last)
+            return p;
         const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&p));
         v = b2w4_sub2(v, b2w4_pack2(f.x, f.y));
     } else {
         asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(p) : "f"(hi), "f"(lo));
+        if (last)
+            return p;
         v = b2w4_sub2(v, b2w4_pack2(__uint_as_float(p << 16), __uint_as_float(p & 0xffff0000u)));
     }
     return p;
@@ -160,7 +168,10 @@ __device__ __forceinline__ uint32_t place(int row, int chunk) {
     return (uint32_t)((row >> 3) * 1024 + (row & 7) * 128 + ((chunk ^ (row & 7)) << 4));
 }
 
-constexpr float kHalfScale = 1024.f;  // of probabilities beside an fp16 cache
+// 2^kLift times a row's probabilities are what is taken apart and summed: beside an fp16 cache
+// that keeps the small ones' pieces normal numbers.
+template <typename T>
+constexpr float kLift = std::is_same_v<T, __half> ? 10.f : 0.f;
 
 // Whole warp.  Tile `at` of the call's, counted from the last sequence's last tile; false: there is
 // none.  t0: its first token of the sequence's rows.
@@ -198,17 +209,18 @@ template <typename T, int DIM>
 __global__ void __launch_bounds__(Cfg<T, DIM>::kThreads, 1)
 paged_runs_kernel(const Args a, const Attend p, int tq) {
     using C = Cfg<T, DIM>;
-    constexpr int kKeys = C::kKeys, kType = std::is_same_v<T, __half> ? 0 : 1;
+    constexpr int kKeys = C::kKeys, kParts = C::kParts, kRowWarps = C::kRowWarps;
+    constexpr int kMmaWarp = C::kMmaWarp, kLoadWarp0 = C::kLoadWarp0;
+    constexpr int kType = std::is_same_v<T, __half> ? 0 : 1;
     extern __shared__ __align__(1024) uint8_t smem[];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::kBar);
     uint64_t* q_full = bars;        // the queries' pieces
     uint64_t* s_full = bars + 1;    // scores of a block complete
     uint64_t* s_free = bars + 2;    // ... and in registers
-    uint64_t* p_full = bars + 3;    // probabilities' pieces in tensor memory
+    uint64_t* p_full = bars + 3;    // probabilities' pieces in tensor memory, the last P V out of it
     uint64_t* o_full = bars + 4;    // P V of a block complete (and P read)
-    uint64_t* o_free = bars + 5;    // ... and in registers
-    uint64_t* drained = bars + 6;   // [2] every MMA retired
+    uint64_t* drained = bars + 6;   // every MMA retired
     uint64_t* k_full = bars + 8;    // [2]
     uint64_t* k_free = bars + 10;   // [2]
     uint64_t* v_full = bars + 12;   // [2]
@@ -226,9 +238,8 @@ paged_runs_kernel(const Args a, const Attend p, int tq) {
         mbar_init(s_free, kRowWarps);
         mbar_init(p_full, kRowWarps);
         mbar_init(o_full, 1);
-        mbar_init(o_free, kRowWarps);
+        mbar_init(drained, 1);
         for (int b = 0; b < 2; ++b) {
-            mbar_init(&drained[b], 1);
             mbar_init(&k_full[b], C::kLoadWarps);
             mbar_init(&k_free[b], 1);
             mbar_init(&v_full[b], C::kLoadWarps);
@@ -240,7 +251,7 @@ paged_runs_kernel(const Args a, const Attend p, int tq) {
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     b2w4_pdl_wait();
-    if (warp == kOutWarp) {
+    if (warp == kLoadWarp0) {
         int seq = -1, t0 = 0;
         if (!find_tile(a, tq, blockIdx.y, &seq, &t0))
             seq = -1;
@@ -253,7 +264,7 @@ paged_runs_kernel(const Args a, const Attend p, int tq) {
     const int seq = s_tile[0], t0 = s_tile[1];
     if (seq < 0)
         return;
-    if (warp == kScoreWarp) {
+    if (warp == kMmaWarp) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;"
                      ::"r"(smem_u32(tmem_slot)), "r"(512)
                      : "memory");
@@ -288,73 +299,108 @@ paged_runs_kernel(const Args a, const Attend p, int tq) {
     const int from = p.window.from(max(p0, 0)), low = min(p.window.sinks, from);
     const int count = p1 < 0 ? 0 : low + p1 + 1 - from;
     const int steps = (count + kKeys - 1) / kKeys;
+    // r / rep for r < 128: a division for every row of the tile was 5000 cycles of it
+    const int inverse = (65536 + rep - 1) / rep;
+    auto token_of = [&](int r) { return (r * inverse) >> 16; };
     auto row_offset = [&](int r, int ld) {
-        return (size_t)(s.first + t0 + r / rep) * ld + (size_t)(kvh * rep + r % rep) * DIM;
+        const int t = token_of(r);
+        return (size_t)(s.first + t0 + t) * ld + (size_t)(kvh * rep + r - t * rep) * DIM;
     };
-    auto row_exists = [&](int r) { return r < tq * rep && t0 + r / rep < s.count; };
+    auto row_exists = [&](int r) { return r < tq * rep && t0 + token_of(r) < s.count; };
 
     if (warp < kRowWarps) {
         // ================================== rows =====================================
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(C::kRegsRows));
-        const int quarter = warp & 3, half = warp >> 2;
+        // a quarter of the tensor memory's lanes; a part of the keys and of the features
+        const int quarter = warp & 3, part = warp >> 2;
         const int row = quarter * 32 + lane;
         const bool exists = row_exists(row);
-        const int pos = exists ? p0 + row / rep : -1;
+        const int pos = exists ? p0 + token_of(row) : -1;
         const uint32_t lane_addr = tmem + ((uint32_t)(quarter * 32) << 16);
-        auto pair_sync = [&]() { asm volatile("bar.sync %0, 64;" ::"r"(3 + quarter) : "memory"); };
-        // both threads' larger value, through the words of a parity
-        auto pair_max = [&](float v, int parity) {
-            float* mx = s_max + parity * 2 * kRows;
-            mx[half * kRows + row] = v;
-            pair_sync();
-            return fmaxf(v, mx[(1 - half) * kRows + row]);
+        auto row_sync = [&]() {  // the threads of a quarter's rows have come here
+            asm volatile("bar.sync %0, %1;" ::"r"(3 + quarter), "n"(32 * kParts) : "memory");
         };
-        float factor = __fmul_rn(p.scale, 1.4426950408889634f);
+        // the threads' values of the row, through the words of a parity
+        auto share = [&](float v, int parity, auto join) {
+            float* mx = s_max + parity * kParts * kRows + row;
+            mx[part * kRows] = v;
+            row_sync();
+            float r = mx[0];
+#pragma unroll
+            for (int i = 1; i < kParts; ++i)
+                r = join(r, mx[i * kRows]);
+            return r;
+        };
+        auto larger = [](float x, float y) { return fmaxf(x, y); };
+        // The factor of the scores, in base 2.  It is positive: the queries take a negative sign,
+        // and zero is as small a number as can be, so that a masked score stays below all others.
+        const float scale = __fmul_rn(p.scale, 1.4426950408889634f);
+        float factor = fmaxf(fabsf(scale), 0x1p-100f);
+        constexpr int kOwn = DIM / kParts, kMine = kKeys / kParts;  // features, keys
+        // a tile of fp32 rows in shared memory: a warp moves some of its quarter's rows whole
+        constexpr int kRowChunks = DIM / 4, kRowsAtOnce = 32 / kRowChunks;
+        auto staged = [](int r, int chunk) { return (r * kRowChunks + (chunk ^ (r & 7))) * 16; };
+        const int stage_chunk = lane % kRowChunks;
+        auto stage_row = [&](int i) {
+            return quarter * 32 + (part * (32 / kParts / kRowsAtOnce) + i) * kRowsAtOnce +
+                   lane / kRowChunks;
+        };
         if (steps > 0) {
-            const float4* src =
-                reinterpret_cast<const float4*>(p.q + (exists ? row_offset(row, p.ldq) : 0));
-            const float4 zero = make_float4(0.f, 0.f, 0.f, 0.f);
-            float up = 1.f;
+            // Rows come through shared memory, the values' place, which is not filled before: a
+            // thread's own loads would be a line each (5000 cycles of the load path).
+            uint8_t* const stage = smem + C::kVs;
+#pragma unroll
+            for (int i = 0; i < 32 / kParts / kRowsAtOnce; ++i) {
+                const int r = stage_row(i);
+                const float4 v =
+                    row_exists(r) ? *reinterpret_cast<const float4*>(p.q + row_offset(r, p.ldq) +
+                                                                     stage_chunk * 4)
+                                  : make_float4(0.f, 0.f, 0.f, 0.f);
+                *reinterpret_cast<float4*>(stage + staged(r, stage_chunk)) = v;
+            }
+            row_sync();
+            float4 f[kOwn / 4];
+#pragma unroll
+            for (int i = 0; i < kOwn / 4; ++i)
+                f[i] = *reinterpret_cast<const float4*>(stage + staged(row, part * (kOwn / 4) + i));
+            float up = scale < 0.f ? -1.f : 1.f;
             if constexpr (std::is_same_v<T, __half>) {  // the row's largest to [2^10, 2^11)
                 float top = 0.f;
-                if (exists)
-                    for (int c = half * (DIM / 8); c < (half + 1) * (DIM / 8); ++c) {
-                        const float4 f = src[c];
-                        top = fmaxf(fmaxf(fmaxf(top, fabsf(f.x)), fmaxf(fabsf(f.y), fabsf(f.z))),
-                                    fabsf(f.w));
-                    }
-                top = pair_max(top, 1);
+#pragma unroll
+                for (int i = 0; i < kOwn / 4; ++i)
+                    top = fmaxf(fmaxf(fmaxf(top, fabsf(f[i].x)), fmaxf(fabsf(f[i].y), fabsf(f[i].z))),
+                                fabsf(f[i].w));
+                top = share(top, 1, larger);
                 int e = (int)(__float_as_uint(top) >> 23) - 127;
                 e = top == 0.f ? 10 : min(max(e, -100), 120);
-                up = __uint_as_float((unsigned)(127 + 10 - e) << 23);
+                up = __fmul_rn(up, __uint_as_float((unsigned)(127 + 10 - e) << 23));
                 factor = __fmul_rn(factor, __uint_as_float((unsigned)(127 - 10 + e) << 23));
+                factor = fmaxf(factor, 0x1p-100f);
             }
-#pragma unroll 1
-            for (int c = half * (DIM / 2); c < (half + 1) * (DIM / 2); c += 32) {
-                uint64_t v[16];
+            const uint64_t up2 = b2w4_pack2(up, up);
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    float4 f = exists ? src[c / 4 + i] : zero;
-                    if constexpr (std::is_same_v<T, __half>)
-                        f = make_float4(__fmul_rn(f.x, up), __fmul_rn(f.y, up), __fmul_rn(f.z, up),
-                                        __fmul_rn(f.w, up));
-                    v[2 * i] = b2w4_pack2(f.x, f.y);
-                    v[2 * i + 1] = b2w4_pack2(f.z, f.w);
+            for (int c = 0; c < kOwn; c += 16) {
+                uint64_t v[8];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    v[2 * i] = b2w4_mul2(b2w4_pack2(f[c / 4 + i].x, f[c / 4 + i].y), up2);
+                    v[2 * i + 1] = b2w4_mul2(b2w4_pack2(f[c / 4 + i].z, f[c / 4 + i].w), up2);
                 }
+                const int at = part * kOwn + c;  // first feature
 #pragma unroll
                 for (int i = 0; i < C::kQ; ++i) {
-                    uint32_t r[16];
+                    uint32_t r[8];
 #pragma unroll
-                    for (int e = 0; e < 16; ++e)
-                        r[e] = take_piece<T>(v[e]);
+                    for (int e = 0; e < 8; ++e)
+                        r[e] = take_piece<T>(v[e], i == C::kQ - 1);
                     if (i < C::kQTmem) {
-                        tmem_st16(lane_addr + C::kTq + i * (DIM / 2) + c / 2, r);
+                        tmem_st8(lane_addr + C::kTq + i * (DIM / 2) + at / 2, r);
                     } else {
                         uint8_t* to = smem + C::kQs + (i - C::kQTmem) * C::kQPiece +
-                                      c / 64 * C::kQPart;
+                                      at / 64 * C::kQPart;
 #pragma unroll
-                        for (int e = 0; e < 4; ++e)
-                            *reinterpret_cast<uint4*>(to + place(row, c % 64 / 8 + e)) =
+                        for (int e = 0; e < 2; ++e)
+                            *reinterpret_cast<uint4*>(to + place(row, at % 64 / 8 + e)) =
                                 make_uint4(r[4 * e], r[4 * e + 1], r[4 * e + 2], r[4 * e + 3]);
                     }
                 }
@@ -364,13 +410,13 @@ paged_runs_kernel(const Args a, const Attend p, int tq) {
             asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
             warp_arrive(q_full);
         }
-        float m = -INFINITY, l = 0.f, alpha = 1.f;
-        constexpr int kOwn = DIM / 2, kMine = kKeys / 2;  // the thread's features and keys
+        // m: the row's largest score, mf: times the factor, as it is taken from the exponents
+        float m = -INFINITY, mf = -INFINITY, l = 0.f, alpha = 1.f;
         uint64_t acc[kOwn / 2];
 #pragma unroll
         for (int i = 0; i < kOwn / 2; ++i)
             acc[i] = 0ull;
-        bool live = true;  // no way out of the loop: the two threads of a row meet once a step
+        bool live = true;  // no way out of the loop: the threads of a row meet once a step
         auto await = [&](uint64_t* bar, uint32_t parity) {
             if (live && !warp_wait(bar, parity)) {
                 live = false;
@@ -378,156 +424,173 @@ paged_runs_kernel(const Args a, const Attend p, int tq) {
             }
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         };
-        auto take_output = [&]() {
+        // 16 of the thread's features of P V, on their way; and into the running output
+        auto output_ld = [&](int c, uint32_t (&r)[16]) {
+            tmem_ld16(lane_addr + C::kTo + part * kOwn + 16 * c, r);
+        };
+        auto output_add = [&](int c, uint32_t (&r)[16]) {
             const uint64_t al = b2w4_pack2(alpha, alpha);
+            tmem_ld_wait(r);
 #pragma unroll
-            for (int c = 0; c < kOwn; c += 32) {
-                uint32_t r0[16], r1[16];
-                tmem_ld16(lane_addr + C::kTo + half * kOwn + c, r0);
-                tmem_ld16(lane_addr + C::kTo + half * kOwn + c + 16, r1);
-                tmem_ld_wait(r0, r1);
-#pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    const uint32_t* r = i < 8 ? r0 : r1;
-                    acc[c / 2 + i] = b2w4_fma2(acc[c / 2 + i], al,
-                                               b2w4_pack2(__uint_as_float(r[2 * (i & 7)]),
-                                                          __uint_as_float(r[2 * (i & 7) + 1])));
-                }
-            }
-            asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-            warp_arrive(o_free);
+            for (int i = 0; i < 8; ++i)
+                acc[8 * c + i] = b2w4_fma2(acc[8 * c + i], al,
+                                           b2w4_pack2(__uint_as_float(r[2 * i]),
+                                                      __uint_as_float(r[2 * i + 1])));
         };
         // of the list, the row sees [0, sinks) and [lo, hi)
         const int hi = pos < 0 ? 0 : pos - from + low + 1;
         const int lo = p.window.from(max(pos, 0)) - from + low;
         for (int j = 0; j < steps; ++j) {
             await(s_full, j & 1);
-            uint64_t sc[kMine / 2];
+            uint32_t sr[kMine / 16][16];
 #pragma unroll
-            for (int h = 0; h < kMine; h += 32) {
-                uint32_t r0[16], r1[16];
-                tmem_ld16(lane_addr + C::kTs + half * kMine + h, r0);
-                tmem_ld16(lane_addr + C::kTs + half * kMine + h + 16, r1);
-                tmem_ld_wait(r0, r1);
+            for (int h = 0; h < kMine / 16; ++h)
+                tmem_ld16(lane_addr + C::kTs + part * kMine + 16 * h, sr[h]);
 #pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    const uint32_t* r = i < 8 ? r0 : r1;
-                    sc[h / 2 + i] =
-                        b2w4_mul2(b2w4_pack2(__uint_as_float(r[2 * (i & 7)]),
-                                             __uint_as_float(r[2 * (i & 7) + 1])),
-                                  b2w4_pack2(factor, factor));
-                }
-            }
+            for (int h = 0; h < kMine / 16; ++h)
+                tmem_ld_wait(sr[h]);
             asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
             warp_arrive(s_free);
-            const int first = j * kKeys + half * kMine;  // the thread's first key of the list
-            if (first + kMine > hi || (first < lo && first + kMine > p.window.sinks)) {
+            float sc[kMine];
 #pragma unroll
-                for (int i = 0; i < kMine / 2; ++i) {
-                    float x, y;
-                    b2w4_unpack2(sc[i], x, y);
-                    auto sees = [&](int k) { return k < hi && (k >= lo || k < p.window.sinks); };
-                    sc[i] = b2w4_pack2(sees(first + 2 * i) ? x : -INFINITY,
-                                       sees(first + 2 * i + 1) ? y : -INFINITY);
-                }
+            for (int i = 0; i < kMine; ++i)
+                sc[i] = __uint_as_float(sr[i / 16][i % 16]);
+            const int first = j * kKeys + part * kMine;  // the thread's first key of the list
+            if (first + kMine > hi || (first < lo && first + kMine > p.window.sinks)) {
+                static_assert(kMine <= 32);
+                auto below = [](int n) { return n <= 0 ? 0u : n >= 32 ? ~0u : (1u << n) - 1u; };
+                const unsigned seen = below(hi - first) &
+                                      (~below(lo - first) | below(p.window.sinks - first));
+#pragma unroll
+                for (int i = 0; i < kMine; ++i)
+                    if (!(seen >> i & 1))
+                        sc[i] = -INFINITY;
             }
             float top = m;
 #pragma unroll
-            for (int i = 0; i < kMine / 2; ++i) {
-                float x, y;
-                b2w4_unpack2(sc[i], x, y);
-                top = fmaxf(fmaxf(top, x), y);
-            }
-            top = pair_max(top, j & 1);
-            const float base = top == -INFINITY ? 0.f : top;
+            for (int i = 0; i < kMine; i += 2)
+                top = fmaxf(fmaxf(top, sc[i]), sc[i + 1]);
+            m = share(top, j & 1, larger);
+            const float next_mf = m == -INFINITY ? 0.f : __fmul_rn(m, factor);
+            const float shift = __fsub_rn(kLift<T>, next_mf);
+            const uint64_t factor2 = b2w4_pack2(factor, factor), shift2 = b2w4_pack2(shift, shift);
+            uint64_t pr[kMine / 2];
 #pragma unroll
             for (int i = 0; i < kMine / 2; ++i) {
                 float x, y;
-                b2w4_unpack2(sc[i], x, y);
-                sc[i] = b2w4_pack2(exp2_neg(__fsub_rn(x, base)), exp2_neg(__fsub_rn(y, base)));
+                b2w4_unpack2(b2w4_fma2(b2w4_pack2(sc[2 * i], sc[2 * i + 1]), factor2, shift2), x, y);
+                pr[i] = b2w4_pack2(exp2_neg(x), exp2_neg(y));
             }
-            uint64_t sum[4] = {sc[0], sc[1], sc[2], sc[3]};
+            uint64_t sum[4] = {pr[0], pr[1], pr[2], pr[3]};
 #pragma unroll
             for (int i = 4; i < kMine / 2; ++i)
-                sum[i & 3] = add2(sum[i & 3], sc[i]);
+                sum[i & 3] = add2(sum[i & 3], pr[i]);
             sum[0] = add2(add2(sum[0], sum[1]), add2(sum[2], sum[3]));
             float sum0, sum1;
             b2w4_unpack2(sum[0], sum0, sum1);
-            const float next_alpha = exp2_neg(__fsub_rn(m, base));
-            m = top;
+            const float next_alpha = exp2_neg(__fsub_rn(mf, next_mf));
+            mf = m == -INFINITY ? -INFINITY : next_mf;
             l = __fmaf_rn(l, next_alpha, __fadd_rn(sum0, sum1));
-            if constexpr (std::is_same_v<T, __half>) {
+            // The pieces that fit the registers are taken ahead of the wait for the product before,
+            // which reads the probabilities: the MMAs of the next one wait for what is behind it.
+            constexpr int kPs = kMine / 16, kOs = kOwn / 16, kTurns = kPs > kOs ? kPs : kOs;
+            uint32_t pieces[C::kQ][8];
+            auto take = [&](int u) {
 #pragma unroll
-                for (int i = 0; i < kMine / 2; ++i)
-                    sc[i] = b2w4_mul2(sc[i], b2w4_pack2(kHalfScale, kHalfScale));
-            }
-            // the product before has read the probabilities
-            if (j) {
+                for (int i = 0; i < C::kQ; ++i)
+#pragma unroll
+                    for (int e = 0; e < 8; ++e)
+                        pieces[i][e] = take_piece<T>(pr[8 * u + e], i == C::kQ - 1);
+            };
+            take(0);
+            if (j)
                 await(o_full, (j - 1) & 1);
-                take_output();
+#pragma unroll
+            for (int u = 0; u < kTurns; ++u) {
+                uint32_t ro[16];
+                if (j && u < kOs)
+                    output_ld(u, ro);
+                if (u < kPs) {
+                    if (u)
+                        take(u);
+#pragma unroll
+                    for (int i = 0; i < C::kQ; ++i)
+                        tmem_st8(lane_addr + C::kTp + i * (kKeys / 2) + part * (kMine / 2) + 8 * u,
+                                 pieces[i]);
+                }
+                if (j && u < kOs)
+                    output_add(u, ro);
             }
             alpha = next_alpha;
-#pragma unroll
-            for (int i = 0; i < C::kQ; ++i)
-#pragma unroll
-                for (int h = 0; h < kMine / 2; h += 16) {
-                    uint32_t r[16];
-#pragma unroll
-                    for (int e = 0; e < 16; ++e)
-                        r[e] = take_piece<T>(sc[h + e]);
-                    tmem_st16(lane_addr + C::kTp + i * (kKeys / 2) + half * (kMine / 2) + h, r);
-                }
             tmem_st_wait();
             asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
             warp_arrive(p_full);
         }
         if (steps > 0) {
             await(o_full, (steps - 1) & 1);
-            take_output();
+#pragma unroll
+            for (int u = 0; u < kOwn / 16; ++u) {
+                uint32_t ro[16];
+                output_ld(u, ro);
+                output_add(u, ro);
+            }
         }
-        // the other thread's part of the sum (the other parity's words: they may still be read)
-        float* mx = s_max + (steps & 1) * 2 * kRows;
-        mx[half * kRows + row] = l;
-        pair_sync();
-        const float total = __fadd_rn(mx[row], mx[kRows + row]);
-        const float down = std::is_same_v<T, __half> ? 1.f / kHalfScale : 1.f;
+        // (the other parity's words: they may still be read)
+        const float total = share(l, steps & 1, [](float x, float y) { return __fadd_rn(x, y); });
         bool odd = false;
+        const float over = pos < 0 ? 0.f : __fdiv_rn(1.f, total);
 #pragma unroll
         for (int i = 0; i < kOwn / 2; ++i) {
             float x, y;
             b2w4_unpack2(acc[i], x, y);
-            x = pos < 0 ? 0.f : __fdiv_rn(__fmul_rn(x, down), total);
-            y = pos < 0 ? 0.f : __fdiv_rn(__fmul_rn(y, down), total);
+            x = pos < 0 ? 0.f : __fmul_rn(x, over);
+            y = pos < 0 ? 0.f : __fmul_rn(y, over);
             odd |= paged::odd_result<T>(x) || paged::odd_result<T>(y);
             acc[i] = b2w4_pack2(x, y);
         }
-        if (exists && !*s_abort) {
-            ulonglong2* dst =
-                reinterpret_cast<ulonglong2*>(p.out + row_offset(row, p.ldo) + half * kOwn);
+        // out through shared memory too: every product that read it has retired
+        uint8_t* const stage = smem + C::kVs;
 #pragma unroll
-            for (int i = 0; i < kOwn / 4; ++i)
-                dst[i] = make_ulonglong2(acc[2 * i], acc[2 * i + 1]);
-        }
+        for (int i = 0; i < kOwn / 4; ++i)
+            *reinterpret_cast<ulonglong2*>(stage + staged(row, part * (kOwn / 4) + i)) =
+                make_ulonglong2(acc[2 * i], acc[2 * i + 1]);
+        row_sync();
+        if (!*s_abort)
+#pragma unroll
+            for (int i = 0; i < 32 / kParts / kRowsAtOnce; ++i) {
+                const int r = stage_row(i);
+                if (row_exists(r))
+                    *reinterpret_cast<float4*>(p.out + row_offset(r, p.ldo) + stage_chunk * 4) =
+                        *reinterpret_cast<const float4*>(stage + staged(r, stage_chunk));
+            }
         const unsigned again = __ballot_sync(0xffffffffu, exists && odd);
         if (lane == 0 && again)
             atomicOr(&s_odd[quarter], again);
     } else {
       asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::kRegsOther));
-      if (warp == kScoreWarp) {
-        // ============================ MMA issue: scores ==============================
-        if (lane == 0) {
+      if (warp == kMmaWarp) {
+        // ================================= MMA issue =================================
+        // One warp, so that P V of a block goes ahead of the scores of the next but one, which
+        // become possible at the same time: the rows wait for the former.  The warp stays together
+        // and one lane issues: what the MMAs are given is then the same for all lanes and is
+        // worked out once a warp.
+        {
+            const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
             const uint64_t k_desc0 = umma_desc_k_sw128(smem_u32(smem + C::kKs));
             const uint64_t q_desc = umma_desc_k_sw128(smem_u32(smem + C::kQs));
-            constexpr uint32_t id = idesc(kType, kKeys, false);
-            bool ok = steps == 0 || wait(q_full, 0);
-            for (int j = 0; j < steps && ok; ++j) {
-                ok = wait(&k_full[j & 1], (j >> 1) & 1) && (j == 0 || wait(s_free, (j - 1) & 1));
-                if (!ok)
-                    break;
+            const uint64_t v_desc0 = desc_slow(smem_u32(smem + C::kVs), C::kPart);
+            constexpr uint32_t score_id = idesc(kType, kKeys, false);
+            constexpr uint32_t out_id = idesc(kType, DIM, true);
+            // sizes of products, the smallest first: pieces i of Q and size - i of K
+            auto scores = [&](int j) {
+                if (!warp_wait(&k_full[j & 1], (j >> 1) & 1) ||
+                    (j > 0 && !warp_wait(s_free, (j - 1) & 1)))
+                    return false;
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                 const uint64_t d = k_desc0 + (uint64_t)((j & 1) * (C::kBuf >> 4));
+                if (!elect_one())
+                    return true;
                 bool more = false;
-                // sizes of products, the smallest first: pieces i of Q and size - i of K
 #pragma unroll
                 for (int size = C::kQ - 1; size >= 0; --size)
 #pragma unroll
@@ -540,38 +603,27 @@ paged_runs_kernel(const Args a, const Attend p, int tq) {
                                 d + (uint64_t)(((size - i) * C::kPiece + k / 4 * C::kPart +
                                                 k % 4 * 32) >> 4);
                             if (i < C::kQTmem)
-                                umma_ts(tmem + C::kTs, tmem + C::kTq + i * (DIM / 2) + k * 8, kd,
-                                        id, more);
+                                umma_ts(tm + C::kTs, tm + C::kTq + i * (DIM / 2) + k * 8, kd,
+                                        score_id, more);
                             else
-                                umma_ss(tmem + C::kTs,
+                                umma_ss(tm + C::kTs,
                                         q_desc + (uint64_t)(((i - C::kQTmem) * C::kQPiece +
                                                              k / 4 * C::kQPart + k % 4 * 32) >> 4),
-                                        kd, id, more);
+                                        kd, score_id, more);
                             more = true;
                         }
                     }
                 umma_commit(s_full);
                 umma_commit(&k_free[j & 1]);
-            }
-            if (!ok)
-                fail();
-            umma_commit(&drained[0]);
-            if (!mbar_wait(&drained[0], 0))
-                fail();
-        }
-      } else if (warp == kOutWarp) {
-        // ============================== MMA issue: P V ===============================
-        if (lane == 0) {
-            const uint64_t v_desc0 = desc_slow(smem_u32(smem + C::kVs), C::kPart);
-            constexpr uint32_t id = idesc(kType, DIM, true);
-            bool ok = true;
-            for (int j = 0; j < steps; ++j) {
-                ok = wait(&v_full[j & 1], (j >> 1) & 1) &&
-                     (j == 0 || wait(o_free, (j - 1) & 1)) && wait(p_full, j & 1);
-                if (!ok)
-                    break;
+                return true;
+            };
+            auto output = [&](int j) {
+                if (!warp_wait(&v_full[j & 1], (j >> 1) & 1) || !warp_wait(p_full, j & 1))
+                    return false;
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                 const uint64_t d = v_desc0 + (uint64_t)((j & 1) * (C::kBuf >> 4));
+                if (!elect_one())
+                    return true;
                 bool more = false;
 #pragma unroll
                 for (int size = C::kQ - 1; size >= 0; --size)
@@ -581,22 +633,36 @@ paged_runs_kernel(const Args a, const Attend p, int tq) {
                             continue;
 #pragma unroll
                         for (int k = 0; k < kKeys / 16; ++k) {
-                            umma_ts(tmem + C::kTo, tmem + C::kTp + i * (kKeys / 2) + k * 8,
-                                    d + (uint64_t)(((size - i) * C::kPiece + k * 2048) >> 4), id,
-                                    more);
+                            umma_ts(tm + C::kTo, tm + C::kTp + i * (kKeys / 2) + k * 8,
+                                    d + (uint64_t)(((size - i) * C::kPiece + k * 2048) >> 4),
+                                    out_id, more);
                             more = true;
                         }
                     }
                 umma_commit(o_full);
                 umma_commit(&v_free[j & 1]);
+                return true;
+            };
+            bool ok = steps == 0 || (warp_wait(q_full, 0) && scores(0));
+            __syncwarp();
+            if (ok && steps > 1)
+                ok = scores(1);
+            __syncwarp();
+            for (int j = 0; j < steps && ok; ++j) {
+                ok = output(j);
+                __syncwarp();
+                ok = ok && (j + 2 >= steps || scores(j + 2));
+                __syncwarp();
             }
             if (!ok)
                 fail();
-            umma_commit(&drained[1]);
-            if (!mbar_wait(&drained[1], 0))
+            if (elect_one())
+                umma_commit(drained);
+            __syncwarp();
+            if (!mbar_wait(drained, 0))
                 fail();
         }
-      } else {
+      } else if (warp < kLoadWarp0 + 2 * C::kLoadWarps) {
         // ============================== keys and values ==============================
         // Where key i of the list lies; -1: it does not exist.  One whose page is not the pool's
         // is left out, which a masked row cannot be: the tile's rows are done again.
@@ -615,113 +681,107 @@ paged_runs_kernel(const Args a, const Attend p, int tq) {
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             warp_arrive(bar);
         };
-        const int w0 = warp - kLoadWarp0;
+        // Half of the warps have the keys, the others the values.
+        const bool values = warp >= kLoadWarp0 + C::kLoadWarps;
+        const int w0 = (warp - kLoadWarp0) % C::kLoadWarps;
+        uint64_t *filled = values ? v_full : k_full, *freed = values ? v_free : k_free;
+        const T* pool = static_cast<const T*>(values ? a.v : a.k);
+        uint8_t* ring = smem + (values ? C::kVs : C::kKs);
         constexpr int kChunks = DIM / 8, kPer = 32 / kChunks;  // of eight features; rows at a time
         const int c = lane % kChunks, sub = lane / kChunks;
-        bool ok = true;
-        auto free = [&](uint64_t* bars2, int j) {
-            if (j >= 2 && !warp_wait(&bars2[j & 1], ((j >> 1) - 1) & 1)) {
-                ok = false;
+        uint8_t* const mine = ring + (c >> 3) * C::kPart;
+        auto free = [&](int j) {
+            // (the values' place holds the queries at first)
+            const bool ok = j < 2 ? !values || warp_wait(q_full, 0)
+                                  : warp_wait(&freed[j & 1], ((j >> 1) - 1) & 1);
+            if (!ok)
                 fail();
-            }
             return ok;
         };
         if constexpr (C::kWide) {
-            // a warp has every kLoadWarps-th set of kPer rows of a block
+            // a warp has every kLoadWarps-th set of kPer rows of a block; the next block's numbers
+            // are on their way
             constexpr int kSets = kKeys / kPer, kMine = (kSets + C::kLoadWarps - 1) / C::kLoadWarps;
-            int rows[kMine];
-            auto look = [&](int j) {
+            ulonglong2 next[kMine][2];
+            auto load = [&](int j) {
+                int rows[kMine];
 #pragma unroll
                 for (int u = 0; u < kMine; ++u) {
                     const int set = w0 + u * C::kLoadWarps;
                     rows[u] = set < kSets ? row_of(j * kKeys + set * kPer + sub) : -1;
                 }
-            };
-            auto bring = [&](const float* pool, uint8_t* to) {
-                ulonglong2 f[kMine][2];
 #pragma unroll
                 for (int u = 0; u < kMine; ++u)
 #pragma unroll
                     for (int h = 0; h < 2; ++h)
-                        f[u][h] = rows[u] >= 0 ? reinterpret_cast<const ulonglong2*>(
-                                                     pool + (size_t)rows[u] * DIM + c * 8)[h]
-                                               : make_ulonglong2(0ull, 0ull);
+                        next[u][h] = rows[u] >= 0 ? reinterpret_cast<const ulonglong2*>(
+                                                        pool + (size_t)rows[u] * DIM + c * 8)[h]
+                                                  : make_ulonglong2(0ull, 0ull);
+            };
+            load(0);
+            for (int j = 0; j < steps && free(j); ++j) {
 #pragma unroll
                 for (int u = 0; u < kMine; ++u) {
                     const int set = w0 + u * C::kLoadWarps;
                     if (set >= kSets)
                         break;
-                    uint64_t x[4] = {f[u][0].x, f[u][0].y, f[u][1].x, f[u][1].y};
-                    uint8_t* dst = to + (c >> 3) * C::kPart + place(set * kPer + sub, c & 7);
+                    uint64_t x[4] = {next[u][0].x, next[u][0].y, next[u][1].x, next[u][1].y};
+                    uint8_t* dst = mine + (j & 1) * C::kBuf + place(set * kPer + sub, c & 7);
 #pragma unroll
                     for (int i = 0; i < C::kK; ++i) {
                         uint4 o;
-                        o.x = take_piece<T>(x[0]);
-                        o.y = take_piece<T>(x[1]);
-                        o.z = take_piece<T>(x[2]);
-                        o.w = take_piece<T>(x[3]);
+                        o.x = take_piece<T>(x[0], i == C::kK - 1);
+                        o.y = take_piece<T>(x[1], i == C::kK - 1);
+                        o.z = take_piece<T>(x[2], i == C::kK - 1);
+                        o.w = take_piece<T>(x[3], i == C::kK - 1);
                         *reinterpret_cast<uint4*>(dst + i * C::kPiece) = o;
                     }
                 }
+                full(&filled[j & 1]);
+                load(j + 1);
+            }
+        } else {
+            // the warp's lanes know where four of a block's keys lie each, a block ahead
+            static_assert(C::kWide || (C::kLoadWarps == 1 && kKeys == 128));
+            int next[4], rows[4];
+            auto look = [&](int j) {
+#pragma unroll
+                for (int u = 0; u < 4; ++u)
+                    next[u] = row_of(j * kKeys + u * 32 + lane);
             };
             look(0);
-            for (int j = 0; j < steps && free(k_free, j); ++j) {
-                bring(static_cast<const float*>(a.k), smem + C::kKs + (j & 1) * C::kBuf);
-                full(&k_full[j & 1]);
-                if (!free(v_free, j))
-                    break;
-                bring(static_cast<const float*>(a.v), smem + C::kVs + (j & 1) * C::kBuf);
-                look(j + 1);
-                full(&v_full[j & 1]);
-            }
-        } else if (w0 < C::kLoadWarps) {
-            // a warp has 32 keys of a block, a lane knows where one of them lies
-            static_assert(C::kWide || C::kLoadWarps * 32 == kKeys);
-            auto bring = [&](const void* pool, uint8_t* to, int row) {
+            for (int j = 0; j < steps && free(j); ++j) {
 #pragma unroll
-                for (int i = 0; i < 32 / kPer; ++i) {
-                    const int in = i * kPer + sub;
-                    const int r = __shfl_sync(0xffffffffu, row, in);
-                    cp16(smem_u32(to + (c >> 3) * C::kPart + place(w0 * 32 + in, c & 7)),
-                         static_cast<const T*>(pool) + (size_t)max(r, 0) * DIM + c * 8, r >= 0);
-                }
+                for (int u = 0; u < 4; ++u)
+                    rows[u] = next[u];
+                look(j + 1);
+                uint8_t* const to = mine + (j & 1) * C::kBuf;
+                // the rows of eight copies are fetched ahead of them: one by one, every copy
+                // waited for its shuffle (80 cycles each)
+#pragma unroll
+                for (int u = 0; u < 4; ++u)
+#pragma unroll
+                    for (int i = 0; i < 32 / kPer; i += 8) {
+                        int r[8];
+#pragma unroll
+                        for (int e = 0; e < 8; ++e)
+                            r[e] = __shfl_sync(0xffffffffu, rows[u], (i + e) * kPer + sub);
+#pragma unroll
+                        for (int e = 0; e < 8; ++e)
+                            cp16(smem_u32(to + place(u * 32 + (i + e) * kPer + sub, c & 7)),
+                                 pool + (size_t)max(r[e], 0) * DIM + c * 8, r[e] >= 0);
+                    }
                 asm volatile("cp.async.commit_group;" ::: "memory");
-            };
-            int row = row_of(w0 * 32 + lane), done = 0;
-            for (int j = 0; j < steps; ++j) {
-                // the block before is handed on as it arrives, ahead of a wait for a free place
-                if (j) {
-                    asm volatile("cp.async.wait_group 1;" ::: "memory");
-                    full(&k_full[(j - 1) & 1]);
-                }
-                if (!free(k_free, j))
-                    break;
-                bring(a.k, smem + C::kKs + (j & 1) * C::kBuf, row);
-                if (j) {
-                    asm volatile("cp.async.wait_group 1;" ::: "memory");
-                    full(&v_full[(j - 1) & 1]);
-                }
-                if (!free(v_free, j))
-                    break;
-                const int now = row;
-                row = row_of((j + 1) * kKeys + w0 * 32 + lane);
-                bring(a.v, smem + C::kVs + (j & 1) * C::kBuf, now);
-                done = j + 1;
-            }
-            if (ok && done) {
-                asm volatile("cp.async.wait_group 1;" ::: "memory");
-                full(&k_full[(done - 1) & 1]);
                 asm volatile("cp.async.wait_group 0;" ::: "memory");
-                full(&v_full[(done - 1) & 1]);
+                full(&filled[j & 1]);
             }
-            asm volatile("cp.async.wait_group 0;" ::: "memory");
         }
       }
     }
 
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
-    if (warp == kScoreWarp) {
+    if (warp == kMmaWarp) {
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;"
                      ::"r"(tmem), "r"(512)
@@ -730,7 +790,7 @@ paged_runs_kernel(const Args a, const Attend p, int tq) {
     if (warp < kRowWarps && !*s_abort)
         for (int r = warp; r < kRows; r += kRowWarps)
             if ((s_odd[r >> 5] >> (r & 31) & 1) && row_exists(r))
-                paged::attend_row<T, DIM>(a, s, p.q + row_offset(r, p.ldq), p0 + r / rep, kvh,
+                paged::attend_row<T, DIM>(a, s, p.q + row_offset(r, p.ldq), p0 + token_of(r), kvh,
                                           p.scale, p.window, p.out + row_offset(r, p.ldo));
 }
 

@@ -194,3 +194,21 @@ def test_pages_calls_reject_null_contexts():
     assert lib.b2w4_pages_free(None, None, None, 1) == -1
     assert lib.b2w4_pages_compact(None, None, None, None, None) == -1
     assert lib.b2w4_pages_copy(None, None, None, None, 1) == -1
+
+
+@pytest.mark.parametrize("page", [1, 2, 3, 5, 7, 8, 16, 24, 100, 641, 65536, (1 << 30) - 1, 1 << 30])
+def test_tokens_by_the_kernels_division(page):
+    """Every quotient that a table can hold: pages of any size, positions up to 2^31 - 1."""
+    rng = np.random.default_rng(page)
+    top = (1 << 31) - 2
+    positions = {0, 1, page - 1, page, page + 1, top, top - top % page, top - top % page - 1}
+    positions |= {int(x) for x in rng.integers(0, top, 20)}
+    for j in sorted(p for p in positions if 0 <= p <= top):
+        n = j // page
+        if n > 300000:
+            continue
+        table = np.full((1, n + 1), -1, dtype=np.int32)
+        table[0, n] = 0
+        c = cache(page_size=page, pages=1, kv_heads=1)
+        length = min((n + 1) * page, top + 1)
+        assert place(c, table, [length], 0, j, 0, max_length=top + 1)[0] == j - n * page
