@@ -16,8 +16,8 @@
 // What bounds it: the MMAs, which the pieces multiply: 128 rows x 128 keys x 128 features in three
 // pieces are 48 MMAs of 66 cycles, about 3200 cycles; a softmax takes about 2000 beside them.
 //
-// Roles: warps of rows, four threads to a row (two beside an fp32 cache); a warp that issues the scores' MMAs, a block
-// ahead, and one for P V; the rest bring keys and values.  Both lie in shared memory as they lie in
+// Roles: warps of rows, two or four threads to a row; a warp that issues the MMAs, the scores' up to
+// two blocks ahead; the rest bring keys and values.  Both lie in shared memory as they lie in
 // the cache, a key's features in 128-byte rows: the keys are the scores' B operand with features
 // running fastest, the values P V's with them running slowest, so neither is transposed.  Rows
 // come one by one with their pages' addresses, so a page may end anywhere.
@@ -38,20 +38,25 @@ constexpr int kRows = 128;
 template <typename T, int DIM>
 struct Cfg {
     static constexpr bool kWide = sizeof(T) == 4;
-    static constexpr int kKeys = kWide ? 64 : 128;
+    // heads of 64 in 16 bits: two smaller blocks to a multiprocessor, one's softmax, start and end
+    // beside the other's products
+    static constexpr bool kTwo = !kWide && DIM == 64;
+    static constexpr int kKeys = kWide || kTwo ? 64 : 128;
     static constexpr int kK = kWide ? 3 : 1;                             // pieces of a key
     static constexpr int kQ = std::is_same_v<T, __half> ? 2 : 3;         // of a query
     // of them in tensor memory: an MMA whose operands both come from shared memory takes twice as
     // long (its A is 128 bytes a cycle's worth of the port)
-    static constexpr int kQTmem = kWide ? 2 : kQ == 3 && DIM > 64 ? 1 : kQ;
-    static constexpr int kParts = kWide ? 2 : 4;  // threads to a row
+    static constexpr int kQTmem = kWide ? 2 : kQ == 3 ? 1 : kQ;
+    static constexpr int kParts = kWide || kTwo ? 2 : 4;  // threads to a row
     static constexpr int kRowWarps = 4 * kParts, kMmaWarp = kRowWarps;
     // for the keys, and as many for the values
     static constexpr int kLoadWarp0 = kRowWarps + 1, kLoadWarps = kWide ? 7 : 1;
     static constexpr int kThreads = (kLoadWarp0 + 2 * kLoadWarps + 1) * 32;  // one is idle
     static_assert(kThreads % 128 == 0, "warpgroups");
-    static constexpr int kRegsStart = kWide ? 80 : 96;
-    static constexpr int kRegsRows = kWide ? 128 : 104, kRegsOther = kWide ? 56 : 64;
+    static constexpr int kBlocks = kTwo ? 2 : 1;  // of a multiprocessor
+    static constexpr int kRegsStart = kWide || kTwo ? 80 : 96;
+    static constexpr int kRegsRows = kWide ? 128 : kTwo ? 96 : 104;
+    static constexpr int kRegsOther = kWide ? 56 : kTwo ? 48 : 64;
     static_assert(kParts * kRegsRows + (kThreads / 128 - kParts) * kRegsOther <=
                       kThreads / 128 * kRegsStart,
                   "registers of the block");
@@ -63,11 +68,16 @@ struct Cfg {
     static constexpr int kMax = kQs + (kQ - kQTmem) * kQPiece;  // float [2 parities][kParts][kRows]
     static constexpr int kBar = kMax + 2 * kParts * kRows * 4;
     static constexpr int kTotal = kBar + 512;
-    static_assert(kTotal <= 227 * 1024, "shared memory");
+    static_assert(kTotal <= (228 / kBlocks - 1) * 1024, "shared memory");
+    // the rows' queries and results in 32 bits, in the values' place or theirs and the keys'
+    static constexpr bool kStageBoth = kRows * DIM * 4 > 2 * kBuf;
+    static constexpr int kStage = kStageBoth ? kKs : kVs;
+    static_assert(kRows * DIM * 4 <= (kStageBoth ? 4 : 2) * kBuf);
     // tensor memory, columns
     static constexpr int kTq = 0, kTs = kTq + kQTmem * DIM / 2, kTp = kTs + kKeys;
     static constexpr int kTo = kTp + kQ * kKeys / 2;
-    static_assert(kTo + DIM <= 512, "tensor memory");
+    static constexpr int kColumns = 512 / kBlocks;
+    static_assert(kTo + DIM <= kColumns, "tensor memory");
 };
 
 // fp32 accumulate, M = 128, N = n; type 0: fp16, 1: bf16; b_slow: B's columns run fastest
@@ -206,7 +216,7 @@ __device__ bool find_tile(const Args& a, int tq, int at, int* seq, int* t0) {
 }
 
 template <typename T, int DIM>
-__global__ void __launch_bounds__(Cfg<T, DIM>::kThreads, 1)
+__global__ void __launch_bounds__(Cfg<T, DIM>::kThreads, Cfg<T, DIM>::kBlocks)
 paged_runs_kernel(const Args a, const Attend p, int tq) {
     using C = Cfg<T, DIM>;
     constexpr int kKeys = C::kKeys, kParts = C::kParts, kRowWarps = C::kRowWarps;
@@ -231,7 +241,6 @@ paged_runs_kernel(const Args a, const Attend p, int tq) {
     uint32_t* s_odd = tmem_slot + 4;  // [4] rows to be done again
     float* s_max = reinterpret_cast<float*>(smem + C::kMax);
 
-    b2w4_pdl_launch_dependents();
     if (threadIdx.x == 0) {
         mbar_init(q_full, kRowWarps);
         mbar_init(s_full, 1);
@@ -266,7 +275,7 @@ paged_runs_kernel(const Args a, const Attend p, int tq) {
         return;
     if (warp == kMmaWarp) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;"
-                     ::"r"(smem_u32(tmem_slot)), "r"(512)
+                     ::"r"(smem_u32(tmem_slot)), "r"(C::kColumns)
                      : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
@@ -274,6 +283,9 @@ paged_runs_kernel(const Args a, const Attend p, int tq) {
     __syncthreads();
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     const uint32_t tmem = *tmem_slot;
+    // Not before tensor memory is this block's: a block of the next kernel beside it, which may
+    // take tensor memory ahead of its wait for this kernel, would wait for the one that waits.
+    b2w4_pdl_launch_dependents();
     auto fail = [&]() {
         *s_abort = 1;
         b2w4_report_timeout(a.status);
@@ -348,7 +360,7 @@ paged_runs_kernel(const Args a, const Attend p, int tq) {
         if (steps > 0) {
             // Rows come through shared memory, the values' place, which is not filled before: a
             // thread's own loads would be a line each (5000 cycles of the load path).
-            uint8_t* const stage = smem + C::kVs;
+            uint8_t* const stage = smem + C::kStage;
 #pragma unroll
             for (int i = 0; i < 32 / kParts / kRowsAtOnce; ++i) {
                 const int r = stage_row(i);
@@ -549,7 +561,7 @@ paged_runs_kernel(const Args a, const Attend p, int tq) {
             acc[i] = b2w4_pack2(x, y);
         }
         // out through shared memory too: every product that read it has retired
-        uint8_t* const stage = smem + C::kVs;
+        uint8_t* const stage = smem + C::kStage;
 #pragma unroll
         for (int i = 0; i < kOwn / 4; ++i)
             *reinterpret_cast<ulonglong2*>(stage + staged(row, part * (kOwn / 4) + i)) =
@@ -691,8 +703,8 @@ paged_runs_kernel(const Args a, const Attend p, int tq) {
         const int c = lane % kChunks, sub = lane / kChunks;
         uint8_t* const mine = ring + (c >> 3) * C::kPart;
         auto free = [&](int j) {
-            // (the values' place holds the queries at first)
-            const bool ok = j < 2 ? !values || warp_wait(q_full, 0)
+            // (the stage holds the queries at first)
+            const bool ok = j < 2 ? (!values && !C::kStageBoth) || warp_wait(q_full, 0)
                                   : warp_wait(&freed[j & 1], ((j >> 1) - 1) & 1);
             if (!ok)
                 fail();
@@ -741,25 +753,26 @@ paged_runs_kernel(const Args a, const Attend p, int tq) {
                 load(j + 1);
             }
         } else {
-            // the warp's lanes know where four of a block's keys lie each, a block ahead
-            static_assert(C::kWide || (C::kLoadWarps == 1 && kKeys == 128));
-            int next[4], rows[4];
+            // the warp's lanes know where some of a block's keys lie each, a block ahead
+            static_assert(C::kWide || C::kLoadWarps == 1);
+            constexpr int kEach = kKeys / 32;
+            int next[kEach], rows[kEach];
             auto look = [&](int j) {
 #pragma unroll
-                for (int u = 0; u < 4; ++u)
+                for (int u = 0; u < kEach; ++u)
                     next[u] = row_of(j * kKeys + u * 32 + lane);
             };
             look(0);
             for (int j = 0; j < steps && free(j); ++j) {
 #pragma unroll
-                for (int u = 0; u < 4; ++u)
+                for (int u = 0; u < kEach; ++u)
                     rows[u] = next[u];
                 look(j + 1);
                 uint8_t* const to = mine + (j & 1) * C::kBuf;
                 // the rows of eight copies are fetched ahead of them: one by one, every copy
                 // waited for its shuffle (80 cycles each)
 #pragma unroll
-                for (int u = 0; u < 4; ++u)
+                for (int u = 0; u < kEach; ++u)
 #pragma unroll
                     for (int i = 0; i < 32 / kPer; i += 8) {
                         int r[8];
@@ -784,7 +797,7 @@ paged_runs_kernel(const Args a, const Attend p, int tq) {
     if (warp == kMmaWarp) {
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;"
-                     ::"r"(tmem), "r"(512)
+                     ::"r"(tmem), "r"(C::kColumns)
                      : "memory");
     }
     if (warp < kRowWarps && !*s_abort)
