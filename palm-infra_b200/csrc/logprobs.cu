@@ -6,11 +6,17 @@
 // Every thread keeps a running maximum m and sums relative to it, in 32 bits; two such triples
 // join as M = max, S = S1 e^(m1 - M) + S2 e^(m2 - M), T likewise of T_i + (m_i - M) S_i.
 //
-// The k largest: a number below which the k-th largest cannot lie comes from the first tile (the
-// k-th largest of the maxima of 128 groups of its numbers, all different), and what is not below
-// it goes to a list in shared memory, about a hundred numbers of a chunk of 19,000.  The list's
-// first k are found by counting, for each, how many are before it.
+// The k largest: a number below which the k-th largest cannot lie comes from the block's first tile
+// (the k-th largest of the maxima of 64 groups of its numbers), and what is not below it goes to a
+// list of its warp in shared memory, about a hundred numbers of a chunk of 19,000.  The first k of
+// the lists are found by counting, for each, how many are before it.
+//
+// What bounds it: issue slots, about nine instructions for a number that takes four bytes of the
+// card's bandwidth; sums take two numbers an instruction, and a warp looks for numbers above the
+// limit only where a thread's largest of 16 is.
 #include "b200w4_internal.cuh"
+
+#include <math.h>
 
 #include <climits>
 
@@ -22,10 +28,11 @@ constexpr int kThreads = 256, kWarps = kThreads / 32;
 constexpr int kVecs = 4;                    // of four numbers, a thread's share of a tile
 constexpr int kTile = kThreads * kVecs * 4;
 constexpr int kMostTop = 32;
-constexpr int kGroups = kThreads / 2;       // two threads each
+constexpr int kGroups = 64;                 // of four threads each
 constexpr int kTrim = 256;                  // a longer list is cut back to the k largest
-constexpr int kList = kTrim + kTile;
+constexpr int kList = kTrim + 32 * kVecs * 4;
 constexpr int kMostCluster = 8;
+constexpr float kSlack = 8.f;
 
 struct Args {
     const float* x;
@@ -72,45 +79,49 @@ __device__ __forceinline__ Sums join(const Sums& a, const Sums& b) {
     return r;
 }
 
-struct Shared {
-    unsigned long long list[kList];
-    unsigned long long group[kGroups];
-    unsigned long long first[kMostTop];
+struct alignas(16) Shared {
+    unsigned long long flat[kWarps * 2 * kMostTop + 8];
+    unsigned long long list[kWarps][kList];
+    unsigned long long first[kWarps][kMostTop];
     unsigned long long best[kMostCluster][kMostTop];  // of the cluster's blocks, in block 0
     Sums part[kMostCluster];                          // likewise
     Sums warp[kWarps];
-    unsigned long long kth;
-    int count;
+    float group[kGroups];
+    float limit;
+    int count[kWarps];
 };
 
-// Cuts the list to its `top` largest, in order (or to all that there are); whole block.
-__device__ void trim(Shared& s, int top) {
-    __syncthreads();
-    const int n = s.count;
-    for (int i = threadIdx.x; i < n; i += kThreads) {
-        const unsigned long long w = s.list[i];
+// Cuts the warp's list to its `top` largest, in order (or to all that there are); whole warp.
+// Returns the least word that may still be wanted.
+__device__ unsigned long long trim(Shared& s, int warp, int& n, int top) {
+    const int lane = threadIdx.x & 31;
+    unsigned long long *list = s.list[warp], *first = s.first[warp];
+    __syncwarp();
+    for (int i = lane; i < n; i += 32) {
+        const unsigned long long w = list[i];
         int before = 0;
         for (int j = 0; j < n && before < top; ++j)
-            before += s.list[j] > w;
+            before += list[j] > w;
         if (before < top)
-            s.first[before] = w;
+            first[before] = w;
     }
-    __syncthreads();
-    if ((int)threadIdx.x < min(n, top))
-        s.list[threadIdx.x] = s.first[threadIdx.x];
-    if (threadIdx.x == 0) {
-        s.count = min(n, top);
-        s.kth = n >= top ? s.first[top - 1] : 0ull;
-    }
-    __syncthreads();
+    __syncwarp();
+    const int left = min(n, top);
+    if (lane < left)
+        list[lane] = first[lane];
+    const unsigned long long least = n >= top ? first[top - 1] : 0ull;
+    n = left;
+    __syncwarp();
+    return least;
 }
 
 // A cluster per row, a chunk of the row per block.
-__global__ void __launch_bounds__(kThreads)
+__global__ void __launch_bounds__(kThreads, 4)
 logprobs_kernel(const Args a, bool aligned) {
     namespace cg = cooperative_groups;
     b2w4_pdl_chain_entry();
-    __shared__ Shared s;
+    extern __shared__ __align__(16) uint8_t s_dyn[];
+    Shared& s = *reinterpret_cast<Shared*>(s_dyn);
     cg::cluster_group cluster = cg::this_cluster();
     const int blocks = (int)cluster.num_blocks(), block = (int)cluster.block_rank();
     const int row = blockIdx.x / blocks;
@@ -118,29 +129,35 @@ logprobs_kernel(const Args a, bool aligned) {
     const int chunk = ((a.vocab + blocks - 1) / blocks + 3) & ~3;
     const int lo = min(a.vocab, block * chunk), hi = min(a.vocab, lo + chunk);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    if (tid == 0) {
-        s.count = 0;
-        s.kth = 0ull;
-    }
     // number e of the thread's vector u of the tile at `base`
     auto place = [&](int base, int u) { return base + (tid + u * kThreads) * 4; };
     auto load = [&](int base, float4 (&v)[kVecs]) {
+        if (aligned && base + kTile <= hi) {
+#pragma unroll
+            for (int u = 0; u < kVecs; ++u)
+                v[u] = __ldg(reinterpret_cast<const float4*>(x + place(base, u)));
+            return;
+        }
 #pragma unroll
         for (int u = 0; u < kVecs; ++u) {
             const int i = place(base, u);
             if (aligned && i + 4 <= hi) {
-                v[u] = __ldcs(reinterpret_cast<const float4*>(x + i));
+                v[u] = __ldg(reinterpret_cast<const float4*>(x + i));
             } else {
-                v[u].x = i < hi ? __ldcs(x + i) : -INFINITY;
-                v[u].y = i + 1 < hi ? __ldcs(x + i + 1) : -INFINITY;
-                v[u].z = i + 2 < hi ? __ldcs(x + i + 2) : -INFINITY;
-                v[u].w = i + 3 < hi ? __ldcs(x + i + 3) : -INFINITY;
+                v[u].x = i < hi ? __ldg(x + i) : -INFINITY;
+                v[u].y = i + 1 < hi ? __ldg(x + i + 1) : -INFINITY;
+                v[u].z = i + 2 < hi ? __ldg(x + i + 2) : -INFINITY;
+                v[u].w = i + 3 < hi ? __ldg(x + i + 3) : -INFINITY;
             }
         }
     };
-    float m = -INFINITY, sum = 0.f, t = 0.f;
-    unsigned long long kth = 0ull;
-    float limit = -INFINITY;
+    if (tid < kWarps)
+        s.count[tid] = 0;
+    __syncthreads();
+    float m = -INFINITY;
+    uint64_t sum2 = 0ull, t2 = 0ull;  // two sums each
+    float limit = -INFINITY;  // what is below it is not among the largest
+    int n = 0;  // of the warp's list; the same in all lanes
     float4 next[kVecs];
     load(lo, next);
     for (int base = lo; base < hi; base += kTile) {
@@ -153,79 +170,95 @@ logprobs_kernel(const Args a, bool aligned) {
             v[4 * u + 3] = next[u].w;
         }
         load(base + kTile, next);
-        float top = m;
+        float top = v[0];
 #pragma unroll
-        for (int i = 0; i < kVecs * 4; ++i)
+        for (int i = 1; i < kVecs * 4; ++i)
             top = fmaxf(top, v[i]);
-        if (top > m) {
+        // Not for every larger number: what is summed may be e^kSlack times as large as the largest
+        // would make it, and the sums are scaled again a few times instead of nearly every tile.
+        if (top > m + kSlack) {
             if (m > -INFINITY) {
                 const float d = __fsub_rn(m, top), e = expf(d);
+                float s0, s1, t0, t1;
+                b2w4_unpack2(sum2, s0, s1);
+                b2w4_unpack2(t2, t0, t1);
                 // (below, d may be -inf where top is)
-                t = e == 0.f ? 0.f : __fmul_rn(__fmaf_rn(sum, d, t), e);
-                sum = __fmul_rn(sum, e);
+                t2 = e == 0.f ? 0ull : b2w4_pack2(__fmul_rn(__fmaf_rn(s0, d, t0), e),
+                                                  __fmul_rn(__fmaf_rn(s1, d, t1), e));
+                sum2 = b2w4_pack2(__fmul_rn(s0, e), __fmul_rn(s1, e));
             }
             m = top;
         }
         const float from = m == -INFINITY ? 0.f : m;
+        const uint64_t from2 = b2w4_pack2(from, from);
+        const uint64_t log2e = b2w4_pack2(1.4426950408889634f, 1.4426950408889634f);
 #pragma unroll
-        for (int i = 0; i < kVecs * 4; ++i) {
-            const float d = __fsub_rn(v[i], from);
-            float e;
-            asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(__fmul_rn(d, 1.4426950408889634f)));
-            sum = __fadd_rn(sum, e);
-            t = __fmaf_rn(e, fmaxf(d, -200.f), t);  // e = 0 where d = -inf
+        for (int i = 0; i < kVecs * 4; i += 2) {
+            const uint64_t d = b2w4_sub2(b2w4_pack2(v[i], v[i + 1]), from2);
+            float d0, d1, z0, z1, e0, e1;
+            b2w4_unpack2(d, d0, d1);
+            b2w4_unpack2(b2w4_mul2(d, log2e), z0, z1);
+            asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e0) : "f"(z0));
+            asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e1) : "f"(z1));
+            const uint64_t e = b2w4_pack2(e0, e1);
+            asm("add.rn.f32x2 %0, %0, %1;" : "+l"(sum2) : "l"(e));
+            // e = 0 where d = -inf
+            t2 = b2w4_fma2(e, b2w4_pack2(fmaxf(d0, -200.f), fmaxf(d1, -200.f)), t2);
         }
         if (a.top > 0) {
-            if (base == lo) {
-                unsigned long long w = 0ull;
-#pragma unroll
-                for (int i = 0; i < kVecs * 4; ++i) {
-                    const int at = place(base, i / 4) + i % 4;
-                    if (at < hi)
-                        w = max(w, word(v[i], at));
-                }
-                w = max(w, __shfl_xor_sync(0xffffffffu, w, 1));
-                if (!(tid & 1))
-                    s.group[tid >> 1] = w;
+            if (base == lo) {  // the whole block, if any of it is here
+                float g = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+                g = fmaxf(g, __shfl_xor_sync(0xffffffffu, g, 2));
+                if (!(tid & 3))
+                    s.group[tid >> 2] = g;
+                if (tid == 0)
+                    s.limit = -INFINITY;
                 __syncthreads();
                 if (tid < kGroups) {
-                    w = s.group[tid];
-                    int before = 0;
-                    for (int j = 0; j < kGroups; ++j)
-                        before += s.group[j] > w;
-                    if (before == a.top - 1 && w)
-                        s.kth = w;
+                    const float mine = s.group[tid];
+                    int above = 0, level = 0;
+#pragma unroll 8
+                    for (int j = 0; j < kGroups; ++j) {
+                        above += s.group[j] > mine;
+                        level += s.group[j] >= mine;
+                    }
+                    if (above < a.top && a.top <= level)
+                        s.limit = mine;  // the same number from every thread that writes
                 }
                 __syncthreads();
-                kth = s.kth;
-                limit = floor_of(kth);
+                limit = s.limit;
             }
-            bool some = false;
+            // a NaN is wanted only while there is no limit
+            if (top >= limit || limit == -INFINITY) {
+                unsigned mine = 0;
 #pragma unroll
-            for (int i = 0; i < kVecs * 4; ++i)
-                some |= !(v[i] < limit);
-            bool over = false;
-            if (some) {
-#pragma unroll
-                for (int i = 0; i < kVecs * 4; ++i) {
-                    const int at = place(base, i / 4) + i % 4;
-                    if (!(v[i] < limit) && at < hi) {
-                        const unsigned long long w = word(v[i], at);
-                        if (w >= kth) {
-                            const int n = atomicAdd(&s.count, 1);
-                            s.list[n] = w;
-                            over |= n >= kTrim;
-                        }
-                    }
+                for (int i = 0; i < kVecs * 4; ++i)
+                    mine |= (unsigned)!(v[i] < limit) << i;
+                // the number from memory again: one or two, where the registers would want a look
+                // at each of the 16
+                for (; mine; mine &= mine - 1) {
+                    const int i = __ffs(mine) - 1;
+                    const int at = place(base, i >> 2) + (i & 3);
+                    if (at < hi)
+                        s.list[warp][atomicAdd(&s.count[warp], 1)] = word(__ldg(x + at), at);
                 }
             }
-            if (__syncthreads_or(over)) {
-                trim(s, a.top);
-                kth = s.kth;
-                limit = floor_of(kth);
+            __syncwarp();
+            n = s.count[warp];
+            __syncwarp();
+            if (n > kTrim) {
+                limit = fmaxf(limit, floor_of(trim(s, warp, n, a.top)));
+                if (lane == 0)
+                    s.count[warp] = n;
+                __syncwarp();
             }
         }
     }
+    float sum, t, sum_odd, t_odd;
+    b2w4_unpack2(sum2, sum, sum_odd);
+    b2w4_unpack2(t2, t, t_odd);
+    sum = __fadd_rn(sum, sum_odd);
+    t = __fadd_rn(t, t_odd);
     // the block's sums, in a fixed order
     Sums mine = {m, sum, t};
 #pragma unroll
@@ -238,8 +271,43 @@ logprobs_kernel(const Args a, bool aligned) {
     }
     if (lane == 0)
         s.warp[warp] = mine;
-    trim(s, max(a.top, 1));
+    __syncthreads();
     Shared* out = cluster.map_shared_rank(&s, 0);
+    // The first of all lists: long ones are cut first, then all lie one behind the other.
+    if (a.top > 0) {
+        if (n > 2 * kMostTop) {
+            trim(s, warp, n, a.top);
+            if (lane == 0)
+                s.count[warp] = n;
+        }
+        __syncthreads();
+        int all = 0, mine = 0;
+#pragma unroll
+        for (int k = 0; k < kWarps; ++k) {
+            mine += k < warp ? s.count[k] : 0;
+            all += s.count[k];
+        }
+        for (int i = lane; i < n; i += 32)
+            s.flat[mine + i] = s.list[warp][i];
+        if (tid < 8)
+            s.flat[all + tid] = 0ull;
+        if (tid < a.top)
+            s.first[0][tid] = 0ull;
+        __syncthreads();
+        for (int i = tid; i < all; i += kThreads) {
+            const unsigned long long w = s.flat[i];
+            int before = 0;
+            for (int j = 0; j < all; j += 8)
+#pragma unroll
+                for (int e = 0; e < 8; e += 2) {
+                    const ulonglong2 o = *reinterpret_cast<const ulonglong2*>(s.flat + j + e);
+                    before += (o.x > w) + (o.y > w);
+                }
+            if (before < a.top)
+                s.first[0][before] = w;
+        }
+    }
+    __syncthreads();
     if (tid == 0) {
         Sums all = s.warp[0];
         for (int w = 1; w < kWarps; ++w)
@@ -247,7 +315,7 @@ logprobs_kernel(const Args a, bool aligned) {
         out->part[block] = all;
     }
     if (tid < a.top)
-        out->best[block][tid] = tid < s.count ? s.list[tid] : 0ull;
+        out->best[block][tid] = s.first[0][tid];
     cluster.sync();
     if (block != 0)
         return;
@@ -289,12 +357,23 @@ logprobs_kernel(const Args a, bool aligned) {
     }
 }
 
-// Blocks that share a row.
-int cluster_for(int vocab) {
-    int blocks = kMostCluster;
-    while (blocks > 1 && vocab < blocks * 2 * kTile)
-        blocks /= 2;
-    return blocks;
+// Blocks that share a row: as many as make the shortest run of waves, a block's own work being
+// about that of kFixed numbers (a limit, lists, the join).
+constexpr int kFixed = 6000;
+int cluster_for(int rows, int vocab, int resident) {
+    int best = 1;
+    double least = 0;
+    for (int blocks = 1; blocks <= kMostCluster; blocks *= 2) {
+        if (blocks > 1 && vocab < blocks * kTile)
+            break;
+        const double waves = ceil((double)rows * blocks / resident);
+        const double time = waves * (vocab / blocks + kFixed);
+        if (blocks == 1 || time < least) {
+            best = blocks;
+            least = time;
+        }
+    }
+    return best;
 }
 
 }  // namespace
@@ -322,10 +401,12 @@ extern "C" int b2w4_logprobs(b2w4_ctx* ctx, const float* logits_dev, int ld, int
                     top_values_dev, top_indices_dev, ld,          rows,
                     vocab,          top,             ctx->status_dev};
     const bool aligned = !((reinterpret_cast<uintptr_t>(logits_dev) & 15) || (ld & 3));
-    const int blocks = cluster_for(vocab);
+    static b2w4_smem_optin cfg;
+    B2W4_CUDA(ctx, b2w4_opt_in_smem(ctx, logprobs_kernel, sizeof(Shared), cfg));
+    const int blocks = cluster_for(rows, vocab, 4 * ctx->sm_count);
     B2W4_CUDA(ctx, b2w4_launch_chained_cluster(ctx->pdl, logprobs_kernel,
                                                dim3((unsigned)rows * blocks), dim3(kThreads),
-                                               blocks, 0, ctx->stream, a, aligned));
+                                               blocks, sizeof(Shared), ctx->stream, a, aligned));
     ctx->launches++;
     return B2W4_OK;
 }
