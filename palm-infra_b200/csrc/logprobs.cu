@@ -8,8 +8,9 @@
 //
 // The k largest: a number below which the k-th largest cannot lie comes from the block's first tile
 // (the k-th largest of the maxima of 64 groups of its numbers), and what is not below it goes to a
-// list of its warp in shared memory, about a hundred numbers of a chunk of 19,000.  The first k of
-// the lists are found by counting, for each, how many are before it.
+// list of its warp in shared memory.  After two tiles, four, eight, .. of a long chunk the lists are cut
+// back to the k largest so far, by counting for each entry how many are before it, and the k-th is the new
+// limit: about k numbers come between one time and the next.
 //
 // What bounds it: issue slots, about nine instructions for a number that takes four bytes of the
 // card's bandwidth; sums take two numbers an instruction, and a warp looks for numbers above the
@@ -29,7 +30,7 @@ constexpr int kVecs = 4;                    // of four numbers, a thread's share
 constexpr int kTile = kThreads * kVecs * 4;
 constexpr int kMostTop = 32;
 constexpr int kGroups = 64;                 // of four threads each
-constexpr int kTrim = 256;                  // a longer list is cut back to the k largest
+constexpr int kTrim = 64;                   // a longer list is cut back to the k largest
 constexpr int kList = kTrim + 32 * kVecs * 4;
 constexpr int kMostCluster = 8;
 constexpr float kSlack = 8.f;
@@ -65,22 +66,9 @@ __device__ __forceinline__ float floor_of(unsigned long long w) {
 struct Sums {
     float m, s, t;
 };
-__device__ __forceinline__ Sums join(const Sums& a, const Sums& b) {
-    const float m = fmaxf(a.m, b.m), base = m == -INFINITY ? 0.f : m;
-    const float da = fmaxf(__fsub_rn(a.m, base), -1e30f), db = fmaxf(__fsub_rn(b.m, base), -1e30f);
-    const float ea = expf(da), eb = expf(db);
-    Sums r;
-    r.m = m;
-    r.s = __fmaf_rn(a.s, ea, __fmul_rn(b.s, eb));
-    // a side without numbers, or without any that count, has s = 0 and t = 0
-    const float ta = ea == 0.f ? __fmul_rn(a.s, 0.f) : __fmul_rn(__fmaf_rn(a.s, da, a.t), ea);
-    const float tb = eb == 0.f ? __fmul_rn(b.s, 0.f) : __fmul_rn(__fmaf_rn(b.s, db, b.t), eb);
-    r.t = __fadd_rn(ta, tb);
-    return r;
-}
-
 struct alignas(16) Shared {
-    unsigned long long flat[kWarps * 2 * kMostTop + 8];
+    unsigned long long flat[kWarps * kTrim + kMostTop + 8];
+    unsigned long long kept[kMostTop];  // the largest so far, in order; 0: there are not so many
     unsigned long long list[kWarps][kList];
     unsigned long long first[kWarps][kMostTop];
     unsigned long long best[kMostCluster][kMostTop];  // of the cluster's blocks, in block 0
@@ -113,6 +101,65 @@ __device__ unsigned long long trim(Shared& s, int warp, int& n, int top) {
     n = left;
     __syncwarp();
     return least;
+}
+
+// The lists and what was kept before, cut to the `top` largest in s.kept; the lists are empty then.
+// Whole block.
+__device__ void settle(Shared& s, int warp, int& n, int top) {
+    const int tid = threadIdx.x, lane = tid & 31;
+    if (lane == 0)
+        s.count[warp] = n;
+    __syncthreads();
+    int all = 0, mine = 0;
+#pragma unroll
+    for (int k = 0; k < kWarps; ++k) {
+        mine += k < warp ? s.count[k] : 0;
+        all += s.count[k];
+    }
+    for (int i = lane; i < n; i += 32)
+        s.flat[mine + i] = s.list[warp][i];
+    if (tid < top)
+        s.flat[all + tid] = s.kept[tid];
+    all += top;
+    if (tid < 8)
+        s.flat[all + tid] = 0ull;
+    __syncthreads();
+    if (tid < top)
+        s.kept[tid] = 0ull;
+    if (lane == 0)
+        s.count[warp] = 0;
+    n = 0;
+    __syncthreads();
+    for (int i = tid; i < all; i += kThreads) {
+        const unsigned long long w = s.flat[i];
+        int before = 0;
+        for (int j = 0; j < all; j += 8)
+#pragma unroll
+            for (int e = 0; e < 8; e += 2) {
+                const ulonglong2 o = *reinterpret_cast<const ulonglong2*>(s.flat + j + e);
+                before += (o.x > w) + (o.y > w);
+            }
+        if (before < top && w)
+            s.kept[before] = w;
+    }
+    __syncthreads();
+}
+
+// The lanes' sums as one, in all lanes: n lanes, a power of two, next to each other.
+__device__ __forceinline__ Sums join_lanes(Sums v, int n) {
+    float m = v.m;
+    for (int off = n / 2; off > 0; off >>= 1)
+        m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, off));
+    const float base = m == -INFINITY ? 0.f : m;
+    const float d = fmaxf(__fsub_rn(v.m, base), -1e30f), e = expf(d);
+    // a side without numbers, or without any that count, has s = 0 and t = 0
+    float t = e == 0.f ? __fmul_rn(v.s, 0.f) : __fmul_rn(__fmaf_rn(v.s, d, v.t), e);
+    float sum = __fmul_rn(v.s, e);
+    for (int off = n / 2; off > 0; off >>= 1) {
+        sum = __fadd_rn(sum, __shfl_xor_sync(0xffffffffu, sum, off));
+        t = __fadd_rn(t, __shfl_xor_sync(0xffffffffu, t, off));
+    }
+    return {m, sum, t};
 }
 
 // A cluster per row, a chunk of the row per block.
@@ -153,6 +200,8 @@ logprobs_kernel(const Args a, bool aligned) {
     };
     if (tid < kWarps)
         s.count[tid] = 0;
+    if (tid < kMostTop)
+        s.kept[tid] = 0ull;
     __syncthreads();
     float m = -INFINITY;
     uint64_t sum2 = 0ull, t2 = 0ull;  // two sums each
@@ -160,6 +209,7 @@ logprobs_kernel(const Args a, bool aligned) {
     int n = 0;  // of the warp's list; the same in all lanes
     float4 next[kVecs];
     load(lo, next);
+    int tile = 0;
     for (int base = lo; base < hi; base += kTile) {
         float v[kVecs * 4];
 #pragma unroll
@@ -252,6 +302,12 @@ logprobs_kernel(const Args a, bool aligned) {
                     s.count[warp] = n;
                 __syncwarp();
             }
+            ++tile;
+            // (worth its barriers where as much again and more is to come)
+            if (tile > 1 && !(tile & (tile - 1)) && hi - base > 2 * tile * kTile) {
+                settle(s, warp, n, a.top);
+                limit = fmaxf(limit, floor_of(s.kept[a.top - 1]));
+            }
         }
     }
     float sum, t, sum_odd, t_odd;
@@ -260,68 +316,25 @@ logprobs_kernel(const Args a, bool aligned) {
     sum = __fadd_rn(sum, sum_odd);
     t = __fadd_rn(t, t_odd);
     // the block's sums, in a fixed order
-    Sums mine = {m, sum, t};
-#pragma unroll
-    for (int off = 1; off < 32; off <<= 1) {
-        Sums o;
-        o.m = __shfl_xor_sync(0xffffffffu, mine.m, off);
-        o.s = __shfl_xor_sync(0xffffffffu, mine.s, off);
-        o.t = __shfl_xor_sync(0xffffffffu, mine.t, off);
-        mine = lane & off ? join(o, mine) : join(mine, o);
-    }
+    const Sums mine = join_lanes({m, sum, t}, 32);
     if (lane == 0)
         s.warp[warp] = mine;
-    __syncthreads();
+    if (a.top > 0)
+        settle(s, warp, n, a.top);
+    else
+        __syncthreads();
     Shared* out = cluster.map_shared_rank(&s, 0);
-    // The first of all lists: long ones are cut first, then all lie one behind the other.
-    if (a.top > 0) {
-        if (n > 2 * kMostTop) {
-            trim(s, warp, n, a.top);
-            if (lane == 0)
-                s.count[warp] = n;
-        }
-        __syncthreads();
-        int all = 0, mine = 0;
-#pragma unroll
-        for (int k = 0; k < kWarps; ++k) {
-            mine += k < warp ? s.count[k] : 0;
-            all += s.count[k];
-        }
-        for (int i = lane; i < n; i += 32)
-            s.flat[mine + i] = s.list[warp][i];
-        if (tid < 8)
-            s.flat[all + tid] = 0ull;
-        if (tid < a.top)
-            s.first[0][tid] = 0ull;
-        __syncthreads();
-        for (int i = tid; i < all; i += kThreads) {
-            const unsigned long long w = s.flat[i];
-            int before = 0;
-            for (int j = 0; j < all; j += 8)
-#pragma unroll
-                for (int e = 0; e < 8; e += 2) {
-                    const ulonglong2 o = *reinterpret_cast<const ulonglong2*>(s.flat + j + e);
-                    before += (o.x > w) + (o.y > w);
-                }
-            if (before < a.top)
-                s.first[0][before] = w;
-        }
-    }
-    __syncthreads();
-    if (tid == 0) {
-        Sums all = s.warp[0];
-        for (int w = 1; w < kWarps; ++w)
-            all = join(all, s.warp[w]);
-        out->part[block] = all;
+    if (warp == 0) {
+        const Sums all = join_lanes(s.warp[lane % kWarps], kWarps);
+        if (lane == 0)
+            out->part[block] = all;
     }
     if (tid < a.top)
-        out->best[block][tid] = s.first[0][tid];
+        out->best[block][tid] = s.kept[tid];
     cluster.sync();
     if (block != 0)
         return;
-    Sums all = s.part[0];
-    for (int b = 1; b < blocks; ++b)
-        all = join(all, s.part[b]);
+    const Sums all = join_lanes(s.part[lane % blocks], blocks);
     const float log_s = logf(all.s);
     auto answer = [&](float v) { return __fsub_rn(__fsub_rn(v, all.m), log_s); };
     if (tid == 0) {
@@ -357,17 +370,19 @@ logprobs_kernel(const Args a, bool aligned) {
     }
 }
 
-// Blocks that share a row: as many as make the shortest run of waves, a block's own work being
-// about that of kFixed numbers (a limit, lists, the join).
-constexpr int kFixed = 6000;
-int cluster_for(int rows, int vocab, int resident) {
+// Blocks that share a row.  A block's work is its numbers and a share of its own, about that of
+// kFixed numbers (a limit, lists, the join); a multiprocessor's blocks are done side by side as fast
+// as one up to kBeside of them, from where on they share it.
+constexpr int kFixed = 8000;
+constexpr double kBeside = 3.5;
+int cluster_for(int rows, int vocab, int sm_count) {
     int best = 1;
     double least = 0;
     for (int blocks = 1; blocks <= kMostCluster; blocks *= 2) {
         if (blocks > 1 && vocab < blocks * kTile)
             break;
-        const double waves = ceil((double)rows * blocks / resident);
-        const double time = waves * (vocab / blocks + kFixed);
+        const double each = ceil((double)rows * blocks / sm_count) / kBeside;
+        const double time = (each > 1 ? each : 1) * (vocab / blocks + kFixed);
         if (blocks == 1 || time < least) {
             best = blocks;
             least = time;
@@ -403,7 +418,7 @@ extern "C" int b2w4_logprobs(b2w4_ctx* ctx, const float* logits_dev, int ld, int
     const bool aligned = !((reinterpret_cast<uintptr_t>(logits_dev) & 15) || (ld & 3));
     static b2w4_smem_optin cfg;
     B2W4_CUDA(ctx, b2w4_opt_in_smem(ctx, logprobs_kernel, sizeof(Shared), cfg));
-    const int blocks = cluster_for(rows, vocab, 4 * ctx->sm_count);
+    const int blocks = cluster_for(rows, vocab, ctx->sm_count);
     B2W4_CUDA(ctx, b2w4_launch_chained_cluster(ctx->pdl, logprobs_kernel,
                                                dim3((unsigned)rows * blocks), dim3(kThreads),
                                                blocks, sizeof(Shared), ctx->stream, a, aligned));
