@@ -33,7 +33,6 @@ using paged::Attend;
 using paged::Sequence;
 
 constexpr int kKeys = 16;  // of a block
-constexpr int kSet = 16;   // heads of a set: rows of the products
 
 template <typename T>
 struct Pieces {  // of a query or probability, and of a key or value
@@ -48,15 +47,26 @@ struct Pieces<float> {
     static constexpr int kQ = 3, kK = 3;
 };
 
-template <typename T, int DIM>
+// Operands of a product's rows.  SET 16: a row for each of 16 heads, an operand for each piece.  SET
+// 8: eight heads, their first pieces in rows 0 to 7 and their second ones in rows 8 to 15 of one
+// operand, their third ones, if any, in a second: two thirds or half of the products, and of the
+// registers, for groups of up to eight heads; a score is the sum of two rows.
+template <typename T, int SET>
+constexpr int kOperands = SET == 16 ? Pieces<T>::kQ : Pieces<T>::kQ - 1;
+
+template <typename T, int DIM, int SET>
 struct Ring {
     static constexpr int kRow = DIM * sizeof(T);       // bytes
     static constexpr int kHalf = kKeys * kRow;          // keys; the values behind them
     static constexpr int kSlot = 2 * kHalf;
-    static constexpr int kSlots = kSlot > 8192 ? 2 : kSlot > 4096 ? 3 : 5;
-    static constexpr int kWarps = kSlot > 8192 ? 7 : 8;
+    static constexpr int kWarps = kSlot > 8192 ? 7 : SET == 16 ? 8 : kSlot > 4096 ? 12 : 16;
+    static constexpr int kSlots = 208 * 1024 / (kWarps * kSlot) < 2
+                                      ? 2
+                                      : 208 * 1024 / (kWarps * kSlot) > 5
+                                            ? 5
+                                            : 208 * 1024 / (kWarps * kSlot);
     static constexpr int kBytes = kWarps * kSlots * kSlot;
-    static_assert(kWarps <= 8, "the work area");
+    static_assert(kBytes <= 227 * 1024 && kWarps <= 16, "shared memory, the work area");
 };
 
 // The line of blocks: how many a warp takes, and where sequences begin in it.
@@ -122,10 +132,10 @@ __device__ int find(const Args& a, const paged::Window& w, int tiles, int at, in
     return a.sequences;
 }
 
-// A part: m and l of its 16 rows, then their outputs.
-template <int DIM>
+// A part: m and l of its SET rows, then their outputs.
+template <int DIM, int SET>
 struct Part {
-    static constexpr int kFloats = 2 * kSet + kSet * DIM;
+    static constexpr int kFloats = 2 * SET + SET * DIM;
 };
 // Whose part it is: the tile's sequence, its heads, and the warps that have parts of it, the
 // first's in its second place if `second`.  count 0: no part.
@@ -133,10 +143,9 @@ struct Owner {
     int seq, head0, count, w0, w1, second, pad[2];
 };
 // The work area: two parts of every warp, and their owners.
-constexpr int kMostWarps = 8;
-template <int DIM>
+template <int DIM, int SET>
 __host__ __device__ size_t owners_at(int warps) {
-    return sizeof(float) * 2 * Part<DIM>::kFloats * (size_t)warps;
+    return sizeof(float) * 2 * Part<DIM, SET>::kFloats * (size_t)warps;
 }
 
 __device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool there) {
@@ -202,20 +211,50 @@ __device__ __forceinline__ float exp2_neg(float x) {
     return r;
 }
 
-constexpr float kHalfScale = 1024.f;  // of probabilities beside an fp16 cache
+// 2^kLift times a row's probabilities are what is taken apart and summed: beside an fp16 cache
+// that keeps the small ones' pieces normal numbers.
+template <typename T>
+constexpr float kLift = std::is_same_v<T, __half> ? 10.f : 0.f;
 
-template <typename T, int DIM>
-__global__ void __launch_bounds__(Ring<T, DIM>::kWarps * 32, 1)
+// Pieces of a row's column pairs (2t and 2t + 8, of rows r and r + 8) as operands: at(i, e) is
+// register e of operand i.
+template <int Q, int N, typename At>
+__device__ __forceinline__ void operands(const uint32_t (&piece)[Q][N], At at) {
+    if constexpr (N == 4) {
+#pragma unroll
+        for (int i = 0; i < Q; ++i) {
+            at(i, 0) = piece[i][0];
+            at(i, 1) = piece[i][2];
+            at(i, 2) = piece[i][1];
+            at(i, 3) = piece[i][3];
+        }
+    } else {
+        at(0, 0) = piece[0][0];
+        at(0, 1) = piece[1][0];
+        at(0, 2) = piece[0][1];
+        at(0, 3) = piece[1][1];
+        if constexpr (Q == 3) {
+            at(1, 0) = piece[2][0];
+            at(1, 1) = 0u;
+            at(1, 2) = piece[2][1];
+            at(1, 3) = 0u;
+        }
+    }
+}
+template <typename T, int DIM, int SET>
+__global__ void __launch_bounds__(Ring<T, DIM, SET>::kWarps * 32, 1)
 paged_split_kernel(const Args a, const Attend p, float* __restrict__ parts,
                    Owner* __restrict__ owners) {
-    using R = Ring<T, DIM>;
+    using R = Ring<T, DIM, SET>;
     constexpr int kQ = Pieces<T>::kQ, kK = Pieces<T>::kK, kSteps = DIM / 16, kTiles = DIM / 8;
+    constexpr int kHalves = SET / 8;  // of a product's rows, heads
+    constexpr int kA = kOperands<T, SET>;
     constexpr bool kWide = sizeof(T) == 4;  // an fp32 cache
     extern __shared__ __align__(1024) uint8_t smem[];
     b2w4_pdl_chain_entry();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int r = lane >> 2, t = lane & 3;  // row of the products' operands, column pair
-    const int group = p.heads / a.kv_heads, sets = (group + kSet - 1) / kSet;
+    const int group = p.heads / a.kv_heads, sets = (group + SET - 1) / SET;
     const int tiles = a.kv_heads * sets;
     const int warps = gridDim.x * R::kWarps;
     const int me = warp * gridDim.x + blockIdx.x;  // few shares: a multiprocessor each
@@ -251,19 +290,19 @@ paged_split_kernel(const Args a, const Attend p, float* __restrict__ parts,
         // the tile, and the share's blocks of it
         const int tile = (at - begin) / blocks;
         const int b0 = at - begin - tile * blocks, b1 = min(blocks, b0 + end - at);
-        const int kvh = tile / sets, head0 = kvh * group + (tile - kvh * sets) * kSet;
-        const int heads = min(kSet, (kvh + 1) * group - head0);
+        const int kvh = tile / sets, head0 = kvh * group + (tile - kvh * sets) * SET;
+        const int heads = min(SET, (kvh + 1) * group - head0);
 
         // ---- the heads' queries as operands ------------------------------------------
-        uint32_t q[kQ][kSteps][4];
-        float unscale[2] = {1.f, 1.f};
+        uint32_t q[kA][kSteps][4];
+        float unscale[kHalves];
         {
             const float* row = p.q + (size_t)s.first * p.ldq + (size_t)head0 * DIM;
-            float x[kSteps][8];
+            float x[kSteps][4 * kHalves];
 #pragma unroll
             for (int k = 0; k < kSteps; ++k)
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {
+                for (int h = 0; h < kHalves; ++h) {
                     const bool in = r + 8 * h < heads;
                     const float* src = row + (r + 8 * h) * DIM + 16 * k;
                     if (kWide) {  // column pairs 2t and 2t + 8 hold features 4t .. 4t + 3
@@ -283,9 +322,10 @@ paged_split_kernel(const Args a, const Attend p, float* __restrict__ parts,
                         x[k][4 * h + 3] = w.y;
                     }
                 }
-            if constexpr (std::is_same_v<T, __half>) {  // the row's largest to [2^10, 2^11)
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {
+            for (int h = 0; h < kHalves; ++h) {
+                unscale[h] = 1.f;
+                if constexpr (std::is_same_v<T, __half>) {  // the row's largest to [2^10, 2^11)
                     float top = 0.f;
 #pragma unroll
                     for (int k = 0; k < kSteps; ++k)
@@ -306,14 +346,15 @@ paged_split_kernel(const Args a, const Attend p, float* __restrict__ parts,
                 }
             }
 #pragma unroll
-            for (int i = 0; i < kQ; ++i)
+            for (int k = 0; k < kSteps; ++k) {
+                uint32_t piece[kQ][2 * kHalves];
 #pragma unroll
-                for (int k = 0; k < kSteps; ++k) {
-                    q[i][k][0] = take_piece<T>(x[k][0], x[k][1]);
-                    q[i][k][1] = take_piece<T>(x[k][4], x[k][5]);
-                    q[i][k][2] = take_piece<T>(x[k][2], x[k][3]);
-                    q[i][k][3] = take_piece<T>(x[k][6], x[k][7]);
-                }
+                for (int i = 0; i < kQ; ++i)
+#pragma unroll
+                    for (int e = 0; e < 2 * kHalves; ++e)
+                        piece[i][e] = take_piece<T>(x[k][2 * e], x[k][2 * e + 1]);
+                operands(piece, [&](int i, int e) -> uint32_t& { return q[i][k][e]; });
+            }
         }
 
         // ---- the stream of blocks ----------------------------------------------------
@@ -358,20 +399,24 @@ paged_split_kernel(const Args a, const Attend p, float* __restrict__ parts,
             there[i] = fetch(i, row_of(b0 + i));
         int next_row = row_of(b0 + R::kSlots - 1);
 
-        float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
-        float o[kTiles][4];
+        float m[kHalves], l[kHalves], factor[kHalves];
+#pragma unroll
+        for (int h = 0; h < kHalves; ++h) {
+            m[h] = -INFINITY;
+            l[h] = 0.f;
+            factor[h] = __fmul_rn(__fmul_rn(p.scale, 1.4426950408889634f), unscale[h]);
+        }
+        float o[kTiles][2 * kHalves];
 #pragma unroll
         for (int i = 0; i < kTiles; ++i)
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
+            for (int e = 0; e < 2 * kHalves; ++e)
                 o[i][e] = 0.f;
-        const float factor[2] = {__fmul_rn(__fmul_rn(p.scale, 1.4426950408889634f), unscale[0]),
-                                 __fmul_rn(__fmul_rn(p.scale, 1.4426950408889634f), unscale[1])};
 
         auto block = [&](int slot, unsigned keys) {
             const uint32_t ks = ring + slot * R::kSlot, vs = ks + R::kHalf;
-            // a sum for each size of products: six chains instead of two
-            float by[kQ][2][4] = {};
+            // sums of their own for products of different sizes: more chains side by side
+            float by[kA][2][4] = {};
 #pragma unroll
             for (int k = 0; k < kSteps; ++k) {
                 if constexpr (kWide) {
@@ -385,12 +430,19 @@ paged_split_kernel(const Args a, const Attend p, float* __restrict__ parts,
                             b[i][0] = take_piece<T>(v[0], v[1]);
                             b[i][1] = take_piece<T>(v[2], v[3]);
                         }
-                        mma<T>(by[2][n], q[2][k], b[0][0], b[0][1]);
-                        mma<T>(by[1][n], q[1][k], b[0][0], b[0][1]);
-                        mma<T>(by[0][n], q[0][k], b[0][0], b[0][1]);
-                        mma<T>(by[2][n], q[1][k], b[1][0], b[1][1]);
-                        mma<T>(by[1][n], q[0][k], b[1][0], b[1][1]);
-                        mma<T>(by[2][n], q[0][k], b[2][0], b[2][1]);
+                        if constexpr (SET == 16) {
+                            mma<T>(by[2][n], q[2][k], b[0][0], b[0][1]);
+                            mma<T>(by[1][n], q[1][k], b[0][0], b[0][1]);
+                            mma<T>(by[0][n], q[0][k], b[0][0], b[0][1]);
+                            mma<T>(by[2][n], q[1][k], b[1][0], b[1][1]);
+                            mma<T>(by[1][n], q[0][k], b[1][0], b[1][1]);
+                            mma<T>(by[2][n], q[0][k], b[2][0], b[2][1]);
+                        } else {
+                            mma<T>(by[1][n], q[1][k], b[0][0], b[0][1]);
+                            mma<T>(by[0][n], q[0][k], b[2][0], b[2][1]);
+                            mma<T>(by[0][n], q[0][k], b[1][0], b[1][1]);
+                            mma<T>(by[0][n], q[0][k], b[0][0], b[0][1]);
+                        }
                     }
                 } else {
                     // matrices: keys 0-7 and 8-15, features 0-7 and 8-15 of the step
@@ -398,64 +450,70 @@ paged_split_kernel(const Args a, const Attend p, float* __restrict__ parts,
                     ldmatrix(b, ks + swizzled((lane & 7) + (lane >> 4) * 8,
                                               2 * k + ((lane >> 3) & 1), false));
 #pragma unroll
-                    for (int i = kQ - 1; i >= 0; --i) {
+                    for (int i = kA - 1; i >= 0; --i) {
                         mma<T>(by[i][0], q[i][k], b[0], b[1]);
                         mma<T>(by[i][1], q[i][k], b[2], b[3]);
                     }
                 }
             }
-            float alpha[2], pr[2][4], sc[2][4];
+            float alpha[kHalves], pr[kHalves][4];  // of keys 2t, 2t + 1 and those behind 8
 #pragma unroll
-            for (int n = 0; n < 2; ++n)
+            for (int h = 0; h < kHalves; ++h) {
+                float sc[4], top = m[h];
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    sc[n][e] = by[kQ - 1][n][e];
+                    const int n = e >> 1, c = e & 1;
+                    if constexpr (SET == 16) {
+                        sc[e] = by[kA - 1][n][2 * h + c];
 #pragma unroll
-                    for (int i = kQ - 2; i >= 0; --i)
-                        sc[n][e] = __fadd_rn(sc[n][e], by[i][n][e]);
-                }
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                float top = m[h];
-#pragma unroll
-                for (int n = 0; n < 2; ++n)
-#pragma unroll
-                    for (int e = 0; e < 2; ++e) {
-                        float& x = sc[n][2 * h + e];
-                        x = __fmul_rn(x, factor[h]);
-                        if (!(keys >> (8 * n + 2 * t + e) & 1))
-                            x = -INFINITY;
-                        top = fmaxf(top, x);
+                        for (int i = kA - 2; i >= 0; --i)
+                            sc[e] = __fadd_rn(sc[e], by[i][n][2 * h + c]);
+                    } else {
+                        sc[e] = by[0][n][2 + c];
+                        if (kA > 1)
+                            sc[e] = __fadd_rn(by[kA - 1][n][c], sc[e]);
+                        sc[e] = __fadd_rn(sc[e], by[0][n][c]);
                     }
+                    sc[e] = __fmul_rn(sc[e], factor[h]);
+                    if (!(keys >> (8 * n + 2 * t + c) & 1))
+                        sc[e] = -INFINITY;
+                    top = fmaxf(top, sc[e]);
+                }
                 top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
                 top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
                 const float base = top == -INFINITY ? 0.f : top;
                 alpha[h] = exp2_neg(__fsub_rn(m[h], base));
                 m[h] = top;
+                const float shift = __fsub_rn(kLift<T>, base);
                 float sum = 0.f;
 #pragma unroll
-                for (int n = 0; n < 2; ++n)
-#pragma unroll
-                    for (int e = 0; e < 2; ++e) {
-                        const float v = exp2_neg(__fsub_rn(sc[n][2 * h + e], base));
-                        sum = __fadd_rn(sum, v);
-                        pr[n][2 * h + e] =
-                            std::is_same_v<T, __half> ? __fmul_rn(v, kHalfScale) : v;
-                    }
+                for (int e = 0; e < 4; ++e) {
+                    pr[h][e] = exp2_neg(__fadd_rn(sc[e], shift));
+                    sum = __fadd_rn(sum, pr[h][e]);
+                }
                 l[h] = __fmaf_rn(l[h], alpha[h], sum);
             }
-            uint32_t pp[kQ][4];
+            uint32_t pp[kA][4];
+            {
+                uint32_t piece[kQ][2 * kHalves];
 #pragma unroll
-            for (int i = 0; i < kQ; ++i) {
-                pp[i][0] = take_piece<T>(pr[0][0], pr[0][1]);
-                pp[i][1] = take_piece<T>(pr[0][2], pr[0][3]);
-                pp[i][2] = take_piece<T>(pr[1][0], pr[1][1]);
-                pp[i][3] = take_piece<T>(pr[1][2], pr[1][3]);
+                for (int i = 0; i < kQ; ++i)
+#pragma unroll
+                    for (int e = 0; e < 2 * kHalves; ++e)
+                        piece[i][e] = take_piece<T>(pr[e >> 1][2 * (e & 1)],
+                                                    pr[e >> 1][2 * (e & 1) + 1]);
+                operands(piece, [&](int i, int e) -> uint32_t& { return pp[i][e]; });
             }
             auto add = [&](int n, const float (&x)[4]) {
+                if constexpr (SET == 16) {
 #pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    o[n][e] = __fmaf_rn(o[n][e], alpha[e >> 1], x[e]);
+                    for (int e = 0; e < 4; ++e)
+                        o[n][e] = __fmaf_rn(o[n][e], alpha[e >> 1], x[e]);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 2; ++e)
+                        o[n][e] = __fmaf_rn(o[n][e], alpha[0], __fadd_rn(x[2 + e], x[e]));
+                }
             };
             if constexpr (kWide) {
                 // a group of 32 features: lane's four of each of its keys, one per tile
@@ -480,12 +538,15 @@ paged_split_kernel(const Args a, const Attend p, float* __restrict__ parts,
                             b[n][i][0] = take_piece<T>(v[0][n], v[1][n]);
                             b[n][i][1] = take_piece<T>(v[2][n], v[3][n]);
                         }
-                    constexpr int kPa[6] = {2, 0, 1, 1, 0, 0}, kPb[6] = {0, 2, 1, 0, 1, 0};
+                    constexpr int kPairs = SET == 16 ? 6 : 4;
+                    constexpr int kPa[2][6] = {{2, 0, 1, 1, 0, 0}, {1, 0, 0, 0}};
+                    constexpr int kPb[2][6] = {{0, 2, 1, 0, 1, 0}, {0, 2, 1, 0}};
 #pragma unroll
-                    for (int i = 0; i < 6; ++i)
+                    for (int i = 0; i < kPairs; ++i)
 #pragma unroll
                         for (int n = 0; n < 4; ++n)
-                            mma<T>(x[n], pp[kPa[i]], b[n][kPb[i]][0], b[n][kPb[i]][1]);
+                            mma<T>(x[n], pp[kPa[SET == 8][i]], b[n][kPb[SET == 8][i]][0],
+                                   b[n][kPb[SET == 8][i]][1]);
 #pragma unroll
                     for (int n = 0; n < 4; ++n)
                         add(4 * j + n, x[n]);
@@ -501,7 +562,7 @@ paged_split_kernel(const Args a, const Attend p, float* __restrict__ parts,
                                                            n + 2 * j + (lane >> 4), true));
                     float x[4][4] = {};
 #pragma unroll
-                    for (int i = kQ - 1; i >= 0; --i)
+                    for (int i = kA - 1; i >= 0; --i)
 #pragma unroll
                         for (int j = 0; j < 4; ++j)
                             mma<T>(x[j], pp[i], b[j >> 1][(j & 1) * 2], b[j >> 1][(j & 1) * 2 + 1]);
@@ -535,13 +596,12 @@ paged_split_kernel(const Args a, const Attend p, float* __restrict__ parts,
 
         // ---- the part, or the result -------------------------------------------------
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
+        for (int h = 0; h < kHalves; ++h) {
             l[h] = __fadd_rn(l[h], __shfl_xor_sync(0xffffffffu, l[h], 1));
             l[h] = __fadd_rn(l[h], __shfl_xor_sync(0xffffffffu, l[h], 2));
         }
         const bool whole = b0 == 0 && b1 == blocks;
-        constexpr float kDown = std::is_same_v<T, __half> ? 1.f / kHalfScale : 1.f;
-        float* part = parts + ((size_t)2 * me + (at != first)) * Part<DIM>::kFloats;
+        float* part = parts + ((size_t)2 * me + (at != first)) * Part<DIM, SET>::kFloats;
         if (!whole && lane == 0) {
             const int from = begin + tile * blocks, w0 = from / line.share;
             owners[2 * me + (at != first)] = {seq, head0, heads, w0,
@@ -550,18 +610,17 @@ paged_split_kernel(const Args a, const Attend p, float* __restrict__ parts,
         }
         bool odd = false;
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
+        for (int h = 0; h < kHalves; ++h) {
             const int row = r + 8 * h;
             if (row >= heads)
                 continue;
             float* dst = whole ? p.out + (size_t)s.first * p.ldo + (size_t)(head0 + row) * DIM
-                               : part + 2 * kSet + row * DIM;
+                               : part + 2 * SET + row * DIM;
             if (!whole && t == 0) {
                 part[row] = m[h];
-                part[kSet + row] = l[h];
+                part[SET + row] = l[h];
             }
             auto final = [&](float x) {
-                x = __fmul_rn(x, kDown);
                 if (!whole)
                     return x;
                 x = __fdiv_rn(x, l[h]);
@@ -605,7 +664,7 @@ paged_split_kernel(const Args a, const Attend p, float* __restrict__ parts,
 // other blocks that have parts of the same tile it shares out the tile's heads, to warps where
 // there are few parts, else to blocks whose warps take the parts in turn.
 constexpr int kJoinWarps = 8;
-template <typename T, int DIM>
+template <typename T, int DIM, int SET>
 __global__ void __launch_bounds__(kJoinWarps * 32)
 paged_join_kernel(const Args a, const Attend p, const float* __restrict__ parts,
                   const Owner* __restrict__ owners) {
@@ -630,12 +689,12 @@ paged_join_kernel(const Args a, const Attend p, const float* __restrict__ parts,
 #pragma unroll 4
             for (int w = t.w0 + (few ? 0 : warp); w <= t.w1; w += few ? 1 : kJoinWarps) {
                 const float* part =
-                    parts + ((size_t)2 * w + (w == t.w0 && t.second)) * Part<DIM>::kFloats;
-                const float pm = part[row], pl = part[kSet + row];
+                    parts + ((size_t)2 * w + (w == t.w0 && t.second)) * Part<DIM, SET>::kFloats;
+                const float pm = part[row], pl = part[SET + row];
                 float x[kOwn];
 #pragma unroll
                 for (int i = 0; i < kOwn; ++i)
-                    x[i] = part[2 * kSet + row * DIM + lane + 32 * i];
+                    x[i] = part[2 * SET + row * DIM + lane + 32 * i];
                 const float top = fmaxf(m, pm), base = top == -INFINITY ? 0.f : top;
                 const float ea = exp2_neg(__fsub_rn(m, base)), eb = exp2_neg(__fsub_rn(pm, base));
                 m = top;
@@ -694,32 +753,48 @@ paged_join_kernel(const Args a, const Attend p, const float* __restrict__ parts,
     }
 }
 
-template <typename T, int DIM>
-int launch(b2w4_ctx* ctx, const Args& a, const Attend& p, void* work) {
-    using R = Ring<T, DIM>;
+template <typename T, int DIM, int SET>
+int launch_set(b2w4_ctx* ctx, const Args& a, const Attend& p, void* work) {
+    using R = Ring<T, DIM, SET>;
     static b2w4_smem_optin cfg;
-    auto kern = paged_split_kernel<T, DIM>;
+    auto kern = paged_split_kernel<T, DIM, SET>;
     B2W4_CUDA(ctx, b2w4_opt_in_smem(ctx, kern, R::kBytes, cfg));
-    const int blocks = ctx->sm_count;
+    const int blocks = ctx->sm_count, warps = blocks * R::kWarps;
     float* parts = static_cast<float*>(work);
-    Owner* owners = reinterpret_cast<Owner*>(static_cast<uint8_t*>(work) +
-                                             owners_at<DIM>(blocks * R::kWarps));
+    Owner* owners =
+        reinterpret_cast<Owner*>(static_cast<uint8_t*>(work) + owners_at<DIM, SET>(warps));
     B2W4_CUDA(ctx, b2w4_launch_chained(ctx->pdl, kern, dim3(blocks), dim3(R::kWarps * 32),
                                        R::kBytes, ctx->stream, a, p, parts, owners));
     ctx->launches++;
-    B2W4_CUDA(ctx, b2w4_launch_chained(ctx->pdl, paged_join_kernel<T, DIM>,
-                                       dim3(blocks * R::kWarps), dim3(kJoinWarps * 32), 0,
-                                       ctx->stream, a, p, static_cast<const float*>(parts),
+    B2W4_CUDA(ctx, b2w4_launch_chained(ctx->pdl, paged_join_kernel<T, DIM, SET>, dim3(warps),
+                                       dim3(kJoinWarps * 32), 0, ctx->stream, a, p,
+                                       static_cast<const float*>(parts),
                                        static_cast<const Owner*>(owners)));
     ctx->launches++;
     return B2W4_OK;
 }
+template <typename T, int DIM>
+int launch(b2w4_ctx* ctx, const Args& a, const Attend& p, void* work) {
+    return p.heads / a.kv_heads <= 8 ? launch_set<T, DIM, 8>(ctx, a, p, work)
+                                     : launch_set<T, DIM, 16>(ctx, a, p, work);
+}
 
 }  // namespace
 
+// Two parts of every warp, and their owners: the most that a set of eight heads or of sixteen takes.
 size_t b2w4_paged_split_work(int sm_count, int dim) {
-    const size_t warps = (size_t)kMostWarps * sm_count;
-    return (dim <= 64 ? owners_at<64>(warps) : owners_at<128>(warps)) + 2 * warps * sizeof(Owner);
+    auto bytes = [&](auto d, auto set, int warps) {
+        const int all = warps * sm_count;
+        return owners_at<d(), set()>(all) + 2 * sizeof(Owner) * (size_t)all;
+    };
+    using std::integral_constant;
+    const integral_constant<int, 8> eight;
+    const integral_constant<int, 16> sixteen;
+    const integral_constant<int, 64> d64;
+    const integral_constant<int, 128> d128;
+    const size_t x = dim <= 64 ? bytes(d64, eight, 16) : bytes(d128, eight, 16);
+    const size_t y = dim <= 64 ? bytes(d64, sixteen, 8) : bytes(d128, sixteen, 8);
+    return x > y ? x : y;
 }
 
 bool b2w4_paged_split_takes(int dim) { return dim <= 128; }
