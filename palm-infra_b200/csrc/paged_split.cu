@@ -7,9 +7,11 @@
 // What bounds it: the bytes of the cache.  So the keys that the batch sees, in blocks of 16, lie
 // in one line over sequences, kv heads and sets of 16 heads, of which every warp of the chip takes
 // an equal share, whatever the lengths: one long sequence fills the chip as well as many short
-// ones.  A warp streams its blocks through a cp.async ring of its own and meets no other warp.  A
-// part of the cache that began or ended inside another warp's share goes to the work area; a
-// second launch joins those.
+// ones.  A warp streams its blocks through a cp.async ring of its own, across the ends of
+// sequences, and meets no other warp.  A part of the cache that began or ended inside another
+// warp's share goes to the work area; a second launch joins those.  (Joined by each thread block
+// first, what its warps have of a tile costs more than it saves: 64 sequences of 1028 keys 36 -> 37
+// us, two of 120,000 85 -> 93.)
 //
 // Products are mma.sync m16n8k16, the heads as the rows: with 16 heads a key costs 8192
 // multiply-adds, more than the fp32 pipe has in the time that the key's bytes take.  Every operand
@@ -54,6 +56,7 @@ struct Pieces<float> {
 template <typename T, int SET>
 constexpr int kOperands = SET == 16 ? Pieces<T>::kQ : Pieces<T>::kQ - 1;
 
+constexpr int kMostWarps = 16;
 template <typename T, int DIM, int SET>
 struct Ring {
     static constexpr int kRow = DIM * sizeof(T);       // bytes
@@ -66,15 +69,8 @@ struct Ring {
                                             ? 5
                                             : 208 * 1024 / (kWarps * kSlot);
     static constexpr int kBytes = kWarps * kSlots * kSlot;
-    static_assert(kBytes <= 227 * 1024 && kWarps <= 16, "shared memory, the work area");
+    static_assert(kWarps <= kMostWarps, "the work area");
 };
-
-// The line of blocks: how many a warp takes, and where sequences begin in it.
-struct Line {
-    int total, share;
-};
-// The least share: below that, parts cost more than they save.
-constexpr int kLeastShare = 1;
 
 // Keys that the one token of a sequence sees: [0, low) and [from, length).
 struct Seen {
@@ -98,21 +94,25 @@ __device__ __forceinline__ int blocks_of(const Args& a, const paged::Window& w, 
 }
 
 // Whole warp.  Blocks of all sequences; every tile (kv head and set of heads) of a sequence has as
-// many.
-__device__ Line line_of(const Args& a, const paged::Window& w, int tiles, int warps, bool report) {
-    int sum = 0;
-    for (int i = threadIdx.x & 31; i < a.sequences; i += 32)
+// many.  mine: those of sequence `lane`.
+__device__ int line_of(const Args& a, const paged::Window& w, int tiles, bool report, int* mine) {
+    const int lane = threadIdx.x & 31;
+    *mine = lane < a.sequences ? blocks_of(a, w, lane, report) : 0;
+    int sum = *mine;
+#pragma unroll 4
+    for (int i = lane + 32; i < a.sequences; i += 32)
         sum += blocks_of(a, w, i, report);
-    sum = __reduce_add_sync(0xffffffffu, sum) * tiles;
-    return {sum, max(kLeastShare, (sum + warps - 1) / warps)};
+    return __reduce_add_sync(0xffffffffu, sum) * tiles;
 }
 
 // Whole warp.  The sequence whose blocks hold block `at` of the line, and where they begin.
-__device__ int find(const Args& a, const paged::Window& w, int tiles, int at, int* begin) {
+__device__ int find(const Args& a, const paged::Window& w, int tiles, int at, int mine, int* begin) {
     const int lane = threadIdx.x & 31;
     int before = 0;
     for (int base = 0; base < a.sequences; base += 32) {
-        const int n = base + lane < a.sequences ? blocks_of(a, w, base + lane, false) * tiles : 0;
+        int n = mine * tiles;
+        if (base > 0)
+            n = base + lane < a.sequences ? blocks_of(a, w, base + lane, false) * tiles : 0;
         int x = n;
 #pragma unroll
         for (int off = 1; off < 32; off <<= 1) {
@@ -137,16 +137,23 @@ template <int DIM, int SET>
 struct Part {
     static constexpr int kFloats = 2 * SET + SET * DIM;
 };
-// Whose part it is: the tile's sequence, its heads, and the warps that have parts of it, the
-// first's in its second place if `second`.  count 0: no part.
+// Whose part it is: the tile's heads, in the rows of q and out of its sequence, and the warps that
+// have parts of it, the first's in its second place if `second`.  heads 0: no part.
 struct Owner {
-    int seq, head0, count, w0, w1, second, pad[2];
+    int seq, head0, heads, row;
+    int first, last, second, pad;
 };
 // The work area: two parts of every warp, and their owners.
 template <int DIM, int SET>
-__host__ __device__ size_t owners_at(int warps) {
-    return sizeof(float) * 2 * Part<DIM, SET>::kFloats * (size_t)warps;
+__host__ __device__ constexpr size_t owners_at(int blocks) {
+    return sizeof(float) * 2 * Part<DIM, SET>::kFloats * (size_t)kMostWarps * blocks;
 }
+// Where a warp's stream of blocks is: what its next blocks' tile needs.
+struct Stream {
+    const int32_t* table;
+    int low, from, count, blocks, seq;
+    int tile, kv_row;  // kv_row: of the tile's kv head, in a page
+};
 
 __device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool there) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src),
@@ -241,6 +248,83 @@ __device__ __forceinline__ void operands(const uint32_t (&piece)[Q][N], At at) {
         }
     }
 }
+// A row's sums over parts, by one warp: lane + 32 i are its features.
+template <int DIM, int SET>
+struct Joined {
+    static constexpr int kOwn = DIM / 32;
+    float m = -INFINITY, l = 0.f, o[kOwn] = {};
+    // parts w, w + step, .. up to `last`, kBatch of them on their way together
+    template <typename PartOf>
+    __device__ __forceinline__ void add(PartOf part_of, int w, int last, int step, int row) {
+        constexpr int kBatch = 10;
+        const int lane = threadIdx.x & 31;
+        for (; w <= last; w += kBatch * step) {
+            float pm[kBatch], pl[kBatch], x[kBatch][kOwn];
+#pragma unroll
+            for (int b = 0; b < kBatch; ++b) {
+                const bool in = w + b * step <= last;
+                const float* part = part_of(in ? w + b * step : w);
+                pm[b] = in ? part[row] : -INFINITY;
+                pl[b] = in ? part[SET + row] : 0.f;
+#pragma unroll
+                for (int i = 0; i < kOwn; ++i)
+                    x[b][i] = in ? part[2 * SET + row * DIM + lane + 32 * i] : 0.f;
+            }
+            float top = m;
+#pragma unroll
+            for (int b = 0; b < kBatch; ++b)
+                top = fmaxf(top, pm[b]);
+            const float base = top == -INFINITY ? 0.f : top;
+            const float before = exp2_neg(__fsub_rn(m, base));
+            m = top;
+            l = __fmul_rn(l, before);
+#pragma unroll
+            for (int i = 0; i < kOwn; ++i)
+                o[i] = __fmul_rn(o[i], before);
+#pragma unroll
+            for (int b = 0; b < kBatch; ++b) {
+                const float e = exp2_neg(__fsub_rn(pm[b], base));
+                l = __fmaf_rn(pl[b], e, l);
+#pragma unroll
+                for (int i = 0; i < kOwn; ++i)
+                    o[i] = __fmaf_rn(x[b][i], e, o[i]);
+            }
+        }
+    }
+    __device__ __forceinline__ void store(float* part, int row) const {
+        const int lane = threadIdx.x & 31;
+        if (lane == 0) {
+            part[row] = m;
+            part[SET + row] = l;
+        }
+#pragma unroll
+        for (int i = 0; i < kOwn; ++i)
+            part[2 * SET + row * DIM + lane + 32 * i] = o[i];
+    }
+    // the result of one of the owner's heads
+    template <typename T>
+    __device__ __forceinline__ void finish(const Args& a, const Attend& p, const Owner& t, int head) {
+        const int lane = threadIdx.x & 31;
+        float* out = p.out + (size_t)t.row * p.ldo + (size_t)head * DIM;
+        const float over = __fdiv_rn(1.f, l);
+        bool odd = false;
+#pragma unroll
+        for (int i = 0; i < kOwn; ++i) {
+            const float x = __fmul_rn(o[i], over);
+            odd |= paged::odd_result<T>(x);
+            out[lane + 32 * i] = x;
+        }
+        __syncwarp();
+        if (__any_sync(0xffffffffu, odd)) {
+            bool bad = false;
+            const Sequence s = paged::sequence(a, t.seq, &bad);
+            paged::attend_row<T, DIM>(a, s, p.q + (size_t)t.row * p.ldq + (size_t)head * DIM,
+                                      s.length - 1, head / (p.heads / a.kv_heads), p.scale,
+                                      p.window, out);
+        }
+    }
+};
+
 template <typename T, int DIM, int SET>
 __global__ void __launch_bounds__(Ring<T, DIM, SET>::kWarps * 32, 1)
 paged_split_kernel(const Args a, const Attend p, float* __restrict__ parts,
@@ -256,27 +340,131 @@ paged_split_kernel(const Args a, const Attend p, float* __restrict__ parts,
     const int r = lane >> 2, t = lane & 3;  // row of the products' operands, column pair
     const int group = p.heads / a.kv_heads, sets = (group + SET - 1) / SET;
     const int tiles = a.kv_heads * sets;
-    const int warps = gridDim.x * R::kWarps;
-    const int me = warp * gridDim.x + blockIdx.x;  // few shares: a multiprocessor each
-    const Line line = line_of(a, p.window, tiles, warps, me == 0);
-    int at = min(line.total, me * line.share);
-    const int end = min(line.total, at + line.share);
-    if (lane < 2)
-        owners[2 * me + lane].count = 0;
-    for (int i = me; i < a.sequences; i += warps) {  // sequences that see no key
+    Stream& stream = reinterpret_cast<Stream*>(smem + R::kBytes)[warp];
+    int mine;
+    const int total = line_of(a, p.window, tiles, blockIdx.x + warp == 0, &mine);
+    // a share for every warp, or, where there are fewer blocks, for some warps of every thread block
+    const int active = min(R::kWarps, max(1, (total + (int)gridDim.x - 1) / (int)gridDim.x));
+    const int warps = gridDim.x * active, share = max(1, (total + warps - 1) / warps);
+    const int me = warp * gridDim.x + blockIdx.x;
+    int at = warp < active ? min(total, me * share) : total;
+    const int end = min(total, at + share);
+    // sequences that see no key
+    for (int i = warp * gridDim.x + blockIdx.x; i < a.sequences; i += gridDim.x * R::kWarps) {
         bool bad = false;
         const Sequence s = paged::sequence(a, i, &bad);
         if (s.count == 1 && seen_by(s, p.window).count == 0)
             for (int d = lane; d < p.heads * DIM; d += 32)
                 p.out[(size_t)s.first * p.ldo + d] = 0.f;
     }
+    // (of the warps behind those at work too)
+    if (lane < 2)
+        owners[2 * me + lane].heads = 0;
     if (at >= end)
         return;
-    __syncwarp();
-    int begin;
-    int seq = find(a, p.window, tiles, at, &begin);
     const uint32_t ring = (uint32_t)__cvta_generic_to_shared(smem) + warp * R::kSlots * R::kSlot;
     const int first = at;
+    int begin;
+    int seq = find(a, p.window, tiles, at, mine, &begin);
+    auto prefetch_queries = [&](int row, int kvh, int head0) {
+        const float* q = p.q + (size_t)row * p.ldq + (size_t)head0 * DIM;
+        for (int d = lane * 32; d < min(SET, (kvh + 1) * group - head0) * DIM; d += 1024)
+            asm volatile("prefetch.global.L1 [%0];" ::"l"(q + d));
+    };
+
+    // ---- the stream of blocks --------------------------------------------------------
+    // It is ahead of the blocks that are worked on, in the next tile or sequence too.
+    int f_at = at, f_b = 0;  // the next block, in the line and in its tile
+    const int page_stride = a.kv_heads * a.page_size;
+    auto to_tile = [&](int tile) {  // of the stream's sequence
+        __syncwarp();
+        const int kvh = tile / sets;
+        if (lane == 0) {
+            stream.tile = tile;
+            stream.kv_row = kvh * a.page_size;
+        }
+        bool bad = false;
+        prefetch_queries(paged::sequence(a, stream.seq, &bad).first, kvh,
+                         kvh * group + (tile - kvh * sets) * SET);
+        __syncwarp();
+    };
+    auto to_sequence = [&](int i) {  // the first from sequence i on that sees a key
+        bool bad = false;
+        Sequence s = paged::sequence(a, i, &bad);
+        Seen seen = seen_by(s, p.window);
+        while (seen.count == 0 && i + 1 < a.sequences) {
+            s = paged::sequence(a, ++i, &bad);
+            seen = seen_by(s, p.window);
+        }
+        __syncwarp();
+        if (lane == 0)
+            stream = {s.table, seen.low, seen.from, seen.count,
+                      (seen.count + kKeys - 1) / kKeys, i, 0, 0};
+        __syncwarp();
+    };
+    // Lane j < 16 learns where key j of the next block lies; -1: there is no such key.
+    auto next_row_of = [&]() {
+        if (f_at >= end)
+            return -1;
+        if (f_b == stream.blocks) {
+            f_b = 0;
+            int tile = stream.tile + 1;
+            if (tile == tiles) {
+                to_sequence(stream.seq + 1);
+                tile = 0;
+            }
+            to_tile(tile);
+        }
+        const int i = f_b * kKeys + (lane & 15);
+        ++f_b;
+        ++f_at;
+        if (i >= stream.count)
+            return -1;
+        const int low = stream.low, j = i < low ? i : i - low + stream.from;
+        const int n = paged::page_of(a, j), page = stream.table[n];
+        if ((unsigned)page >= (unsigned)a.pages) {
+            b2w4_report(a.status, B2W4_E_INVALID);
+            return -1;
+        }
+        return page * page_stride + stream.kv_row + j - n * a.page_size;
+    };
+    constexpr int kChunks = R::kRow / 16, kRows = kChunks >= 32 ? 1 : 32 / kChunks;
+    auto swizzled = [&](int key, int chunk, bool values) {
+        const int x = kWide ? (values ? key & 6 : (key & 1) << 2) : key & 7;
+        return (uint32_t)(key * R::kRow + ((chunk ^ x) << 4));
+    };
+    auto fetch = [&](int slot, int row) {
+        const uint32_t dst = ring + slot * R::kSlot;
+#pragma unroll
+        for (int i = 0; i < kKeys / kRows; ++i) {
+            const int key = i * kRows + (kRows > 1 ? lane / kChunks : 0);
+            const int from = __shfl_sync(0xffffffffu, row, key);
+            const size_t off = (size_t)max(from, 0) * R::kRow;
+#pragma unroll
+            for (int c = lane % kChunks; c < kChunks; c += 32) {
+                cp16(dst + swizzled(key, c, false), static_cast<const uint8_t*>(a.k) + off + c * 16,
+                     from >= 0);
+                cp16(dst + R::kHalf + swizzled(key, c, true),
+                     static_cast<const uint8_t*>(a.v) + off + c * 16, from >= 0);
+            }
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+        return __ballot_sync(0xffffffffu, row >= 0) & 0xffffu;
+    };
+    // of the keys of the blocks on their way, those that exist: the next block's first
+    unsigned there[R::kSlots - 1];
+    int slot = 0, into = R::kSlots - 1;
+    to_sequence(seq);
+    f_b = (at - begin) % stream.blocks;
+    to_tile((at - begin) / stream.blocks);
+    int rows[R::kSlots];
+#pragma unroll
+    for (int i = 0; i < R::kSlots; ++i)
+        rows[i] = next_row_of();
+#pragma unroll
+    for (int i = 0; i < R::kSlots - 1; ++i)
+        there[i] = fetch(i, rows[i]);
+    int next_row = rows[R::kSlots - 1];
 
     while (at < end) {
         bool bad = false;
@@ -356,48 +544,6 @@ paged_split_kernel(const Args a, const Attend p, float* __restrict__ parts,
                 operands(piece, [&](int i, int e) -> uint32_t& { return q[i][k][e]; });
             }
         }
-
-        // ---- the stream of blocks ----------------------------------------------------
-        // Lane j < 16 knows where key j of a block lies; -1: no such key.
-        auto row_of = [&](int b) {
-            const int i = b * kKeys + (lane & 15);
-            if (b >= b1 || i >= seen.count)
-                return -1;
-            const int j = i < seen.low ? i : i - seen.low + seen.from;
-            const int row = paged::cache_row(a, s.table, j, kvh);
-            if (row < 0)
-                b2w4_report(a.status, B2W4_E_INVALID);
-            return row;
-        };
-        constexpr int kChunks = R::kRow / 16, kRows = kChunks >= 32 ? 1 : 32 / kChunks;
-        auto swizzled = [&](int key, int chunk, bool values) {
-            const int x = kWide ? (values ? key & 6 : (key & 1) << 2) : key & 7;
-            return (uint32_t)(key * R::kRow + ((chunk ^ x) << 4));
-        };
-        auto fetch = [&](int slot, int row) {
-            const uint32_t dst = ring + slot * R::kSlot;
-#pragma unroll
-            for (int i = 0; i < kKeys / kRows; ++i) {
-                const int key = i * kRows + (kRows > 1 ? lane / kChunks : 0);
-                const int from = __shfl_sync(0xffffffffu, row, key);
-                const size_t off = (size_t)max(from, 0) * R::kRow;
-#pragma unroll
-                for (int c = lane % kChunks; c < kChunks; c += 32) {
-                    cp16(dst + swizzled(key, c, false),
-                         static_cast<const uint8_t*>(a.k) + off + c * 16, from >= 0);
-                    cp16(dst + R::kHalf + swizzled(key, c, true),
-                         static_cast<const uint8_t*>(a.v) + off + c * 16, from >= 0);
-                }
-            }
-            asm volatile("cp.async.commit_group;" ::: "memory");
-            return __ballot_sync(0xffffffffu, row >= 0) & 0xffffu;
-        };
-        // of the keys of the blocks on their way, those that exist: the next block's first
-        unsigned there[R::kSlots - 1];
-#pragma unroll
-        for (int i = 0; i < R::kSlots - 1; ++i)
-            there[i] = fetch(i, row_of(b0 + i));
-        int next_row = row_of(b0 + R::kSlots - 1);
 
         float m[kHalves], l[kHalves], factor[kHalves];
 #pragma unroll
@@ -575,7 +721,6 @@ paged_split_kernel(const Args a, const Attend p, float* __restrict__ parts,
 
         // One copy of the body: unrolled over the slots, its code came from beyond the
         // instruction cache.
-        int slot = 0, into = R::kSlots - 1;
 #pragma unroll 1
         for (int b = b0; b < b1; ++b) {
             cp_wait<R::kSlots - 2>();
@@ -585,14 +730,12 @@ paged_split_kernel(const Args a, const Attend p, float* __restrict__ parts,
             for (int i = 0; i + 1 < R::kSlots - 1; ++i)
                 there[i] = there[i + 1];
             there[R::kSlots - 2] = fetch(into, next_row);  // the slot that the block before left
-            next_row = row_of(b + R::kSlots);
+            next_row = next_row_of();
             block(slot, keys);
             __syncwarp();
             into = slot;
             slot = slot + 1 == R::kSlots ? 0 : slot + 1;
         }
-        cp_wait<0>();
-        __syncwarp();
 
         // ---- the part, or the result -------------------------------------------------
 #pragma unroll
@@ -603,10 +746,9 @@ paged_split_kernel(const Args a, const Attend p, float* __restrict__ parts,
         const bool whole = b0 == 0 && b1 == blocks;
         float* part = parts + ((size_t)2 * me + (at != first)) * Part<DIM, SET>::kFloats;
         if (!whole && lane == 0) {
-            const int from = begin + tile * blocks, w0 = from / line.share;
-            owners[2 * me + (at != first)] = {seq, head0, heads, w0,
-                                              (from + blocks - 1) / line.share,
-                                              from != w0 * line.share, {}};
+            const int from = begin + tile * blocks, w0 = from / share;
+            owners[2 * me + (at != first)] = {seq, head0, heads, s.first, w0,
+                                              (from + blocks - 1) / share, from != w0 * share, 0};
         }
         bool odd = false;
 #pragma unroll
@@ -658,98 +800,70 @@ paged_split_kernel(const Args a, const Attend p, float* __restrict__ parts,
             ++seq;
         }
     }
+    cp_wait<0>();
 }
 
-// Joins what several warps' shares hold of a tile.  Block w has the parts of warp w: with the
-// other blocks that have parts of the same tile it shares out the tile's heads, to warps where
-// there are few parts, else to blocks whose warps take the parts in turn.
-constexpr int kJoinWarps = 8;
+// Joins what several warps' shares hold of a tile.  A warp has an owner's place in the work area:
+// with the other owners of the same tile it shares out the tile's heads.  Where a tile has more than
+// kFew parts its heads are shared out to the blocks that have a place of it, and a block's warps take
+// the parts in turn.
+constexpr int kJoinWarps = 16, kFew = 20;
 template <typename T, int DIM, int SET>
 __global__ void __launch_bounds__(kJoinWarps * 32)
 paged_join_kernel(const Args a, const Attend p, const float* __restrict__ parts,
-                  const Owner* __restrict__ owners) {
+                  const Owner* __restrict__ owners, int places) {
     b2w4_pdl_chain_entry();
-    constexpr int kOwn = DIM / 32;
-    __shared__ float s_o[kJoinWarps][DIM];
-    __shared__ float s_m[kJoinWarps], s_l[kJoinWarps];
+    __shared__ float s_part[kJoinWarps][Part<DIM, 1>::kFloats];
+    __shared__ Owner s_own[kJoinWarps];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-#pragma unroll 1
-    for (int side = 0; side < 2; ++side) {
-        const Owner t = owners[2 * blockIdx.x + side];
-        if (t.count == 0)
-            continue;
-        const int n = t.w1 - t.w0 + 1, mine = blockIdx.x - t.w0;
-        const bool few = n <= kJoinWarps;
-        const int step = few ? kJoinWarps * n : n;
-        for (int row = few ? mine * kJoinWarps + warp : mine; row < t.count; row += step) {
-            float m = -INFINITY, l = 0.f, o[kOwn];
-#pragma unroll
-            for (int i = 0; i < kOwn; ++i)
-                o[i] = 0.f;
-#pragma unroll 4
-            for (int w = t.w0 + (few ? 0 : warp); w <= t.w1; w += few ? 1 : kJoinWarps) {
-                const float* part =
-                    parts + ((size_t)2 * w + (w == t.w0 && t.second)) * Part<DIM, SET>::kFloats;
-                const float pm = part[row], pl = part[SET + row];
-                float x[kOwn];
-#pragma unroll
-                for (int i = 0; i < kOwn; ++i)
-                    x[i] = part[2 * SET + row * DIM + lane + 32 * i];
-                const float top = fmaxf(m, pm), base = top == -INFINITY ? 0.f : top;
-                const float ea = exp2_neg(__fsub_rn(m, base)), eb = exp2_neg(__fsub_rn(pm, base));
-                m = top;
-                l = __fmaf_rn(l, ea, __fmul_rn(pl, eb));
-#pragma unroll
-                for (int i = 0; i < kOwn; ++i)
-                    o[i] = __fmaf_rn(o[i], ea, __fmul_rn(x[i], eb));
-            }
-            if (!few) {
-                __syncthreads();  // of the row before
-                if (lane == 0) {
-                    s_m[warp] = m;
-                    s_l[warp] = l;
-                }
-#pragma unroll
-                for (int i = 0; i < kOwn; ++i)
-                    s_o[warp][lane + 32 * i] = o[i];
-                __syncthreads();
-                if (warp != 0)
-                    continue;
-                m = -INFINITY;
-#pragma unroll
-                for (int w = 0; w < kJoinWarps; ++w)
-                    m = fmaxf(m, s_m[w]);
-                const float base = m == -INFINITY ? 0.f : m;
-                l = 0.f;
-#pragma unroll
-                for (int i = 0; i < kOwn; ++i)
-                    o[i] = 0.f;
-#pragma unroll
-                for (int w = 0; w < kJoinWarps; ++w) {
-                    const float e = exp2_neg(__fsub_rn(s_m[w], base));
-                    l = __fmaf_rn(s_l[w], e, l);
-#pragma unroll
-                    for (int i = 0; i < kOwn; ++i)
-                        o[i] = __fmaf_rn(s_o[w][lane + 32 * i], e, o[i]);
-                }
-            }
-            bool bad = false, odd = false;
-            const Sequence s = paged::sequence(a, t.seq, &bad);
-            const int head = t.head0 + row;
-            float* out = p.out + (size_t)s.first * p.ldo + (size_t)head * DIM;
-#pragma unroll
-            for (int i = 0; i < kOwn; ++i) {
-                const float x = __fdiv_rn(o[i], l);
-                odd |= paged::odd_result<T>(x);
-                out[lane + 32 * i] = x;
-            }
-            __syncwarp();
-            if (__any_sync(0xffffffffu, odd))
-                paged::attend_row<T, DIM>(a, s, p.q + (size_t)s.first * p.ldq + (size_t)head * DIM,
-                                          s.length - 1, head / (p.heads / a.kv_heads), p.scale,
-                                          p.window, out);
+    const int place = blockIdx.x * kJoinWarps + warp;
+    Owner mine = {};
+    if (place < places)
+        mine = owners[place];
+    if (lane == 0)
+        s_own[warp] = mine;
+    auto part = [&](const Owner& t, int w) {
+        return parts + (size_t)(2 * w + (w == t.first && t.second)) * Part<DIM, SET>::kFloats;
+    };
+    if (mine.heads && mine.last - mine.first < kFew) {
+        for (int row = place / 2 - mine.first; row < mine.heads; row += mine.last - mine.first + 1) {
+            Joined<DIM, SET> sum;
+            sum.add([&](int w) { return part(mine, w); }, mine.first, mine.last, 1, row);
+            sum.template finish<T>(a, p, mine, mine.head0 + row);
         }
-        __syncthreads();
+    }
+    __syncthreads();
+    // the first place in this block of every tile with many parts; a tile's places are neighbours
+    // or have one without a part between them
+    bool leads = false;
+    if (lane < kJoinWarps) {
+        const Owner& t = s_own[lane];
+        leads = t.heads && t.last - t.first >= kFew;
+        for (int back = 1; back <= 2 && back <= lane && leads; ++back) {
+            const Owner& o = s_own[lane - back];
+            leads = !(o.heads && o.seq == t.seq && o.head0 == t.head0);
+        }
+    }
+    for (unsigned m = __ballot_sync(0xffffffffu, leads); m; m &= m - 1) {
+        const Owner t = s_own[__ffs(m) - 1];
+        const int b0 = (2 * t.first + t.second) / kJoinWarps, b1 = 2 * t.last / kJoinWarps;
+        for (int row = blockIdx.x - b0; row < t.heads; row += b1 - b0 + 1) {
+            Joined<DIM, SET> sum;
+            sum.add([&](int w) { return part(t, w); }, t.first + warp, t.last, kJoinWarps, row);
+            Joined<DIM, 1> all, one;
+            one.m = sum.m;
+            one.l = sum.l;
+#pragma unroll
+            for (int d = 0; d < DIM / 32; ++d)
+                one.o[d] = sum.o[d];
+            __syncthreads();  // of the row before
+            one.store(s_part[warp], 0);
+            __syncthreads();
+            if (warp != 0)
+                continue;
+            all.add([&](int w) { return s_part[w]; }, 0, kJoinWarps - 1, 1, 0);
+            all.template finish<T>(a, p, t, t.head0 + row);
+        }
     }
 }
 
@@ -758,18 +872,22 @@ int launch_set(b2w4_ctx* ctx, const Args& a, const Attend& p, void* work) {
     using R = Ring<T, DIM, SET>;
     static b2w4_smem_optin cfg;
     auto kern = paged_split_kernel<T, DIM, SET>;
-    B2W4_CUDA(ctx, b2w4_opt_in_smem(ctx, kern, R::kBytes, cfg));
-    const int blocks = ctx->sm_count, warps = blocks * R::kWarps;
+    constexpr size_t smem = R::kBytes + R::kWarps * sizeof(Stream);
+    static_assert(smem <= 227 * 1024, "shared memory");
+    B2W4_CUDA(ctx, b2w4_opt_in_smem(ctx, kern, smem, cfg));
+    const int blocks = ctx->sm_count;
     float* parts = static_cast<float*>(work);
     Owner* owners =
-        reinterpret_cast<Owner*>(static_cast<uint8_t*>(work) + owners_at<DIM, SET>(warps));
-    B2W4_CUDA(ctx, b2w4_launch_chained(ctx->pdl, kern, dim3(blocks), dim3(R::kWarps * 32),
-                                       R::kBytes, ctx->stream, a, p, parts, owners));
+        reinterpret_cast<Owner*>(static_cast<uint8_t*>(work) + owners_at<DIM, SET>(blocks));
+    B2W4_CUDA(ctx, b2w4_launch_chained(ctx->pdl, kern, dim3(blocks), dim3(R::kWarps * 32), smem,
+                                       ctx->stream, a, p, parts, owners));
     ctx->launches++;
-    B2W4_CUDA(ctx, b2w4_launch_chained(ctx->pdl, paged_join_kernel<T, DIM, SET>, dim3(warps),
-                                       dim3(kJoinWarps * 32), 0, ctx->stream, a, p,
-                                       static_cast<const float*>(parts),
-                                       static_cast<const Owner*>(owners)));
+    B2W4_CUDA(ctx, b2w4_launch_chained(ctx->pdl, paged_join_kernel<T, DIM, SET>,
+                                       dim3((2 * blocks * R::kWarps + kJoinWarps - 1) / kJoinWarps),
+                                       dim3(kJoinWarps * 32), 0,
+                                       ctx->stream, a, p, static_cast<const float*>(parts),
+                                       static_cast<const Owner*>(owners),
+                                       2 * blocks * R::kWarps));
     ctx->launches++;
     return B2W4_OK;
 }
@@ -781,20 +899,10 @@ int launch(b2w4_ctx* ctx, const Args& a, const Attend& p, void* work) {
 
 }  // namespace
 
-// Two parts of every warp, and their owners: the most that a set of eight heads or of sixteen takes.
+// The most that a set of eight heads or of sixteen takes.
 size_t b2w4_paged_split_work(int sm_count, int dim) {
-    auto bytes = [&](auto d, auto set, int warps) {
-        const int all = warps * sm_count;
-        return owners_at<d(), set()>(all) + 2 * sizeof(Owner) * (size_t)all;
-    };
-    using std::integral_constant;
-    const integral_constant<int, 8> eight;
-    const integral_constant<int, 16> sixteen;
-    const integral_constant<int, 64> d64;
-    const integral_constant<int, 128> d128;
-    const size_t x = dim <= 64 ? bytes(d64, eight, 16) : bytes(d128, eight, 16);
-    const size_t y = dim <= 64 ? bytes(d64, sixteen, 8) : bytes(d128, sixteen, 8);
-    return x > y ? x : y;
+    const size_t parts = dim <= 64 ? owners_at<64, 16>(sm_count) : owners_at<128, 16>(sm_count);
+    return parts + 2 * sizeof(Owner) * (size_t)kMostWarps * sm_count;
 }
 
 bool b2w4_paged_split_takes(int dim) { return dim <= 128; }
