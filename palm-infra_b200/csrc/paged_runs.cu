@@ -16,8 +16,11 @@
 // What bounds it: the MMAs, which the pieces multiply: 128 rows x 128 keys x 128 features in three
 // pieces are 48 MMAs of 66 cycles, about 3200 cycles; a softmax takes about 2000 beside them.
 //
+// Blocks stay and take one tile after the other, so that a tile's first keys and values are on their
+// way while the one before is finished (6000 tokens, below, 455 us with a block per tile).
+//
 // Roles: warps of rows, two or four threads to a row; a warp that issues the MMAs, the scores' up to
-// two blocks ahead; the rest bring keys and values.  Both lie in shared memory as they lie in
+// two blocks ahead; one that looks the tiles up, two ahead; the rest bring keys and values.  Both lie in shared memory as they lie in
 // the cache, a key's features in 128-byte rows: the keys are the scores' B operand with features
 // running fastest, the values P V's with them running slowest, so neither is transposed.  Rows
 // come one by one with their pages' addresses, so a page may end anywhere.
@@ -51,7 +54,7 @@ struct Cfg {
     static constexpr int kRowWarps = 4 * kParts, kMmaWarp = kRowWarps;
     // for the keys, and as many for the values
     static constexpr int kLoadWarp0 = kRowWarps + 1, kLoadWarps = kWide ? 7 : 1;
-    static constexpr int kThreads = (kLoadWarp0 + 2 * kLoadWarps + 1) * 32;  // one is idle
+    static constexpr int kTileWarp = kLoadWarp0 + 2 * kLoadWarps, kThreads = (kTileWarp + 1) * 32;
     static_assert(kThreads % 128 == 0, "warpgroups");
     static constexpr int kBlocks = kTwo ? 2 : 1;  // of a multiprocessor
     static constexpr int kRegsStart = kWide || kTwo ? 80 : 96;
@@ -65,14 +68,16 @@ struct Cfg {
     static constexpr int kBuf = kK * kPiece;
     static constexpr int kQPart = kRows * 128, kQPiece = kQPart * (DIM / 64);
     static constexpr int kKs = 0, kVs = 2 * kBuf, kQs = 4 * kBuf;
-    static constexpr int kMax = kQs + (kQ - kQTmem) * kQPiece;  // float [2 parities][kParts][kRows]
-    static constexpr int kBar = kMax + 2 * kParts * kRows * 4;
+    // The rows' queries and results in 32 bits pass through the place of the queries' pieces, beside
+    // an fp32 cache through the values'.
+    static constexpr int kStageBytes = kRows * DIM * 4, kQBytes = (kQ - kQTmem) * kQPiece;
+    static constexpr bool kStageInValues = kWide;
+    static constexpr int kStage = kStageInValues ? kVs : kQs;
+    static_assert(!kStageInValues || kStageBytes <= 2 * kBuf);
+    static constexpr int kMax = kQs + (kStageInValues || kQBytes > kStageBytes ? kQBytes : kStageBytes);
+    static constexpr int kBar = kMax + 2 * kParts * kRows * 4;  // kMax: float [2][kParts][kRows]
     static constexpr int kTotal = kBar + 512;
     static_assert(kTotal <= (228 / kBlocks - 1) * 1024, "shared memory");
-    // the rows' queries and results in 32 bits, in the values' place or theirs and the keys'
-    static constexpr bool kStageBoth = kRows * DIM * 4 > 2 * kBuf;
-    static constexpr int kStage = kStageBoth ? kKs : kVs;
-    static_assert(kRows * DIM * 4 <= (kStageBoth ? 4 : 2) * kBuf);
     // tensor memory, columns
     static constexpr int kTq = 0, kTs = kTq + kQTmem * DIM / 2, kTp = kTs + kKeys;
     static constexpr int kTo = kTp + kQ * kKeys / 2;
@@ -215,6 +220,15 @@ __device__ bool find_tile(const Args& a, int tq, int at, int* seq, int* t0) {
     return false;
 }
 
+// A tile: its sequence and kv head, its first token of the sequence's rows, and the keys that its
+// rows see, [0, low) and [from, ..), as one list.
+struct Tile {
+    const int32_t* table;
+    int seq, first, count, length, kvh, t0;
+    int low, from, keys, pad;
+    __device__ __forceinline__ int p0() const { return length - count + t0; }  // its position
+};
+
 template <typename T, int DIM>
 __global__ void __launch_bounds__(Cfg<T, DIM>::kThreads, Cfg<T, DIM>::kBlocks)
 paged_runs_kernel(const Args a, const Attend p, int tq) {
@@ -235,10 +249,14 @@ paged_runs_kernel(const Args a, const Attend p, int tq) {
     uint64_t* k_free = bars + 10;   // [2]
     uint64_t* v_full = bars + 12;   // [2]
     uint64_t* v_free = bars + 14;   // [2]
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 16);
+    uint64_t* tile_full = bars + 16;  // [2] what the tile is
+    uint64_t* tile_free = bars + 18;  // [2]
+    Tile* s_tile = reinterpret_cast<Tile*>(bars + 20);  // [2]
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(s_tile + 2);
     volatile int* s_abort = reinterpret_cast<volatile int*>(tmem_slot + 1);
-    volatile int* s_tile = reinterpret_cast<volatile int*>(tmem_slot + 2);  // sequence, token
+    uint32_t* s_bad = tmem_slot + 2;  // [2] a page that is not the pool's
     uint32_t* s_odd = tmem_slot + 4;  // [4] rows to be done again
+    static_assert(20 * 8 + 2 * sizeof(Tile) + 8 * 4 <= 512);
     float* s_max = reinterpret_cast<float*>(smem + C::kMax);
 
     if (threadIdx.x == 0) {
@@ -253,6 +271,9 @@ paged_runs_kernel(const Args a, const Attend p, int tq) {
             mbar_init(&k_free[b], 1);
             mbar_init(&v_full[b], C::kLoadWarps);
             mbar_init(&v_free[b], 1);
+            mbar_init(&tile_full[b], 1);
+            mbar_init(&tile_free[b], kRowWarps + 1 + 2 * C::kLoadWarps);
+            s_bad[b] = 0;
         }
         *s_abort = 0;
         for (int i = 0; i < 4; ++i)
@@ -260,19 +281,6 @@ paged_runs_kernel(const Args a, const Attend p, int tq) {
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     b2w4_pdl_wait();
-    if (warp == kLoadWarp0) {
-        int seq = -1, t0 = 0;
-        if (!find_tile(a, tq, blockIdx.y, &seq, &t0))
-            seq = -1;
-        if (lane == 0) {
-            s_tile[0] = seq;
-            s_tile[1] = t0;
-        }
-    }
-    __syncthreads();
-    const int seq = s_tile[0], t0 = s_tile[1];
-    if (seq < 0)
-        return;
     if (warp == kMmaWarp) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;"
                      ::"r"(smem_u32(tmem_slot)), "r"(C::kColumns)
@@ -302,23 +310,18 @@ paged_runs_kernel(const Args a, const Attend p, int tq) {
             mbar_arrive(bar);
     };
 
-    bool bad = false;
-    const Sequence s = paged::sequence(a, seq, &bad);
-    const int kvh = blockIdx.x, rep = p.heads / a.kv_heads;
-    const int p0 = s.length - s.count + t0;                 // position of the tile's first token
-    const int p1 = s.length - s.count + min(t0 + tq, s.count) - 1;  // and of its last
-    // the keys that the tile's rows see: [0, low) and [from, p1], as one list
-    const int from = p.window.from(max(p0, 0)), low = min(p.window.sinks, from);
-    const int count = p1 < 0 ? 0 : low + p1 + 1 - from;
-    const int steps = (count + kKeys - 1) / kKeys;
+    const int rep = p.heads / a.kv_heads;
     // r / rep for r < 128: a division for every row of the tile was 5000 cycles of it
     const int inverse = (65536 + rep - 1) / rep;
     auto token_of = [&](int r) { return (r * inverse) >> 16; };
-    auto row_offset = [&](int r, int ld) {
-        const int t = token_of(r);
-        return (size_t)(s.first + t0 + t) * ld + (size_t)(kvh * rep + r - t * rep) * DIM;
+    // The block's n-th tile; false: there is none, or a wait ran out.
+    auto next_tile = [&](int n) {
+        if (!warp_wait(&tile_full[n & 1], (n >> 1) & 1)) {
+            fail();
+            return false;
+        }
+        return s_tile[n & 1].seq >= 0;
     };
-    auto row_exists = [&](int r) { return r < tq * rep && t0 + token_of(r) < s.count; };
 
     if (warp < kRowWarps) {
         // ================================== rows =====================================
@@ -326,15 +329,26 @@ paged_runs_kernel(const Args a, const Attend p, int tq) {
         // a quarter of the tensor memory's lanes; a part of the keys and of the features
         const int quarter = warp & 3, part = warp >> 2;
         const int row = quarter * 32 + lane;
-        const bool exists = row_exists(row);
-        const int pos = exists ? p0 + token_of(row) : -1;
         const uint32_t lane_addr = tmem + ((uint32_t)(quarter * 32) << 16);
         auto row_sync = [&]() {  // the threads of a quarter's rows have come here
             asm volatile("bar.sync %0, %1;" ::"r"(3 + quarter), "n"(32 * kParts) : "memory");
         };
-        // the threads' values of the row, through the words of a parity
-        auto share = [&](float v, int parity, auto join) {
-            float* mx = s_max + parity * kParts * kRows + row;
+        auto all_rows_any = [&](bool v) {  // all row warps have come here
+            int r;
+            asm volatile(
+                "{\n\t.reg .pred p, q;\n\t"
+                "setp.ne.s32 p, %1, 0;\n\t"
+                "barrier.cta.red.or.pred q, 2, %2, p;\n\t"
+                "selp.s32 %0, 1, 0, q;\n\t}"
+                : "=r"(r)
+                : "r"((int)v), "n"(kRowWarps * 32)
+                : "memory");
+            return r != 0;
+        };
+        // the threads' values of the row, through words that alternate
+        int turn = 0;
+        auto share = [&](float v, auto join) {
+            float* mx = s_max + (turn++ & 1) * kParts * kRows + row;
             mx[part * kRows] = v;
             row_sync();
             float r = mx[0];
@@ -344,91 +358,18 @@ paged_runs_kernel(const Args a, const Attend p, int tq) {
             return r;
         };
         auto larger = [](float x, float y) { return fmaxf(x, y); };
-        // The factor of the scores, in base 2.  It is positive: the queries take a negative sign,
-        // and zero is as small a number as can be, so that a masked score stays below all others.
-        const float scale = __fmul_rn(p.scale, 1.4426950408889634f);
-        float factor = fmaxf(fabsf(scale), 0x1p-100f);
         constexpr int kOwn = DIM / kParts, kMine = kKeys / kParts;  // features, keys
-        // a tile of fp32 rows in shared memory: a warp moves some of its quarter's rows whole
+        // a tile of fp32 rows in shared memory: a warp moves some of its quarter's rows whole, where
+        // a thread's own accesses would be a line each (5000 cycles of the load path)
         constexpr int kRowChunks = DIM / 4, kRowsAtOnce = 32 / kRowChunks;
+        constexpr int kMoves = 32 / kParts / kRowsAtOnce;
+        uint8_t* const stage = smem + C::kStage;
         auto staged = [](int r, int chunk) { return (r * kRowChunks + (chunk ^ (r & 7))) * 16; };
         const int stage_chunk = lane % kRowChunks;
         auto stage_row = [&](int i) {
-            return quarter * 32 + (part * (32 / kParts / kRowsAtOnce) + i) * kRowsAtOnce +
-                   lane / kRowChunks;
+            return quarter * 32 + (part * kMoves + i) * kRowsAtOnce + lane / kRowChunks;
         };
-        if (steps > 0) {
-            // Rows come through shared memory, the values' place, which is not filled before: a
-            // thread's own loads would be a line each (5000 cycles of the load path).
-            uint8_t* const stage = smem + C::kStage;
-#pragma unroll
-            for (int i = 0; i < 32 / kParts / kRowsAtOnce; ++i) {
-                const int r = stage_row(i);
-                const float4 v =
-                    row_exists(r) ? *reinterpret_cast<const float4*>(p.q + row_offset(r, p.ldq) +
-                                                                     stage_chunk * 4)
-                                  : make_float4(0.f, 0.f, 0.f, 0.f);
-                *reinterpret_cast<float4*>(stage + staged(r, stage_chunk)) = v;
-            }
-            row_sync();
-            float4 f[kOwn / 4];
-#pragma unroll
-            for (int i = 0; i < kOwn / 4; ++i)
-                f[i] = *reinterpret_cast<const float4*>(stage + staged(row, part * (kOwn / 4) + i));
-            float up = scale < 0.f ? -1.f : 1.f;
-            if constexpr (std::is_same_v<T, __half>) {  // the row's largest to [2^10, 2^11)
-                float top = 0.f;
-#pragma unroll
-                for (int i = 0; i < kOwn / 4; ++i)
-                    top = fmaxf(fmaxf(fmaxf(top, fabsf(f[i].x)), fmaxf(fabsf(f[i].y), fabsf(f[i].z))),
-                                fabsf(f[i].w));
-                top = share(top, 1, larger);
-                int e = (int)(__float_as_uint(top) >> 23) - 127;
-                e = top == 0.f ? 10 : min(max(e, -100), 120);
-                up = __fmul_rn(up, __uint_as_float((unsigned)(127 + 10 - e) << 23));
-                factor = __fmul_rn(factor, __uint_as_float((unsigned)(127 - 10 + e) << 23));
-                factor = fmaxf(factor, 0x1p-100f);
-            }
-            const uint64_t up2 = b2w4_pack2(up, up);
-#pragma unroll
-            for (int c = 0; c < kOwn; c += 16) {
-                uint64_t v[8];
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    v[2 * i] = b2w4_mul2(b2w4_pack2(f[c / 4 + i].x, f[c / 4 + i].y), up2);
-                    v[2 * i + 1] = b2w4_mul2(b2w4_pack2(f[c / 4 + i].z, f[c / 4 + i].w), up2);
-                }
-                const int at = part * kOwn + c;  // first feature
-#pragma unroll
-                for (int i = 0; i < C::kQ; ++i) {
-                    uint32_t r[8];
-#pragma unroll
-                    for (int e = 0; e < 8; ++e)
-                        r[e] = take_piece<T>(v[e], i == C::kQ - 1);
-                    if (i < C::kQTmem) {
-                        tmem_st8(lane_addr + C::kTq + i * (DIM / 2) + at / 2, r);
-                    } else {
-                        uint8_t* to = smem + C::kQs + (i - C::kQTmem) * C::kQPiece +
-                                      at / 64 * C::kQPart;
-#pragma unroll
-                        for (int e = 0; e < 2; ++e)
-                            *reinterpret_cast<uint4*>(to + place(row, at % 64 / 8 + e)) =
-                                make_uint4(r[4 * e], r[4 * e + 1], r[4 * e + 2], r[4 * e + 3]);
-                    }
-                }
-            }
-            tmem_st_wait();
-            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-            asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-            warp_arrive(q_full);
-        }
-        // m: the row's largest score, mf: times the factor, as it is taken from the exponents
-        float m = -INFINITY, mf = -INFINITY, l = 0.f, alpha = 1.f;
-        uint64_t acc[kOwn / 2];
-#pragma unroll
-        for (int i = 0; i < kOwn / 2; ++i)
-            acc[i] = 0ull;
-        bool live = true;  // no way out of the loop: the threads of a row meet once a step
+        bool live = true;  // no way out of a tile: the threads of a row meet once a step
         auto await = [&](uint64_t* bar, uint32_t parity) {
             if (live && !warp_wait(bar, parity)) {
                 live = false;
@@ -436,148 +377,277 @@ paged_runs_kernel(const Args a, const Attend p, int tq) {
             }
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         };
-        // 16 of the thread's features of P V, on their way; and into the running output
-        auto output_ld = [&](int c, uint32_t (&r)[16]) {
-            tmem_ld16(lane_addr + C::kTo + part * kOwn + 16 * c, r);
-        };
-        auto output_add = [&](int c, uint32_t (&r)[16]) {
-            const uint64_t al = b2w4_pack2(alpha, alpha);
-            tmem_ld_wait(r);
+        int g = 0;  // steps of the tiles before
+        for (int n = 0;; ++n) {
+            const bool more = next_tile(n);
+            // one answer for all rows
+            if (all_rows_any(!more || !live || *s_abort))
+                break;
+            const Tile& t = s_tile[n & 1];  // read where it is wanted, it costs no registers
+            const int steps = (t.keys + kKeys - 1) / kKeys;
+            auto row_offset = [&](int r, int ld) {
+                const int k = token_of(r);
+                return (size_t)(t.first + t.t0 + k) * ld + (size_t)(t.kvh * rep + r - k * rep) * DIM;
+            };
+            auto row_exists = [&](int r) { return r < tq * rep && t.t0 + token_of(r) < t.count; };
+            const bool exists = row_exists(row);
+            const int pos = exists ? t.p0() + token_of(row) : -1;
+            // The factor of the scores, in base 2.  It is positive: the queries take a negative
+            // sign, and zero is as small a number as can be, so that a masked score stays below all
+            // others.
+            const float scale = __fmul_rn(p.scale, 1.4426950408889634f);
+            float factor = fmaxf(fabsf(scale), 0x1p-100f);
+            if (steps > 0) {
+                // all loads ahead of the first store, which might be to where a load is from for
+                // all that the compiler knows
+                float4 v[kMoves];
 #pragma unroll
-            for (int i = 0; i < 8; ++i)
-                acc[8 * c + i] = b2w4_fma2(acc[8 * c + i], al,
-                                           b2w4_pack2(__uint_as_float(r[2 * i]),
-                                                      __uint_as_float(r[2 * i + 1])));
-        };
-        // of the list, the row sees [0, sinks) and [lo, hi)
-        const int hi = pos < 0 ? 0 : pos - from + low + 1;
-        const int lo = p.window.from(max(pos, 0)) - from + low;
-        for (int j = 0; j < steps; ++j) {
-            await(s_full, j & 1);
-            uint32_t sr[kMine / 16][16];
+                for (int i = 0; i < kMoves; ++i) {
+                    const int r = stage_row(i);
+                    v[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+                    if (row_exists(r))
+                        v[i] = *reinterpret_cast<const float4*>(p.q + row_offset(r, p.ldq) +
+                                                                stage_chunk * 4);
+                }
 #pragma unroll
-            for (int h = 0; h < kMine / 16; ++h)
-                tmem_ld16(lane_addr + C::kTs + part * kMine + 16 * h, sr[h]);
+                for (int i = 0; i < kMoves; ++i)
+                    *reinterpret_cast<float4*>(stage + staged(stage_row(i), stage_chunk)) = v[i];
+                row_sync();
+                float4 f[kOwn / 4];
 #pragma unroll
-            for (int h = 0; h < kMine / 16; ++h)
-                tmem_ld_wait(sr[h]);
-            asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-            warp_arrive(s_free);
-            float sc[kMine];
+                for (int i = 0; i < kOwn / 4; ++i)
+                    f[i] =
+                        *reinterpret_cast<const float4*>(stage + staged(row, part * (kOwn / 4) + i));
+                if (!C::kStageInValues)
+                    all_rows_any(false);  // the pieces go where the rows were
+                float up = scale < 0.f ? -1.f : 1.f;
+                if constexpr (std::is_same_v<T, __half>) {  // the row's largest to [2^10, 2^11)
+                    float top = 0.f;
 #pragma unroll
-            for (int i = 0; i < kMine; ++i)
-                sc[i] = __uint_as_float(sr[i / 16][i % 16]);
-            const int first = j * kKeys + part * kMine;  // the thread's first key of the list
-            if (first + kMine > hi || (first < lo && first + kMine > p.window.sinks)) {
-                static_assert(kMine <= 32);
-                auto below = [](int n) { return n <= 0 ? 0u : n >= 32 ? ~0u : (1u << n) - 1u; };
-                const unsigned seen = below(hi - first) &
-                                      (~below(lo - first) | below(p.window.sinks - first));
+                    for (int i = 0; i < kOwn / 4; ++i)
+                        top = fmaxf(
+                            fmaxf(fmaxf(top, fabsf(f[i].x)), fmaxf(fabsf(f[i].y), fabsf(f[i].z))),
+                            fabsf(f[i].w));
+                    top = share(top, larger);
+                    int e = (int)(__float_as_uint(top) >> 23) - 127;
+                    e = top == 0.f ? 10 : min(max(e, -100), 120);
+                    up = __fmul_rn(up, __uint_as_float((unsigned)(127 + 10 - e) << 23));
+                    factor = __fmul_rn(factor, __uint_as_float((unsigned)(127 - 10 + e) << 23));
+                    factor = fmaxf(factor, 0x1p-100f);
+                }
+                const uint64_t up2 = b2w4_pack2(up, up);
+#pragma unroll
+                for (int c = 0; c < kOwn; c += 16) {
+                    uint64_t v[8];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        v[2 * i] = b2w4_mul2(b2w4_pack2(f[c / 4 + i].x, f[c / 4 + i].y), up2);
+                        v[2 * i + 1] = b2w4_mul2(b2w4_pack2(f[c / 4 + i].z, f[c / 4 + i].w), up2);
+                    }
+                    const int at = part * kOwn + c;  // first feature
+#pragma unroll
+                    for (int i = 0; i < C::kQ; ++i) {
+                        uint32_t r[8];
+#pragma unroll
+                        for (int e = 0; e < 8; ++e)
+                            r[e] = take_piece<T>(v[e], i == C::kQ - 1);
+                        if (i < C::kQTmem) {
+                            tmem_st8(lane_addr + C::kTq + i * (DIM / 2) + at / 2, r);
+                        } else {
+                            uint8_t* to = smem + C::kQs + (i - C::kQTmem) * C::kQPiece +
+                                          at / 64 * C::kQPart;
+#pragma unroll
+                            for (int e = 0; e < 2; ++e)
+                                *reinterpret_cast<uint4*>(to + place(row, at % 64 / 8 + e)) =
+                                    make_uint4(r[4 * e], r[4 * e + 1], r[4 * e + 2], r[4 * e + 3]);
+                        }
+                    }
+                }
+                tmem_st_wait();
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+                warp_arrive(q_full);
+            }
+            // m: the row's largest score, mf: times the factor, as it is taken from the exponents
+            float m = -INFINITY, mf = -INFINITY, l = 0.f, alpha = 1.f;
+            uint64_t acc[kOwn / 2];
+#pragma unroll
+            for (int i = 0; i < kOwn / 2; ++i)
+                acc[i] = 0ull;
+            // 16 of the thread's features of P V, on their way; and into the running output
+            auto output_ld = [&](int c, uint32_t (&r)[16]) {
+                tmem_ld16(lane_addr + C::kTo + part * kOwn + 16 * c, r);
+            };
+            auto output_add = [&](int c, uint32_t (&r)[16]) {
+                const uint64_t al = b2w4_pack2(alpha, alpha);
+                tmem_ld_wait(r);
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                    acc[8 * c + i] = b2w4_fma2(acc[8 * c + i], al,
+                                               b2w4_pack2(__uint_as_float(r[2 * i]),
+                                                          __uint_as_float(r[2 * i + 1])));
+            };
+            // of the list, the row sees [0, sinks) and [lo, hi)
+            const int hi = pos < 0 ? 0 : pos - t.from + t.low + 1;
+            const int lo = p.window.from(max(pos, 0)) - t.from + t.low;
+            for (int j = 0; j < steps; ++j) {
+                await(s_full, (g + j) & 1);
+                uint32_t sr[kMine / 16][16];
+#pragma unroll
+                for (int h = 0; h < kMine / 16; ++h)
+                    tmem_ld16(lane_addr + C::kTs + part * kMine + 16 * h, sr[h]);
+#pragma unroll
+                for (int h = 0; h < kMine / 16; ++h)
+                    tmem_ld_wait(sr[h]);
+                asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+                warp_arrive(s_free);
+                float sc[kMine];
 #pragma unroll
                 for (int i = 0; i < kMine; ++i)
-                    if (!(seen >> i & 1))
-                        sc[i] = -INFINITY;
-            }
-            float top = m;
+                    sc[i] = __uint_as_float(sr[i / 16][i % 16]);
+                const int first = j * kKeys + part * kMine;  // the thread's first key of the list
+                if (first + kMine > hi || (first < lo && first + kMine > p.window.sinks)) {
+                    static_assert(kMine <= 32);
+                    auto below = [](int k) { return k <= 0 ? 0u : k >= 32 ? ~0u : (1u << k) - 1u; };
+                    const unsigned seen = below(hi - first) &
+                                          (~below(lo - first) | below(p.window.sinks - first));
 #pragma unroll
-            for (int i = 0; i < kMine; i += 2)
-                top = fmaxf(fmaxf(top, sc[i]), sc[i + 1]);
-            m = share(top, j & 1, larger);
-            const float next_mf = m == -INFINITY ? 0.f : __fmul_rn(m, factor);
-            const float shift = __fsub_rn(kLift<T>, next_mf);
-            const uint64_t factor2 = b2w4_pack2(factor, factor), shift2 = b2w4_pack2(shift, shift);
-            uint64_t pr[kMine / 2];
+                    for (int i = 0; i < kMine; ++i)
+                        if (!(seen >> i & 1))
+                            sc[i] = -INFINITY;
+                }
+                float top = m;
 #pragma unroll
-            for (int i = 0; i < kMine / 2; ++i) {
-                float x, y;
-                b2w4_unpack2(b2w4_fma2(b2w4_pack2(sc[2 * i], sc[2 * i + 1]), factor2, shift2), x, y);
-                pr[i] = b2w4_pack2(exp2_neg(x), exp2_neg(y));
-            }
-            uint64_t sum[4] = {pr[0], pr[1], pr[2], pr[3]};
+                for (int i = 0; i < kMine; i += 2)
+                    top = fmaxf(fmaxf(top, sc[i]), sc[i + 1]);
+                m = share(top, larger);
+                const float next_mf = m == -INFINITY ? 0.f : __fmul_rn(m, factor);
+                const float shift = __fsub_rn(kLift<T>, next_mf);
+                const uint64_t factor2 = b2w4_pack2(factor, factor);
+                const uint64_t shift2 = b2w4_pack2(shift, shift);
+                uint64_t pr[kMine / 2];
 #pragma unroll
-            for (int i = 4; i < kMine / 2; ++i)
-                sum[i & 3] = add2(sum[i & 3], pr[i]);
-            sum[0] = add2(add2(sum[0], sum[1]), add2(sum[2], sum[3]));
-            float sum0, sum1;
-            b2w4_unpack2(sum[0], sum0, sum1);
-            const float next_alpha = exp2_neg(__fsub_rn(mf, next_mf));
-            mf = m == -INFINITY ? -INFINITY : next_mf;
-            l = __fmaf_rn(l, next_alpha, __fadd_rn(sum0, sum1));
-            // The pieces that fit the registers are taken ahead of the wait for the product before,
-            // which reads the probabilities: the MMAs of the next one wait for what is behind it.
-            constexpr int kPs = kMine / 16, kOs = kOwn / 16, kTurns = kPs > kOs ? kPs : kOs;
-            uint32_t pieces[C::kQ][8];
-            auto take = [&](int u) {
+                for (int i = 0; i < kMine / 2; ++i) {
+                    float x, y;
+                    b2w4_unpack2(b2w4_fma2(b2w4_pack2(sc[2 * i], sc[2 * i + 1]), factor2, shift2), x,
+                                 y);
+                    pr[i] = b2w4_pack2(exp2_neg(x), exp2_neg(y));
+                }
+                uint64_t sum[4] = {pr[0], pr[1], pr[2], pr[3]};
 #pragma unroll
-                for (int i = 0; i < C::kQ; ++i)
-#pragma unroll
-                    for (int e = 0; e < 8; ++e)
-                        pieces[i][e] = take_piece<T>(pr[8 * u + e], i == C::kQ - 1);
-            };
-            take(0);
-            if (j)
-                await(o_full, (j - 1) & 1);
-#pragma unroll
-            for (int u = 0; u < kTurns; ++u) {
-                uint32_t ro[16];
-                if (j && u < kOs)
-                    output_ld(u, ro);
-                if (u < kPs) {
-                    if (u)
-                        take(u);
+                for (int i = 4; i < kMine / 2; ++i)
+                    sum[i & 3] = add2(sum[i & 3], pr[i]);
+                sum[0] = add2(add2(sum[0], sum[1]), add2(sum[2], sum[3]));
+                float sum0, sum1;
+                b2w4_unpack2(sum[0], sum0, sum1);
+                const float next_alpha = exp2_neg(__fsub_rn(mf, next_mf));
+                mf = m == -INFINITY ? -INFINITY : next_mf;
+                l = __fmaf_rn(l, next_alpha, __fadd_rn(sum0, sum1));
+                // The pieces that fit the registers are taken ahead of the wait for the product
+                // before, which reads the probabilities: the MMAs of the next one wait for what is
+                // behind it.
+                constexpr int kPs = kMine / 16, kOs = kOwn / 16, kTurns = kPs > kOs ? kPs : kOs;
+                uint32_t pieces[C::kQ][8];
+                auto take = [&](int u) {
 #pragma unroll
                     for (int i = 0; i < C::kQ; ++i)
-                        tmem_st8(lane_addr + C::kTp + i * (kKeys / 2) + part * (kMine / 2) + 8 * u,
-                                 pieces[i]);
+#pragma unroll
+                        for (int e = 0; e < 8; ++e)
+                            pieces[i][e] = take_piece<T>(pr[8 * u + e], i == C::kQ - 1);
+                };
+                take(0);
+                if (j)
+                    await(o_full, (g + j - 1) & 1);
+#pragma unroll
+                for (int u = 0; u < kTurns; ++u) {
+                    uint32_t ro[16];
+                    if (j && u < kOs)
+                        output_ld(u, ro);
+                    if (u < kPs) {
+                        if (u)
+                            take(u);
+#pragma unroll
+                        for (int i = 0; i < C::kQ; ++i)
+                            tmem_st8(lane_addr + C::kTp + i * (kKeys / 2) + part * (kMine / 2) +
+                                         8 * u,
+                                     pieces[i]);
+                    }
+                    if (j && u < kOs)
+                        output_add(u, ro);
                 }
-                if (j && u < kOs)
+                alpha = next_alpha;
+                tmem_st_wait();
+                asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+                warp_arrive(p_full);
+            }
+            if (steps > 0) {
+                await(o_full, (g + steps - 1) & 1);
+#pragma unroll
+                for (int u = 0; u < kOwn / 16; ++u) {
+                    uint32_t ro[16];
+                    output_ld(u, ro);
                     output_add(u, ro);
+                }
             }
-            alpha = next_alpha;
-            tmem_st_wait();
-            asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-            warp_arrive(p_full);
-        }
-        if (steps > 0) {
-            await(o_full, (steps - 1) & 1);
+            g += steps;
+            const float total = share(l, [](float x, float y) { return __fadd_rn(x, y); });
+            bool odd = false;
+            const float over = pos < 0 ? 0.f : __fdiv_rn(1.f, total);
 #pragma unroll
-            for (int u = 0; u < kOwn / 16; ++u) {
-                uint32_t ro[16];
-                output_ld(u, ro);
-                output_add(u, ro);
+            for (int i = 0; i < kOwn / 2; ++i) {
+                float x, y;
+                b2w4_unpack2(acc[i], x, y);
+                x = pos < 0 ? 0.f : __fmul_rn(x, over);
+                y = pos < 0 ? 0.f : __fmul_rn(y, over);
+                odd |= paged::odd_result<T>(x) || paged::odd_result<T>(y);
+                acc[i] = b2w4_pack2(x, y);
             }
-        }
-        // (the other parity's words: they may still be read)
-        const float total = share(l, steps & 1, [](float x, float y) { return __fadd_rn(x, y); });
-        bool odd = false;
-        const float over = pos < 0 ? 0.f : __fdiv_rn(1.f, total);
+            // out through shared memory too: every product that read it has retired
 #pragma unroll
-        for (int i = 0; i < kOwn / 2; ++i) {
-            float x, y;
-            b2w4_unpack2(acc[i], x, y);
-            x = pos < 0 ? 0.f : __fmul_rn(x, over);
-            y = pos < 0 ? 0.f : __fmul_rn(y, over);
-            odd |= paged::odd_result<T>(x) || paged::odd_result<T>(y);
-            acc[i] = b2w4_pack2(x, y);
-        }
-        // out through shared memory too: every product that read it has retired
-        uint8_t* const stage = smem + C::kStage;
+            for (int i = 0; i < kOwn / 4; ++i)
+                *reinterpret_cast<ulonglong2*>(stage + staged(row, part * (kOwn / 4) + i)) =
+                    make_ulonglong2(acc[2 * i], acc[2 * i + 1]);
+            const unsigned again =
+                __ballot_sync(0xffffffffu, exists && (odd || s_bad[n & 1]));
+            if (lane == 0 && again)
+                atomicOr(&s_odd[quarter], again);
+            row_sync();
+            {
+                float4 v[kMoves];
 #pragma unroll
-        for (int i = 0; i < kOwn / 4; ++i)
-            *reinterpret_cast<ulonglong2*>(stage + staged(row, part * (kOwn / 4) + i)) =
-                make_ulonglong2(acc[2 * i], acc[2 * i + 1]);
-        row_sync();
-        if (!*s_abort)
+                for (int i = 0; i < kMoves; ++i)
+                    v[i] = *reinterpret_cast<const float4*>(stage +
+                                                            staged(stage_row(i), stage_chunk));
+                const bool good = live && !*s_abort;
 #pragma unroll
-            for (int i = 0; i < 32 / kParts / kRowsAtOnce; ++i) {
-                const int r = stage_row(i);
-                if (row_exists(r))
-                    *reinterpret_cast<float4*>(p.out + row_offset(r, p.ldo) + stage_chunk * 4) =
-                        *reinterpret_cast<const float4*>(stage + staged(r, stage_chunk));
+                for (int i = 0; i < kMoves; ++i) {
+                    const int r = stage_row(i);
+                    if (good && row_exists(r))
+                        *reinterpret_cast<float4*>(p.out + row_offset(r, p.ldo) + stage_chunk * 4) =
+                            v[i];
+                }
             }
-        const unsigned again = __ballot_sync(0xffffffffu, exists && odd);
-        if (lane == 0 && again)
-            atomicOr(&s_odd[quarter], again);
+            row_sync();
+            if (const unsigned mine = s_odd[quarter]) {
+                for (int r = part; r < 32; r += kParts)
+                    if ((mine >> r & 1) && live && !*s_abort) {
+                        bool bad = false;
+                        const Sequence s = paged::sequence(a, t.seq, &bad);
+                        const int q = quarter * 32 + r;
+                        paged::attend_row<T, DIM>(a, s, p.q + row_offset(q, p.ldq),
+                                                  t.p0() + token_of(q), t.kvh, p.scale, p.window,
+                                                  p.out + row_offset(q, p.ldo));
+                    }
+                row_sync();
+                if (part == 0 && lane == 0)
+                    s_odd[quarter] = 0;
+                row_sync();
+            }
+            // every row has looked at the word
+            if (all_rows_any(false), threadIdx.x == 0)
+                s_bad[n & 1] = 0;
+            warp_arrive(&tile_free[n & 1]);
+        }
     } else {
       asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::kRegsOther));
       if (warp == kMmaWarp) {
@@ -655,40 +725,69 @@ paged_runs_kernel(const Args a, const Attend p, int tq) {
                 umma_commit(&v_free[j & 1]);
                 return true;
             };
-            bool ok = steps == 0 || (warp_wait(q_full, 0) && scores(0));
-            __syncwarp();
-            if (ok && steps > 1)
-                ok = scores(1);
-            __syncwarp();
-            for (int j = 0; j < steps && ok; ++j) {
-                ok = output(j);
+            int g = 0, queries = 0;
+            for (int n = 0;; ++n) {
+                if (!next_tile(n))
+                    break;
+                const int steps = (s_tile[n & 1].keys + kKeys - 1) / kKeys;
+                warp_arrive(&tile_free[n & 1]);
+                if (steps == 0)
+                    continue;
+                bool ok = warp_wait(q_full, queries++ & 1) && scores(g);
                 __syncwarp();
-                ok = ok && (j + 2 >= steps || scores(j + 2));
+                if (ok && steps > 1)
+                    ok = scores(g + 1);
                 __syncwarp();
+                for (int j = 0; j < steps && ok; ++j) {
+                    ok = output(g + j);
+                    __syncwarp();
+                    ok = ok && (j + 2 >= steps || scores(g + j + 2));
+                    __syncwarp();
+                }
+                g += steps;
+                if (!ok) {
+                    fail();
+                    break;
+                }
             }
-            if (!ok)
-                fail();
             if (elect_one())
                 umma_commit(drained);
             __syncwarp();
             if (!mbar_wait(drained, 0))
                 fail();
         }
-      } else if (warp < kLoadWarp0 + 2 * C::kLoadWarps) {
-        // ============================== keys and values ==============================
-        // Where key i of the list lies; -1: it does not exist.  One whose page is not the pool's
-        // is left out, which a masked row cannot be: the tile's rows are done again.
-        auto row_of = [&](int i) {
-            if (i >= count)
-                return -1;
-            const int row = paged::cache_row(a, s.table, i < low ? i : i - low + from, kvh);
-            if (row < 0) {
-                b2w4_report(a.status, B2W4_E_INVALID);
-                for (int q = 0; q < 4; ++q)
-                    atomicOr(&s_odd[q], 0xffffffffu);
+      } else if (warp == C::kTileWarp) {
+        // ================================ tiles =====================================
+        for (int n = 0;; ++n) {
+            if (n >= 2 && !warp_wait(&tile_free[n & 1], ((n >> 1) - 1) & 1)) {
+                fail();
+                break;
             }
-            return row;
-        };
+            const int at = blockIdx.x + n * gridDim.x;
+            Tile t = {};
+            t.kvh = at % a.kv_heads;
+            if (find_tile(a, tq, at / a.kv_heads, &t.seq, &t.t0)) {
+                bool bad = false;
+                const Sequence s = paged::sequence(a, t.seq, &bad);
+                t.table = s.table;
+                t.first = s.first;
+                t.count = s.count;
+                t.length = s.length;
+                const int p1 = s.length - s.count + min(t.t0 + tq, s.count) - 1;  // its last token
+                t.from = p.window.from(max(t.p0(), 0));
+                t.low = min(p.window.sinks, t.from);
+                t.keys = p1 < 0 ? 0 : t.low + p1 + 1 - t.from;
+            } else {
+                t.seq = -1;
+            }
+            if (lane == 0)
+                s_tile[n & 1] = t;
+            warp_arrive(&tile_full[n & 1]);
+            if (t.seq < 0)
+                break;
+        }
+      } else {
+        // ============================== keys and values ==============================
         auto full = [&](uint64_t* bar) {  // make it visible to the tensor core
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             warp_arrive(bar);
@@ -702,92 +801,121 @@ paged_runs_kernel(const Args a, const Attend p, int tq) {
         constexpr int kChunks = DIM / 8, kPer = 32 / kChunks;  // of eight features; rows at a time
         const int c = lane % kChunks, sub = lane / kChunks;
         uint8_t* const mine = ring + (c >> 3) * C::kPart;
-        auto free = [&](int j) {
-            // (the stage holds the queries at first)
-            const bool ok = j < 2 ? (!values && !C::kStageBoth) || warp_wait(q_full, 0)
-                                  : warp_wait(&freed[j & 1], ((j >> 1) - 1) & 1);
-            if (!ok)
+        int g = 0, queries = 0;
+        bool ok = true;
+        for (int n = 0; ok; ++n) {
+            if (!next_tile(n))
+                break;
+            const Tile& t = s_tile[n & 1];
+            const int steps = (t.keys + kKeys - 1) / kKeys;
+            // Where key i of the list lies; -1: it does not exist.  One whose page is not the
+            // pool's is left out, which a masked row cannot be: the tile's rows are done again.
+            auto row_of = [&](int i) {
+                if (i >= t.keys)
+                    return -1;
+                const int row =
+                    paged::cache_row(a, t.table, i < t.low ? i : i - t.low + t.from, t.kvh);
+                if (row < 0) {
+                    b2w4_report(a.status, B2W4_E_INVALID);
+                    atomicOr(&s_bad[n & 1], 1u);
+                }
+                return row;
+            };
+            auto free = [&](int i) {
+                ok = i < 2 || warp_wait(&freed[i & 1], ((i >> 1) - 1) & 1);
+                if (!ok)
+                    fail();
+                return ok;
+            };
+            // (the values' place holds the queries at first)
+            if (C::kStageInValues && values && steps > 0 && !warp_wait(q_full, queries++ & 1)) {
                 fail();
-            return ok;
-        };
-        if constexpr (C::kWide) {
-            // a warp has every kLoadWarps-th set of kPer rows of a block; the next block's numbers
-            // are on their way
-            constexpr int kSets = kKeys / kPer, kMine = (kSets + C::kLoadWarps - 1) / C::kLoadWarps;
-            ulonglong2 next[kMine][2];
-            auto load = [&](int j) {
-                int rows[kMine];
-#pragma unroll
-                for (int u = 0; u < kMine; ++u) {
-                    const int set = w0 + u * C::kLoadWarps;
-                    rows[u] = set < kSets ? row_of(j * kKeys + set * kPer + sub) : -1;
-                }
-#pragma unroll
-                for (int u = 0; u < kMine; ++u)
-#pragma unroll
-                    for (int h = 0; h < 2; ++h)
-                        next[u][h] = rows[u] >= 0 ? reinterpret_cast<const ulonglong2*>(
-                                                        pool + (size_t)rows[u] * DIM + c * 8)[h]
-                                                  : make_ulonglong2(0ull, 0ull);
-            };
-            load(0);
-            for (int j = 0; j < steps && free(j); ++j) {
-#pragma unroll
-                for (int u = 0; u < kMine; ++u) {
-                    const int set = w0 + u * C::kLoadWarps;
-                    if (set >= kSets)
-                        break;
-                    uint64_t x[4] = {next[u][0].x, next[u][0].y, next[u][1].x, next[u][1].y};
-                    uint8_t* dst = mine + (j & 1) * C::kBuf + place(set * kPer + sub, c & 7);
-#pragma unroll
-                    for (int i = 0; i < C::kK; ++i) {
-                        uint4 o;
-                        o.x = take_piece<T>(x[0], i == C::kK - 1);
-                        o.y = take_piece<T>(x[1], i == C::kK - 1);
-                        o.z = take_piece<T>(x[2], i == C::kK - 1);
-                        o.w = take_piece<T>(x[3], i == C::kK - 1);
-                        *reinterpret_cast<uint4*>(dst + i * C::kPiece) = o;
-                    }
-                }
-                full(&filled[j & 1]);
-                load(j + 1);
+                break;
             }
-        } else {
-            // the warp's lanes know where some of a block's keys lie each, a block ahead
-            static_assert(C::kWide || C::kLoadWarps == 1);
-            constexpr int kEach = kKeys / 32;
-            int next[kEach], rows[kEach];
-            auto look = [&](int j) {
+            if constexpr (C::kWide) {
+                // a warp has every kLoadWarps-th set of kPer rows of a block; the next block's
+                // numbers are on their way
+                constexpr int kSets = kKeys / kPer;
+                constexpr int kMine = (kSets + C::kLoadWarps - 1) / C::kLoadWarps;
+                ulonglong2 next[kMine][2];
+                auto load = [&](int j) {
+                    int rows[kMine];
 #pragma unroll
-                for (int u = 0; u < kEach; ++u)
-                    next[u] = row_of(j * kKeys + u * 32 + lane);
-            };
-            look(0);
-            for (int j = 0; j < steps && free(j); ++j) {
-#pragma unroll
-                for (int u = 0; u < kEach; ++u)
-                    rows[u] = next[u];
-                look(j + 1);
-                uint8_t* const to = mine + (j & 1) * C::kBuf;
-                // the rows of eight copies are fetched ahead of them: one by one, every copy
-                // waited for its shuffle (80 cycles each)
-#pragma unroll
-                for (int u = 0; u < kEach; ++u)
-#pragma unroll
-                    for (int i = 0; i < 32 / kPer; i += 8) {
-                        int r[8];
-#pragma unroll
-                        for (int e = 0; e < 8; ++e)
-                            r[e] = __shfl_sync(0xffffffffu, rows[u], (i + e) * kPer + sub);
-#pragma unroll
-                        for (int e = 0; e < 8; ++e)
-                            cp16(smem_u32(to + place(u * 32 + (i + e) * kPer + sub, c & 7)),
-                                 pool + (size_t)max(r[e], 0) * DIM + c * 8, r[e] >= 0);
+                    for (int u = 0; u < kMine; ++u) {
+                        const int set = w0 + u * C::kLoadWarps;
+                        rows[u] = set < kSets ? row_of(j * kKeys + set * kPer + sub) : -1;
                     }
-                asm volatile("cp.async.commit_group;" ::: "memory");
-                asm volatile("cp.async.wait_group 0;" ::: "memory");
-                full(&filled[j & 1]);
+#pragma unroll
+                    for (int u = 0; u < kMine; ++u)
+#pragma unroll
+                        for (int h = 0; h < 2; ++h)
+                            next[u][h] = rows[u] >= 0
+                                             ? reinterpret_cast<const ulonglong2*>(
+                                                   pool + (size_t)rows[u] * DIM + c * 8)[h]
+                                             : make_ulonglong2(0ull, 0ull);
+                };
+                load(0);
+                for (int j = 0; j < steps && free(g + j); ++j) {
+#pragma unroll
+                    for (int u = 0; u < kMine; ++u) {
+                        const int set = w0 + u * C::kLoadWarps;
+                        if (set >= kSets)
+                            break;
+                        uint64_t x[4] = {next[u][0].x, next[u][0].y, next[u][1].x, next[u][1].y};
+                        uint8_t* dst =
+                            mine + ((g + j) & 1) * C::kBuf + place(set * kPer + sub, c & 7);
+#pragma unroll
+                        for (int i = 0; i < C::kK; ++i) {
+                            uint4 o;
+                            o.x = take_piece<T>(x[0], i == C::kK - 1);
+                            o.y = take_piece<T>(x[1], i == C::kK - 1);
+                            o.z = take_piece<T>(x[2], i == C::kK - 1);
+                            o.w = take_piece<T>(x[3], i == C::kK - 1);
+                            *reinterpret_cast<uint4*>(dst + i * C::kPiece) = o;
+                        }
+                    }
+                    full(&filled[(g + j) & 1]);
+                    load(j + 1);
+                }
+            } else {
+                // the warp's lanes know where some of a block's keys lie each, a block ahead
+                static_assert(C::kWide || C::kLoadWarps == 1);
+                constexpr int kEach = kKeys / 32;
+                int next[kEach], rows[kEach];
+                auto look = [&](int j) {
+#pragma unroll
+                    for (int u = 0; u < kEach; ++u)
+                        next[u] = row_of(j * kKeys + u * 32 + lane);
+                };
+                look(0);
+                for (int j = 0; j < steps && free(g + j); ++j) {
+#pragma unroll
+                    for (int u = 0; u < kEach; ++u)
+                        rows[u] = next[u];
+                    look(j + 1);
+                    uint8_t* const to = mine + ((g + j) & 1) * C::kBuf;
+                    // the rows of eight copies are fetched ahead of them: one by one, every copy
+                    // waited for its shuffle (80 cycles each)
+#pragma unroll
+                    for (int u = 0; u < kEach; ++u)
+#pragma unroll
+                        for (int i = 0; i < 32 / kPer; i += 8) {
+                            int r[8];
+#pragma unroll
+                            for (int e = 0; e < 8; ++e)
+                                r[e] = __shfl_sync(0xffffffffu, rows[u], (i + e) * kPer + sub);
+#pragma unroll
+                            for (int e = 0; e < 8; ++e)
+                                cp16(smem_u32(to + place(u * 32 + (i + e) * kPer + sub, c & 7)),
+                                     pool + (size_t)max(r[e], 0) * DIM + c * 8, r[e] >= 0);
+                        }
+                    asm volatile("cp.async.commit_group;" ::: "memory");
+                    asm volatile("cp.async.wait_group 0;" ::: "memory");
+                    full(&filled[(g + j) & 1]);
+                }
             }
+            g += steps;
+            warp_arrive(&tile_free[n & 1]);
         }
       }
     }
@@ -800,11 +928,6 @@ paged_runs_kernel(const Args a, const Attend p, int tq) {
                      ::"r"(tmem), "r"(C::kColumns)
                      : "memory");
     }
-    if (warp < kRowWarps && !*s_abort)
-        for (int r = warp; r < kRows; r += kRowWarps)
-            if ((s_odd[r >> 5] >> (r & 31) & 1) && row_exists(r))
-                paged::attend_row<T, DIM>(a, s, p.q + row_offset(r, p.ldq), p0 + token_of(r), kvh,
-                                          p.scale, p.window, p.out + row_offset(r, p.ldo));
 }
 
 template <typename T, int DIM>
@@ -814,9 +937,11 @@ int launch(b2w4_ctx* ctx, const Args& a, const Attend& p) {
     auto kern = paged_runs_kernel<T, DIM>;
     const int tq = kRows / (p.heads / a.kv_heads);
     // a sequence's last tile may be short: one more for each
-    const unsigned tiles = (unsigned)(a.rows / tq + a.sequences);
+    const long tiles = ((long)a.rows / tq + a.sequences) * a.kv_heads;
+    const long resident = (long)ctx->sm_count * C::kBlocks;
+    const unsigned blocks = (unsigned)(tiles < resident ? tiles : resident);
     B2W4_CUDA(ctx, b2w4_opt_in_smem(ctx, kern, C::kTotal, cfg));
-    B2W4_CUDA(ctx, b2w4_launch_chained(ctx->pdl, kern, dim3(a.kv_heads, tiles), dim3(C::kThreads),
+    B2W4_CUDA(ctx, b2w4_launch_chained(ctx->pdl, kern, dim3(blocks), dim3(C::kThreads),
                                        C::kTotal, ctx->stream, a, p, tq));
     ctx->launches++;
     return B2W4_OK;
@@ -826,7 +951,9 @@ int launch(b2w4_ctx* ctx, const Args& a, const Attend& p) {
 
 bool b2w4_paged_runs_takes(int dim, int heads, int kv_heads, int rows, int sequences) {
     const int rep = heads / kv_heads;
-    return dim <= 128 && rep <= kRows && rows / (kRows / rep) + sequences <= 65535;
+    // (the tiles are counted in 32 bits)
+    return dim <= 128 && rep <= kRows &&
+           ((double)rows / (kRows / rep) + sequences) * kv_heads < 0x3fffffff;
 }
 
 int b2w4_launch_paged_runs(b2w4_ctx* ctx, int type, int dim, const Args& a, const Attend& p) {
