@@ -665,8 +665,8 @@ paged_runs_kernel(const Args a, const Attend p, int tq) {
             constexpr uint32_t out_id = idesc(kType, DIM, true);
             // sizes of products, the smallest first: pieces i of Q and size - i of K
             auto scores = [&](int j) {
-                if (!warp_wait(&k_full[j & 1], (j >> 1) & 1) ||
-                    (j > 0 && !warp_wait(s_free, (j - 1) & 1)))
+                if (!__all_sync(0xffffffffu, wait(&k_full[j & 1], (j >> 1) & 1) &&
+                                                 (j == 0 || wait(s_free, (j - 1) & 1))))
                     return false;
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                 const uint64_t d = k_desc0 + (uint64_t)((j & 1) * (C::kBuf >> 4));
@@ -700,7 +700,8 @@ paged_runs_kernel(const Args a, const Attend p, int tq) {
                 return true;
             };
             auto output = [&](int j) {
-                if (!warp_wait(&v_full[j & 1], (j >> 1) & 1) || !warp_wait(p_full, j & 1))
+                if (!__all_sync(0xffffffffu,
+                                wait(&v_full[j & 1], (j >> 1) & 1) && wait(p_full, j & 1)))
                     return false;
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                 const uint64_t d = v_desc0 + (uint64_t)((j & 1) * (C::kBuf >> 4));
@@ -733,11 +734,13 @@ paged_runs_kernel(const Args a, const Attend p, int tq) {
                 warp_arrive(&tile_free[n & 1]);
                 if (steps == 0)
                     continue;
+                // (the lanes wait for the one that issues: they would ask for the next barrier)
                 bool ok = warp_wait(q_full, queries++ & 1) && scores(g);
                 __syncwarp();
                 if (ok && steps > 1)
                     ok = scores(g + 1);
                 __syncwarp();
+#pragma unroll 1
                 for (int j = 0; j < steps && ok; ++j) {
                     ok = output(g + j);
                     __syncwarp();
