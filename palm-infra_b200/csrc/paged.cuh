@@ -18,6 +18,7 @@ struct Args {
     int pages, kv_heads, page_size;
     int slots, table_len, sequences, rows, max_length;
     int* status;
+    bool by_row;  // paged::item: every row by itself
     // x / page_size for 0 <= x < 2^31 (Granlund and Montgomery, Division by invariant integers
     // using multiplication, 1994): t = x multiplier >> 32, (t + (x - t >> shift1)) >> shift2
     uint32_t multiplier;
@@ -75,6 +76,42 @@ inline __host__ __device__ Sequence sequence(const Args& a, int i, bool* bad) {
         s.first = s.count = 0;
     }
     return s;
+}
+
+// The sequence that row `row` of the call belongs to: the last one that begins at or before it;
+// -1 where the row lies before the first sequence or behind the last.
+inline __host__ __device__ int sequence_of(const Args& a, int row) {
+    if (!a.starts)
+        return row < a.sequences ? row : -1;
+    if (row < a.starts[0] || row >= a.starts[a.sequences])
+        return -1;
+    int lo = 0, hi = a.sequences;  // starts[lo] <= row < starts[hi]
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (a.starts[mid] <= row)
+            lo = mid;
+        else
+            hi = mid;
+    }
+    return lo;
+}
+
+// What is attended one token at a time: the sequences, with their last token, or with by_row the
+// rows of all, each as a sequence that ends with its token (length 0: it has none; count 0: there
+// is no such row).
+inline __host__ __device__ int items(const Args& a) { return a.by_row ? a.rows : a.sequences; }
+inline __host__ __device__ Sequence item(const Args& a, int i, bool* bad) {
+    if (!a.by_row)
+        return sequence(a, i, bad);
+    const int n = sequence_of(a, i);
+    if (n < 0)
+        return {a.tables, 0, 0, 0};
+    Sequence s = sequence(a, n, bad);
+    const int in = i - s.first;
+    if (in >= s.count)
+        return {a.tables, 0, 0, 0};
+    const int length = s.length - s.count + in + 1;
+    return {s.table, length < 0 ? 0 : length, i, 1};
 }
 
 // Row of the pools (of dim numbers) where token j of a sequence lies, kv head h; -1: its page is

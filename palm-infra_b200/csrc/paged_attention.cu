@@ -2,6 +2,8 @@
 // embedding, append to the pages), and attention over the pages.
 #include "paged_kernels.cuh"
 
+#include <math.h>
+
 #include <climits>
 
 namespace {
@@ -12,24 +14,6 @@ using paged::Sequence;
 using paged::Window;
 
 constexpr int kWarps = 8;
-
-// The sequence that row `row` of the call belongs to: the last one that begins at or before it;
-// -1 where the row lies before the first sequence or behind the last.
-__device__ __forceinline__ int sequence_of(const Args& a, int row) {
-    if (!a.starts)
-        return row < a.sequences ? row : -1;
-    int lo = 0, hi = a.sequences;  // starts[lo] <= row < starts[hi], if the row has a sequence
-    if (row < a.starts[0] || row >= a.starts[a.sequences])
-        return -1;
-    while (hi - lo > 1) {
-        const int mid = (lo + hi) >> 1;
-        if (a.starts[mid] <= row)
-            lo = mid;
-        else
-            hi = mid;
-    }
-    return lo;
-}
 
 // Whether sequence i's slot is that of an earlier sequence too (whole warp).
 __device__ __forceinline__ bool slot_again(const Args& a, int i) {
@@ -72,7 +56,7 @@ paged_prepare_kernel(const Args a, const Prepare p) {
 #pragma unroll
         for (int d = 0; d < kPer; ++d)
             v[e][d] = first + e < slots ? x[e * DIM + lane + 32 * d] : 0.f;
-    const int i = sequence_of(a, row);
+    const int i = paged::sequence_of(a, row);
     if (i < 0)
         return;
     bool bad = false;
@@ -153,29 +137,6 @@ paged_prepare_kernel(const Args a, const Prepare p) {
     }
 }
 
-// One warp per (row, head), key by key.
-template <typename T, int DIM>
-__global__ void __launch_bounds__(32 * kWarps)
-paged_rows_kernel(const Args a, const Attend p) {
-    b2w4_pdl_chain_entry();
-    const unsigned at = blockIdx.x * kWarps + (threadIdx.x >> 5);
-    const int row = (int)(at / p.heads), head = (int)(at - row * p.heads);
-    if (row >= a.rows)
-        return;
-    const int i = sequence_of(a, row);
-    if (i < 0)
-        return;
-    bool bad = false;
-    const Sequence s = paged::sequence(a, i, &bad);
-    if (bad)
-        b2w4_report(a.status, B2W4_E_INVALID);
-    const int in = row - s.first;
-    const int pos = in < s.count ? s.length - s.count + in : -1;
-    paged::attend_row<T, DIM>(a, s, p.q + (size_t)row * p.ldq + head * DIM, pos,
-                              head / (p.heads / a.kv_heads), p.scale, p.window,
-                              p.out + (size_t)row * p.ldo + head * DIM);
-}
-
 bool misaligned(const void* p, int ld = 0) {
     return (reinterpret_cast<uintptr_t>(p) & 15) || (ld & 3);
 }
@@ -202,12 +163,43 @@ Args args_of(b2w4_ctx* ctx, const b2w4_paged_cache& c, const b2w4_paged_batch& b
     Args a = {c.k_dev,   c.v_dev,  b.tables_dev, b.lengths_dev, b.slots_dev,
               b.starts_dev, c.pages, c.kv_heads,   c.page_size,   b.slots,
               b.table_len, b.sequences, b.rows,    b.max_length,
-              ctx ? ctx->status_dev : nullptr, 0,  0, 0};
+              ctx ? ctx->status_dev : nullptr, false, 0,  0, 0};
     paged::set_division(a);
     return a;
 }
 
 }  // namespace
+
+// Runs of rows go to the kernel that takes 128 (row, head) pairs together, or row by row to the one
+// that shares the cache's bytes out over the chip: long runs and many sequences to the former, a few
+// rows behind a long cache to the latter, by their times in us.  A tile's steps are those of
+// paged_runs.cu; row by row every token has its keys read again, from the second level cache for the
+// most part.  Heads of 192 and 256 numbers, and groups of more than 128, go row by row.
+extern "C" int b2w4_paged_runs_wanted_by(int sm_count, int type, int dim, int heads, int kv_heads,
+                                         int rows, int sequences, int max_length, int window,
+                                         int sinks) {
+    const int rep = heads / kv_heads;
+    if (!b2w4_paged_runs_takes(dim, heads, kv_heads, rows, sequences))
+        return 0;
+    const bool wide = type == B2W4_F32, two = !wide && dim == 64;
+    const int tq = 128 / rep, per = wide || two ? 64 : 128;
+    double keys = max_length;
+    if (window > 0 && (double)window + sinks + tq < keys)
+        keys = (double)window + sinks + tq;
+    const double tiles = ((double)rows / tq + 0.5 * sequences) * kv_heads;
+    const double waves = ceil(tiles / (sm_count * (two ? 2 : 1)));
+    const double step = wide ? 3.3 : two ? 1.9 : 2.2;
+    const double together = 6. + waves * (4. + keys / per * step);
+    const double sets = rep <= 8 || dim > 128 ? (rep + 7) / 8 : (rep + 15) / 16;
+    const double bytes = (double)rows * kv_heads * sets * keys * 2 * dim * (wide ? 4 : 2);
+    return together <= 12. + bytes / 6e6;
+}
+
+bool b2w4_paged_runs_wanted(int sm_count, const b2w4_paged_cache& c, const b2w4_paged_batch& b,
+                            int heads, int window, int sinks) {
+    return b2w4_paged_runs_wanted_by(sm_count, c.type, c.dim, heads, c.kv_heads, b.rows,
+                                     b.sequences, b.max_length, window, sinks) != 0;
+}
 
 // What a cache and a batch must be, whatever is done with them; the text of what is wrong, or
 // NULL.  Host only, for the entry points and for checks without a device.
@@ -322,21 +314,14 @@ int b2w4_paged_attention(b2w4_ctx* ctx, const b2w4_paged_cache* cache,
         work_bytes < b2w4_paged_attention_work(ctx, heads, cache->dim))
         return b2w4_fail(ctx, B2W4_E_INVALID, "paged_attention: the work area is too small");
     const b2w4_device_guard device(ctx);
-    const Args a = args_of(ctx, *cache, *batch);
+    Args a = args_of(ctx, *cache, *batch);
     const Attend p = {q_dev, out_dev, scale, {window, sinks}, ldq, ldo, heads};
-    if (batch->max_new == 1 && b2w4_paged_split_takes(cache->dim))
-        return b2w4_launch_paged_split(ctx, cache->type, cache->dim, a, p, work_dev);
-    if (batch->max_new > 1 &&
-        b2w4_paged_runs_takes(cache->dim, heads, cache->kv_heads, batch->rows, batch->sequences))
-        return b2w4_launch_paged_runs(ctx, cache->type, cache->dim, a, p);
-    const unsigned blocks = ((unsigned)batch->rows * heads + kWarps - 1) / kWarps;
-    return by_type(cache->type, cache->dim, [&](auto* t, auto dim) {
-        using T = std::remove_pointer_t<decltype(t)>;
-        B2W4_CUDA(ctx, b2w4_launch_chained(ctx->pdl, paged_rows_kernel<T, dim()>, dim3(blocks),
-                                           dim3(32 * kWarps), 0, ctx->stream, a, p));
-        ctx->launches++;
-        return (int)B2W4_OK;
-    });
+    if (batch->max_new > 1) {
+        if (b2w4_paged_runs_wanted(ctx->sm_count, *cache, *batch, heads, window, sinks))
+            return b2w4_launch_paged_runs(ctx, cache->type, cache->dim, a, p);
+        a.by_row = true;
+    }
+    return b2w4_launch_paged_split(ctx, cache->type, cache->dim, a, p, work_dev);
 }
 
 }  // extern "C"

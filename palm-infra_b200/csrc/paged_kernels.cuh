@@ -30,8 +30,10 @@ bool b2w4_paged_runs_takes(int dim, int heads, int kv_heads, int rows, int seque
 int b2w4_launch_paged_runs(b2w4_ctx* ctx, int type, int dim, const paged::Args& a,
                            const paged::Attend& p);
 
-// One row per sequence (paged_split.cu): heads of 64 or 128 numbers.
-bool b2w4_paged_split_takes(int dim);
+bool b2w4_paged_runs_wanted(int sm_count, const b2w4_paged_cache& c, const b2w4_paged_batch& b,
+                            int heads, int window, int sinks);
+
+// One row per sequence, or row by row (paged_split.cu).
 size_t b2w4_paged_split_work(int sm_count, int dim);
 int b2w4_launch_paged_split(b2w4_ctx* ctx, int type, int dim, const paged::Args& a,
                             const paged::Attend& p, void* work);

@@ -1,5 +1,5 @@
-// Attention of one new token per sequence over a paged cache, split over the cache's length and
-// joined.
+// Attention of one new token per sequence over a paged cache, or of a run's tokens one by one, split
+// over the cache's length and joined.
 //
 // For the heads of a kv head, with the keys of a part of the cache: m = max s_j, l = sum
 // exp(s_j - m), o = sum exp(s_j - m) v_j; parts join by scaling with exp(m_part - m).
@@ -62,7 +62,13 @@ struct Ring {
     static constexpr int kRow = DIM * sizeof(T);       // bytes
     static constexpr int kHalf = kKeys * kRow;          // keys; the values behind them
     static constexpr int kSlot = 2 * kHalf;
-    static constexpr int kWarps = kSlot > 8192 ? 7 : SET == 16 ? 8 : kSlot > 4096 ? 12 : 16;
+    static constexpr int kWarps = kSlot > 24576   ? 3
+                                  : kSlot > 16384 ? 4
+                                  : DIM > 128     ? 7
+                                  : kSlot > 8192  ? 7
+                                  : SET == 16     ? 8
+                                  : kSlot > 4096  ? 12
+                                                  : 16;
     static constexpr int kSlots = 208 * 1024 / (kWarps * kSlot) < 2
                                       ? 2
                                       : 208 * 1024 / (kWarps * kSlot) > 5
@@ -87,7 +93,7 @@ __device__ __forceinline__ Seen seen_by(const Sequence& s, const paged::Window& 
 }
 __device__ __forceinline__ int blocks_of(const Args& a, const paged::Window& w, int i, bool report) {
     bool bad = false;
-    const Sequence s = paged::sequence(a, i, &bad);
+    const Sequence s = paged::item(a, i, &bad);
     if (report && (bad || s.count > 1))
         b2w4_report(a.status, B2W4_E_INVALID);
     return (seen_by(s, w).count + kKeys - 1) / kKeys;
@@ -97,10 +103,10 @@ __device__ __forceinline__ int blocks_of(const Args& a, const paged::Window& w, 
 // many.  mine: those of sequence `lane`.
 __device__ int line_of(const Args& a, const paged::Window& w, int tiles, bool report, int* mine) {
     const int lane = threadIdx.x & 31;
-    *mine = lane < a.sequences ? blocks_of(a, w, lane, report) : 0;
+    *mine = lane < paged::items(a) ? blocks_of(a, w, lane, report) : 0;
     int sum = *mine;
 #pragma unroll 4
-    for (int i = lane + 32; i < a.sequences; i += 32)
+    for (int i = lane + 32; i < paged::items(a); i += 32)
         sum += blocks_of(a, w, i, report);
     return __reduce_add_sync(0xffffffffu, sum) * tiles;
 }
@@ -109,10 +115,10 @@ __device__ int line_of(const Args& a, const paged::Window& w, int tiles, bool re
 __device__ int find(const Args& a, const paged::Window& w, int tiles, int at, int mine, int* begin) {
     const int lane = threadIdx.x & 31;
     int before = 0;
-    for (int base = 0; base < a.sequences; base += 32) {
+    for (int base = 0; base < paged::items(a); base += 32) {
         int n = mine * tiles;
         if (base > 0)
-            n = base + lane < a.sequences ? blocks_of(a, w, base + lane, false) * tiles : 0;
+            n = base + lane < paged::items(a) ? blocks_of(a, w, base + lane, false) * tiles : 0;
         int x = n;
 #pragma unroll
         for (int off = 1; off < 32; off <<= 1) {
@@ -129,7 +135,7 @@ __device__ int find(const Args& a, const paged::Window& w, int tiles, int at, in
         before += __shfl_sync(0xffffffffu, x, 31);
     }
     *begin = before;
-    return a.sequences;
+    return paged::items(a);
 }
 
 // A part: m and l of its SET rows, then their outputs.
@@ -317,7 +323,7 @@ struct Joined {
         __syncwarp();
         if (__any_sync(0xffffffffu, odd)) {
             bool bad = false;
-            const Sequence s = paged::sequence(a, t.seq, &bad);
+            const Sequence s = paged::item(a, t.seq, &bad);
             paged::attend_row<T, DIM>(a, s, p.q + (size_t)t.row * p.ldq + (size_t)head * DIM,
                                       s.length - 1, head / (p.heads / a.kv_heads), p.scale,
                                       p.window, out);
@@ -350,9 +356,9 @@ paged_split_kernel(const Args a, const Attend p, float* __restrict__ parts,
     int at = warp < active ? min(total, me * share) : total;
     const int end = min(total, at + share);
     // sequences that see no key
-    for (int i = warp * gridDim.x + blockIdx.x; i < a.sequences; i += gridDim.x * R::kWarps) {
+    for (int i = warp * gridDim.x + blockIdx.x; i < paged::items(a); i += gridDim.x * R::kWarps) {
         bool bad = false;
-        const Sequence s = paged::sequence(a, i, &bad);
+        const Sequence s = paged::item(a, i, &bad);
         if (s.count == 1 && seen_by(s, p.window).count == 0)
             for (int d = lane; d < p.heads * DIM; d += 32)
                 p.out[(size_t)s.first * p.ldo + d] = 0.f;
@@ -384,16 +390,16 @@ paged_split_kernel(const Args a, const Attend p, float* __restrict__ parts,
             stream.kv_row = kvh * a.page_size;
         }
         bool bad = false;
-        prefetch_queries(paged::sequence(a, stream.seq, &bad).first, kvh,
+        prefetch_queries(paged::item(a, stream.seq, &bad).first, kvh,
                          kvh * group + (tile - kvh * sets) * SET);
         __syncwarp();
     };
     auto to_sequence = [&](int i) {  // the first from sequence i on that sees a key
         bool bad = false;
-        Sequence s = paged::sequence(a, i, &bad);
+        Sequence s = paged::item(a, i, &bad);
         Seen seen = seen_by(s, p.window);
-        while (seen.count == 0 && i + 1 < a.sequences) {
-            s = paged::sequence(a, ++i, &bad);
+        while (seen.count == 0 && i + 1 < paged::items(a)) {
+            s = paged::item(a, ++i, &bad);
             seen = seen_by(s, p.window);
         }
         __syncwarp();
@@ -468,7 +474,7 @@ paged_split_kernel(const Args a, const Attend p, float* __restrict__ parts,
 
     while (at < end) {
         bool bad = false;
-        const Sequence s = paged::sequence(a, seq, &bad);
+        const Sequence s = paged::item(a, seq, &bad);
         const Seen seen = seen_by(s, p.window);
         const int blocks = (seen.count + kKeys - 1) / kKeys;
         if (blocks == 0) {
@@ -893,27 +899,35 @@ int launch_set(b2w4_ctx* ctx, const Args& a, const Attend& p, void* work) {
 }
 template <typename T, int DIM>
 int launch(b2w4_ctx* ctx, const Args& a, const Attend& p, void* work) {
-    return p.heads / a.kv_heads <= 8 ? launch_set<T, DIM, 8>(ctx, a, p, work)
-                                     : launch_set<T, DIM, 16>(ctx, a, p, work);
+    // (the registers of wide heads have no room for sixteen)
+    if constexpr (DIM <= 128)
+        if (p.heads / a.kv_heads > 8)
+            return launch_set<T, DIM, 16>(ctx, a, p, work);
+    return launch_set<T, DIM, 8>(ctx, a, p, work);
+}
+template <typename T>
+int launch_dim(b2w4_ctx* ctx, int dim, const Args& a, const Attend& p, void* work) {
+    switch (dim) {
+    case 64: return launch<T, 64>(ctx, a, p, work);
+    case 128: return launch<T, 128>(ctx, a, p, work);
+    case 192: return launch<T, 192>(ctx, a, p, work);
+    default: return launch<T, 256>(ctx, a, p, work);
+    }
 }
 
 }  // namespace
 
 // The most that a set of eight heads or of sixteen takes.
 size_t b2w4_paged_split_work(int sm_count, int dim) {
-    const size_t parts = dim <= 64 ? owners_at<64, 16>(sm_count) : owners_at<128, 16>(sm_count);
+    const size_t parts = dim <= 64    ? owners_at<64, 16>(sm_count)
+                         : dim <= 128 ? owners_at<128, 16>(sm_count)
+                                      : owners_at<256, 8>(sm_count);
     return parts + 2 * sizeof(Owner) * (size_t)kMostWarps * sm_count;
 }
 
-bool b2w4_paged_split_takes(int dim) { return dim <= 128; }
-
 int b2w4_launch_paged_split(b2w4_ctx* ctx, int type, int dim, const Args& a, const Attend& p,
                             void* work) {
-    if (dim == 64)
-        return type == B2W4_F16    ? launch<__half, 64>(ctx, a, p, work)
-               : type == B2W4_BF16 ? launch<__nv_bfloat16, 64>(ctx, a, p, work)
-                                   : launch<float, 64>(ctx, a, p, work);
-    return type == B2W4_F16    ? launch<__half, 128>(ctx, a, p, work)
-           : type == B2W4_BF16 ? launch<__nv_bfloat16, 128>(ctx, a, p, work)
-                               : launch<float, 128>(ctx, a, p, work);
+    return type == B2W4_F16    ? launch_dim<__half>(ctx, dim, a, p, work)
+           : type == B2W4_BF16 ? launch_dim<__nv_bfloat16>(ctx, dim, a, p, work)
+                               : launch_dim<float>(ctx, dim, a, p, work);
 }

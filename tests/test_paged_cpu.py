@@ -212,3 +212,17 @@ def test_tokens_by_the_kernels_division(page):
         c = cache(page_size=page, pages=1, kv_heads=1)
         length = min((n + 1) * page, top + 1)
         assert place(c, table, [length], 0, j, 0, max_length=top + 1)[0] == j - n * page
+
+
+def test_the_rule_between_runs_and_rows():
+    """Prompts go together, a few rows behind a long cache one by one; heads that the former does not
+    take never do."""
+    rule = capi.lib().b2w4_paged_runs_wanted_by
+    wanted = lambda kind, dim, heads, kv, rows, seqs, length, window=0, sinks=0: rule(  # noqa: E731
+        148, kind, dim, heads, kv, rows, seqs, length, window, sinks)
+    assert wanted(capi.BF16, 128, 32, 8, 6000, 1, 6000, 2048, 4) == 1
+    assert wanted(capi.F16, 64, 64, 8, 2100, 6, 3500, 512, 8) == 1
+    assert wanted(capi.F32, 128, 32, 8, 333, 1, 1233) == 1
+    assert wanted(capi.BF16, 128, 32, 8, 4, 1, 30000) == 0
+    assert wanted(capi.BF16, 192, 32, 8, 6000, 1, 6000) == 0
+    assert wanted(capi.BF16, 64, 129, 1, 6000, 1, 6000) == 0

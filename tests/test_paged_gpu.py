@@ -123,6 +123,24 @@ def test_long_single_token_in_an_order_of_pages(ctx, dtype):
     run(ctx, dict(lengths=[20011, 5, 9000], page=32, heads=8, kv=2, dim=64, dtype=dtype), 5)
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("heads,kv,dim", [(8, 2, 128), (32, 2, 64), (5, 1, 192), (20, 2, 256),
+                                          (130, 1, 64)])
+@pytest.mark.parametrize("window,sinks", [(0, 0), (700, 5)])
+def test_a_few_rows_behind_a_long_cache(ctx, dtype, heads, kv, dim, window, sinks):
+    run(ctx, dict(lengths=[5000, 5, 1, 1200], news=[3, 0, 1, 2], slots=[3, 0, 1, 4], page=24,
+                  heads=heads, kv=kv, dim=dim, dtype=dtype), 15, window=window, sinks=sinks, pad=2)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("news", [[5, 7], [140, 90]])
+def test_more_rows_than_tokens(ctx, dtype, news):
+    """Rows ahead of a sequence's first token have none: zeros."""
+    got, _, _, _ = run(ctx, dict(lengths=[2, 60], news=news, page=16, heads=8, kv=2, dim=128,
+                                 dtype=dtype), 16)
+    assert (got[:news[0] - 2] == 0).all() and (got[news[0] - 2:news[0]] != 0).any()
+
+
 @pytest.mark.parametrize("news", [None, [9, 1, 30]])
 def test_slots_of_a_larger_table(ctx, news):
     run(ctx, dict(lengths=[100, 7, 55], news=news, slots=[5, 0, 3], page=16, heads=8, kv=2,
