@@ -665,13 +665,7 @@ paged_runs_kernel(const Args a, const Attend p, int tq) {
             constexpr uint32_t out_id = idesc(kType, DIM, true);
             // sizes of products, the smallest first: pieces i of Q and size - i of K
             auto scores = [&](int j) {
-                if (!__all_sync(0xffffffffu, wait(&k_full[j & 1], (j >> 1) & 1) &&
-                                                 (j == 0 || wait(s_free, (j - 1) & 1))))
-                    return false;
-                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                 const uint64_t d = k_desc0 + (uint64_t)((j & 1) * (C::kBuf >> 4));
-                if (!elect_one())
-                    return true;
                 bool more = false;
 #pragma unroll
                 for (int size = C::kQ - 1; size >= 0; --size)
@@ -697,34 +691,57 @@ paged_runs_kernel(const Args a, const Attend p, int tq) {
                     }
                 umma_commit(s_full);
                 umma_commit(&k_free[j & 1]);
-                return true;
             };
-            auto output = [&](int j) {
+            // products of one size
+            auto output = [&](int j, int size) {
+                const uint64_t d = v_desc0 + (uint64_t)((j & 1) * (C::kBuf >> 4));
+#pragma unroll
+                for (int i = size; i >= 0; --i) {
+                    if (size - i >= C::kK)
+                        continue;
+#pragma unroll
+                    for (int k = 0; k < kKeys / 16; ++k)
+                        umma_ts(tm + C::kTo, tm + C::kTp + i * (kKeys / 2) + k * 8,
+                                d + (uint64_t)(((size - i) * C::kPiece + k * 2048) >> 4), out_id,
+                                size < C::kQ - 1 || i < size || k > 0);
+                }
+            };
+            auto scores_wait = [&](int j) {
+                const bool ok = __all_sync(0xffffffffu, wait(&k_full[j & 1], (j >> 1) & 1) &&
+                                                            (j == 0 || wait(s_free, (j - 1) & 1)));
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                return ok;
+            };
+            // P V of block j, then the scores of block `next`, unless that is -1.  What the scores
+            // wait for comes a little after the probabilities: the warp asks for it with a part of
+            // P V on its way, so that no gap is left between the products.
+            auto step = [&](int j, int next) {
                 if (!__all_sync(0xffffffffu,
                                 wait(&v_full[j & 1], (j >> 1) & 1) && wait(p_full, j & 1)))
                     return false;
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                const uint64_t d = v_desc0 + (uint64_t)((j & 1) * (C::kBuf >> 4));
-                if (!elect_one())
-                    return true;
-                bool more = false;
+                if (elect_one())
+                    output(j, C::kQ - 1);
+                __syncwarp();
+                const bool ok = next < 0 || scores_wait(next);
+                if (elect_one()) {
 #pragma unroll
-                for (int size = C::kQ - 1; size >= 0; --size)
-#pragma unroll
-                    for (int i = size; i >= 0; --i) {
-                        if (size - i >= C::kK)
-                            continue;
-#pragma unroll
-                        for (int k = 0; k < kKeys / 16; ++k) {
-                            umma_ts(tm + C::kTo, tm + C::kTp + i * (kKeys / 2) + k * 8,
-                                    d + (uint64_t)(((size - i) * C::kPiece + k * 2048) >> 4),
-                                    out_id, more);
-                            more = true;
-                        }
-                    }
-                umma_commit(o_full);
-                umma_commit(&v_free[j & 1]);
-                return true;
+                    for (int size = C::kQ - 2; size >= 0; --size)
+                        output(j, size);
+                    umma_commit(o_full);
+                    umma_commit(&v_free[j & 1]);
+                    if (next >= 0 && ok)
+                        scores(next);
+                }
+                __syncwarp();
+                return ok;
+            };
+            auto first_scores = [&](int j) {
+                const bool ok = scores_wait(j);
+                if (ok && elect_one())
+                    scores(j);
+                __syncwarp();
+                return ok;
             };
             int g = 0, queries = 0;
             for (int n = 0;; ++n) {
@@ -734,19 +751,11 @@ paged_runs_kernel(const Args a, const Attend p, int tq) {
                 warp_arrive(&tile_free[n & 1]);
                 if (steps == 0)
                     continue;
-                // (the lanes wait for the one that issues: they would ask for the next barrier)
-                bool ok = warp_wait(q_full, queries++ & 1) && scores(g);
-                __syncwarp();
-                if (ok && steps > 1)
-                    ok = scores(g + 1);
-                __syncwarp();
+                bool ok = warp_wait(q_full, queries++ & 1) && first_scores(g) &&
+                          (steps == 1 || first_scores(g + 1));
 #pragma unroll 1
-                for (int j = 0; j < steps && ok; ++j) {
-                    ok = output(g + j);
-                    __syncwarp();
-                    ok = ok && (j + 2 >= steps || scores(g + j + 2));
-                    __syncwarp();
-                }
+                for (int j = 0; j < steps && ok; ++j)
+                    ok = step(g + j, j + 2 < steps ? g + j + 2 : -1);
                 g += steps;
                 if (!ok) {
                     fail();
