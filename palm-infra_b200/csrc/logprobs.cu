@@ -20,6 +20,7 @@
 #include <math.h>
 
 #include <climits>
+#include <utility>
 
 #include <cooperative_groups.h>
 
@@ -171,6 +172,8 @@ logprobs_kernel(const Args a, bool aligned) {
     Shared& s = *reinterpret_cast<Shared*>(s_dyn);
     cg::cluster_group cluster = cg::this_cluster();
     const int blocks = (int)cluster.num_blocks(), block = (int)cluster.block_rank();
+    // that every block of the cluster has begun is asked for before one writes to another
+    auto begun = cluster.barrier_arrive();
     const int row = blockIdx.x / blocks;
     const float* x = a.x + (size_t)row * a.ld;
     const int chunk = ((a.vocab + blocks - 1) / blocks + 3) & ~3;
@@ -323,6 +326,7 @@ logprobs_kernel(const Args a, bool aligned) {
         settle(s, warp, n, a.top);
     else
         __syncthreads();
+    cluster.barrier_wait(std::move(begun));
     Shared* out = cluster.map_shared_rank(&s, 0);
     if (warp == 0) {
         const Sums all = join_lanes(s.warp[lane % kWarps], kWarps);

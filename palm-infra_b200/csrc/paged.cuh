@@ -18,7 +18,8 @@ struct Args {
     int pages, kv_heads, page_size;
     int slots, table_len, sequences, rows, max_length;
     int* status;
-    bool by_row;  // paged::item: every row by itself
+    bool by_row;             // paged::item: every row by itself
+    int first_item, items;  // ... of a launch
     // x / page_size for 0 <= x < 2^31 (Granlund and Montgomery, Division by invariant integers
     // using multiplication, 1994): t = x multiplier >> 32, (t + (x - t >> shift1)) >> shift2
     uint32_t multiplier;
@@ -98,9 +99,9 @@ inline __host__ __device__ int sequence_of(const Args& a, int row) {
 
 // What is attended one token at a time: the sequences, with their last token, or with by_row the
 // rows of all, each as a sequence that ends with its token (length 0: it has none; count 0: there
-// is no such row).
-inline __host__ __device__ int items(const Args& a) { return a.by_row ? a.rows : a.sequences; }
+// is no such row).  i: counted from the launch's first.
 inline __host__ __device__ Sequence item(const Args& a, int i, bool* bad) {
+    i += a.first_item;
     if (!a.by_row)
         return sequence(a, i, bad);
     const int n = sequence_of(a, i);

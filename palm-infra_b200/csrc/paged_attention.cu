@@ -163,7 +163,7 @@ Args args_of(b2w4_ctx* ctx, const b2w4_paged_cache& c, const b2w4_paged_batch& b
     Args a = {c.k_dev,   c.v_dev,  b.tables_dev, b.lengths_dev, b.slots_dev,
               b.starts_dev, c.pages, c.kv_heads,   c.page_size,   b.slots,
               b.table_len, b.sequences, b.rows,    b.max_length,
-              ctx ? ctx->status_dev : nullptr, false, 0,  0, 0};
+              ctx ? ctx->status_dev : nullptr, false, 0, 0, 0, 0, 0};
     paged::set_division(a);
     return a;
 }

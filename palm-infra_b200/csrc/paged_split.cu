@@ -5,9 +5,9 @@
 // exp(s_j - m), o = sum exp(s_j - m) v_j; parts join by scaling with exp(m_part - m).
 //
 // What bounds it: the bytes of the cache.  So the keys that the batch sees, in blocks of 16, lie
-// in one line over sequences, kv heads and sets of 16 heads, of which every warp of the chip takes
-// an equal share, whatever the lengths: one long sequence fills the chip as well as many short
-// ones.  A warp streams its blocks through a cp.async ring of its own, across the ends of
+// in one line over sequences, kv heads and sets of 8 or 16 heads, of which every warp of the chip
+// takes an equal share, whatever the lengths: one long sequence fills the chip as well as many
+// short ones.  A warp streams its blocks through a cp.async ring of its own, across the ends of
 // sequences, and meets no other warp.  A part of the cache that began or ended inside another
 // warp's share goes to the work area; a second launch joins those.  (Joined by each thread block
 // first, what its warps have of a tile costs more than it saves: 64 sequences of 1028 keys 36 -> 37
@@ -25,6 +25,8 @@
 // What pieces cannot hold -- infinities, NaN, results that are not finite -- is done key by key in
 // 32 bits (paged::attend_row), which has the rule for values of probability zero.
 #include "paged_kernels.cuh"
+
+#include <math.h>
 
 #include <climits>
 
@@ -103,10 +105,10 @@ __device__ __forceinline__ int blocks_of(const Args& a, const paged::Window& w, 
 // many.  mine: those of sequence `lane`.
 __device__ int line_of(const Args& a, const paged::Window& w, int tiles, bool report, int* mine) {
     const int lane = threadIdx.x & 31;
-    *mine = lane < paged::items(a) ? blocks_of(a, w, lane, report) : 0;
+    *mine = lane < a.items ? blocks_of(a, w, lane, report) : 0;
     int sum = *mine;
 #pragma unroll 4
-    for (int i = lane + 32; i < paged::items(a); i += 32)
+    for (int i = lane + 32; i < a.items; i += 32)
         sum += blocks_of(a, w, i, report);
     return __reduce_add_sync(0xffffffffu, sum) * tiles;
 }
@@ -115,10 +117,10 @@ __device__ int line_of(const Args& a, const paged::Window& w, int tiles, bool re
 __device__ int find(const Args& a, const paged::Window& w, int tiles, int at, int mine, int* begin) {
     const int lane = threadIdx.x & 31;
     int before = 0;
-    for (int base = 0; base < paged::items(a); base += 32) {
+    for (int base = 0; base < a.items; base += 32) {
         int n = mine * tiles;
         if (base > 0)
-            n = base + lane < paged::items(a) ? blocks_of(a, w, base + lane, false) * tiles : 0;
+            n = base + lane < a.items ? blocks_of(a, w, base + lane, false) * tiles : 0;
         int x = n;
 #pragma unroll
         for (int off = 1; off < 32; off <<= 1) {
@@ -135,7 +137,7 @@ __device__ int find(const Args& a, const paged::Window& w, int tiles, int at, in
         before += __shfl_sync(0xffffffffu, x, 31);
     }
     *begin = before;
-    return paged::items(a);
+    return a.items;
 }
 
 // A part: m and l of its SET rows, then their outputs.
@@ -356,7 +358,7 @@ paged_split_kernel(const Args a, const Attend p, float* __restrict__ parts,
     int at = warp < active ? min(total, me * share) : total;
     const int end = min(total, at + share);
     // sequences that see no key
-    for (int i = warp * gridDim.x + blockIdx.x; i < paged::items(a); i += gridDim.x * R::kWarps) {
+    for (int i = warp * gridDim.x + blockIdx.x; i < a.items; i += gridDim.x * R::kWarps) {
         bool bad = false;
         const Sequence s = paged::item(a, i, &bad);
         if (s.count == 1 && seen_by(s, p.window).count == 0)
@@ -398,7 +400,7 @@ paged_split_kernel(const Args a, const Attend p, float* __restrict__ parts,
         bool bad = false;
         Sequence s = paged::item(a, i, &bad);
         Seen seen = seen_by(s, p.window);
-        while (seen.count == 0 && i + 1 < paged::items(a)) {
+        while (seen.count == 0 && i + 1 < a.items) {
             s = paged::item(a, ++i, &bad);
             seen = seen_by(s, p.window);
         }
@@ -897,11 +899,12 @@ int launch_set(b2w4_ctx* ctx, const Args& a, const Attend& p, void* work) {
     ctx->launches++;
     return B2W4_OK;
 }
+// Heads of a set: the registers of wide heads have no room for sixteen.
+int set_of(int dim, int group) { return dim <= 128 && group > 8 ? 16 : 8; }
 template <typename T, int DIM>
 int launch(b2w4_ctx* ctx, const Args& a, const Attend& p, void* work) {
-    // (the registers of wide heads have no room for sixteen)
     if constexpr (DIM <= 128)
-        if (p.heads / a.kv_heads > 8)
+        if (set_of(DIM, p.heads / a.kv_heads) == 16)
             return launch_set<T, DIM, 16>(ctx, a, p, work);
     return launch_set<T, DIM, 8>(ctx, a, p, work);
 }
@@ -925,9 +928,34 @@ size_t b2w4_paged_split_work(int sm_count, int dim) {
     return parts + 2 * sizeof(Owner) * (size_t)kMostWarps * sm_count;
 }
 
-int b2w4_launch_paged_split(b2w4_ctx* ctx, int type, int dim, const Args& a, const Attend& p,
-                            void* work) {
-    return type == B2W4_F16    ? launch_dim<__half>(ctx, dim, a, p, work)
-           : type == B2W4_BF16 ? launch_dim<__nv_bfloat16>(ctx, dim, a, p, work)
-                               : launch_dim<float>(ctx, dim, a, p, work);
+// A launch counts its blocks of keys in 32 bits: the items (paged::item) that it may have, each of
+// `keys` keys at most; 0: not even one.
+extern "C" int b2w4_paged_split_items(int items, double keys, int dim, int heads, int kv_heads) {
+    const int set = set_of(dim, heads / kv_heads);
+    const double tiles = (double)kv_heads * ((heads / kv_heads + set - 1) / set);
+    const double most = floor(0x40000000 / (ceil(keys / kKeys) * tiles));
+    return most < items ? (int)most : items;
+}
+
+int b2w4_launch_paged_split(b2w4_ctx* ctx, int type, int dim, Args a, const Attend& p, void* work) {
+    const int items = a.by_row ? a.rows : a.sequences;
+    double keys = a.max_length < (double)a.table_len * a.page_size
+                      ? a.max_length
+                      : (double)a.table_len * a.page_size;
+    if (p.window.size > 0 && (double)p.window.size + p.window.sinks < keys)
+        keys = (double)p.window.size + p.window.sinks;
+    const int most = b2w4_paged_split_items(items, keys, dim, p.heads, a.kv_heads);
+    if (most == 0)
+        return b2w4_fail(ctx, B2W4_E_INVALID, "paged_attention: max_length is too large (%d)",
+                         a.max_length);
+    for (int first = 0; first < items; first += a.items) {
+        a.first_item = first;
+        a.items = most < items - first ? most : items - first;
+        const int rc = type == B2W4_F16    ? launch_dim<__half>(ctx, dim, a, p, work)
+                       : type == B2W4_BF16 ? launch_dim<__nv_bfloat16>(ctx, dim, a, p, work)
+                                           : launch_dim<float>(ctx, dim, a, p, work);
+        if (rc != B2W4_OK)
+            return rc;
+    }
+    return B2W4_OK;
 }

@@ -42,13 +42,13 @@ __device__ __forceinline__ int room(const Pool& p) {
 }
 
 // Sum of the threads' values before this one's; total: of all.  s_part: a word per warp.
-template <int THREADS>
-__device__ int scan(int v, int* s_part, int* total) {
+template <int THREADS, typename N>
+__device__ N scan(N v, N* s_part, N* total) {
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    int x = v;
+    N x = v;
 #pragma unroll
     for (int off = 1; off < 32; off <<= 1) {
-        const int y = __shfl_up_sync(0xffffffffu, x, off);
+        const N y = __shfl_up_sync(0xffffffffu, x, off);
         if (lane >= off)
             x += y;
     }
@@ -56,7 +56,7 @@ __device__ int scan(int v, int* s_part, int* total) {
     if (lane == 31)
         s_part[warp] = x;
     __syncthreads();
-    int before = 0, all = 0;
+    N before = 0, all = 0;
 #pragma unroll
     for (int w = 0; w < THREADS / 32; ++w) {
         before += w < warp ? s_part[w] : 0;
@@ -96,7 +96,9 @@ __global__ void __launch_bounds__(kMostItems)
 pages_extend_kernel(const Pool p, const int32_t* __restrict__ slots,
                     const int32_t* __restrict__ counts, int n, int32_t* __restrict__ granted) {
     b2w4_pdl_chain_entry();
-    __shared__ int s_part[32], s_slot[kMostItems], s_off[kMostItems + 1], s_first[kMostItems];
+    __shared__ int s_part[32], s_slot[kMostItems], s_first[kMostItems];
+    // (what the sequences ask for may pass 32 bits)
+    __shared__ long long s_sum[32], s_off[kMostItems + 1];
     const int i = threadIdx.x;
     const int slot = i < n ? (slots ? slots[i] : i) : -1;
     const int count = i < n ? (counts ? counts[i] : 1) : 0;
@@ -115,16 +117,17 @@ pages_extend_kernel(const Pool p, const int32_t* __restrict__ slots,
     }
     if (i < n && !good && slot != -1)
         bad(p);
-    int total;
-    const int off = scan<kMostItems>(need, s_part, &total);
+    long long total;
+    const long long off = scan<kMostItems>((long long)need, s_sum, &total);
     s_off[i] = off;
     s_first[i] = good ? pages_of(p, length) : 0;
     if (i == 0)
         s_off[kMostItems] = total;
     __syncthreads();
     int have = 0;
-    if (total > 0)
-        have = free_pages<kMostItems>(p, total, s_part, [&](int rank, int page) {
+    const int want = (int)min(total, (long long)p.pages);
+    if (want > 0)
+        have = free_pages<kMostItems>(p, want, s_part, [&](int rank, int page) {
             int lo = 0, hi = kMostItems;  // the last item that begins at or before the rank
             while (hi - lo > 1) {
                 const int mid = (lo + hi) >> 1;
@@ -133,7 +136,8 @@ pages_extend_kernel(const Pool p, const int32_t* __restrict__ slots,
                 else
                     hi = mid;
             }
-            p.tables[(size_t)s_slot[lo] * p.table_len + s_first[lo] + rank - s_off[lo]] = page;
+            p.tables[(size_t)s_slot[lo] * p.table_len + s_first[lo] + rank - (int)s_off[lo]] =
+                page;
             p.refs[page] = 1;
         });
     const bool fits = good && (need == 0 || off + need <= have);
@@ -143,7 +147,7 @@ pages_extend_kernel(const Pool p, const int32_t* __restrict__ slots,
         return;
     if (!fits) {  // back with what it got
         const int32_t* row = p.tables + (size_t)slot * p.table_len + s_first[i];
-        for (int r = off; r < have; ++r)
+        for (long long r = off; r < have; ++r)
             p.refs[row[r - off]] = 0;
         b2w4_report(p.status, B2W4_E_NOMEM);
         return;
@@ -491,6 +495,8 @@ extern "C" const char* b2w4_pages_refusal(const b2w4_page_pool* p, const b2w4_pa
             return "no pool";
         if (p->pages <= 0 || p->page_size <= 0 || p->slots <= 0 || p->table_len <= 0)
             return "pages, page_size, slots and table_len must be positive";
+        if (p->pages > INT_MAX / 2)
+            return "fewer than 2^30 pages";
     }
     if (wants_planes) {
         if (!pl || !pl->planes || pl->count <= 0 || pl->pages <= 0)

@@ -350,7 +350,9 @@ class PagedDecoder(DenseDecoder):
     one captured step serves every mix of sequences.
 
     cache_type: torch.float32, float16 or bfloat16.  window, sinks: as b2w4_paged_attention's; a
-    window bounds what a step reads, not the pages that a sequence keeps.
+    window bounds what a step reads, not the pages that a sequence keeps.  max_length: tokens of a
+    sequence, rounded up to whole pages; a step leaves a longer one as it is, and sync raises.
+    Calls run on torch's current stream, which they set the context to.
 
     The matmuls of one row (a decoder of one slot, a prompt of one token) take the rule per 128
     values, those of several rows `multi_row_rule`."""
@@ -363,11 +365,11 @@ class PagedDecoder(DenseDecoder):
         self.pages, self.page_size, self.slots = pages, page_size, slots
         self.cache_type = cache_type or torch.float32
         self.window, self.sinks = window, sinks
-        max_length = max_length or pages * page_size
+        max_length = -(-(max_length or pages * page_size) // page_size) * page_size
         super().__init__(ctx, cfg, weights, max_length, multi_row_rule=multi_row_rule)
         zeros = lambda *shape: torch.zeros(shape, dtype=torch.int32, device="cuda")
-        table_len = -(-max_length // page_size)
-        self.pool = capi.PagePool(zeros(pages), zeros(slots, table_len), zeros(slots), page_size)
+        self.pool = capi.PagePool(zeros(pages), zeros(slots, max_length // page_size),
+                                  zeros(slots), page_size)
         self.refs, self.tables, self.lengths = self.pool.keep
         for L in self.layers:
             L["cache"] = capi.PagedCache(L["k_cache"], L["v_cache"])
@@ -391,6 +393,18 @@ class PagedDecoder(DenseDecoder):
         shape = (self.pages, self.cfg.kv_heads, self.page_size, self.cfg.head_dim)
         return {k: self.torch.zeros(shape, dtype=self.cache_type, device=self.device)
                 for k in ("k_cache", "v_cache")}
+
+    def _b(self, name, rows, cols):
+        """The step's rows have buffers of their own, which a captured step holds; prompts, of any
+        number of rows, share one that grows."""
+        if rows == self.slots:
+            return super()._b(name, rows, cols)
+        if name not in self._buf or self._buf[name].numel() < rows * cols:
+            self._buf[name] = self.torch.empty(rows * cols, device=self.device)
+        return self._buf[name][:rows * cols].view(rows, cols)
+
+    def _on_current_stream(self):
+        self.ctx.set_stream(self.torch.cuda.current_stream().cuda_stream)
 
     def _ints(self, values):
         return self.torch.tensor(list(values), dtype=self.torch.int32, device="cuda")
@@ -446,6 +460,7 @@ class PagedDecoder(DenseDecoder):
         if len(counts) != len(slots) or min(counts, default=0) < 1:
             raise ValueError("a prompt of at least one token for every slot")
         starts = np.concatenate([[0], np.cumsum(counts)]).tolist()
+        self._on_current_stream()
         ids = self._ints(t for p in prompts for t in p)
         where = self._ints(slots)
         self.ctx.pages_extend(self.pool, where, self._ints(counts))
@@ -498,11 +513,13 @@ class PagedDecoder(DenseDecoder):
     def drop(self, slots):
         """The slots give their pages back."""
         self.stop(slots)
+        self._on_current_stream()
         self.ctx.pages_free(self.pool, self._ints(slots))
 
     def fork(self, parent, children):
         """The children, empty slots, go on from where the parent is."""
         self._check_slots([parent] + list(children))
+        self._on_current_stream()
         where = self._ints(children)
         self.ctx.pages_fork(self.pool, self.planes, self._ints([parent] * len(children)), where)
         self.ctx.sync()
@@ -511,6 +528,7 @@ class PagedDecoder(DenseDecoder):
 
     def compact(self):
         """Moves the pages in use to the front of the pool; returns how many they are."""
+        self._on_current_stream()
         self.ctx.pages_compact(self.pool, self.planes, self.compact_work, self.used)
         self.ctx.sync()
         return int(self.used.item())

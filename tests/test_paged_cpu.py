@@ -226,3 +226,15 @@ def test_the_rule_between_runs_and_rows():
     assert wanted(capi.BF16, 128, 32, 8, 4, 1, 30000) == 0
     assert wanted(capi.BF16, 192, 32, 8, 6000, 1, 6000) == 0
     assert wanted(capi.BF16, 64, 129, 1, 6000, 1, 6000) == 0
+
+
+def test_how_many_rows_a_launch_takes():
+    """Blocks of 16 keys of a launch stay below 2^30, by tiles of eight or sixteen heads of a kv head."""
+    items = capi.lib().b2w4_paged_split_items
+    items.argtypes = [C.c_int, C.c_double, C.c_int, C.c_int, C.c_int]
+    assert items(64, 131072.0, 128, 64, 8) == 64
+    assert items(100000, 100000.0, 256, 8, 8) == 2 ** 30 // (6250 * 8)
+    assert items(100000, 100000.0, 256, 72, 8) == 2 ** 30 // (6250 * 16)
+    assert items(100000, 100000.0, 128, 128, 8) == 2 ** 30 // (6250 * 8)
+    assert items(20, 2.0 ** 31 - 1, 64, 1, 1) == 8
+    assert items(20, 2.0 ** 31 - 1, 64, 16, 16) == 0

@@ -190,6 +190,38 @@ def test_the_pool_runs_out_and_the_decoder_goes_on(model):
     d.free()
 
 
+def test_a_full_sequence_stays_and_the_others_go_on(model):
+    _, _, _, prompts, want = model
+    d = paged(model, max_length=35)       # five pages of eight: 40 tokens
+    d.add([prompts[2], prompts[0]], [0, 3])
+    tokens = [[], []]
+    for i in range(12):
+        tokens[0].append(int(d.token[0]))
+        tokens[1].append(int(d.token[3]))
+        d.step(replay=True)
+        if i == 6:
+            d.sync()
+    with pytest.raises(capi.B200W4Error):
+        d.sync()
+    assert d.lengths.tolist() == [40, 0, 0, 24, 0, 0]
+    assert same(tokens[0][:8], want[2]) and tokens[0][7:] == [tokens[0][7]] * 5
+    assert same(tokens[1], want[0])
+    d.free()
+
+
+def test_on_a_stream_of_the_callers(model):
+    _, _, ctx, prompts, want = model
+    d = paged(model)
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        got = d.generate(prompts, 24)
+        got_again = d.generate(prompts[::-1], 24, replay=True)
+    ctx.set_stream(0)
+    assert all(map(same, got, want)) and all(map(same, got_again[::-1], want))
+    d.free()
+
+
 def test_scores_of_a_prompt(model):
     cfg, _, ctx, prompts, _ = model
     d = paged(model)

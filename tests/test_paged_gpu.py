@@ -359,3 +359,64 @@ def test_a_slot_named_twice_is_reported(ctx):
     with pytest.raises(capi.B200W4Error, match="outside of what the call has"):
         ctx.sync()
     assert (cache.keep[1][1, 0, 2] == 1.0).all() and cache.keep[1].sum() == 64
+
+
+@pytest.mark.parametrize("dim,news", [(64, None), (192, [5, 9, 6])])
+def test_a_length_that_takes_several_launches(ctx, dim, news):
+    """A table with room for 2^31 - 1 tokens: eight rows to a launch."""
+    g, page = gen(5), 2 ** 20
+    lengths = [1 + 11 * i for i in range(20)] if not news else [5, 200, 90]
+    starts = starts_of(news or [1] * 20)
+    k = torch.randn(1, 1, 256, dim, generator=g).to(BF16)
+    v = torch.randn(1, 1, 256, dim, generator=g).to(BF16)
+    pools = [torch.zeros(1, 1, page, dim, dtype=BF16, device="cuda") for _ in range(2)]
+    for pool, x in zip(pools, (k, v)):
+        pool[:, :, :256] = x.cuda()
+    q = torch.randn(20, 2 * dim, generator=g)
+    tables = torch.zeros(len(lengths), 2048, dtype=torch.int32)
+    want, bound = ref.attention(q, k, v, tables, torch.tensor(lengths), page, starts,
+                                range(len(lengths)), 2, dim ** -0.5, 0, 0)
+    ints = lambda x: torch.tensor(x, dtype=torch.int32, device="cuda")  # noqa: E731
+    batch = capi.PagedBatch(tables.cuda(), ints(lengths), 2 ** 31 - 1,
+                            starts=ints(starts) if news else None, rows=20,
+                            max_new=max(news) if news else 1)
+    out = torch.full((20, 2 * dim), math.nan, device="cuda")
+    work = torch.empty(ctx.paged_attention_work(2, dim), dtype=torch.uint8, device="cuda")
+    before = ctx.launches
+    ctx.paged_attention(capi.PagedCache(*pools), batch, q.cuda(), 2, out, dim ** -0.5, work)
+    ctx.sync()
+    assert ctx.launches - before == 6
+    assert ((out.cpu().double() - want).abs() <= bound).all()
+
+
+def test_more_keys_than_a_launch_can_count_are_refused(ctx):
+    pool = torch.zeros(1, 16, 2 ** 20, 64, dtype=BF16, device="cuda")
+    q = torch.zeros(1, 16 * 64, device="cuda")
+    batch = capi.PagedBatch(torch.zeros(1, 2048, dtype=torch.int32, device="cuda"),
+                            torch.zeros(1, dtype=torch.int32, device="cuda"), 2 ** 31 - 1)
+    work = torch.empty(ctx.paged_attention_work(16, 64), dtype=torch.uint8, device="cuda")
+    with pytest.raises(capi.B200W4Error, match="max_length"):
+        ctx.paged_attention(capi.PagedCache(pool, pool), batch, q, 16, torch.empty_like(q), 1.0,
+                            work)
+
+
+@pytest.mark.parametrize("news", [None, [130, 20, 77]])
+def test_two_streams_at_once(ctx, news):
+    """Two contexts with work areas of their own give the bits that each gives alone."""
+    case = dict(lengths=[3000, 20, 777], news=news, page=16, heads=8, kv=2, dim=128, dtype=BF16)
+    first = run(ctx, case, 31)
+    second = run(ctx, dict(case, dtype=F16), 32)
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    contexts = [capi.Context(0), capi.Context(0)]
+    outs = []
+    torch.cuda.synchronize()
+    for c, s in zip(contexts, streams):
+        c.set_stream(s.cuda_stream)
+    for _ in range(20):
+        for c, (_, _, _, (cache, batch, qd, out, work, width)) in zip(contexts, (first, second)):
+            c.paged_attention(cache, batch, qd, 8, out[:, :width], 128 ** -0.5, work)
+    for c, (got, _, _, (_, _, _, out, _, width)) in zip(contexts, (first, second)):
+        c.sync()
+        outs.append(torch.equal(out.cpu()[:, :width], got))
+        c.close()
+    assert outs == [True, True]

@@ -312,3 +312,25 @@ def test_refusals(ctx):
             call()
     assert ctx.launches == launches
     d.check()
+
+
+def test_demands_whose_sum_passes_32_bits(ctx):
+    """1024 sequences that ask for 2^21 + 1 pages each of a pool of 16: none gets one."""
+    each = 2 ** 21 + 1
+    pool = capi.PagePool(ints([0] * 16), torch.empty((1024, each), dtype=torch.int32, device="cuda"),
+                         ints([0] * 1024), 1)
+    granted = ints([7] * 1024)
+    ctx.pages_extend(pool, counts=ints([0] + [each] * 1022 + [1]), granted=granted)
+    with pytest.raises(capi.B200W4Error, match="out of pages"):
+        ctx.sync()
+    refs, _, lengths = pool.keep
+    assert granted.tolist() == [0] + [-1] * 1023
+    assert int(lengths.abs().sum()) == 0 and int(refs.abs().sum()) == 0
+
+
+def test_a_pool_of_too_many_pages_is_refused(ctx):
+    one = ints([0])
+    pool = capi.PagePool(one, one.view(1, 1), one, 1)
+    pool.pages = 2 ** 30
+    with pytest.raises(capi.B200W4Error, match="2.30"):
+        ctx.pages_free(pool)
