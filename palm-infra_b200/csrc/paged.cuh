@@ -18,8 +18,7 @@ struct Args {
     int pages, kv_heads, page_size;
     int slots, table_len, sequences, rows, max_length;
     int* status;
-    bool by_row;             // paged::item: every row by itself
-    int first_item, items;  // ... of a launch
+    int first_item, items;  // paged::item: of a launch
     // x / page_size for 0 <= x < 2^31 (Granlund and Montgomery, Division by invariant integers
     // using multiplication, 1994): t = x multiplier >> 32, (t + (x - t >> shift1)) >> shift2
     uint32_t multiplier;
@@ -97,12 +96,13 @@ inline __host__ __device__ int sequence_of(const Args& a, int row) {
     return lo;
 }
 
-// What is attended one token at a time: the sequences, with their last token, or with by_row the
+// What is attended one token at a time: the sequences, with their last token, or with BY_ROW the
 // rows of all, each as a sequence that ends with its token (length 0: it has none; count 0: there
 // is no such row).  i: counted from the launch's first.
+template <bool BY_ROW>
 inline __host__ __device__ Sequence item(const Args& a, int i, bool* bad) {
     i += a.first_item;
-    if (!a.by_row)
+    if (!BY_ROW)
         return sequence(a, i, bad);
     const int n = sequence_of(a, i);
     if (n < 0)

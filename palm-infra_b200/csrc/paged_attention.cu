@@ -163,7 +163,7 @@ Args args_of(b2w4_ctx* ctx, const b2w4_paged_cache& c, const b2w4_paged_batch& b
     Args a = {c.k_dev,   c.v_dev,  b.tables_dev, b.lengths_dev, b.slots_dev,
               b.starts_dev, c.pages, c.kv_heads,   c.page_size,   b.slots,
               b.table_len, b.sequences, b.rows,    b.max_length,
-              ctx ? ctx->status_dev : nullptr, false, 0, 0, 0, 0, 0};
+              ctx ? ctx->status_dev : nullptr, 0, 0, 0, 0, 0};
     paged::set_division(a);
     return a;
 }
@@ -314,14 +314,12 @@ int b2w4_paged_attention(b2w4_ctx* ctx, const b2w4_paged_cache* cache,
         work_bytes < b2w4_paged_attention_work(ctx, heads, cache->dim))
         return b2w4_fail(ctx, B2W4_E_INVALID, "paged_attention: the work area is too small");
     const b2w4_device_guard device(ctx);
-    Args a = args_of(ctx, *cache, *batch);
+    const Args a = args_of(ctx, *cache, *batch);
     const Attend p = {q_dev, out_dev, scale, {window, sinks}, ldq, ldo, heads};
-    if (batch->max_new > 1) {
-        if (b2w4_paged_runs_wanted(ctx->sm_count, *cache, *batch, heads, window, sinks))
-            return b2w4_launch_paged_runs(ctx, cache->type, cache->dim, a, p);
-        a.by_row = true;
-    }
-    return b2w4_launch_paged_split(ctx, cache->type, cache->dim, a, p, work_dev);
+    const bool runs = batch->max_new > 1;
+    if (runs && b2w4_paged_runs_wanted(ctx->sm_count, *cache, *batch, heads, window, sinks))
+        return b2w4_launch_paged_runs(ctx, cache->type, cache->dim, a, p);
+    return b2w4_launch_paged_split(ctx, cache->type, cache->dim, a, p, runs, work_dev);
 }
 
 }  // extern "C"

@@ -36,4 +36,4 @@ bool b2w4_paged_runs_wanted(int sm_count, const b2w4_paged_cache& c, const b2w4_
 // One row per sequence, or row by row (paged_split.cu).
 size_t b2w4_paged_split_work(int sm_count, int dim);
 int b2w4_launch_paged_split(b2w4_ctx* ctx, int type, int dim, paged::Args a,
-                            const paged::Attend& p, void* work);
+                            const paged::Attend& p, bool by_row, void* work);

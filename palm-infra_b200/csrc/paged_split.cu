@@ -93,9 +93,10 @@ __device__ __forceinline__ Seen seen_by(const Sequence& s, const paged::Window& 
     v.count = v.low + s.length - v.from;
     return v;
 }
+template <bool BY_ROW>
 __device__ __forceinline__ int blocks_of(const Args& a, const paged::Window& w, int i, bool report) {
     bool bad = false;
-    const Sequence s = paged::item(a, i, &bad);
+    const Sequence s = paged::item<BY_ROW>(a, i, &bad);
     if (report && (bad || s.count > 1))
         b2w4_report(a.status, B2W4_E_INVALID);
     return (seen_by(s, w).count + kKeys - 1) / kKeys;
@@ -103,24 +104,26 @@ __device__ __forceinline__ int blocks_of(const Args& a, const paged::Window& w, 
 
 // Whole warp.  Blocks of all sequences; every tile (kv head and set of heads) of a sequence has as
 // many.  mine: those of sequence `lane`.
+template <bool BY_ROW>
 __device__ int line_of(const Args& a, const paged::Window& w, int tiles, bool report, int* mine) {
     const int lane = threadIdx.x & 31;
-    *mine = lane < a.items ? blocks_of(a, w, lane, report) : 0;
+    *mine = lane < a.items ? blocks_of<BY_ROW>(a, w, lane, report) : 0;
     int sum = *mine;
 #pragma unroll 4
     for (int i = lane + 32; i < a.items; i += 32)
-        sum += blocks_of(a, w, i, report);
+        sum += blocks_of<BY_ROW>(a, w, i, report);
     return __reduce_add_sync(0xffffffffu, sum) * tiles;
 }
 
 // Whole warp.  The sequence whose blocks hold block `at` of the line, and where they begin.
+template <bool BY_ROW>
 __device__ int find(const Args& a, const paged::Window& w, int tiles, int at, int mine, int* begin) {
     const int lane = threadIdx.x & 31;
     int before = 0;
     for (int base = 0; base < a.items; base += 32) {
         int n = mine * tiles;
         if (base > 0)
-            n = base + lane < a.items ? blocks_of(a, w, base + lane, false) * tiles : 0;
+            n = base + lane < a.items ? blocks_of<BY_ROW>(a, w, base + lane, false) * tiles : 0;
         int x = n;
 #pragma unroll
         for (int off = 1; off < 32; off <<= 1) {
@@ -310,7 +313,7 @@ struct Joined {
             part[2 * SET + row * DIM + lane + 32 * i] = o[i];
     }
     // the result of one of the owner's heads
-    template <typename T>
+    template <typename T, bool BY_ROW>
     __device__ __forceinline__ void finish(const Args& a, const Attend& p, const Owner& t, int head) {
         const int lane = threadIdx.x & 31;
         float* out = p.out + (size_t)t.row * p.ldo + (size_t)head * DIM;
@@ -325,7 +328,7 @@ struct Joined {
         __syncwarp();
         if (__any_sync(0xffffffffu, odd)) {
             bool bad = false;
-            const Sequence s = paged::item(a, t.seq, &bad);
+            const Sequence s = paged::item<BY_ROW>(a, t.seq, &bad);
             paged::attend_row<T, DIM>(a, s, p.q + (size_t)t.row * p.ldq + (size_t)head * DIM,
                                       s.length - 1, head / (p.heads / a.kv_heads), p.scale,
                                       p.window, out);
@@ -333,7 +336,7 @@ struct Joined {
     }
 };
 
-template <typename T, int DIM, int SET>
+template <typename T, int DIM, int SET, bool BY_ROW>
 __global__ void __launch_bounds__(Ring<T, DIM, SET>::kWarps * 32, 1)
 paged_split_kernel(const Args a, const Attend p, float* __restrict__ parts,
                    Owner* __restrict__ owners) {
@@ -350,7 +353,7 @@ paged_split_kernel(const Args a, const Attend p, float* __restrict__ parts,
     const int tiles = a.kv_heads * sets;
     Stream& stream = reinterpret_cast<Stream*>(smem + R::kBytes)[warp];
     int mine;
-    const int total = line_of(a, p.window, tiles, blockIdx.x + warp == 0, &mine);
+    const int total = line_of<BY_ROW>(a, p.window, tiles, blockIdx.x + warp == 0, &mine);
     // a share for every warp, or, where there are fewer blocks, for some warps of every thread block
     const int active = min(R::kWarps, max(1, (total + (int)gridDim.x - 1) / (int)gridDim.x));
     const int warps = gridDim.x * active, share = max(1, (total + warps - 1) / warps);
@@ -360,7 +363,7 @@ paged_split_kernel(const Args a, const Attend p, float* __restrict__ parts,
     // sequences that see no key
     for (int i = warp * gridDim.x + blockIdx.x; i < a.items; i += gridDim.x * R::kWarps) {
         bool bad = false;
-        const Sequence s = paged::item(a, i, &bad);
+        const Sequence s = paged::item<BY_ROW>(a, i, &bad);
         if (s.count == 1 && seen_by(s, p.window).count == 0)
             for (int d = lane; d < p.heads * DIM; d += 32)
                 p.out[(size_t)s.first * p.ldo + d] = 0.f;
@@ -373,7 +376,7 @@ paged_split_kernel(const Args a, const Attend p, float* __restrict__ parts,
     const uint32_t ring = (uint32_t)__cvta_generic_to_shared(smem) + warp * R::kSlots * R::kSlot;
     const int first = at;
     int begin;
-    int seq = find(a, p.window, tiles, at, mine, &begin);
+    int seq = find<BY_ROW>(a, p.window, tiles, at, mine, &begin);
     auto prefetch_queries = [&](int row, int kvh, int head0) {
         const float* q = p.q + (size_t)row * p.ldq + (size_t)head0 * DIM;
         for (int d = lane * 32; d < min(SET, (kvh + 1) * group - head0) * DIM; d += 1024)
@@ -392,16 +395,16 @@ paged_split_kernel(const Args a, const Attend p, float* __restrict__ parts,
             stream.kv_row = kvh * a.page_size;
         }
         bool bad = false;
-        prefetch_queries(paged::item(a, stream.seq, &bad).first, kvh,
+        prefetch_queries(paged::item<BY_ROW>(a, stream.seq, &bad).first, kvh,
                          kvh * group + (tile - kvh * sets) * SET);
         __syncwarp();
     };
     auto to_sequence = [&](int i) {  // the first from sequence i on that sees a key
         bool bad = false;
-        Sequence s = paged::item(a, i, &bad);
+        Sequence s = paged::item<BY_ROW>(a, i, &bad);
         Seen seen = seen_by(s, p.window);
         while (seen.count == 0 && i + 1 < a.items) {
-            s = paged::item(a, ++i, &bad);
+            s = paged::item<BY_ROW>(a, ++i, &bad);
             seen = seen_by(s, p.window);
         }
         __syncwarp();
@@ -476,7 +479,7 @@ paged_split_kernel(const Args a, const Attend p, float* __restrict__ parts,
 
     while (at < end) {
         bool bad = false;
-        const Sequence s = paged::item(a, seq, &bad);
+        const Sequence s = paged::item<BY_ROW>(a, seq, &bad);
         const Seen seen = seen_by(s, p.window);
         const int blocks = (seen.count + kKeys - 1) / kKeys;
         if (blocks == 0) {
@@ -816,7 +819,7 @@ paged_split_kernel(const Args a, const Attend p, float* __restrict__ parts,
 // kFew parts its heads are shared out to the blocks that have a place of it, and a block's warps take
 // the parts in turn.
 constexpr int kJoinWarps = 16, kFew = 20;
-template <typename T, int DIM, int SET>
+template <typename T, int DIM, int SET, bool BY_ROW>
 __global__ void __launch_bounds__(kJoinWarps * 32)
 paged_join_kernel(const Args a, const Attend p, const float* __restrict__ parts,
                   const Owner* __restrict__ owners, int places) {
@@ -837,7 +840,7 @@ paged_join_kernel(const Args a, const Attend p, const float* __restrict__ parts,
         for (int row = place / 2 - mine.first; row < mine.heads; row += mine.last - mine.first + 1) {
             Joined<DIM, SET> sum;
             sum.add([&](int w) { return part(mine, w); }, mine.first, mine.last, 1, row);
-            sum.template finish<T>(a, p, mine, mine.head0 + row);
+            sum.template finish<T, BY_ROW>(a, p, mine, mine.head0 + row);
         }
     }
     __syncthreads();
@@ -870,16 +873,16 @@ paged_join_kernel(const Args a, const Attend p, const float* __restrict__ parts,
             if (warp != 0)
                 continue;
             all.add([&](int w) { return s_part[w]; }, 0, kJoinWarps - 1, 1, 0);
-            all.template finish<T>(a, p, t, t.head0 + row);
+            all.template finish<T, BY_ROW>(a, p, t, t.head0 + row);
         }
     }
 }
 
-template <typename T, int DIM, int SET>
+template <typename T, int DIM, int SET, bool BY_ROW>
 int launch_set(b2w4_ctx* ctx, const Args& a, const Attend& p, void* work) {
     using R = Ring<T, DIM, SET>;
     static b2w4_smem_optin cfg;
-    auto kern = paged_split_kernel<T, DIM, SET>;
+    auto kern = paged_split_kernel<T, DIM, SET, BY_ROW>;
     constexpr size_t smem = R::kBytes + R::kWarps * sizeof(Stream);
     static_assert(smem <= 227 * 1024, "shared memory");
     B2W4_CUDA(ctx, b2w4_opt_in_smem(ctx, kern, smem, cfg));
@@ -890,7 +893,7 @@ int launch_set(b2w4_ctx* ctx, const Args& a, const Attend& p, void* work) {
     B2W4_CUDA(ctx, b2w4_launch_chained(ctx->pdl, kern, dim3(blocks), dim3(R::kWarps * 32), smem,
                                        ctx->stream, a, p, parts, owners));
     ctx->launches++;
-    B2W4_CUDA(ctx, b2w4_launch_chained(ctx->pdl, paged_join_kernel<T, DIM, SET>,
+    B2W4_CUDA(ctx, b2w4_launch_chained(ctx->pdl, paged_join_kernel<T, DIM, SET, BY_ROW>,
                                        dim3((2 * blocks * R::kWarps + kJoinWarps - 1) / kJoinWarps),
                                        dim3(kJoinWarps * 32), 0,
                                        ctx->stream, a, p, static_cast<const float*>(parts),
@@ -901,21 +904,27 @@ int launch_set(b2w4_ctx* ctx, const Args& a, const Attend& p, void* work) {
 }
 // Heads of a set: the registers of wide heads have no room for sixteen.
 int set_of(int dim, int group) { return dim <= 128 && group > 8 ? 16 : 8; }
-template <typename T, int DIM>
+template <typename T, int DIM, bool BY_ROW>
 int launch(b2w4_ctx* ctx, const Args& a, const Attend& p, void* work) {
     if constexpr (DIM <= 128)
         if (set_of(DIM, p.heads / a.kv_heads) == 16)
-            return launch_set<T, DIM, 16>(ctx, a, p, work);
-    return launch_set<T, DIM, 8>(ctx, a, p, work);
+            return launch_set<T, DIM, 16, BY_ROW>(ctx, a, p, work);
+    return launch_set<T, DIM, 8, BY_ROW>(ctx, a, p, work);
 }
-template <typename T>
+template <typename T, bool BY_ROW>
 int launch_dim(b2w4_ctx* ctx, int dim, const Args& a, const Attend& p, void* work) {
     switch (dim) {
-    case 64: return launch<T, 64>(ctx, a, p, work);
-    case 128: return launch<T, 128>(ctx, a, p, work);
-    case 192: return launch<T, 192>(ctx, a, p, work);
-    default: return launch<T, 256>(ctx, a, p, work);
+    case 64: return launch<T, 64, BY_ROW>(ctx, a, p, work);
+    case 128: return launch<T, 128, BY_ROW>(ctx, a, p, work);
+    case 192: return launch<T, 192, BY_ROW>(ctx, a, p, work);
+    default: return launch<T, 256, BY_ROW>(ctx, a, p, work);
     }
+}
+template <bool BY_ROW>
+int launch_type(b2w4_ctx* ctx, int type, int dim, const Args& a, const Attend& p, void* work) {
+    return type == B2W4_F16    ? launch_dim<__half, BY_ROW>(ctx, dim, a, p, work)
+           : type == B2W4_BF16 ? launch_dim<__nv_bfloat16, BY_ROW>(ctx, dim, a, p, work)
+                               : launch_dim<float, BY_ROW>(ctx, dim, a, p, work);
 }
 
 }  // namespace
@@ -937,8 +946,9 @@ extern "C" int b2w4_paged_split_items(int items, double keys, int dim, int heads
     return most < items ? (int)most : items;
 }
 
-int b2w4_launch_paged_split(b2w4_ctx* ctx, int type, int dim, Args a, const Attend& p, void* work) {
-    const int items = a.by_row ? a.rows : a.sequences;
+int b2w4_launch_paged_split(b2w4_ctx* ctx, int type, int dim, Args a, const Attend& p,
+                            bool by_row, void* work) {
+    const int items = by_row ? a.rows : a.sequences;
     double keys = a.max_length < (double)a.table_len * a.page_size
                       ? a.max_length
                       : (double)a.table_len * a.page_size;
@@ -951,9 +961,8 @@ int b2w4_launch_paged_split(b2w4_ctx* ctx, int type, int dim, Args a, const Atte
     for (int first = 0; first < items; first += a.items) {
         a.first_item = first;
         a.items = most < items - first ? most : items - first;
-        const int rc = type == B2W4_F16    ? launch_dim<__half>(ctx, dim, a, p, work)
-                       : type == B2W4_BF16 ? launch_dim<__nv_bfloat16>(ctx, dim, a, p, work)
-                                           : launch_dim<float>(ctx, dim, a, p, work);
+        const int rc = by_row ? launch_type<true>(ctx, type, dim, a, p, work)
+                              : launch_type<false>(ctx, type, dim, a, p, work);
         if (rc != B2W4_OK)
             return rc;
     }
