@@ -492,8 +492,8 @@ typedef struct b2w4_paged_cache {
  * call's rows among them.  Its rows are starts_dev[i] .. starts_dev[i + 1] - 1 (starts_dev NULL:
  * row i alone), its last tokens in order: row r has position length - (starts_dev[i + 1] - r).
  * A row whose position is negative has no token (an empty slot, or -1 for a slot, which names
- * none); rows behind the last sequence are left as they were.  max_new and max_length bound a sequence's rows and tokens;
- * they choose kernels and sizes.
+ * none); rows behind the last sequence are left as they were.  max_new and max_length bound a
+ * sequence's rows and tokens (both at least 1); they choose kernels and sizes.
  * The arrays are device memory, read when the call runs, so a captured call can be replayed as
  * they change.  What they say is bounded on the device: a slot, row count, length or page that
  * the call does not have is left out and b2w4_sync answers B2W4_E_INVALID. */
@@ -527,9 +527,10 @@ int b2w4_paged_attention(b2w4_ctx* ctx, const b2w4_paged_cache* cache,
  * b2w4_paged_batch.  All zero is an empty pool of empty slots.  Free pages are handed out lowest
  * first, so a call's result follows from the state and its arguments alone; entries of a table
  * behind a sequence's pages mean nothing.  None of the calls waits for the host or allocates, and
- * all can be captured.  A slot of -1 names none: its item does nothing.  Work that a call refuses on the device (a slot, page or length that is not
- * there, a slot named twice, a pool without enough pages) is left undone item by item, and
- * b2w4_sync answers B2W4_E_INVALID or B2W4_E_NOMEM. */
+ * all can be captured.  A slot of -1 names none: its item does nothing.  Work that a call refuses
+ * on the device (a slot, page or length that is not there, a slot named twice, a pool without enough
+ * pages) is left undone item by item, and b2w4_sync answers B2W4_E_INVALID or B2W4_E_NOMEM.  Fewer
+ * than 2^30 pages. */
 typedef struct b2w4_page_pool {
     int32_t *refs_dev, *tables_dev, *lengths_dev;
     int pages, page_size, slots, table_len;

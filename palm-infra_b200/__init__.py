@@ -5,7 +5,8 @@
   synth.py   seeded synthetic weights / activations of the benchmark shapes
   shard.py   tensor-parallel (row) and expert-parallel sharding of weights across ranks
   expert_parallel.py  routed MoE over ranks: local expert outputs, all-reduce, ordered combine
-  decoder.py a Qwen3-shaped dense decoder driven through the C ABI (benchmark configuration 3)
+  decoder.py a Qwen3-shaped decoder driven through the C ABI (benchmark configuration 3), and one
+             of several sequences on a paged cache (PagedDecoder)
   package.py reader for the reference's .mollm packages (dense Qwen3, W4G128 weights)
   build.py   in-tree nvcc build
 

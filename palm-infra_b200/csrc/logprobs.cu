@@ -8,13 +8,14 @@
 //
 // The k largest: a number below which the k-th largest cannot lie comes from the block's first tile
 // (the k-th largest of the maxima of 64 groups of its numbers), and what is not below it goes to a
-// list of its warp in shared memory.  After two tiles, four, eight, .. of a long chunk the lists are cut
-// back to the k largest so far, by counting for each entry how many are before it, and the k-th is the new
-// limit: about k numbers come between one time and the next.
+// list of its warp in shared memory.  After two tiles, four, eight, .. of a long chunk the lists are
+// cut back to the k largest so far, by counting for each entry how many are before it, and the k-th
+// is the new limit: about k numbers come between one time and the next.
 //
-// What bounds it: issue slots, about nine instructions for a number that takes four bytes of the
-// card's bandwidth; sums take two numbers an instruction, and a warp looks for numbers above the
-// limit only where a thread's largest of 16 is.
+// What bounds it: issue slots (64 % busy), about nine instructions for a number that takes four bytes
+// of the card's bandwidth; sums take two numbers an instruction, and a warp looks for numbers above
+// the limit only where a thread's largest of 16 is.  600 rows of 151,936 with the 20 largest: 86 us,
+// 4.2 TB/s.  One row of as many: 9.1 us, a first tile, its limit and the joins one after the other.
 #include "b200w4_internal.cuh"
 
 #include <math.h>

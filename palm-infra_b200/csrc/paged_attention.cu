@@ -37,8 +37,9 @@ struct Prepare {
 // what the row needs -- its sequence, position, cosines and sines -- is looked up once.  The
 // arithmetic is that of b2w4_qkv_prepare, operation for operation; keys and values are rounded to
 // the cache's type as they are stored.
-// What bounds it: memory traffic, for a few rows the chain of lookups.  With a warp for every head
-// and a lookup in each, 5980 rows of 32 / 8 heads of 128 into an fp32 cache took 48 us.
+// What bounds it: memory traffic, for a few rows the chain of lookups.  3208 rows of 32 / 8 heads of
+// 128 into an fp32 cache take 35 us (4.5 TB/s), 48 with a warp for every head and a lookup in each;
+// 64 rows 2.9 us with a warp for every head.
 template <typename T, int DIM, int EACH>
 __global__ void __launch_bounds__(32 * kWarps)
 paged_prepare_kernel(const Args a, const Prepare p) {
@@ -174,7 +175,12 @@ Args args_of(b2w4_ctx* ctx, const b2w4_paged_cache& c, const b2w4_paged_batch& b
 // that shares the cache's bytes out over the chip: long runs and many sequences to the former, a few
 // rows behind a long cache to the latter, by their times in us.  A tile's steps are those of
 // paged_runs.cu; row by row every token has its keys read again, from the second level cache for the
-// most part.  Heads of 192 and 256 numbers, and groups of more than 128, go row by row.
+// most part.  Heads of 192 and 256 numbers, and groups of more than 128, go row by row.  Measured, us
+// together / row by row, 32 heads over 8 of 128 in bf16: 2 rows behind 30,000 keys 591 / 50; 16 behind
+// 2000 46 / 32; 32 behind 4000 78 / 77; 64 behind 8000 153 / 266; 128 behind 4000 79 / 266.  In fp32: 16
+// behind 2000 101 / 55; 32 behind 4000 199 / 175; 128 behind 4000 202 / 656.  Of 120 shapes of three
+// types and four head layouts the rule takes the slower one by more than 15 % four times, by 53 % at
+// most (64 rows of 64 / 8 heads of 64 in fp32 behind 8000 keys, 296 where together takes 193).
 extern "C" int b2w4_paged_runs_wanted_by(int sm_count, int type, int dim, int heads, int kv_heads,
                                          int rows, int sequences, int max_length, int window,
                                          int sinks) {

@@ -13,17 +13,24 @@
 // fp32 cache; small products first.  Sums in tensor memory truncate, so those of an output are of
 // one block of keys, and the running output is in registers, one rounding per block.
 //
-// What bounds it: the MMAs, which the pieces multiply: 128 rows x 128 keys x 128 features in three
-// pieces are 48 MMAs of 66 cycles, about 3200 cycles; a softmax takes about 2000 beside them.
+// What bounds it: a step's rows, then the MMAs, which the pieces multiply.  128 rows x 128 keys x 128
+// features in three pieces are 48 MMAs of about 58 cycles, 2800 cycles; the rows' part of a step --
+// scores out of tensor memory, 2^x, the sum, three pieces, the running output -- is about 3500
+// beside them, and a step about 4150 (clock readings; the tensor pipe is 64 % busy).  6000 tokens of
+// 32 heads over 8 of 128, bf16, a window of 2048: 422 to 460 us from one GPU to another, 0.4 PFLOP/s
+// of the formula's products and 1.2 with the pieces'.  A tile's start and end, queries in and results
+// out, take about 10,000 cycles, which tell where rows see few keys: 333 tokens behind 900, fp32,
+// 69 us; six chunks of 50 to 700, fp16, 64 / 8 heads of 64 under a window of 512, 79.
 //
 // Blocks stay and take one tile after the other, so that a tile's first keys and values are on their
-// way while the one before is finished (6000 tokens, below, 455 us with a block per tile).
+// way while the one before is finished (6000 tokens as above with a block per tile: 455 to 498 us).
 //
 // Roles: warps of rows, two or four threads to a row; a warp that issues the MMAs, the scores' up to
-// two blocks ahead; one that looks the tiles up, two ahead; the rest bring keys and values.  Both lie in shared memory as they lie in
-// the cache, a key's features in 128-byte rows: the keys are the scores' B operand with features
-// running fastest, the values P V's with them running slowest, so neither is transposed.  Rows
-// come one by one with their pages' addresses, so a page may end anywhere.
+// two blocks ahead; one that looks the tiles up, two ahead; the rest bring keys and values.  Both lie
+// in shared memory as they lie in the cache, a key's features in 128-byte rows: the keys are the
+// scores' B operand with features running fastest, the values P V's with them running slowest, so
+// neither is transposed.  Rows come one by one with their pages' addresses, so a page may end
+// anywhere.
 //
 // A row whose result is not finite is done again key by key (paged::attend_row): a key that it does
 // not see, or that has no probability, may hold anything.  Every wait is bounded.
@@ -47,8 +54,8 @@ struct Cfg {
     static constexpr int kKeys = kWide || kTwo ? 64 : 128;
     static constexpr int kK = kWide ? 3 : 1;                             // pieces of a key
     static constexpr int kQ = std::is_same_v<T, __half> ? 2 : 3;         // of a query
-    // of them in tensor memory: an MMA whose operands both come from shared memory takes twice as
-    // long (its A is 128 bytes a cycle's worth of the port)
+    // of them in tensor memory, as many as it holds beside the rest (an MMA with both operands in
+    // shared memory takes as long, but the pieces' place there is wanted too)
     static constexpr int kQTmem = kWide ? 2 : kQ == 3 ? 1 : kQ;
     static constexpr int kParts = kWide || kTwo ? 2 : 4;  // threads to a row
     static constexpr int kRowWarps = 4 * kParts, kMmaWarp = kRowWarps;

@@ -11,7 +11,7 @@
 // sequences, and meets no other warp.  A part of the cache that began or ended inside another
 // warp's share goes to the work area; a second launch joins those.  (Joined by each thread block
 // first, what its warps have of a tile costs more than it saves: 64 sequences of 1028 keys 36 -> 37
-// us, two of 120,000 85 -> 93.)
+// us, two of 120,001 and 58,650 85 -> 93.)
 //
 // Products are mma.sync m16n8k16, the heads as the rows: with 16 heads a key costs 8192
 // multiply-adds, more than the fp32 pipe has in the time that the key's bytes take.  Every operand
