@@ -178,9 +178,9 @@ Args args_of(b2w4_ctx* ctx, const b2w4_paged_cache& c, const b2w4_paged_batch& b
 // most part.  Heads of 192 and 256 numbers, and groups of more than 128, go row by row.  Measured, us
 // together / row by row, 32 heads over 8 of 128 in bf16: 2 rows behind 30,000 keys 591 / 50; 16 behind
 // 2000 46 / 32; 32 behind 4000 78 / 77; 64 behind 8000 153 / 266; 128 behind 4000 79 / 266.  In fp32: 16
-// behind 2000 101 / 55; 32 behind 4000 199 / 175; 128 behind 4000 202 / 656.  Of 120 shapes of three
-// types and four head layouts the rule takes the slower one by more than 15 % four times, by 53 % at
-// most (64 rows of 64 / 8 heads of 64 in fp32 behind 8000 keys, 296 where together takes 193).
+// behind 2000 91 / 55; 32 behind 4000 180 / 175; 128 behind 4000 182 / 656.  Of 120 shapes of three
+// types and four head layouts the rule takes one that is slower by more than 5 % once, by 13 % (64 rows
+// of 64 / 4 heads of 128 in fp16 behind 8000 keys, 153 where together takes 135).
 extern "C" int b2w4_paged_runs_wanted_by(int sm_count, int type, int dim, int heads, int kv_heads,
                                          int rows, int sequences, int max_length, int window,
                                          int sinks) {
@@ -194,11 +194,15 @@ extern "C" int b2w4_paged_runs_wanted_by(int sm_count, int type, int dim, int he
         keys = (double)window + sinks + tq;
     const double tiles = ((double)rows / tq + 0.5 * sequences) * kv_heads;
     const double waves = ceil(tiles / (sm_count * (two ? 2 : 1)));
-    const double step = wide ? 3.3 : two ? 1.9 : 2.2;
+    // (two blocks beside each other share the products' rate)
+    const double step = wide ? (dim == 64 ? 1.6 : 2.8)
+                        : two ? (tiles <= sm_count ? 1.25 : 1.9) : 2.2;
     const double together = 6. + waves * (4. + keys / per * step);
-    const double sets = rep <= 8 || dim > 128 ? (rep + 7) / 8 : (rep + 15) / 16;
+    // row by row: bytes a microsecond, by what their products cost
+    const double sets = rep <= 8 ? 1 : (rep + 15) / 16;
     const double bytes = (double)rows * kv_heads * sets * keys * 2 * dim * (wide ? 4 : 2);
-    return together <= 12. + bytes / 6e6;
+    const double rate = (wide ? 6.8e6 : type == B2W4_F16 ? 12e6 : 8e6) * (rep <= 8 ? 1 : 0.66);
+    return together <= 12. + bytes / rate;
 }
 
 bool b2w4_paged_runs_wanted(int sm_count, const b2w4_paged_cache& c, const b2w4_paged_batch& b,

@@ -20,7 +20,7 @@
 // 32 heads over 8 of 128, bf16, a window of 2048: 422 to 460 us from one GPU to another, 0.4 PFLOP/s
 // of the formula's products and 1.2 with the pieces'.  A tile's start and end, queries in and results
 // out, take about 10,000 cycles, which tell where rows see few keys: 333 tokens behind 900, fp32,
-// 69 us; six chunks of 50 to 700, fp16, 64 / 8 heads of 64 under a window of 512, 79.
+// 62 us; six chunks of 50 to 700, fp16, 64 / 8 heads of 64 under a window of 512, 79.
 //
 // Blocks stay and take one tile after the other, so that a tile's first keys and values are on their
 // way while the one before is finished (6000 tokens as above with a block per tile: 455 to 498 us).
@@ -60,13 +60,13 @@ struct Cfg {
     static constexpr int kParts = kWide || kTwo ? 2 : 4;  // threads to a row
     static constexpr int kRowWarps = 4 * kParts, kMmaWarp = kRowWarps;
     // for the keys, and as many for the values
-    static constexpr int kLoadWarp0 = kRowWarps + 1, kLoadWarps = kWide ? 7 : 1;
+    static constexpr int kLoadWarp0 = kRowWarps + 1, kLoadWarps = kWide ? 9 : 1;
     static constexpr int kTileWarp = kLoadWarp0 + 2 * kLoadWarps, kThreads = (kTileWarp + 1) * 32;
     static_assert(kThreads % 128 == 0, "warpgroups");
     static constexpr int kBlocks = kTwo ? 2 : 1;  // of a multiprocessor
-    static constexpr int kRegsStart = kWide || kTwo ? 80 : 96;
+    static constexpr int kRegsStart = kWide ? 72 : kTwo ? 80 : 96;
     static constexpr int kRegsRows = kWide ? 128 : kTwo ? 96 : 104;
-    static constexpr int kRegsOther = kWide ? 56 : kTwo ? 48 : 64;
+    static constexpr int kRegsOther = kWide ? 48 : kTwo ? 48 : 64;
     static_assert(kParts * kRegsRows + (kThreads / 128 - kParts) * kRegsOther <=
                       kThreads / 128 * kRegsStart,
                   "registers of the block");
@@ -852,37 +852,44 @@ paged_runs_kernel(const Args a, const Attend p, int tq) {
                 break;
             }
             if constexpr (C::kWide) {
-                // a warp has every kLoadWarps-th set of kPer rows of a block; the next block's
-                // numbers are on their way
+                // A warp has every kLoadWarps-th set of kPer rows of a block.  Its lanes know where a
+                // block's rows lie, a block ahead, and the numbers of the next kDepth sets are on
+                // their way: as many as 48 registers hold (all five sets of seven warps in 56, some
+                // in local memory: 333 tokens behind 900 70 us, so 63).
                 constexpr int kSets = kKeys / kPer;
-                constexpr int kMine = (kSets + C::kLoadWarps - 1) / C::kLoadWarps;
-                ulonglong2 next[kMine][2];
-                auto load = [&](int j) {
-                    int rows[kMine];
-#pragma unroll
-                    for (int u = 0; u < kMine; ++u) {
-                        const int set = w0 + u * C::kLoadWarps;
-                        rows[u] = set < kSets ? row_of(j * kKeys + set * kPer + sub) : -1;
-                    }
-#pragma unroll
-                    for (int u = 0; u < kMine; ++u)
-#pragma unroll
-                        for (int h = 0; h < 2; ++h)
-                            next[u][h] = rows[u] >= 0
-                                             ? reinterpret_cast<const ulonglong2*>(
-                                                   pool + (size_t)rows[u] * DIM + c * 8)[h]
-                                             : make_ulonglong2(0ull, 0ull);
+                constexpr int kMine = (kSets + C::kLoadWarps - 1) / C::kLoadWarps, kDepth = 2;
+                static_assert(kMine * kPer <= 32 && kMine % kDepth == 0);
+                ulonglong2 next[kDepth][2];
+                auto look = [&](int j) {
+                    const int set = w0 + lane / kPer * C::kLoadWarps;
+                    return set < kSets ? row_of(j * kKeys + set * kPer + lane % kPer) : -1;
                 };
-                load(0);
+                auto load = [&](int rows, int u) {
+                    const int row = __shfl_sync(0xffffffffu, rows, u * kPer + sub);
+#pragma unroll
+                    for (int h = 0; h < 2; ++h)
+                        next[u % kDepth][h] = row >= 0 ? reinterpret_cast<const ulonglong2*>(
+                                                             pool + (size_t)row * DIM + c * 8)[h]
+                                                       : make_ulonglong2(0ull, 0ull);
+                };
+                int rows = look(0), ahead = look(1);
+#pragma unroll
+                for (int u = 0; u < kDepth; ++u)
+                    load(rows, u);
                 for (int j = 0; j < steps && free(g + j); ++j) {
 #pragma unroll
                     for (int u = 0; u < kMine; ++u) {
                         const int set = w0 + u * C::kLoadWarps;
-                        if (set >= kSets)
-                            break;
-                        uint64_t x[4] = {next[u][0].x, next[u][0].y, next[u][1].x, next[u][1].y};
+                        const ulonglong2 (&n)[2] = next[u % kDepth];
+                        uint64_t x[4] = {n[0].x, n[0].y, n[1].x, n[1].y};
                         uint8_t* dst =
                             mine + ((g + j) & 1) * C::kBuf + place(set * kPer + sub, c & 7);
+                        if (u + kDepth < kMine)
+                            load(rows, u + kDepth);
+                        else
+                            load(ahead, u + kDepth - kMine);
+                        if (set >= kSets)
+                            continue;
 #pragma unroll
                         for (int i = 0; i < C::kK; ++i) {
                             uint4 o;
@@ -894,7 +901,8 @@ paged_runs_kernel(const Args a, const Attend p, int tq) {
                         }
                     }
                     full(&filled[(g + j) & 1]);
-                    load(j + 1);
+                    rows = ahead;
+                    ahead = look(j + 2);
                 }
             } else {
                 // the warp's lanes know where some of a block's keys lie each, a block ahead
