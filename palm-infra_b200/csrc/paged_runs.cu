@@ -274,9 +274,10 @@ paged_runs_kernel(const Args a, const Attend p, int tq) {
         mbar_init(o_full, 1);
         mbar_init(drained, 1);
         for (int b = 0; b < 2; ++b) {
-            mbar_init(&k_full[b], C::kLoadWarps);
+            // (a lane's copies arrive by themselves)
+            mbar_init(&k_full[b], C::kWide ? C::kLoadWarps : 32);
             mbar_init(&k_free[b], 1);
-            mbar_init(&v_full[b], C::kLoadWarps);
+            mbar_init(&v_full[b], C::kWide ? C::kLoadWarps : 32);
             mbar_init(&v_free[b], 1);
             mbar_init(&tile_full[b], 1);
             mbar_init(&tile_free[b], kRowWarps + 1 + 2 * C::kLoadWarps);
@@ -713,9 +714,16 @@ paged_runs_kernel(const Args a, const Attend p, int tq) {
                                 size < C::kQ - 1 || i < size || k > 0);
                 }
             };
+            // what the loaders' asynchronous copies wrote is for the tensor core to read; where they
+            // write it themselves they say so
+            auto copied = [&]() {
+                if (!C::kWide)
+                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            };
             auto scores_wait = [&](int j) {
                 const bool ok = __all_sync(0xffffffffu, wait(&k_full[j & 1], (j >> 1) & 1) &&
                                                             (j == 0 || wait(s_free, (j - 1) & 1)));
+                copied();
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                 return ok;
             };
@@ -726,6 +734,7 @@ paged_runs_kernel(const Args a, const Attend p, int tq) {
                 if (!__all_sync(0xffffffffu,
                                 wait(&v_full[j & 1], (j >> 1) & 1) && wait(p_full, j & 1)))
                     return false;
+                copied();
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                 if (elect_one())
                     output(j, C::kQ - 1);
@@ -905,9 +914,16 @@ paged_runs_kernel(const Args a, const Attend p, int tq) {
                     ahead = look(j + 2);
                 }
             } else {
-                // the warp's lanes know where some of a block's keys lie each, a block ahead
+                // The warp's lanes know where some of a block's keys lie each, a block ahead.  A copy
+                // is a shuffle, an address and the copy: what of its place depends on the lane is
+                // the same for every eighth row, and whether a row exists is asked once for a block.
                 static_assert(C::kWide || C::kLoadWarps == 1);
-                constexpr int kEach = kKeys / 32;
+                constexpr int kEach = kKeys / 32, kPeriod = 8 / kPer;
+                uint32_t place_of[kPeriod];
+#pragma unroll
+                for (int e = 0; e < kPeriod; ++e)
+                    place_of[e] = smem_u32(mine) + place(e * kPer + sub, c & 7);
+                const T* const source = pool + c * 8;
                 int next[kEach], rows[kEach];
                 auto look = [&](int j) {
 #pragma unroll
@@ -916,34 +932,53 @@ paged_runs_kernel(const Args a, const Attend p, int tq) {
                 };
                 look(0);
                 for (int j = 0; j < steps && free(g + j); ++j) {
+                    bool whole = true;
 #pragma unroll
-                    for (int u = 0; u < kEach; ++u)
+                    for (int u = 0; u < kEach; ++u) {
                         rows[u] = next[u];
+                        whole &= rows[u] >= 0;
+                    }
+                    whole = __all_sync(0xffffffffu, whole);
                     look(j + 1);
-                    uint8_t* const to = mine + ((g + j) & 1) * C::kBuf;
+                    const uint32_t to = ((g + j) & 1) * C::kBuf;
                     // the rows of eight copies are fetched ahead of them: one by one, every copy
                     // waited for its shuffle (80 cycles each)
+                    auto copy = [&](int rows, int i0, int first, bool whole) {
+                        int r[8];
 #pragma unroll
-                    for (int u = 0; u < kEach; ++u)
+                        for (int e = 0; e < 8; ++e)
+                            r[e] = __shfl_sync(0xffffffffu, rows, (i0 + e) * kPer + sub);
 #pragma unroll
-                        for (int i = 0; i < 32 / kPer; i += 8) {
-                            int r[8];
-#pragma unroll
-                            for (int e = 0; e < 8; ++e)
-                                r[e] = __shfl_sync(0xffffffffu, rows[u], (i + e) * kPer + sub);
-#pragma unroll
-                            for (int e = 0; e < 8; ++e)
-                                cp16(smem_u32(to + place(u * 32 + (i + e) * kPer + sub, c & 7)),
-                                     pool + (size_t)max(r[e], 0) * DIM + c * 8, r[e] >= 0);
+                        for (int e = 0; e < 8; ++e) {
+                            const int at = first + (i0 + e) * kPer;
+                            const bool there = whole || r[e] >= 0;
+                            cp16(place_of[e % kPeriod] + to + at / 8 * 1024,
+                                 source + (size_t)(there ? (unsigned)r[e] : 0u) * DIM, there);
                         }
-                    asm volatile("cp.async.commit_group;" ::: "memory");
-                    asm volatile("cp.async.wait_group 0;" ::: "memory");
-                    full(&filled[(g + j) & 1]);
+                    };
+                    if (whole) {
+#pragma unroll
+                        for (int u = 0; u < kEach; ++u)
+#pragma unroll
+                            for (int i = 0; i < 32 / kPer; i += 8)
+                                copy(rows[u], i, u * 32, true);
+                    } else {
+#pragma unroll
+                        for (int u = 0; u < kEach; ++u)
+#pragma unroll 1
+                            for (int i = 0; i < 32 / kPer; i += 8)
+                                copy(rows[u], i, u * 32, false);
+                    }
+                    // when they have all come; the warp goes on with the next block
+                    asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];"
+                                 ::"r"(smem_u32(&filled[(g + j) & 1]))
+                                 : "memory");
                 }
             }
             g += steps;
             warp_arrive(&tile_free[n & 1]);
         }
+        asm volatile("cp.async.wait_all;" ::: "memory");
       }
     }
 
