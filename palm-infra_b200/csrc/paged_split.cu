@@ -12,6 +12,9 @@
 // warp's share goes to the work area; a second launch joins those.  (Joined by each thread block
 // first, what its warps have of a tile costs more than it saves: 64 sequences of 1028 keys 36 -> 37
 // us, two of 120,001 and 58,650 85 -> 93.)
+// 120,001 and 58,650 keys of 64 heads over 4 of 128, bf16: 83 us (4.4 TB/s; 255 registers leave two
+// warps a scheduler, whose latencies show); 64 sequences under a window of 1024, 64 heads over 8 of 64,
+// fp16: 32 us; one of 300 tokens: 11 us, 7 of them lookups and first loads, 3 the join.
 //
 // Products are mma.sync m16n8k16, the heads as the rows: with 16 heads a key costs 8192
 // multiply-adds, more than the fp32 pipe has in the time that the key's bytes take.  Every operand
@@ -211,17 +214,24 @@ __device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint3
 template <typename T>
 __device__ __forceinline__ uint32_t take_piece(float& lo, float& hi) {
     uint32_t p;
+    float x, y;
     if constexpr (std::is_same_v<T, __half>) {
         asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(p) : "f"(hi), "f"(lo));
         const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&p));
-        lo = __fsub_rn(lo, f.x);
-        hi = __fsub_rn(hi, f.y);
+        x = f.x;
+        y = f.y;
     } else {
         asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(p) : "f"(hi), "f"(lo));
-        lo = __fsub_rn(lo, __uint_as_float(p << 16));
-        hi = __fsub_rn(hi, __uint_as_float(p & 0xffff0000u));
+        x = __uint_as_float(p << 16);
+        y = __uint_as_float(p & 0xffff0000u);
     }
+    b2w4_unpack2(b2w4_sub2(b2w4_pack2(lo, hi), b2w4_pack2(x, y)), lo, hi);
     return p;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+    uint64_t d;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
 }
 __device__ __forceinline__ float exp2_neg(float x) {
     float r;
@@ -563,12 +573,12 @@ paged_split_kernel(const Args a, const Attend p, float* __restrict__ parts,
             l[h] = 0.f;
             factor[h] = __fmul_rn(__fmul_rn(p.scale, 1.4426950408889634f), unscale[h]);
         }
-        float o[kTiles][2 * kHalves];
+        uint64_t o[kTiles][kHalves];  // two columns each
 #pragma unroll
         for (int i = 0; i < kTiles; ++i)
 #pragma unroll
-            for (int e = 0; e < 2 * kHalves; ++e)
-                o[i][e] = 0.f;
+            for (int h = 0; h < kHalves; ++h)
+                o[i][h] = 0ull;
 
         auto block = [&](int slot, unsigned keys) {
             const uint32_t ks = ring + slot * R::kSlot, vs = ks + R::kHalf;
@@ -661,15 +671,17 @@ paged_split_kernel(const Args a, const Attend p, float* __restrict__ parts,
                                                     pr[e >> 1][2 * (e & 1) + 1]);
                 operands(piece, [&](int i, int e) -> uint32_t& { return pp[i][e]; });
             }
+            uint64_t alpha2[kHalves];
+#pragma unroll
+            for (int h = 0; h < kHalves; ++h)
+                alpha2[h] = b2w4_pack2(alpha[h], alpha[h]);
             auto add = [&](int n, const float (&x)[4]) {
+                const uint64_t x0 = b2w4_pack2(x[0], x[1]), x1 = b2w4_pack2(x[2], x[3]);
                 if constexpr (SET == 16) {
-#pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        o[n][e] = __fmaf_rn(o[n][e], alpha[e >> 1], x[e]);
+                    o[n][0] = b2w4_fma2(o[n][0], alpha2[0], x0);
+                    o[n][1] = b2w4_fma2(o[n][1], alpha2[1], x1);
                 } else {
-#pragma unroll
-                    for (int e = 0; e < 2; ++e)
-                        o[n][e] = __fmaf_rn(o[n][e], alpha[0], __fadd_rn(x[2 + e], x[e]));
+                    o[n][0] = b2w4_fma2(o[n][0], alpha2[0], add2(x1, x0));
                 }
             };
             if constexpr (kWide) {
@@ -782,18 +794,23 @@ paged_split_kernel(const Args a, const Attend p, float* __restrict__ parts,
             };
             if constexpr (kWide) {
 #pragma unroll
-                for (int j = 0; j < DIM / 32; ++j)
+                for (int j = 0; j < DIM / 32; ++j) {
+                    float x[4][2];
+#pragma unroll
+                    for (int n = 0; n < 4; ++n)
+                        b2w4_unpack2(o[4 * j + n][h], x[n][0], x[n][1]);
 #pragma unroll
                     for (int e = 0; e < 2; ++e)
-                        *reinterpret_cast<float4*>(dst + 32 * j + 8 * t + 4 * e) =
-                            make_float4(final(o[4 * j][2 * h + e]), final(o[4 * j + 1][2 * h + e]),
-                                        final(o[4 * j + 2][2 * h + e]),
-                                        final(o[4 * j + 3][2 * h + e]));
+                        *reinterpret_cast<float4*>(dst + 32 * j + 8 * t + 4 * e) = make_float4(
+                            final(x[0][e]), final(x[1][e]), final(x[2][e]), final(x[3][e]));
+                }
             } else {
 #pragma unroll
-                for (int n = 0; n < kTiles; ++n)
-                    *reinterpret_cast<float2*>(dst + 8 * n + 2 * t) =
-                        make_float2(final(o[n][2 * h]), final(o[n][2 * h + 1]));
+                for (int n = 0; n < kTiles; ++n) {
+                    float x, y;
+                    b2w4_unpack2(o[n][h], x, y);
+                    *reinterpret_cast<float2*>(dst + 8 * n + 2 * t) = make_float2(final(x), final(y));
+                }
             }
         }
         __syncwarp();
