@@ -14,6 +14,8 @@ weights; torch provides device memory only.
 Activation rule of the matmuls: the reference's -- per 128 values for one row (decode), per 32
 values for several (prefill) -- unless `multi_row_rule` says otherwise.
 """
+import contextlib
+
 import numpy as np
 
 from . import capi, synth
@@ -453,6 +455,21 @@ class PagedDecoder(DenseDecoder):
         if len(set(slots)) != len(slots) or not all(0 <= s < self.slots for s in slots):
             raise ValueError(f"slots {slots}: different ones of {self.slots} are wanted")
 
+    @contextlib.contextmanager
+    def _whole_or_not(self):
+        """What is done to the sequences within is done whole or, where it raises, not at all.  The
+        device refuses item by item: of several prompts the first may have its pages when the pool
+        has none for the second, and would then count tokens that nothing was computed for.  Pages
+        are taken behind the sequences' ends, where tables and pages mean nothing, so lengths and
+        counts are all that there is to put back."""
+        kept = self.lengths.clone(), self.refs.clone()
+        try:
+            yield
+        except BaseException:
+            self.lengths.copy_(kept[0])
+            self.refs.copy_(kept[1])
+            raise
+
     def _prompts(self, prompts, slots):
         """Extends the slots by their prompts and runs those; (hidden rows, starts)."""
         self._check_slots(slots)
@@ -464,19 +481,21 @@ class PagedDecoder(DenseDecoder):
         ids = self._ints(t for p in prompts for t in p)
         where = self._ints(slots)
         self.ctx.pages_extend(self.pool, where, self._ints(counts))
-        # the pool may have refused: nothing runs on a sequence that is not there
+        # the pool may have refused: nothing runs on a sequence without its pages
         self.ctx.sync()
         batch = capi.PagedBatch(self.tables, self.lengths, self.capacity, slots=where,
                                 starts=self._ints(starts), rows=starts[-1], max_new=max(counts))
         return self._rows(self.ctx, ids, batch, starts[-1]), starts
 
     def add(self, prompts, slots):
-        """Runs prompts into slots (empty ones, or behind what is there) and starts them."""
-        h, starts = self._prompts(prompts, slots)
-        last = self._ints(s - 1 for s in starts[1:])
-        rows = h.index_select(0, last)
-        tokens = self.torch.empty(len(slots), dtype=self.torch.int32, device="cuda")
-        self._greedy(self.ctx, rows, tokens)
+        """Runs prompts into slots (empty ones, or behind what is there) and starts them: all of
+        them, or, where it raises, none."""
+        with self._whole_or_not():
+            h, starts = self._prompts(prompts, slots)
+            last = self._ints(s - 1 for s in starts[1:])
+            rows = h.index_select(0, last)
+            tokens = self.torch.empty(len(slots), dtype=self.torch.int32, device="cuda")
+            self._greedy(self.ctx, rows, tokens)
         where = self._ints(slots).long()
         self.token.index_copy_(0, where, tokens)
         self.running.index_copy_(0, where, self._ints(slots))
@@ -484,24 +503,27 @@ class PagedDecoder(DenseDecoder):
     def score(self, ids, slot, top=0):
         """Runs ids into an empty slot that then stops; of each token after the first the log
         probability, the entropy of its distribution and, with top, the most likely tokens and
-        their log probabilities (tensors of len(ids) - 1 rows)."""
+        their log probabilities (tensors of len(ids) - 1 rows).  Where it raises, the slot is as it
+        was."""
         torch = self.torch
         if len(ids) < 2:
             raise ValueError("two tokens or more")
-        h, _ = self._prompts([ids], [slot])
         n = len(ids) - 1
-        targets = self._ints(ids[1:])
-        out = {"logprob": torch.empty(n, device="cuda"), "entropy": torch.empty(n, device="cuda")}
-        if top:
-            out["top_values"] = torch.empty((n, top), device="cuda")
-            out["top_indices"] = torch.empty((n, top), dtype=torch.int32, device="cuda")
-        step = 256  # rows of logits at a time
-        for first in range(0, n, step):
-            rows = min(step, n - first)
-            logits = self._b("logits", rows, self.cfg.vocab)
-            self.ctx.matmul(self.lm_head, h[first:first + rows], logits, rule=capi.ACT_G128)
-            self.ctx.logprobs(logits, targets[first:first + rows],
-                              **{k: v[first:first + rows] for k, v in out.items()})
+        with self._whole_or_not():
+            h, _ = self._prompts([ids], [slot])
+            targets = self._ints(ids[1:])
+            out = {"logprob": torch.empty(n, device="cuda"),
+                   "entropy": torch.empty(n, device="cuda")}
+            if top:
+                out["top_values"] = torch.empty((n, top), device="cuda")
+                out["top_indices"] = torch.empty((n, top), dtype=torch.int32, device="cuda")
+            step = 256  # rows of logits at a time
+            for first in range(0, n, step):
+                rows = min(step, n - first)
+                logits = self._b("logits", rows, self.cfg.vocab)
+                self.ctx.matmul(self.lm_head, h[first:first + rows], logits, rule=capi.ACT_G128)
+                self.ctx.logprobs(logits, targets[first:first + rows],
+                                  **{k: v[first:first + rows] for k, v in out.items()})
         self.stop([slot])
         return out
 

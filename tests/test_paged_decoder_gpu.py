@@ -251,3 +251,43 @@ def test_refusals(model):
             call()
     assert int(d.refs.sum()) == 0
     d.free()
+
+
+def state_of(d):
+    return [t.clone() for t in (d.lengths, d.refs, d.running, d.token)]
+
+
+def test_prompts_that_do_not_all_fit_change_nothing(model):
+    """The first prompt fits and the second does not: neither is taken, in an empty slot or in one
+    that is running, and what comes behind the refusal is as if it had not been asked for."""
+    _, _, _, prompts, want = model
+    d = paged(model, pages=13)
+    d.add([prompts[0]], [2])              # 12 tokens: two pages
+    d.step()
+    before = state_of(d)
+    for first, slot in ((prompts[2], 0), (prompts[3] + prompts[2], 2)):
+        with pytest.raises(capi.B200W4Error, match="out of pages"):
+            d.add([first, prompts[4]], [slot, 1])   # five or seven pages, and nine: eleven are left
+        assert all(torch.equal(a, b) for a, b in zip(state_of(d), before))
+    with pytest.raises(capi.B200W4Error):
+        d.add([prompts[1], [1] * 161], [0, 1])      # longer than a sequence may be
+    assert all(torch.equal(a, b) for a, b in zip(state_of(d), before))
+    d.add([prompts[2]], [0])
+    tokens = [[], []]
+    for _ in range(10):
+        for t, slot in zip(tokens, (2, 0)):
+            t.append(int(d.token[slot]))
+        d.step(replay=True)
+    d.sync()
+    assert same(tokens[0], want[0][1:]) and same(tokens[1], want[2])
+    d.free()
+
+
+@pytest.mark.parametrize("top", [-1, 33])
+def test_a_score_that_is_refused_takes_no_slot(model, top):
+    _, _, _, prompts, _ = model
+    d = paged(model)
+    with pytest.raises(RuntimeError):
+        d.score(prompts[0], 3, top=top)
+    assert int(d.refs.sum()) == 0 and int(d.lengths.sum()) == 0
+    d.free()
