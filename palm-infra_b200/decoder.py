@@ -545,7 +545,7 @@ class PagedDecoder(DenseDecoder):
         where = self._ints(children)
         self.ctx.pages_fork(self.pool, self.planes, self._ints([parent] * len(children)), where)
         self.ctx.sync()
-        self.token.index_copy_(0, where.long(), self.token[parent].expand(len(children)))
+        self.token.index_fill_(0, where.long(), self.token[parent])
         self.running.index_copy_(0, where.long(), where)
 
     def compact(self):

@@ -291,3 +291,18 @@ def test_a_score_that_is_refused_takes_no_slot(model, top):
         d.score(prompts[0], 3, top=top)
     assert int(d.refs.sum()) == 0 and int(d.lengths.sum()) == 0
     d.free()
+
+
+def test_a_fork_with_one_child(model):
+    _, _, _, prompts, want = model
+    d = paged(model)
+    d.add([prompts[0]], [0])
+    d.fork(0, [4])
+    tokens = {0: [], 4: []}
+    for _ in range(6):
+        for s, t in tokens.items():
+            t.append(int(d.token[s]))
+        d.step()
+    d.sync()
+    assert tokens[0] == tokens[4] and same(tokens[4], want[0])
+    d.free()
