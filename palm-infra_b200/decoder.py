@@ -539,12 +539,15 @@ class PagedDecoder(DenseDecoder):
         self.ctx.pages_free(self.pool, self._ints(slots))
 
     def fork(self, parent, children):
-        """The children, empty slots, go on from where the parent is."""
+        """The children, empty slots, go on from where the parent is: all of them, or, where it
+        raises, none."""
         self._check_slots([parent] + list(children))
         self._on_current_stream()
         where = self._ints(children)
-        self.ctx.pages_fork(self.pool, self.planes, self._ints([parent] * len(children)), where)
-        self.ctx.sync()
+        with self._whole_or_not():
+            self.ctx.pages_fork(self.pool, self.planes, self._ints([parent] * len(children)),
+                                where)
+            self.ctx.sync()
         self.token.index_fill_(0, where.long(), self.token[parent])
         self.running.index_copy_(0, where.long(), where)
 

@@ -306,3 +306,27 @@ def test_a_fork_with_one_child(model):
     d.sync()
     assert tokens[0] == tokens[4] and same(tokens[4], want[0])
     d.free()
+
+
+def test_forks_that_do_not_all_fit_change_nothing(model):
+    _, _, _, prompts, want = model
+    d = paged(model, pages=5)
+    d.add([prompts[0]], [0])              # 12 tokens: a full page and one that every child copies
+    before = state_of(d)
+    with pytest.raises(capi.B200W4Error, match="out of pages"):
+        d.fork(0, [1, 2, 3, 4])
+    assert all(torch.equal(a, b) for a, b in zip(state_of(d), before))
+    d.fork(0, [1])
+    before = state_of(d)
+    with pytest.raises(capi.B200W4Error):
+        d.fork(0, [3, 1])                 # a child that is not empty
+    assert all(torch.equal(a, b) for a, b in zip(state_of(d), before))
+    d.fork(0, [3, 4])
+    tokens = {s: [] for s in (0, 1, 3, 4)}
+    for _ in range(4):
+        for s, t in tokens.items():
+            t.append(int(d.token[s]))
+        d.step()
+    d.sync()
+    assert all(same(t, want[0]) for t in tokens.values())
+    d.free()
