@@ -391,6 +391,14 @@ class PagedDecoder(DenseDecoder):
         self.step_batch = capi.PagedBatch(self.tables, self.lengths, max_length,
                                           slots=self.granted)
 
+    def _one_sequence(self, *args, **kw):
+        """What takes the cache for a contiguous one of 32-bit numbers: in the pages it would write
+        over other sequences' rows, and past the end of a pool of 16-bit numbers."""
+        raise NotImplementedError("a paged decoder has slots: add, step, stop, fork, drop, generate")
+
+    forward = prefill = decode_step = _one_sequence
+    capture_decode_step = replay_decode_step = reset = _one_sequence
+
     def _layer_cache(self):
         shape = (self.pages, self.cfg.kv_heads, self.page_size, self.cfg.head_dim)
         return {k: self.torch.zeros(shape, dtype=self.cache_type, device=self.device)

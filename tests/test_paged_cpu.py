@@ -238,3 +238,14 @@ def test_how_many_rows_a_launch_takes():
     assert items(100000, 100000.0, 128, 128, 8) == 2 ** 30 // (6250 * 8)
     assert items(20, 2.0 ** 31 - 1, 64, 1, 1) == 8
     assert items(20, 2.0 ** 31 - 1, 64, 16, 16) == 0
+
+
+@pytest.mark.parametrize("name,args", [
+    ("forward", (None, 1)), ("prefill", ([1],)), ("decode_step", ()), ("capture_decode_step", ()),
+    ("replay_decode_step", ()), ("reset", ())])
+def test_a_paged_decoder_refuses_the_calls_of_one_sequence(name, args):
+    """They take the cache for a contiguous one of 32-bit numbers: in the pages they would write
+    over other sequences, and beyond the pool's end where that is of 16 bits."""
+    d = pkg.decoder.PagedDecoder.__new__(pkg.decoder.PagedDecoder)
+    with pytest.raises(NotImplementedError, match="slots"):
+        getattr(d, name)(*args)
