@@ -496,7 +496,8 @@ typedef struct b2w4_paged_cache {
  * sequence's rows and tokens (both at least 1); they choose kernels and sizes.
  * The arrays are device memory, read when the call runs, so a captured call can be replayed as
  * they change.  What they say is bounded on the device: a slot, row count, length or page that
- * the call does not have is left out and b2w4_sync answers B2W4_E_INVALID. */
+ * the call does not have is left out and b2w4_sync answers B2W4_E_INVALID.  A sequence with such
+ * a length (negative, beyond max_length or its table) has no token in the call. */
 typedef struct b2w4_paged_batch {
     const int32_t *tables_dev, *lengths_dev, *slots_dev, *starts_dev;
     int slots, table_len, sequences, rows, max_new, max_length;

@@ -78,6 +78,17 @@ inline __host__ __device__ Sequence sequence(const Args& a, int i, bool* bad) {
     return s;
 }
 
+// As the kernels take it: a sequence whose length is not one that the call can have has no token in
+// it.  (With its length only bounded, a new key would be written over a good one further ahead.)
+inline __host__ __device__ Sequence taken(const Args& a, int i, bool* bad) {
+    bool wrong = false;
+    Sequence s = sequence(a, i, &wrong);
+    if (wrong)
+        s.length = 0;
+    *bad |= wrong;
+    return s;
+}
+
 // The sequence that row `row` of the call belongs to: the last one that begins at or before it;
 // -1 where the row lies before the first sequence or behind the last.
 inline __host__ __device__ int sequence_of(const Args& a, int row) {
@@ -103,11 +114,11 @@ template <bool BY_ROW>
 inline __host__ __device__ Sequence item(const Args& a, int i, bool* bad) {
     i += a.first_item;
     if (!BY_ROW)
-        return sequence(a, i, bad);
+        return taken(a, i, bad);
     const int n = sequence_of(a, i);
     if (n < 0)
         return {a.tables, 0, 0, 0};
-    Sequence s = sequence(a, n, bad);
+    Sequence s = taken(a, n, bad);
     const int in = i - s.first;
     if (in >= s.count)
         return {a.tables, 0, 0, 0};

@@ -61,7 +61,7 @@ paged_prepare_kernel(const Args a, const Prepare p) {
     if (i < 0)
         return;
     bool bad = false;
-    const Sequence s = paged::sequence(a, i, &bad);
+    const Sequence s = paged::taken(a, i, &bad);
     if (bad)
         b2w4_report(a.status, B2W4_E_INVALID);
     const int in = row - s.first;
@@ -243,7 +243,7 @@ extern "C" const char* b2w4_paged_refusal(const b2w4_paged_cache* c, const b2w4_
 // Where token j of a sequence lies, by the kernels' own arithmetic: for checks without a device
 // (every pointer of the batch is host memory).  The row of the pools, -1 for a page that is not
 // theirs, -2 where the sequence is not one of the batch's or has no such token; length, first
-// and count as the kernels bound them.
+// and count as they are bounded (what is out of bounds has no token: paged::taken).
 extern "C" int b2w4_paged_row(const b2w4_paged_cache* c, const b2w4_paged_batch* b, int i, int j,
                               int h, int* length, int* first, int* count) {
     const Args a = args_of(nullptr, *c, *b);

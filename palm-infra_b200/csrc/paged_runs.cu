@@ -204,7 +204,7 @@ __device__ bool find_tile(const Args& a, int tq, int at, int* seq, int* t0) {
         int n = 0;
         if (i >= 0) {
             bool bad = false;
-            n = (paged::sequence(a, i, &bad).count + tq - 1) / tq;
+            n = (paged::taken(a, i, &bad).count + tq - 1) / tq;
             if (bad)
                 b2w4_report(a.status, B2W4_E_INVALID);
         }
@@ -640,7 +640,7 @@ paged_runs_kernel(const Args a, const Attend p, int tq) {
                 for (int r = part; r < 32; r += kParts)
                     if ((mine >> r & 1) && live && !*s_abort) {
                         bool bad = false;
-                        const Sequence s = paged::sequence(a, t.seq, &bad);
+                        const Sequence s = paged::taken(a, t.seq, &bad);
                         const int q = quarter * 32 + r;
                         paged::attend_row<T, DIM>(a, s, p.q + row_offset(q, p.ldq),
                                                   t.p0() + token_of(q), t.kvh, p.scale, p.window,
@@ -796,7 +796,7 @@ paged_runs_kernel(const Args a, const Attend p, int tq) {
             t.kvh = at % a.kv_heads;
             if (find_tile(a, tq, at / a.kv_heads, &t.seq, &t.t0)) {
                 bool bad = false;
-                const Sequence s = paged::sequence(a, t.seq, &bad);
+                const Sequence s = paged::taken(a, t.seq, &bad);
                 t.table = s.table;
                 t.first = s.first;
                 t.count = s.count;

@@ -420,3 +420,40 @@ def test_two_streams_at_once(ctx, news):
         outs.append(torch.equal(out.cpu()[:, :width], got))
         c.close()
     assert outs == [True, True]
+
+
+@pytest.mark.parametrize("news", [None, [2, 3], [150, 150]])
+@pytest.mark.parametrize("length,room", [(65, 64), (81, 128), (-1, 64)])
+def test_a_length_that_the_call_does_not_have_writes_nothing(ctx, news, length, room):
+    """Beyond max_length, beyond the table, negative: the sequence has no token in this call.  Its
+    pages stay as they were, its rows are zeros, the other sequence's are what they are alone."""
+    g, heads, kv, dim = gen(21), 8, 4, 64
+    pools = [torch.randn(16, kv, 16, dim, generator=g).cuda() for _ in range(2)]
+    cache = capi.PagedCache(*pools)
+    before = [t.clone() for t in pools]
+    ints = lambda x: torch.tensor(x, dtype=torch.int32, device="cuda")  # noqa: E731
+    starts = starts_of(news or [1, 1])
+    rows = starts[-1]
+    qkv = torch.randn(rows, (heads + 2 * kv) * dim, generator=g).cuda()
+    tables = ints([list(range(5)), list(range(8, 13))])
+    angle = torch.rand(128, dim // 2, generator=g).cuda()
+    q, out = (torch.full((rows, heads * dim), 5.0, device="cuda") for _ in range(2))
+    work = torch.empty(ctx.paged_attention_work(heads, dim), dtype=torch.uint8, device="cuda")
+
+    def both(lengths):
+        batch = capi.PagedBatch(tables, ints(lengths), room, starts=ints(starts) if news else None,
+                                rows=rows, max_new=max(news) if news else 1)
+        ctx.paged_prepare(cache, batch, qkv, heads, None, None, 1e-6, angle.cos(), angle.sin(), q)
+        ctx.paged_attention(cache, batch, q, heads, out, 0.125, work)
+    both([0, 60])
+    ctx.sync()
+    want, pools_want = out.clone(), [t.clone() for t in pools]
+    for pool, x in zip(pools, before):
+        pool.copy_(x)
+    out.fill_(5.0)
+    both([length, 60])
+    with pytest.raises(capi.B200W4Error, match="outside of what the call has"):
+        ctx.sync()
+    assert torch.equal(pools[0], pools_want[0]) and torch.equal(pools[1], pools_want[1])
+    assert (q[:starts[1]] == 0).all() and (out[:starts[1]] == 0).all()
+    assert torch.equal(out, want)
