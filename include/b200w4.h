@@ -55,6 +55,8 @@ int b2w4_ctx_create(int device, b2w4_ctx** out);
 void b2w4_ctx_destroy(b2w4_ctx* ctx);
 int b2w4_ctx_set_stream(b2w4_ctx* ctx, void* stream);
 int b2w4_sync(b2w4_ctx* ctx); /* end_graph(), engine/cuda_backend.cu:631-639 */
+/* Answers with the gravest of what the context's kernels reported since the call before, and
+ * clears it all: B2W4_E_TIMEOUT, then B2W4_E_INVALID, then B2W4_E_NOMEM. */
 /* Bound of the device-side waits for ANOTHER GPU's stores (the exchanges inside
  * the kernels, below), 1..10000 ms, default about 2 s.  It must cover the skew
  * between the ranks' host threads -- a peer still loading a kernel's code while

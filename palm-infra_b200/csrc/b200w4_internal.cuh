@@ -61,9 +61,10 @@ struct b2w4_ctx {
     int few_used = 0;
     std::mutex few_lock;  // one quantiser and its matmul at a time
     int* flag_dev = nullptr;  // device words: arrival counters, greedy-token cells
-    // The status word a kernel sets when a bounded wait gives up lives in mapped pinned HOST
-    // memory: the host reads it after a stream synchronise with no copy.  status_dev is the
-    // same word's device address.
+    // The status words (STATUS_*) a kernel sets when a bounded wait gives up, or when it leaves out
+    // what its device data wrongly ask for, live in mapped pinned HOST memory: the host reads them
+    // after a stream synchronise with no copy.  status_dev is the same words' device address.  A
+    // word each, so that what one call reports hides nothing of another's.
     int* status_host = nullptr;
     int* status_dev = nullptr;
 };
@@ -77,6 +78,13 @@ enum ScratchSlot {
     SCR_MOE_B = 5,
     SCR_MOE_C = 6,
     SCR_MOE_D = 7,
+};
+
+enum StatusWord {  // the gravest first
+    STATUS_TIMEOUT = 0,
+    STATUS_INVALID = 1,
+    STATUS_NOMEM = 2,
+    STATUS_WORDS = 3,
 };
 
 int b2w4_fail(b2w4_ctx* ctx, int code, const char* fmt, ...);
@@ -359,12 +367,14 @@ __device__ __forceinline__ uint4 b2w4_ldg_stream(const uint4* p) {
 // host-mapped status word.  The store drains at the latest at the end of the grid, which is
 // before the host's stream synchronise returns.
 __device__ __forceinline__ void b2w4_report_timeout(int* status) {
-    *reinterpret_cast<volatile int*>(status) = B2W4_E_TIMEOUT;
+    *reinterpret_cast<volatile int*>(status + STATUS_TIMEOUT) = B2W4_E_TIMEOUT;
 }
 
-// What a kernel found wrong in the device data that it was given, to the same word.
+// What a kernel found wrong in the device data that it was given (B2W4_E_INVALID), or that a pool
+// had no pages for (B2W4_E_NOMEM).
 __device__ __forceinline__ void b2w4_report(int* status, int code) {
-    *reinterpret_cast<volatile int*>(status) = code;
+    *reinterpret_cast<volatile int*>(status + (code == B2W4_E_NOMEM ? STATUS_NOMEM
+                                                                    : STATUS_INVALID)) = code;
 }
 
 __device__ __forceinline__ void b2w4_pdl_wait() {

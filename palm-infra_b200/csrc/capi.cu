@@ -123,7 +123,8 @@ int b2w4_ctx_create(int device, b2w4_ctx** out) {
         delete ctx;
         return B2W4_E_NOMEM;
     }
-    *ctx->status_host = 0;
+    for (int i = 0; i < STATUS_WORDS; ++i)
+        ctx->status_host[i] = 0;
     *out = ctx;
     return B2W4_OK;
 }
@@ -173,13 +174,19 @@ int b2w4_ctx_set_moe_rule(b2w4_ctx* ctx, int act_rule) {
     return B2W4_OK;
 }
 
-// Drains the stream and reads the status word a kernel sets when one of its bounded waits
-// gave up, or when its device data name a page, slot or row that is not there; clears it so that the context stays usable.
+// Drains the stream and reads the status words a kernel sets when one of its bounded waits gave
+// up, or when its device data name a page, slot or row that is not there; answers with the gravest
+// and clears them, so that the context stays usable.
 static int drain_and_check(b2w4_ctx* ctx) {
     B2W4_CUDA(ctx, cudaStreamSynchronize(ctx->stream));
-    const int status = *reinterpret_cast<volatile int*>(ctx->status_host);
+    volatile int* words = ctx->status_host;
+    int status = 0;
+    for (int i = STATUS_WORDS - 1; i >= 0; --i) {
+        if (words[i] != 0)
+            status = words[i];
+        words[i] = 0;
+    }
     if (status != 0) {
-        *reinterpret_cast<volatile int*>(ctx->status_host) = 0;
         cudaMemset(ctx->flag_dev + 2, 0, sizeof(int));  // the persistent kernel's abort word
         return b2w4_fail(ctx, status,
                          status == B2W4_E_INVALID ? "a page, slot, row or count that a call's device "

@@ -208,3 +208,39 @@ def test_token_gather_with_a_silent_peer_times_out():
     assert int(tok.item()) == -1  # no token rather than a guess from one rank's maximum
     for c in ctxs:
         c.close()
+
+
+@pytest.mark.parametrize("first", [True, False])
+def test_a_time_out_is_not_hidden_by_what_another_call_reports(first):
+    """A wait that ran out leaves outputs undefined; a pool without pages leaves items undone.  With
+    both before one sync the answer is the former, whichever came first; both are cleared."""
+    import torch
+    n, k = 64, 256
+    blocks = pkg.synth.bg128_weight(13, 1, n, k)
+    ctxs, stages, groups = _ranks(2, n)
+    ctx = ctxs[0]
+    sh, n_local, lo = pkg.shard.shard_blocks(blocks, n, k, 0, 2)
+    w = ctx.upload_weight(sh, n_local, k)
+    xd = torch.from_numpy(pkg.synth.activations(5, 0, 1, k)).cuda()
+    row = torch.zeros((1, n), dtype=torch.float32, device="cuda")
+    ints = lambda *shape: torch.zeros(shape, dtype=torch.int32, device="cuda")  # noqa: E731
+    pool = pkg.capi.PagePool(ints(1), ints(3, 2), ints(3), 16)  # three slots, one page
+    ctx.set_peer_wait_ms(20)
+
+    def extend():
+        ctx.pages_extend(pool)
+    if not first:
+        extend()
+    ctx.matmul_tp(w, xd, n, lo, groups[0])
+    ctx.tp_gather(groups[0], row, n)
+    if first:
+        extend()
+    with pytest.raises(pkg.capi.B200W4Error, match="ran out of iterations"):
+        ctx.sync()
+    ctx.sync()
+    extend()
+    with pytest.raises(pkg.capi.B200W4Error, match="out of pages"):
+        ctx.sync()
+    ctx.sync()
+    for c in ctxs:
+        c.close()
