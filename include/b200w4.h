@@ -513,12 +513,13 @@ int b2w4_paged_prepare(b2w4_ctx* ctx, const b2w4_paged_cache* cache,
                        const float* q_weight_dev, const float* k_weight_dev, float eps,
                        const float* cos_dev, const float* sin_dev, float* q_out_dev, int ldq);
 /* Attention of the batch's rows over their sequences' pages; everything but the cache is fp32,
- * and so are the results to rounding, whatever the cache's type.  The token at position p sees
- * key j if j <= p and, with a window > 0, j > p - window or j < sinks (the first `sinks` tokens
- * stay visible).  A key whose probability is zero in 32 bits contributes nothing, whatever its
- * value row holds.  Rows without a token: zeros.  q, out: 16-byte aligned rows [heads * dim]
- * that do not overlap.  work_dev: b2w4_paged_attention_work bytes, 16-byte aligned, which no
- * other call uses at the same time; what it holds between calls does not matter. */
+ * and so are the results to rounding, whatever the cache's type (beside an fp16 cache a query or
+ * probability below 2^-28 of its row's largest counts as a multiple of 2^-50 of that).  The token
+ * at position p sees key j if j <= p and, with a window > 0, j > p - window or j < sinks (the first
+ * `sinks` tokens stay visible).  A key whose probability is zero in 32 bits contributes nothing,
+ * whatever its value row holds.  Rows without a token: zeros.  q, out: 16-byte aligned rows [heads
+ * * dim] that do not overlap.  work_dev: b2w4_paged_attention_work bytes, 16-byte aligned, which
+ * no other call uses at the same time; what it holds between calls does not matter. */
 size_t b2w4_paged_attention_work(const b2w4_ctx* ctx, int heads, int dim);
 int b2w4_paged_attention(b2w4_ctx* ctx, const b2w4_paged_cache* cache,
                          const b2w4_paged_batch* batch, const float* q_dev, int ldq, int heads,

@@ -9,8 +9,10 @@
 //
 // Operands of 32 bits are sums of pieces of the cache's 16-bit type, as in paged_split.cu: three
 // bf16 pieces of queries and probabilities beside a bf16 cache, two fp16 pieces of a row's queries
-// times a power of two beside an fp16 cache, three pieces of both sides, six products, beside an
-// fp32 cache; small products first.  Sums in tensor memory truncate, so those of an output are of
+// times a power of two and of its probabilities beside an fp16 cache, the second one of what is left
+// times 2^12 (paged_kernels.cuh); three pieces of both sides, six products, beside an fp32 cache; small
+// products first.  The first product behind those of the second fp16 pieces takes their sum times
+// 2^-12 (an MMA's scale of its input).  Sums in tensor memory truncate, so those of an output are of
 // one block of keys, and the running output is in registers, one rounding per block.
 //
 // What bounds it: a step's rows, then the MMAs, which the pieces multiply.  128 rows x 128 keys x 128
@@ -20,7 +22,8 @@
 // 32 heads over 8 of 128, bf16, a window of 2048: 408 to 462 us from one GPU to another, 0.4 PFLOP/s
 // of the formula's products and 1.2 with the pieces'.  A tile's start and end take about 17,000
 // cycles: queries in 3600 and into pieces 1500, the first scores 2500, the last P V 2250, results out
-// 5500.  They tell where rows see few keys: 333 tokens behind 900, fp32, 62 us; six chunks of 50 to 700, fp16, 64 / 8 heads of 64 under a window of 512, 79.
+// 5500.  They tell where rows see few keys: 333 tokens behind 900, fp32, 62 us; six chunks of 50 to
+// 700, fp16, 64 / 8 heads of 64 under a window of 512, 82.
 //
 // Blocks stay and take one tile after the other, so that a tile's first keys and values are on their
 // way while the one before is finished (6000 tokens as above with a block per tile: 455 to 498 us).
@@ -39,9 +42,16 @@
 
 namespace {
 
+using paged::add2;
 using paged::Args;
 using paged::Attend;
+using paged::cp16;
+using paged::exp2_neg;
+using paged::kHalf;
+using paged::kLift;
+using paged::kTop;
 using paged::Sequence;
+using paged::take_piece;
 
 constexpr int kRows = 128;
 
@@ -53,10 +63,13 @@ struct Cfg {
     static constexpr bool kTwo = !kWide && DIM == 64;
     static constexpr int kKeys = kWide || kTwo ? 64 : 128;
     static constexpr int kK = kWide ? 3 : 1;                             // pieces of a key
-    static constexpr int kQ = std::is_same_v<T, __half> ? 2 : 3;         // of a query
+    static constexpr int kQ = kHalf<T> ? 2 : 3;                          // of a query
     // of them in tensor memory, as many as it holds beside the rest (an MMA with both operands in
     // shared memory takes as long, but the pieces' place there is wanted too)
     static constexpr int kQTmem = kWide ? 2 : kQ == 3 ? 1 : kQ;
+    // what of a query or probability its first piece leaves is taken times 2^kUpBits
+    static constexpr int kUpBits = kHalf<T> ? paged::kUpBits : 0;
+    static constexpr float kUp = kUpBits ? paged::kUp : 1.f;
     static constexpr int kParts = kWide || kTwo ? 2 : 4;  // threads to a row
     static constexpr int kRowWarps = 4 * kParts, kMmaWarp = kRowWarps;
     // for the keys, and as many for the values
@@ -103,14 +116,24 @@ __device__ __forceinline__ uint64_t desc_slow(uint32_t at, uint32_t next) {
     return (uint64_t)((at & 0x3FFFF) >> 4) | (uint64_t)(next >> 4) << 16 |
            (uint64_t)(1024 >> 4) << 32 | (uint64_t)1 << 46 | (uint64_t)2 << 61;
 }
+// DOWN > 0: what is there already counts 2^-DOWN
+template <int DOWN = 0>
 __device__ __forceinline__ void umma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t id,
                                         uint32_t accumulate) {
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "setp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
-        ::"r"(d), "r"(a), "l"(b), "r"(id), "r"(accumulate)
-        : "memory");
+    if constexpr (DOWN > 0)
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t"
+            "setp.ne.b32 p, %4, 0;\n\t"
+            "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p, %5;\n\t}"
+            ::"r"(d), "r"(a), "l"(b), "r"(id), "r"(accumulate), "n"(DOWN)
+            : "memory");
+    else
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t"
+            "setp.ne.b32 p, %4, 0;\n\t"
+            "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+            ::"r"(d), "r"(a), "l"(b), "r"(id), "r"(accumulate)
+            : "memory");
 }
 __device__ __forceinline__ void umma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t id,
                                         uint32_t accumulate) {
@@ -149,51 +172,10 @@ __device__ __forceinline__ void tmem_st8(uint32_t at, const uint32_t (&r)[8]) {
 __device__ __forceinline__ void tmem_st_wait() {
     asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
 }
-__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
-    uint64_t d;
-    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
-    return d;
-}
-// The next piece of two numbers, low half = lo; they keep what is left (exact), but not behind the
-// last piece.
-template <typename T>
-__device__ __forceinline__ uint32_t take_piece(uint64_t& v, bool last = false) {
-    float lo, hi;
-    b2w4_unpack2(v, lo, hi);
-    uint32_t p;
-    if constexpr (std::is_same_v<T, __half>) {
-        asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(p) : "f"(hi), "f"(lo));
-        if (last)
-            return p;
-        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&p));
-        v = b2w4_sub2(v, b2w4_pack2(f.x, f.y));
-    } else {
-        asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(p) : "f"(hi), "f"(lo));
-        if (last)
-            return p;
-        v = b2w4_sub2(v, b2w4_pack2(__uint_as_float(p << 16), __uint_as_float(p & 0xffff0000u)));
-    }
-    return p;
-}
-__device__ __forceinline__ float exp2_neg(float x) {
-    float r;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
-    return r;
-}
-__device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool there) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src),
-                 "r"(there ? 16 : 0)
-                 : "memory");
-}
 // row, chunk of 16 bytes -> bytes in 128-byte rows: 8-row atoms, chunks swizzled with the row
 __device__ __forceinline__ uint32_t place(int row, int chunk) {
     return (uint32_t)((row >> 3) * 1024 + (row & 7) * 128 + ((chunk ^ (row & 7)) << 4));
 }
-
-// 2^kLift times a row's probabilities are what is taken apart and summed: beside an fp16 cache
-// that keeps the small ones' pieces normal numbers.
-template <typename T>
-constexpr float kLift = std::is_same_v<T, __half> ? 10.f : 0.f;
 
 // Whole warp.  Tile `at` of the call's, counted from the last sequence's last tile; false: there is
 // none.  t0: its first token of the sequence's rows.
@@ -429,7 +411,7 @@ paged_runs_kernel(const Args a, const Attend p, int tq) {
                 if (!C::kStageInValues)
                     all_rows_any(false);  // the pieces go where the rows were
                 float up = scale < 0.f ? -1.f : 1.f;
-                if constexpr (std::is_same_v<T, __half>) {  // the row's largest to [2^10, 2^11)
+                if constexpr (kHalf<T>) {
                     float top = 0.f;
 #pragma unroll
                     for (int i = 0; i < kOwn / 4; ++i)
@@ -438,9 +420,9 @@ paged_runs_kernel(const Args a, const Attend p, int tq) {
                             fabsf(f[i].w));
                     top = share(top, larger);
                     int e = (int)(__float_as_uint(top) >> 23) - 127;
-                    e = top == 0.f ? 10 : min(max(e, -100), 120);
-                    up = __fmul_rn(up, __uint_as_float((unsigned)(127 + 10 - e) << 23));
-                    factor = __fmul_rn(factor, __uint_as_float((unsigned)(127 - 10 + e) << 23));
+                    e = top == 0.f ? kTop : min(max(e, -100), 120);
+                    up = __fmul_rn(up, __uint_as_float((unsigned)(127 + kTop - e) << 23));
+                    factor = __fmul_rn(factor, __uint_as_float((unsigned)(127 - kTop + e) << 23));
                     factor = fmaxf(factor, 0x1p-100f);
                 }
                 const uint64_t up2 = b2w4_pack2(up, up);
@@ -458,7 +440,7 @@ paged_runs_kernel(const Args a, const Attend p, int tq) {
                         uint32_t r[8];
 #pragma unroll
                         for (int e = 0; e < 8; ++e)
-                            r[e] = take_piece<T>(v[e], i == C::kQ - 1);
+                            r[e] = take_piece<T>(v[e], C::kUp, i == C::kQ - 1);
                         if (i < C::kQTmem) {
                             tmem_st8(lane_addr + C::kTq + i * (DIM / 2) + at / 2, r);
                         } else {
@@ -561,7 +543,7 @@ paged_runs_kernel(const Args a, const Attend p, int tq) {
                     for (int i = 0; i < C::kQ; ++i)
 #pragma unroll
                         for (int e = 0; e < 8; ++e)
-                            pieces[i][e] = take_piece<T>(pr[8 * u + e], i == C::kQ - 1);
+                            pieces[i][e] = take_piece<T>(pr[8 * u + e], C::kUp, i == C::kQ - 1);
                 };
                 take(0);
                 if (j)
@@ -686,7 +668,9 @@ paged_runs_kernel(const Args a, const Attend p, int tq) {
                             const uint64_t kd =
                                 d + (uint64_t)(((size - i) * C::kPiece + k / 4 * C::kPart +
                                                 k % 4 * 32) >> 4);
-                            if (i < C::kQTmem)
+                            if (C::kUpBits && size == 0 && k == 0)
+                                umma_ts<C::kUpBits>(tm + C::kTs, tm + C::kTq, kd, score_id, 1);
+                            else if (i < C::kQTmem)
                                 umma_ts(tm + C::kTs, tm + C::kTq + i * (DIM / 2) + k * 8, kd,
                                         score_id, more);
                             else
@@ -709,9 +693,12 @@ paged_runs_kernel(const Args a, const Attend p, int tq) {
                         continue;
 #pragma unroll
                     for (int k = 0; k < kKeys / 16; ++k)
-                        umma_ts(tm + C::kTo, tm + C::kTp + i * (kKeys / 2) + k * 8,
-                                d + (uint64_t)(((size - i) * C::kPiece + k * 2048) >> 4), out_id,
-                                size < C::kQ - 1 || i < size || k > 0);
+                        if (C::kUpBits && size == 0 && k == 0)
+                            umma_ts<C::kUpBits>(tm + C::kTo, tm + C::kTp, d, out_id, 1);
+                        else
+                            umma_ts(tm + C::kTo, tm + C::kTp + i * (kKeys / 2) + k * 8,
+                                    d + (uint64_t)(((size - i) * C::kPiece + k * 2048) >> 4), out_id,
+                                    size < C::kQ - 1 || i < size || k > 0);
                 }
             };
             // what the loaders' asynchronous copies wrote is for the tensor core to read; where they
@@ -902,10 +889,10 @@ paged_runs_kernel(const Args a, const Attend p, int tq) {
 #pragma unroll
                         for (int i = 0; i < C::kK; ++i) {
                             uint4 o;
-                            o.x = take_piece<T>(x[0], i == C::kK - 1);
-                            o.y = take_piece<T>(x[1], i == C::kK - 1);
-                            o.z = take_piece<T>(x[2], i == C::kK - 1);
-                            o.w = take_piece<T>(x[3], i == C::kK - 1);
+                            o.x = take_piece<T>(x[0], 1.f, i == C::kK - 1);
+                            o.y = take_piece<T>(x[1], 1.f, i == C::kK - 1);
+                            o.z = take_piece<T>(x[2], 1.f, i == C::kK - 1);
+                            o.w = take_piece<T>(x[3], 1.f, i == C::kK - 1);
                             *reinterpret_cast<uint4*>(dst + i * C::kPiece) = o;
                         }
                     }

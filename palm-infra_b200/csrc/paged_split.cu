@@ -20,10 +20,10 @@
 // multiply-adds, more than the fp32 pipe has in the time that the key's bytes take.  Every operand
 // of 32 bits is a sum of pieces of the cache's 16-bit type, products small ones first, sums in 32
 // bits: three bf16 pieces (24 bits) beside a bf16 cache; two fp16 pieces (22 bits) of the row's
-// query or probabilities times a power of two beside an fp16 cache, which loses below 2^-22 of the
-// row's largest; three pieces of both sides beside an fp32 cache, six products of the nine.  A sum
-// in the tensor core truncates, so an output's sum over a block of keys starts from zero and is
-// added to the running one with one rounding.
+// query or probabilities times a power of two beside an fp16 cache, the second one of what is left
+// times 2^12 (paged_kernels.cuh); three pieces of both sides beside an fp32 cache, six products of the
+// nine.  A sum in the tensor core truncates, so an output's sum over a block of keys starts from zero
+// and is added to the running one with one rounding.
 //
 // What pieces cannot hold -- infinities, NaN, results that are not finite -- is done key by key in
 // 32 bits (paged::attend_row), which has the rule for values of probability zero.
@@ -35,8 +35,15 @@
 
 namespace {
 
+using paged::add2;
 using paged::Args;
 using paged::Attend;
+using paged::cp16;
+using paged::exp2_neg;
+using paged::kDown;
+using paged::kHalf;
+using paged::kLift;
+using paged::kTop;
 using paged::Sequence;
 
 constexpr int kKeys = 16;  // of a block
@@ -169,11 +176,6 @@ struct Stream {
     int tile, kv_row;  // kv_row: of the tile's kv head, in a page
 };
 
-__device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool there) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src),
-                 "r"(there ? 16 : 0)
-                 : "memory");
-}
 template <int N>
 __device__ __forceinline__ void cp_wait() {
     asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
@@ -210,39 +212,23 @@ __device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint3
             : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
             : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-// The next piece of two numbers, lo in the low half; they keep what is left (exact).
+// What is left of a query or probability behind its first piece, in pieces' units (paged::kUp).
 template <typename T>
 __device__ __forceinline__ uint32_t take_piece(float& lo, float& hi) {
-    uint32_t p;
-    float x, y;
-    if constexpr (std::is_same_v<T, __half>) {
-        asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(p) : "f"(hi), "f"(lo));
-        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&p));
-        x = f.x;
-        y = f.y;
-    } else {
-        asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(p) : "f"(hi), "f"(lo));
-        x = __uint_as_float(p << 16);
-        y = __uint_as_float(p & 0xffff0000u);
-    }
-    b2w4_unpack2(b2w4_sub2(b2w4_pack2(lo, hi), b2w4_pack2(x, y)), lo, hi);
+    uint64_t v = b2w4_pack2(lo, hi);
+    const uint32_t p = paged::take_piece<T>(v, kHalf<T> ? paged::kUp : 1.f);
+    b2w4_unpack2(v, lo, hi);
     return p;
 }
-__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
-    uint64_t d;
-    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
-    return d;
-}
-__device__ __forceinline__ float exp2_neg(float x) {
-    float r;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
-    return r;
-}
-
-// 2^kLift times a row's probabilities are what is taken apart and summed: beside an fp16 cache
-// that keeps the small ones' pieces normal numbers.
+// Sums of products of first pieces, and of second ones, as one.
 template <typename T>
-constexpr float kLift = std::is_same_v<T, __half> ? 10.f : 0.f;
+__device__ __forceinline__ float joined(float second, float first) {
+    return kHalf<T> ? __fmaf_rn(second, kDown, first) : __fadd_rn(second, first);
+}
+template <typename T>
+__device__ __forceinline__ uint64_t joined2(uint64_t second, uint64_t first) {
+    return kHalf<T> ? b2w4_fma2(second, b2w4_pack2(kDown, kDown), first) : add2(second, first);
+}
 
 // Pieces of a row's column pairs (2t and 2t + 8, of rows r and r + 8) as operands: at(i, e) is
 // register e of operand i.
@@ -534,7 +520,7 @@ paged_split_kernel(const Args a, const Attend p, float* __restrict__ parts,
 #pragma unroll
             for (int h = 0; h < kHalves; ++h) {
                 unscale[h] = 1.f;
-                if constexpr (std::is_same_v<T, __half>) {  // the row's largest to [2^10, 2^11)
+                if constexpr (kHalf<T>) {
                     float top = 0.f;
 #pragma unroll
                     for (int k = 0; k < kSteps; ++k)
@@ -544,9 +530,9 @@ paged_split_kernel(const Args a, const Attend p, float* __restrict__ parts,
                     top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
                     top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
                     int e = (int)(__float_as_uint(top) >> 23) - 127;
-                    e = top == 0.f ? 10 : min(max(e, -100), 120);
-                    const float up = __uint_as_float((unsigned)(127 + 10 - e) << 23);
-                    unscale[h] = __uint_as_float((unsigned)(127 - 10 + e) << 23);
+                    e = top == 0.f ? kTop : min(max(e, -100), 120);
+                    const float up = __uint_as_float((unsigned)(127 + kTop - e) << 23);
+                    unscale[h] = __uint_as_float((unsigned)(127 - kTop + e) << 23);
 #pragma unroll
                     for (int k = 0; k < kSteps; ++k)
 #pragma unroll
@@ -634,12 +620,12 @@ paged_split_kernel(const Args a, const Attend p, float* __restrict__ parts,
                         sc[e] = by[kA - 1][n][2 * h + c];
 #pragma unroll
                         for (int i = kA - 2; i >= 0; --i)
-                            sc[e] = __fadd_rn(sc[e], by[i][n][2 * h + c]);
+                            sc[e] = joined<T>(sc[e], by[i][n][2 * h + c]);
                     } else {
                         sc[e] = by[0][n][2 + c];
                         if (kA > 1)
                             sc[e] = __fadd_rn(by[kA - 1][n][c], sc[e]);
-                        sc[e] = __fadd_rn(sc[e], by[0][n][c]);
+                        sc[e] = joined<T>(sc[e], by[0][n][c]);
                     }
                     sc[e] = __fmul_rn(sc[e], factor[h]);
                     if (!(keys >> (8 * n + 2 * t + c) & 1))
@@ -681,8 +667,14 @@ paged_split_kernel(const Args a, const Attend p, float* __restrict__ parts,
                     o[n][0] = b2w4_fma2(o[n][0], alpha2[0], x0);
                     o[n][1] = b2w4_fma2(o[n][1], alpha2[1], x1);
                 } else {
-                    o[n][0] = b2w4_fma2(o[n][0], alpha2[0], add2(x1, x0));
+                    o[n][0] = b2w4_fma2(o[n][0], alpha2[0], joined2<T>(x1, x0));
                 }
+            };
+            // sums of two fp16 pieces that are apart, rows of first ones in x, of second ones in y
+            auto join_rows = [&](float (&x)[4], const float (&y)[4]) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    x[e] = joined<T>(y[e], x[e]);
             };
             if constexpr (kWide) {
                 // a group of 32 features: lane's four of each of its keys, one per tile
@@ -730,11 +722,25 @@ paged_split_kernel(const Args a, const Attend p, float* __restrict__ parts,
                         ldmatrix_trans(b[j], vs + swizzled((lane & 7) + ((lane >> 3) & 1) * 8,
                                                            n + 2 * j + (lane >> 4), true));
                     float x[4][4] = {};
+                    if constexpr (kHalf<T> && SET == 16) {
+                        float y[4][4] = {};
 #pragma unroll
-                    for (int i = kA - 1; i >= 0; --i)
+                        for (int i = kA - 1; i >= 0; --i)
+#pragma unroll
+                            for (int j = 0; j < 4; ++j)
+                                mma<T>(i ? y[j] : x[j], pp[i], b[j >> 1][(j & 1) * 2],
+                                       b[j >> 1][(j & 1) * 2 + 1]);
 #pragma unroll
                         for (int j = 0; j < 4; ++j)
-                            mma<T>(x[j], pp[i], b[j >> 1][(j & 1) * 2], b[j >> 1][(j & 1) * 2 + 1]);
+                            join_rows(x[j], y[j]);
+                    } else {
+#pragma unroll
+                        for (int i = kA - 1; i >= 0; --i)
+#pragma unroll
+                            for (int j = 0; j < 4; ++j)
+                                mma<T>(x[j], pp[i], b[j >> 1][(j & 1) * 2],
+                                       b[j >> 1][(j & 1) * 2 + 1]);
+                    }
 #pragma unroll
                     for (int j = 0; j < 4; ++j)
                         add(n + j, x[j]);

@@ -457,3 +457,87 @@ def test_a_length_that_the_call_does_not_have_writes_nothing(ctx, news, length, 
     assert torch.equal(pools[0], pools_want[0]) and torch.equal(pools[1], pools_want[1])
     assert (q[:starts[1]] == 0).all() and (out[:starts[1]] == 0).all()
     assert torch.equal(out, want)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("heads,kv,dim,lengths,news,together", [
+    (4, 1, 64, [400, 33], None, False), (8, 1, 128, [400], None, False),
+    (16, 1, 128, [400, 200], None, False), (40, 2, 64, [300], None, False),
+    (6, 2, 256, [300], None, False), (4, 1, 192, [400], [5], False),
+    (16, 4, 128, [2000], [300], True), (16, 4, 64, [2000], [300], True)])
+@pytest.mark.parametrize("ahead", [0, 8, 12, 16, 21, 26])
+def test_a_first_token_far_ahead_that_holds_zeros(ctx, dtype, heads, kv, dim, lengths, news,
+                                                  together, ahead):
+    """A sink: the first key's score is `ahead` and more above all others, its value row zero, so that
+    the result is made of probabilities that are small against the row's largest.
+
+    Scores are sums of products of small numbers, exact in 32 bits; values are positive, so that
+    errors of the probabilities are errors of the result, relative.  In units of eps = 2^-24, with S
+    the sink's score and s the others': the factor of the scores (three roundings) 3 (S - s); a
+    score's product with it, its difference from the maximum, that one's rounding: S + |s|, S - s,
+    S + 15; the exponential 4; its pieces 4; a block's sum, whose products and sums may be truncated:
+    at most 24 sums and 17 numbers of each, 82; a rounding of the running sums and of their scale for
+    each of at most n / 16 blocks, n / 8; the joins and the division 12.  Beside fp16 a probability is
+    a multiple of 2^-51 of the row's largest: 2^-52 of each value more."""
+    rule = capi.lib().b2w4_paged_runs_wanted_by
+    kind = {F32: capi.F32, F16: capi.F16, BF16: capi.BF16}[dtype]
+    rows = sum(news or [1] * len(lengths))
+    if news:
+        assert rule(148, kind, dim, heads, kv, rows, len(lengths), max(lengths), 0, 0) == together
+    g, page, scale = gen(17), 16, 0.125
+    q = torch.randint(-1, 2, (rows, heads, dim), generator=g).float()
+    q[..., 0] = 1.0
+    k, v, tables, held = ref.make_pool(lengths, page, kv, dim, dtype, g)
+    k = (torch.randint(-4, 5, k.shape, generator=g) / 4).to(dtype)
+    k[..., 0] = 0
+    v = (v.float().abs() + 0.25).to(dtype)
+    spread = dim ** 0.5 * 0.7 * 4.5 * scale / 2  # of the others' scores, about four sigma either way
+    for s in range(len(lengths)):
+        k[tables[s, 0], :, 0] = 0
+        k[tables[s, 0], :, 0, 0] = round((ahead + spread) / scale)
+        v[tables[s, 0], :, 0] = 0
+    cache = capi.PagedCache(k.cuda(), v.cuda())
+    tables, held = tables[:len(lengths)].cuda(), held[:len(lengths)].cuda()
+    starts = starts_of(news or [1] * len(lengths))
+    ints = lambda x: torch.tensor(x, dtype=torch.int32, device="cuda")  # noqa: E731
+    batch = capi.PagedBatch(tables, held, max(lengths), starts=ints(starts) if news else None,
+                            rows=rows, max_new=max(news) if news else 1)
+    out = torch.empty(rows, heads * dim, device="cuda")
+    work = torch.empty(ctx.paged_attention_work(heads, dim), dtype=torch.uint8, device="cuda")
+    ctx.paged_attention(cache, batch, q.view(rows, -1).cuda(), heads, out, scale, work)
+    ctx.sync()
+    eps, group = 2.0 ** -24, heads // kv
+    for s, length in enumerate(lengths):
+        n = starts[s + 1] - starts[s]
+        keys = ref.rows_of(cache.keep[0], tables[s], page, length).double()
+        values = ref.rows_of(cache.keep[1], tables[s], page, length).double()
+        x = q[starts[s]:starts[s + 1]].cuda().double().view(n, kv, group, dim)
+        score = torch.einsum("nhgd,mhd->hgnm", x, keys) * scale
+        seen = torch.arange(length)[None] <= torch.arange(length - n, length)[:, None]
+        score.masked_fill_(~seen.cuda(), -math.inf)
+        top = score[..., :1]
+        others = score[..., 1:].masked_fill(~seen.cuda()[:, 1:], 0.0)
+        p = (score - score.amax(-1, keepdim=True)).exp()
+        weighted = torch.einsum("hgnm,mhd->hgnd", p, values)
+        want = weighted / p.sum(-1, keepdim=True)
+        size = top.abs()[..., 0] + others.abs().amax(-1)
+        rel = (3 * size + 2 * size + size + top.abs()[..., 0] + 15 + 8 + 82 + length / 8 + 12) * eps
+        bound = want * rel[..., None]
+        if dtype == F16:
+            bound = bound + 2.0 ** -52 * values.sum(0)[:, None, None] / p.sum(-1, keepdim=True)
+        got = out[starts[s]:starts[s + 1]].double().view(n, kv, group, dim).permute(1, 2, 0, 3)
+        off = ((got - want).abs() / bound).max()
+        assert off <= 1.0, float(off)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("heads,kv,dim,lengths,news", [
+    (4, 1, 128, [300], None), (16, 1, 64, [300], None), (16, 4, 128, [600], [100]),
+    (16, 4, 64, [600], [100])])
+def test_queries_far_above_the_others_where_keys_are_zero(ctx, dtype, heads, kv, dim, lengths, news):
+    """A feature of 2^20 in every row that no key has: the scores are made of the others."""
+    def change(q, k, v, tables, held):
+        q.view(q.shape[0], heads, dim)[:, :, 5] = 2.0 ** 20
+        k[..., 5] = 0
+    run(ctx, dict(lengths=lengths, news=news, page=16, heads=heads, kv=kv, dim=dim, dtype=dtype),
+        18, change=change)
