@@ -175,7 +175,8 @@ Args args_of(b2w4_ctx* ctx, const b2w4_paged_cache& c, const b2w4_paged_batch& b
 // that shares the cache's bytes out over the chip: long runs and many sequences to the former, a few
 // rows behind a long cache to the latter, by their times in us.  A tile's steps are those of
 // paged_runs.cu; row by row every token has its keys read again, from the second level cache for the
-// most part.  Heads of 192 and 256 numbers, and groups of more than 128, go row by row.  Measured, us
+// most part.  Heads of 192 and 256 numbers, groups of more than 128, and what
+// b2w4_paged_runs_takes has no room or time for, go row by row.  Measured, us
 // together / row by row, 32 heads over 8 of 128 in bf16: 2 rows behind 30,000 keys 591 / 50; 16 behind
 // 2000 46 / 32; 32 behind 4000 78 / 77; 64 behind 8000 153 / 266; 128 behind 4000 79 / 266.  In fp32: 16
 // behind 2000 91 / 55; 32 behind 4000 180 / 175; 128 behind 4000 182 / 656.  Of 120 shapes of three
@@ -185,7 +186,7 @@ extern "C" int b2w4_paged_runs_wanted_by(int sm_count, int type, int dim, int he
                                          int rows, int sequences, int max_length, int window,
                                          int sinks) {
     const int rep = heads / kv_heads;
-    if (!b2w4_paged_runs_takes(dim, heads, kv_heads, rows, sequences))
+    if (!b2w4_paged_runs_takes(sm_count, dim, heads, kv_heads, rows, sequences, max_length))
         return 0;
     const bool wide = type == B2W4_F32, two = !wide && dim == 64;
     const int tq = 128 / rep, per = wide || two ? 64 : 128;
@@ -328,7 +329,7 @@ int b2w4_paged_attention(b2w4_ctx* ctx, const b2w4_paged_cache* cache,
     const Attend p = {q_dev, out_dev, scale, {window, sinks}, ldq, ldo, heads};
     const bool runs = batch->max_new > 1;
     if (runs && b2w4_paged_runs_wanted(ctx->sm_count, *cache, *batch, heads, window, sinks))
-        return b2w4_launch_paged_runs(ctx, cache->type, cache->dim, a, p);
+        return b2w4_launch_paged_runs(ctx, cache->type, cache->dim, a, p, work_dev);
     return b2w4_launch_paged_split(ctx, cache->type, cache->dim, a, p, runs, work_dev);
 }
 

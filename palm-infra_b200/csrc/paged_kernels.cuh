@@ -82,10 +82,11 @@ __device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool there) 
 
 }  // namespace paged
 
-// Runs of rows (paged_runs.cu): heads of 64 or 128 numbers.
-bool b2w4_paged_runs_takes(int dim, int heads, int kv_heads, int rows, int sequences);
+// Runs of rows (paged_runs.cu): heads of 64 or 128 numbers.  work: as the split kernel's.
+bool b2w4_paged_runs_takes(int sm_count, int dim, int heads, int kv_heads, int rows, int sequences,
+                           int max_length);
 int b2w4_launch_paged_runs(b2w4_ctx* ctx, int type, int dim, const paged::Args& a,
-                           const paged::Attend& p);
+                           const paged::Attend& p, void* work);
 
 bool b2w4_paged_runs_wanted(int sm_count, const b2w4_paged_cache& c, const b2w4_paged_batch& b,
                             int heads, int window, int sinks);

@@ -22,7 +22,7 @@
 // 32 heads over 8 of 128, bf16, a window of 2048: 408 to 462 us from one GPU to another, 0.4 PFLOP/s
 // of the formula's products and 1.2 with the pieces'.  A tile's start and end take about 17,000
 // cycles: queries in 3600 and into pieces 1500, the first scores 2500, the last P V 2250, results out
-// 5500.  They tell where rows see few keys: 333 tokens behind 900, fp32, 62 us; six chunks of 50 to
+// 5500.  They tell where rows see few keys: 333 tokens behind 900, fp32, 64 us; six chunks of 50 to
 // 700, fp16, 64 / 8 heads of 64 under a window of 512, 82.
 //
 // Blocks stay and take one tile after the other, so that a tile's first keys and values are on their
@@ -36,7 +36,9 @@
 // anywhere.
 //
 // A row whose result is not finite is done again key by key (paged::attend_row): a key that it does
-// not see, or that has no probability, may hold anything.  Every wait is bounded.
+// not see, or that has no probability, may hold anything.  That takes as long as the cache is (a warp
+// does a row, 0.6 us a key), so it waits until the block's other warps are done: every wait is bounded
+// (2 s), and within the tiles none is for more than a tile's steps.
 #include "paged_kernels.cuh"
 #include "tcgen05_ops.cuh"
 
@@ -218,9 +220,22 @@ struct Tile {
     __device__ __forceinline__ int p0() const { return length - count + t0; }  // its position
 };
 
+// Rows of a tile to be done again: bit r of `rows` is row r of the quarter.  In the work area a list
+// for every quarter of every block's rows, an entry a tile.
+struct alignas(16) Again {
+    int seq, t0, kvh;
+    unsigned rows;
+};
+// The most tiles of a call: a sequence's last one may be short, one more for each.
+long tiles_of(int rows, int sequences, int heads, int kv_heads) {
+    return ((long)rows / (kRows / (heads / kv_heads)) + sequences) * kv_heads;
+}
+constexpr int kMostBlocks = 2;  // of a multiprocessor
+
 template <typename T, int DIM>
 __global__ void __launch_bounds__(Cfg<T, DIM>::kThreads, Cfg<T, DIM>::kBlocks)
-paged_runs_kernel(const Args a, const Attend p, int tq) {
+paged_runs_kernel(const Args a, const Attend p, int tq, Again* __restrict__ lists,
+                  int most_tiles) {
     using C = Cfg<T, DIM>;
     constexpr int kKeys = C::kKeys, kParts = C::kParts, kRowWarps = C::kRowWarps;
     constexpr int kMmaWarp = C::kMmaWarp, kLoadWarp0 = C::kLoadWarp0;
@@ -245,7 +260,8 @@ paged_runs_kernel(const Args a, const Attend p, int tq) {
     volatile int* s_abort = reinterpret_cast<volatile int*>(tmem_slot + 1);
     uint32_t* s_bad = tmem_slot + 2;  // [2] a page that is not the pool's
     uint32_t* s_odd = tmem_slot + 4;  // [4] rows to be done again
-    static_assert(20 * 8 + 2 * sizeof(Tile) + 8 * 4 <= 512);
+    int* s_listed = reinterpret_cast<int*>(tmem_slot + 8);  // [4] tiles with such rows
+    static_assert(20 * 8 + 2 * sizeof(Tile) + 12 * 4 <= 512);
     float* s_max = reinterpret_cast<float*>(smem + C::kMax);
 
     if (threadIdx.x == 0) {
@@ -267,7 +283,7 @@ paged_runs_kernel(const Args a, const Attend p, int tq) {
         }
         *s_abort = 0;
         for (int i = 0; i < 4; ++i)
-            s_odd[i] = 0;
+            s_odd[i] = s_listed[i] = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     b2w4_pdl_wait();
@@ -368,6 +384,7 @@ paged_runs_kernel(const Args a, const Attend p, int tq) {
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         };
         int g = 0;  // steps of the tiles before
+        auto list_of = [&]() { return lists + (size_t)(blockIdx.x * 4 + quarter) * most_tiles; };
         for (int n = 0;; ++n) {
             const bool more = next_tile(n);
             // one answer for all rows
@@ -619,24 +636,42 @@ paged_runs_kernel(const Args a, const Attend p, int tq) {
             }
             row_sync();
             if (const unsigned mine = s_odd[quarter]) {
-                for (int r = part; r < 32; r += kParts)
-                    if ((mine >> r & 1) && live && !*s_abort) {
-                        bool bad = false;
-                        const Sequence s = paged::taken(a, t.seq, &bad);
-                        const int q = quarter * 32 + r;
-                        paged::attend_row<T, DIM>(a, s, p.q + row_offset(q, p.ldq),
-                                                  t.p0() + token_of(q), t.kvh, p.scale, p.window,
-                                                  p.out + row_offset(q, p.ldo));
+                row_sync();  // all have looked
+                if (part == 0 && lane == 0) {
+                    // (more tiles than the call's rows make: starts that are wrong)
+                    const int at = s_listed[quarter];
+                    if (at < most_tiles) {
+                        list_of()[at] = {t.seq, t.t0, t.kvh, mine};
+                        s_listed[quarter] = at + 1;
+                    } else {
+                        b2w4_report(a.status, B2W4_E_INVALID);
                     }
-                row_sync();
-                if (part == 0 && lane == 0)
                     s_odd[quarter] = 0;
+                }
                 row_sync();
             }
             // every row has looked at the word
             if (all_rows_any(false), threadIdx.x == 0)
                 s_bad[n & 1] = 0;
             warp_arrive(&tile_free[n & 1]);
+        }
+        // No warp waits for this with a limit: the others stand at the block's last barrier.
+#pragma unroll 1
+        for (int i = 0; i < s_listed[quarter] && live && !*s_abort; ++i) {
+            const Again t = list_of()[i];
+            bool bad = false;
+            const Sequence s = paged::taken(a, t.seq, &bad);
+#pragma unroll 1
+            for (int r = part; r < 32; r += kParts) {
+                if (!(t.rows >> r & 1))
+                    continue;
+                const int token = t.t0 + token_of(quarter * 32 + r);
+                const int head = t.kvh * rep + quarter * 32 + r - (token - t.t0) * rep;
+                const size_t row = s.first + token;
+                paged::attend_row<T, DIM>(a, s, p.q + row * p.ldq + (size_t)head * DIM,
+                                          s.length - s.count + token, t.kvh, p.scale, p.window,
+                                          p.out + row * p.ldo + (size_t)head * DIM);
+            }
         }
     } else {
       asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::kRegsOther));
@@ -980,37 +1015,44 @@ paged_runs_kernel(const Args a, const Attend p, int tq) {
 }
 
 template <typename T, int DIM>
-int launch(b2w4_ctx* ctx, const Args& a, const Attend& p) {
+int launch(b2w4_ctx* ctx, const Args& a, const Attend& p, void* work) {
     using C = Cfg<T, DIM>;
+    static_assert(C::kBlocks <= kMostBlocks);
     static b2w4_smem_optin cfg;
     auto kern = paged_runs_kernel<T, DIM>;
     const int tq = kRows / (p.heads / a.kv_heads);
-    // a sequence's last tile may be short: one more for each
-    const long tiles = ((long)a.rows / tq + a.sequences) * a.kv_heads;
+    const long tiles = tiles_of(a.rows, a.sequences, p.heads, a.kv_heads);
     const long resident = (long)ctx->sm_count * C::kBlocks;
     const unsigned blocks = (unsigned)(tiles < resident ? tiles : resident);
+    const int most_tiles = (int)((tiles + blocks - 1) / blocks);
     B2W4_CUDA(ctx, b2w4_opt_in_smem(ctx, kern, C::kTotal, cfg));
     B2W4_CUDA(ctx, b2w4_launch_chained(ctx->pdl, kern, dim3(blocks), dim3(C::kThreads),
-                                       C::kTotal, ctx->stream, a, p, tq));
+                                       C::kTotal, ctx->stream, a, p, tq, static_cast<Again*>(work),
+                                       most_tiles));
     ctx->launches++;
     return B2W4_OK;
 }
 
 }  // namespace
 
-bool b2w4_paged_runs_takes(int dim, int heads, int kv_heads, int rows, int sequences) {
-    const int rep = heads / kv_heads;
-    // (the tiles are counted in 32 bits)
-    return dim <= 128 && rep <= kRows &&
-           ((double)rows / (kRows / rep) + sequences) * kv_heads < 0x3fffffff;
+// Tiles are counted in 32 bits; the work area holds an entry of every block's lists for each, and a
+// tile of 2^24 keys takes 0.7 s of a wait's 2.
+bool b2w4_paged_runs_takes(int sm_count, int dim, int heads, int kv_heads, int rows, int sequences,
+                           int max_length) {
+    if (dim > 128 || heads / kv_heads > kRows || max_length > 1 << 24)
+        return false;
+    const long tiles = tiles_of(rows, sequences, heads, kv_heads);
+    return tiles < 0x3fffffff && 4 * sizeof(Again) * (tiles + (long)sm_count * kMostBlocks) <=
+                                     b2w4_paged_split_work(sm_count, dim);
 }
 
-int b2w4_launch_paged_runs(b2w4_ctx* ctx, int type, int dim, const Args& a, const Attend& p) {
+int b2w4_launch_paged_runs(b2w4_ctx* ctx, int type, int dim, const Args& a, const Attend& p,
+                           void* work) {
     if (dim == 64)
-        return type == B2W4_F16    ? launch<__half, 64>(ctx, a, p)
-               : type == B2W4_BF16 ? launch<__nv_bfloat16, 64>(ctx, a, p)
-                                   : launch<float, 64>(ctx, a, p);
-    return type == B2W4_F16    ? launch<__half, 128>(ctx, a, p)
-           : type == B2W4_BF16 ? launch<__nv_bfloat16, 128>(ctx, a, p)
-                               : launch<float, 128>(ctx, a, p);
+        return type == B2W4_F16    ? launch<__half, 64>(ctx, a, p, work)
+               : type == B2W4_BF16 ? launch<__nv_bfloat16, 64>(ctx, a, p, work)
+                                   : launch<float, 64>(ctx, a, p, work);
+    return type == B2W4_F16    ? launch<__half, 128>(ctx, a, p, work)
+           : type == B2W4_BF16 ? launch<__nv_bfloat16, 128>(ctx, a, p, work)
+                               : launch<float, 128>(ctx, a, p, work);
 }

@@ -541,3 +541,38 @@ def test_queries_far_above_the_others_where_keys_are_zero(ctx, dtype, heads, kv,
         k[..., 5] = 0
     run(ctx, dict(lengths=lengths, news=news, page=16, heads=heads, kv=kv, dim=dim, dtype=dtype),
         18, change=change)
+
+
+def test_rows_done_again_behind_a_long_cache(ctx):
+    """A key of probability zero whose value is infinite: every row of its kv head is done again key
+    by key, behind 400,000 keys, which is longer than a wait may be (2 s).  No row is left out and
+    no wait runs out.  A serial sum of n numbers in 32 bits is off by at most n eps of itself."""
+    heads, kv, dim, n, page, rows = 32, 2, 64, 400_000, 64, 600
+    rule = capi.lib().b2w4_paged_runs_wanted_by
+    assert rule(148, capi.F16, dim, heads, kv, rows, 1, n, 0, 0) == 1
+    g = torch.Generator(device="cuda").manual_seed(3)
+    k, v = (torch.randn((n // page, kv, page, dim), device="cuda", generator=g).half()
+            for _ in range(2))
+    q = torch.randn((rows, heads, dim), device="cuda", generator=g)
+    q[..., 0] = 4.0
+    k[..., 0] = 0
+    k[0, 0, 7] = 0
+    k[0, 0, 7, 0] = -2000.0          # a score of -1000
+    v[0, 0, 7] = math.inf
+    ints = lambda x: torch.tensor(x, dtype=torch.int32, device="cuda")  # noqa: E731
+    batch = capi.PagedBatch(torch.arange(n // page, dtype=torch.int32, device="cuda")[None],
+                            ints([n]), n, starts=ints([0, rows]), rows=rows, max_new=rows)
+    out = torch.full((rows, heads * dim), math.nan, device="cuda")
+    work = torch.empty(ctx.paged_attention_work(heads, dim), dtype=torch.uint8, device="cuda")
+    torch.cuda.synchronize()
+    ctx.paged_attention(capi.PagedCache(k, v), batch, q.view(rows, -1), heads, out, 0.125, work)
+    ctx.sync()
+    assert torch.isfinite(out).all()
+    v[0, 0, 7] = 0
+    for row in (0, 7, 300, 599):
+        for head in (0, 9, 15, 20):
+            last = n - rows + row + 1
+            keys, values = (t[:, head // 16].reshape(-1, dim)[:last].double() for t in (k, v))
+            p = torch.softmax(keys @ q[row, head].double() * 0.125, 0)
+            off = (out[row, head * dim:(head + 1) * dim].double() - p @ values).abs()
+            assert (off <= 2 * (n + 200) * 2.0 ** -24 * (p @ values.abs())).all()
