@@ -3,8 +3,12 @@
 //
 // With M the row's maximum, S = sum exp(x - M) and T = sum exp(x - M) (x - M):
 //   log p(t) = x_t - M - log S,   entropy = log S - T / S   (a sum of two terms >= 0).
-// Every thread keeps a running maximum m and sums relative to it, in 32 bits; two such triples
-// join as M = max, S = S1 e^(m1 - M) + S2 e^(m2 - M), T likewise of T_i + (m_i - M) S_i.
+// Every warp keeps a running maximum m, every thread sums relative to its warp's, in 32 bits; two such
+// triples join as M = max, S = S1 e^(m1 - M) + S2 e^(m2 - M), T likewise of T_i + (m_i - M) S_i.  The
+// largest number's own term is 1 without a rounding, no term of T is above zero, so that S >= 1, T <= 0,
+// no log probability is above zero and no entropy below, and a likely token's log probability, which
+// is -log S, is as good as the sum of the others' terms.  (A maximum per thread would change in nearly
+// every tile for some thread of a warp; a warp's changes about ln(tiles) times.)
 //
 // The k largest: a number below which the k-th largest cannot lie comes from the block's first tile
 // (the k-th largest of the maxima of 64 groups of its numbers), and what is not below it goes to a
@@ -35,7 +39,6 @@ constexpr int kGroups = 64;                 // of four threads each
 constexpr int kTrim = 64;                   // a longer list is cut back to the k largest
 constexpr int kList = kTrim + 32 * kVecs * 4;
 constexpr int kMostCluster = 8;
-constexpr float kSlack = 8.f;
 
 struct Args {
     const float* x;
@@ -228,20 +231,22 @@ logprobs_kernel(const Args a, bool aligned) {
 #pragma unroll
         for (int i = 1; i < kVecs * 4; ++i)
             top = fmaxf(top, v[i]);
-        // Not for every larger number: what is summed may be e^kSlack times as large as the largest
-        // would make it, and the sums are scaled again a few times instead of nearly every tile.
-        if (top > m + kSlack) {
+        if (__any_sync(0xffffffffu, top > m)) {
+            float up = fmaxf(m, top);
+#pragma unroll
+            for (int off = 16; off > 0; off >>= 1)
+                up = fmaxf(up, __shfl_xor_sync(0xffffffffu, up, off));
             if (m > -INFINITY) {
-                const float d = __fsub_rn(m, top), e = expf(d);
+                const float d = __fsub_rn(m, up), e = expf(d);
                 float s0, s1, t0, t1;
                 b2w4_unpack2(sum2, s0, s1);
                 b2w4_unpack2(t2, t0, t1);
-                // (below, d may be -inf where top is)
+                // (d may be -inf where up is inf)
                 t2 = e == 0.f ? 0ull : b2w4_pack2(__fmul_rn(__fmaf_rn(s0, d, t0), e),
                                                   __fmul_rn(__fmaf_rn(s1, d, t1), e));
                 sum2 = b2w4_pack2(__fmul_rn(s0, e), __fmul_rn(s1, e));
             }
-            m = top;
+            m = up;
         }
         const float from = m == -INFINITY ? 0.f : m;
         const uint64_t from2 = b2w4_pack2(from, from);

@@ -202,3 +202,43 @@ def test_refusals(ctx):
         with pytest.raises(ValueError):
             ctx.logprobs(**{**dict(logits=x), **args})
     assert ctx.launches == launches
+
+
+@pytest.mark.parametrize("vocab", [9000, 151936])
+@pytest.mark.parametrize("winner_first", [False, True])
+def test_confident_rows(ctx, vocab, winner_first):
+    """A winner and a rival 1 to 30 below it, in numbers that one thread meets one after the other
+    or that lie anywhere; nothing else is left.  No log probability is above zero, no entropy below.
+    With R = e^-gap: log p = -log(1 + R), entropy = log(1 + R) + R gap / (1 + R).  R is off by its
+    exponent's roundings (two of a size up to 1.5 gap), two units of ex2 and two of joins: rel =
+    (3 gap + 8) eps + 2^-22 of it; the sum 1 + R, its logarithm (two units) and the difference by eps
+    of 1 each at most, beside which everything is a share of R or of R gap."""
+    gaps = [1.0, 3.0, 5.0, 5.7, 6.5, 7.9, 8.1, 10.0, 14.0, 20.0, 30.0]
+    places = [(7, 7 + 4096), (4093, 4093 + 4096), (0, vocab - 1), (100, 101)]
+    x = torch.full((len(gaps) * len(places), vocab), -math.inf, device="cuda")
+    want_lp, want_h, rel = [], [], []
+    for i, (gap, (a, b)) in enumerate((g, p) for g in gaps for p in places):
+        win, lose = (a, b) if winner_first else (b, a)
+        x[i, win] = 3.25
+        x[i, lose] = 3.25 - gap
+        gap = 3.25 - float(x[i, lose])
+        r = math.exp(-gap)
+        want_lp.append((-math.log1p(r), -gap - math.log1p(r)))
+        want_h.append(math.log1p(r) + r * gap / (1 + r))
+        rel.append((3 * gap + 8) * 2.0 ** -24 + 2.0 ** -22)
+    target = x.argmax(-1).to(torch.int32)
+    lp, ent, values, indices = call(ctx, x, target, 2)
+    want_lp, want_h, rel = (torch.tensor(t, dtype=torch.float64) for t in (want_lp, want_h, rel))
+    assert (lp <= 0).all() and (ent >= 0).all() and (values <= 0).all()
+    eps = 2.0 ** -24
+    slack = 3 * eps + (rel + 4 * eps) * want_h.clamp_min(0)
+    assert ((lp.double() - want_lp[:, 0]).abs() <= slack).all()
+    assert torch.equal(values[:, 0], lp)
+    assert ((values[:, 1].double() - want_lp[:, 1]).abs() <= slack - 2 * eps * want_lp[:, 1]).all()
+    assert ((ent.double() - want_h).abs() <= slack).all()
+    # many numbers, one far above them
+    y = logits(40, vocab, 3)
+    y[torch.arange(40), torch.arange(40) * (vocab // 41) + 5] = torch.linspace(10, 40, 40).cuda()
+    lp, ent, values, _ = call(ctx, y, y.argmax(-1).to(torch.int32), 20)
+    assert (lp <= 0).all() and (ent >= 0).all() and (values <= 0).all()
+    check(ctx, y)
