@@ -685,12 +685,16 @@ class Context:
         shapes = ((targets, "int32", (rows,)), (logprob, "float32", (rows,)),
                   (entropy, "float32", (rows,)), (top_values, "float32", (rows, top)),
                   (top_indices, "int32", (rows, top)))
+        if str(logits.dtype) != "torch.float32":
+            raise ValueError("logprobs: float32 logits are wanted")
         for t, kind, shape in shapes:
             if t is not None and (tuple(t.shape) != shape or str(t.dtype) != "torch." + kind or
                                   not t.is_contiguous()):
                 raise ValueError(f"logprobs: a contiguous {kind} tensor {shape} is wanted")
         if logits.stride(1) != 1 and vocab > 1:
             raise ValueError("logprobs: a row's logits lie one after the other")
+        if rows > 1 and logits.stride(0) < vocab:
+            raise ValueError("logprobs: rows that share memory")
         rc = lib().b2w4_logprobs(self.handle, _dptr(logits), max(logits.stride(0), vocab), rows,
                                  vocab, _dptr(targets), _dptr(logprob), _dptr(entropy), top,
                                  _dptr(top_values), _dptr(top_indices))

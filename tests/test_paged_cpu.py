@@ -249,3 +249,24 @@ def test_a_paged_decoder_refuses_the_calls_of_one_sequence(name, args):
     d = pkg.decoder.PagedDecoder.__new__(pkg.decoder.PagedDecoder)
     with pytest.raises(NotImplementedError, match="slots"):
         getattr(d, name)(*args)
+
+
+def bare_context():
+    """A context whose calls get as far as the library, which refuses a context that is none."""
+    c = capi.Context.__new__(capi.Context)
+    c.handle = None
+    return c
+
+
+def test_logits_that_the_kernel_would_read_past_are_refused():
+    """16-bit logits, and rows of a broadcast: read as 32-bit rows of their own they end behind the
+    tensor's memory."""
+    import torch
+    c = bare_context()
+    entropy = torch.zeros(4)
+    for x in (torch.zeros(4, 100, dtype=torch.bfloat16), torch.zeros(4, 100, dtype=torch.float16),
+              torch.zeros(1, 100).expand(4, 100), torch.zeros(500).as_strided((4, 100), (50, 1))):
+        with pytest.raises(ValueError, match="logprobs"):
+            c.logprobs(x, entropy=entropy)
+    with pytest.raises(capi.B200W4Error):   # one row: its stride does not matter
+        c.logprobs(torch.zeros(100).as_strided((1, 100), (0, 1)), entropy=entropy[:1])
