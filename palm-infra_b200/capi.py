@@ -91,6 +91,11 @@ def _int32(name, t, dims):
     return t.data_ptr()
 
 
+# What the paged kernels would read or write past otherwise; asked in the calls themselves, which a
+# step makes for every layer (a helper took 4 of their 12 us).
+_ROWS = "%s: a float32 tensor of at least %d rows of numbers without gaps is wanted"
+
+
 class PagedBatch(C.Structure):
     """b2w4_paged_batch: the sequences of a call, int32 tensors.  tables [slots, table_len],
     lengths [slots] (the call's rows counted), slots [sequences] (None: sequence i is slot i),
@@ -612,9 +617,23 @@ class Context:
     # -- a paged key-value cache
     def paged_prepare(self, cache, batch, qkv, heads, q_weight, k_weight, eps, cos, sin, q_out):
         """Merged qkv rows -> normalised + rotated Q in q_out, K and V in their pages."""
-        rc = lib().b2w4_paged_prepare(self.handle, C.byref(cache), C.byref(batch), _dptr(qkv),
-                                      qkv.stride(0), heads, _dptr(q_weight), _dptr(k_weight), eps,
-                                      _dptr(cos), _dptr(sin), _dptr(q_out), q_out.stride(0))
+        n, dim, length = batch.rows, cache.dim, batch.max_length
+        x, q = qkv.stride(), q_out.stride()
+        if qkv.element_size() != 4 or x[-1] != 1 or qkv.shape[0] < n:
+            raise ValueError(_ROWS % ("qkv", n))
+        if q_out.element_size() != 4 or q[-1] != 1 or q_out.shape[0] < n:
+            raise ValueError(_ROWS % ("q_out", n))
+        if qkv.numel() < n * (heads + 2 * cache.kv_heads) * dim or q_out.numel() < n * heads * dim:
+            raise B200W4Error("paged_prepare: rows of qkv or q_out that are too short")
+        for name, t in (("cos", cos), ("sin", sin)):
+            if t.element_size() != 4 or t.numel() * 2 < length * dim or not t.is_contiguous():
+                raise ValueError(_ROWS % (name, length))
+        for name, t in (("q_weight", q_weight), ("k_weight", k_weight)):
+            if t is not None and (t.element_size() != 4 or t.numel() < dim):
+                raise ValueError(_ROWS % (name, dim))
+        rc = lib().b2w4_paged_prepare(self.handle, cache, batch, qkv.data_ptr(), x[0], heads,
+                                      _dptr(q_weight), _dptr(k_weight), eps, cos.data_ptr(),
+                                      sin.data_ptr(), q_out.data_ptr(), q[0])
         if rc != 0:
             self._check(rc)
 
@@ -625,9 +644,17 @@ class Context:
     def paged_attention(self, cache, batch, q, heads, out, scale, work, window=0, sinks=0):
         """Attention of the batch's rows q [rows, heads * dim] over their pages.  window > 0: the
         last `window` keys of a token and the sequence's first `sinks`."""
-        rc = lib().b2w4_paged_attention(self.handle, C.byref(cache), C.byref(batch), _dptr(q),
-                                        q.stride(0), heads, scale, window, sinks, _dptr(out),
-                                        out.stride(0), _dptr(work), work.numel())
+        n, width = batch.rows, heads * cache.dim
+        x, o = q.stride(), out.stride()
+        if q.element_size() != 4 or x[-1] != 1 or q.shape[0] < n:
+            raise ValueError(_ROWS % ("q", n))
+        if out.element_size() != 4 or o[-1] != 1 or out.shape[0] < n:
+            raise ValueError(_ROWS % ("out", n))
+        if q.numel() < n * width or out.numel() < n * width:
+            raise B200W4Error("paged_attention: rows of q or out that are too short")
+        rc = lib().b2w4_paged_attention(self.handle, cache, batch, q.data_ptr(), x[0], heads, scale,
+                                        window, sinks, out.data_ptr(), o[0], work.data_ptr(),
+                                        work.numel())
         if rc != 0:
             self._check(rc)
 
@@ -685,17 +712,18 @@ class Context:
         shapes = ((targets, "int32", (rows,)), (logprob, "float32", (rows,)),
                   (entropy, "float32", (rows,)), (top_values, "float32", (rows, top)),
                   (top_indices, "int32", (rows, top)))
-        if str(logits.dtype) != "torch.float32":
+        if logits.element_size() != 4:
             raise ValueError("logprobs: float32 logits are wanted")
         for t, kind, shape in shapes:
             if t is not None and (tuple(t.shape) != shape or str(t.dtype) != "torch." + kind or
                                   not t.is_contiguous()):
                 raise ValueError(f"logprobs: a contiguous {kind} tensor {shape} is wanted")
-        if logits.stride(1) != 1 and vocab > 1:
+        ld, step = logits.stride()
+        if step != 1 and vocab > 1:
             raise ValueError("logprobs: a row's logits lie one after the other")
-        if rows > 1 and logits.stride(0) < vocab:
+        if rows > 1 and ld < vocab:
             raise ValueError("logprobs: rows that share memory")
-        rc = lib().b2w4_logprobs(self.handle, _dptr(logits), max(logits.stride(0), vocab), rows,
+        rc = lib().b2w4_logprobs(self.handle, _dptr(logits), max(ld, vocab), rows,
                                  vocab, _dptr(targets), _dptr(logprob), _dptr(entropy), top,
                                  _dptr(top_values), _dptr(top_indices))
         if rc != 0:

@@ -270,3 +270,43 @@ def test_logits_that_the_kernel_would_read_past_are_refused():
             c.logprobs(x, entropy=entropy)
     with pytest.raises(capi.B200W4Error):   # one row: its stride does not matter
         c.logprobs(torch.zeros(100).as_strided((1, 100), (0, 1)), entropy=entropy[:1])
+
+
+def test_tensors_that_the_paged_kernels_would_read_or_write_past_are_refused():
+    import torch
+    c = bare_context()
+    k = torch.zeros(4, 2, 16, 64, dtype=torch.bfloat16)
+    ints = lambda *shape: torch.zeros(shape, dtype=torch.int32)  # noqa: E731
+    paged, b = capi.PagedCache(k, k), capi.PagedBatch(ints(3, 4), ints(3), 64)
+    rows = lambda n, width, **kw: torch.zeros(n, width, **kw)  # noqa: E731
+    half = dict(dtype=torch.bfloat16)
+    attend = dict(cache=paged, batch=b, q=rows(3, 256), heads=4, out=rows(3, 256), scale=1.0,
+                  work=torch.zeros(8, dtype=torch.uint8))
+    prepare = dict(cache=paged, batch=b, qkv=rows(3, 512), heads=4, q_weight=torch.zeros(64),
+                   k_weight=None, eps=1e-6, cos=rows(64, 32), sin=rows(70, 32), q_out=rows(3, 256))
+    for call, good, bad in (
+            (c.paged_attention, attend, dict(q=rows(3, 256, **half))),
+            (c.paged_attention, attend, dict(q=rows(2, 256))),
+            (c.paged_attention, attend, dict(q=rows(3, 512)[:, ::2])),
+            (c.paged_attention, attend, dict(q=rows(1, 768))),
+            (c.paged_attention, attend, dict(out=rows(3, 256, **half))),
+            (c.paged_attention, attend, dict(out=rows(2, 256))),
+            (c.paged_prepare, prepare, dict(qkv=rows(3, 512, **half))),
+            (c.paged_prepare, prepare, dict(qkv=rows(2, 512))),
+            (c.paged_prepare, prepare, dict(q_out=rows(3, 256, dtype=torch.float64))),
+            (c.paged_prepare, prepare, dict(q_weight=torch.zeros(64, **half))),
+            (c.paged_prepare, prepare, dict(k_weight=torch.zeros(32))),
+            (c.paged_prepare, prepare, dict(cos=rows(63, 32))),
+            (c.paged_prepare, prepare, dict(sin=rows(64, 32, **half))),
+            (c.paged_prepare, prepare, dict(sin=rows(64, 64)[:, :32]))):
+        with pytest.raises(capi.B200W4Error):   # as far as the library
+            call(**good)
+        with pytest.raises(ValueError, match=next(iter(bad))):
+            call(**{**good, **bad})
+    for call, good, bad in (   # the last row would end behind the tensor
+            (c.paged_attention, attend, dict(q=rows(3, 256)[:, 64:])),
+            (c.paged_attention, attend, dict(out=rows(3, 256)[:, 4:])),
+            (c.paged_prepare, prepare, dict(qkv=rows(3, 512)[:, 4:])),
+            (c.paged_prepare, prepare, dict(q_out=rows(3, 256)[:, 128:]))):
+        with pytest.raises(capi.B200W4Error, match="too short"):
+            call(**{**good, **bad})
