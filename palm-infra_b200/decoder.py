@@ -484,9 +484,12 @@ class PagedDecoder(DenseDecoder):
         counts = [len(p) for p in prompts]
         if len(counts) != len(slots) or min(counts, default=0) < 1:
             raise ValueError("a prompt of at least one token for every slot")
+        tokens = [t for p in prompts for t in p]
+        if min(tokens) < 0 or max(tokens) >= self.cfg.vocab:
+            raise ValueError(f"tokens of a vocabulary of {self.cfg.vocab}")
         starts = np.concatenate([[0], np.cumsum(counts)]).tolist()
         self._on_current_stream()
-        ids = self._ints(t for p in prompts for t in p)
+        ids = self._ints(tokens)
         where = self._ints(slots)
         self.ctx.pages_extend(self.pool, where, self._ints(counts))
         # the pool may have refused: nothing runs on a sequence without its pages

@@ -310,3 +310,17 @@ def test_tensors_that_the_paged_kernels_would_read_or_write_past_are_refused():
             (c.paged_prepare, prepare, dict(q_out=rows(3, 256)[:, 128:]))):
         with pytest.raises(capi.B200W4Error, match="too short"):
             call(**{**good, **bad})
+
+
+@pytest.mark.parametrize("prompts", [[[5, 100]], [[-1]], [[1, 2], [3, 1 << 40]]])
+def test_tokens_beyond_the_vocabulary_are_refused(prompts):
+    """Their embedding rows lie outside of the table."""
+    import types
+    import torch
+    d = pkg.decoder.PagedDecoder.__new__(pkg.decoder.PagedDecoder)
+    d.cfg, d.slots, d.torch = types.SimpleNamespace(vocab=100), 4, torch
+    d.lengths, d.refs = (torch.zeros(4, dtype=torch.int32) for _ in range(2))
+    with pytest.raises(ValueError, match="vocabulary of 100"):
+        d.add(prompts, list(range(len(prompts))))
+    with pytest.raises(ValueError, match="vocabulary of 100"):
+        d.score([7] + prompts[-1], 1)
