@@ -351,10 +351,10 @@ class PagedDecoder(DenseDecoder):
     compacted.  Nothing of a step waits for the host -- pages are handed out on the device -- so
     one captured step serves every mix of sequences.
 
-    cache_type: torch.float32, float16 or bfloat16.  window, sinks: as b2w4_paged_attention's; a
-    window bounds what a step reads, not the pages that a sequence keeps.  max_length: tokens of a
-    sequence, rounded up to whole pages; a step leaves a longer one as it is, and sync raises.
-    Calls run on torch's current stream, which they set the context to.
+    slots: up to 1024.  cache_type: torch.float32, float16 or bfloat16.  window, sinks: as
+    b2w4_paged_attention's; a window bounds what a step reads, not the pages that a sequence keeps.
+    max_length: tokens of a sequence, rounded up to whole pages; a step leaves a longer one as it
+    is, and sync raises.  Calls run on torch's current stream, which they set the context to.
 
     The matmuls of one row (a decoder of one slot, a prompt of one token) take the rule per 128
     values, those of several rows `multi_row_rule`."""
@@ -364,6 +364,8 @@ class PagedDecoder(DenseDecoder):
         import torch
         if cfg.head_dim % 64 or cfg.head_dim > 256:
             raise ValueError("a paged decoder takes heads of 64, 128, 192 or 256 numbers")
+        if not 1 <= slots <= 1024 or pages < 1 or page_size < 1:
+            raise ValueError("a paged decoder takes 1 to 1024 slots and pages of a token or more")
         self.pages, self.page_size, self.slots = pages, page_size, slots
         self.cache_type = cache_type or torch.float32
         self.window, self.sinks = window, sinks

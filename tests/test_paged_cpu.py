@@ -324,3 +324,11 @@ def test_tokens_beyond_the_vocabulary_are_refused(prompts):
         d.add(prompts, list(range(len(prompts))))
     with pytest.raises(ValueError, match="vocabulary of 100"):
         d.score([7] + prompts[-1], 1)
+
+
+@pytest.mark.parametrize("bad", [dict(slots=1025), dict(slots=0), dict(pages=0), dict(page_size=0)])
+def test_a_paged_decoder_that_no_step_could_run_is_refused(bad):
+    """More slots than one call of pages_extend takes: every step would raise."""
+    cfg = pkg.decoder.DecoderConfig(1, 64, 1, 1, 64, 64, 64)
+    with pytest.raises(ValueError, match="1 to 1024 slots"):
+        pkg.decoder.PagedDecoder(None, cfg, None, **{**dict(slots=4, pages=4), **bad})
