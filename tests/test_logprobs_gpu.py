@@ -242,3 +242,34 @@ def test_confident_rows(ctx, vocab, winner_first):
     lp, ent, values, _ = call(ctx, y, y.argmax(-1).to(torch.int32), 20)
     assert (lp <= 0).all() and (ent >= 0).all() and (values <= 0).all()
     check(ctx, y)
+
+
+@pytest.mark.parametrize("left", [10, 100, 1000])
+def test_rows_of_which_a_mask_leaves_few_tokens(ctx, left):
+    """Their answers, and that they do not take many times as long as rows of as many tokens: while
+    numbers equal to the last of the largest came into the lists, -inf too, they took 21 to 44 times as
+    long; 1.5 to 2.4 now."""
+    rows, vocab, top = 64, 151936, 20
+    x = logits(rows, vocab, 12, ruled_out=0.0)
+    masked = torch.full_like(x, -math.inf)
+    g = torch.Generator(device="cuda").manual_seed(left)
+    kept = torch.rand((rows, vocab), device="cuda", generator=g).topk(left, -1).indices
+    masked.scatter_(1, kept, x.gather(1, kept))
+    check(ctx, masked, top=top)
+    check(ctx, masked, top=32)
+    entropy = torch.empty(rows, device="cuda")
+    values = torch.empty((rows, top), device="cuda")
+    ctx.set_stream(torch.cuda.current_stream().cuda_stream)
+
+    def time(t):
+        best = math.inf
+        for _ in range(5):
+            a, b = (torch.cuda.Event(enable_timing=True) for _ in range(2))
+            a.record()
+            for _ in range(10):
+                ctx.logprobs(t, entropy=entropy, top_values=values)
+            b.record()
+            torch.cuda.synchronize()
+            best = min(best, a.elapsed_time(b))
+        return best
+    assert time(masked) < 8 * time(x)
