@@ -176,12 +176,15 @@ Args args_of(b2w4_ctx* ctx, const b2w4_paged_cache& c, const b2w4_paged_batch& b
 // rows behind a long cache to the latter, by their times in us.  A tile's steps are those of
 // paged_runs.cu; row by row every token has its keys read again, from the second level cache for the
 // most part.  Heads of 192 and 256 numbers, groups of more than 128, and what
-// b2w4_paged_runs_takes has no room or time for, go row by row.  Measured, us
-// together / row by row, 32 heads over 8 of 128 in bf16: 2 rows behind 30,000 keys 591 / 50; 16 behind
-// 2000 46 / 32; 32 behind 4000 78 / 77; 64 behind 8000 153 / 266; 128 behind 4000 79 / 266.  In fp32: 16
-// behind 2000 91 / 55; 32 behind 4000 180 / 175; 128 behind 4000 182 / 656.  Of 120 shapes of three
-// types and four head layouts the rule takes one that is slower by more than 5 % once, by 13 % (64 rows
-// of 64 / 4 heads of 128 in fp16 behind 8000 keys, 153 where together takes 135).
+// b2w4_paged_runs_takes has no room or time for, go row by row whatever that costs (a prompt of 2000 of
+// 16 / 4 heads of 256: 7.1 ms in fp32, 2.5 in bf16, 1.8 in fp16; of 128, together, 0.14, 0.07, 0.06).
+// Measured, us together / row by row, 32 heads over 8 of 128 in bf16: 2 rows behind 30,000 keys 506 /
+// 52; 16 behind 2000 44 / 33; 32 behind 4000 75 / 81; 64 behind 8000 138 / 278; 128 behind 4000 75 /
+// 278; under a window of 512 16 rows 21.5 / 18, 64 rows 22.5 / 33.  In fp32: 16 behind 2000 92 / 55; 32
+// behind 4000 172 / 180; 128 behind 4000 184 / 669.  Of 174 shapes (three types, four head layouts,
+// 54 of them under windows of 512 and 2048) three take the one that is slower by more than 5 %: 64 rows
+// of 64 / 4 heads of 128 in fp16 behind 8000 keys (166, together 122), 64 of 64 / 8 of 64 in fp16 under
+// a window of 512 (20.5, 18.0), 32 of 32 / 8 of 128 in bf16 behind 4000 (81, 75).
 extern "C" int b2w4_paged_runs_wanted_by(int sm_count, int type, int dim, int heads, int kv_heads,
                                          int rows, int sequences, int max_length, int window,
                                          int sinks) {
