@@ -39,7 +39,7 @@ struct Prepare {
 // the cache's type as they are stored.
 // What bounds it: memory traffic, for a few rows the chain of lookups.  3208 rows of 32 / 8 heads of
 // 128 into an fp32 cache take 35 us (4.5 TB/s), 48 with a warp for every head and a lookup in each;
-// 64 rows 2.9 us with a warp for every head.
+// 64 rows 3 us with a warp for every head.
 template <typename T, int DIM, int EACH>
 __global__ void __launch_bounds__(32 * kWarps)
 paged_prepare_kernel(const Args a, const Prepare p) {

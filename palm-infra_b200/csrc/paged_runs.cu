@@ -19,7 +19,7 @@
 // features in three pieces are 48 MMAs of about 58 cycles, 2800 cycles; the rows' part of a step --
 // scores out of tensor memory, 2^x, the sum, three pieces, the running output -- is about 3500
 // beside them, and a step about 4000 (clock readings; the tensor pipe is 64 % busy).  6000 tokens of
-// 32 heads over 8 of 128, bf16, a window of 2048: 408 to 462 us from one GPU to another, 0.4 PFLOP/s
+// 32 heads over 8 of 128, bf16, a window of 2048: 408 to 473 us from one GPU to another, 0.4 PFLOP/s
 // of the formula's products and 1.2 with the pieces'.  A tile's start and end take about 17,000
 // cycles: queries in 3600 and into pieces 1500, the first scores 2500, the last P V 2250, results out
 // 5500.  They tell where rows see few keys: 333 tokens behind 900, fp32, 64 us; six chunks of 50 to

@@ -9,8 +9,10 @@
 //
 // What bounds it: the bytes that move, each read and written once.  Compaction of a pool of 2048
 // pages in 16 planes, 64 KB a page of a plane, 491 of which move: 184 us, 5.6 TB/s both ways.  Eight
-// children of a sequence of 1001 tokens, their last pages copied in 72 planes, and given back: 19 us,
-// the plan's and the commit's chains of lookups rather than the 38 MB.
+// children of a sequence of 1001 tokens, their last pages copied in 72 planes, and given back: 19 to
+// 22 us, the plan's and the commit's chains of lookups rather than the 38 MB.  A step's extend takes 4.9
+// us where no sequence needs a page; where one does, one block looks through the counts from page 0: 11
+// to 37 us in pools of 65,536 pages, 0.3 ms behind 900,000 pages in use.
 //
 // Only full pages are ever shared: a fork copies a last page that is not full.  So the page that
 // a sequence's next token goes to is its own.
