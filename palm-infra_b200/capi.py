@@ -397,6 +397,7 @@ class Context:
                               "an sm_100 (B200) device is required; there is no CPU path")
         self.handle = h
         self.device = device
+        self.moe_rule = ACT_G32
 
     def _check(self, rc):
         if rc != 0:
@@ -418,6 +419,7 @@ class Context:
         """ACT_G32: the reference's rule (per 32 values for an expert that holds several rows,
         per 128 for a lone row); ACT_G128: per 128 for every row."""
         self._check(lib().b2w4_ctx_set_moe_rule(self.handle, rule))
+        self.moe_rule = rule
 
     def set_peer_wait_ms(self, milliseconds):
         """Bound of the device-side waits for another GPU's stores (default about 2 s)."""

@@ -357,7 +357,8 @@ class PagedDecoder(DenseDecoder):
     is, and sync raises.  Calls run on torch's current stream, which they set the context to.
 
     The matmuls of one row (a decoder of one slot, a prompt of one token) take the rule per 128
-    values, those of several rows `multi_row_rule`."""
+    values, those of several rows `multi_row_rule`; experts the rule that the context has when the
+    decoder is made."""
 
     def __init__(self, ctx, cfg, weights, slots, pages, page_size=32, max_length=None,
                  cache_type=None, window=0, sinks=0, multi_row_rule=capi.ACT_G32):
@@ -384,6 +385,7 @@ class PagedDecoder(DenseDecoder):
         # A step's rows are always the slots, so what its context holds for them keeps its place
         # while the prompts' context grows: a captured step stays valid.
         self.step_ctx = capi.Context(ctx.device)
+        self.step_ctx.set_moe_rule(ctx.moe_rule)
         self.work = {c: torch.empty(ctx.paged_attention_work(cfg.heads, cfg.head_dim),
                                     dtype=torch.uint8, device="cuda")
                      for c in (self.ctx, self.step_ctx)}

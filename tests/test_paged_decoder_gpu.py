@@ -330,3 +330,18 @@ def test_forks_that_do_not_all_fit_change_nothing(model):
     d.sync()
     assert all(same(t, want[0]) for t in tokens.values())
     d.free()
+
+
+def test_steps_and_prompts_take_the_contexts_rule_for_experts(model):
+    """Steps have a context of their own: the same rows through both are the same bits, experts that
+    hold several rows included."""
+    cfg, weights, ctx, prompts, _ = model
+    d = dec.PagedDecoder(ctx, cfg, weights, slots=6, pages=80, page_size=8, max_length=160,
+                         multi_row_rule=RULE)
+    d.add(prompts, [0, 1, 2, 3, 4])
+    d.step_ctx.set_stream(torch.cuda.current_stream().cuda_stream)
+    d.step_ctx.pages_extend(d.pool, d.running, granted=d.granted)
+    rows = [d._rows(c, d.token, d.step_batch, 6).clone() for c in (d.ctx, d.step_ctx)]
+    d.sync()
+    assert torch.equal(rows[0][:5], rows[1][:5])
+    d.free()
