@@ -189,13 +189,15 @@ extern "C" int b2w4_paged_runs_wanted_by(int sm_count, int type, int dim, int he
                                          int rows, int sequences, int max_length, int window,
                                          int sinks) {
     const int rep = heads / kv_heads;
-    if (!b2w4_paged_runs_takes(sm_count, dim, heads, kv_heads, rows, sequences, max_length))
+    if (rep > 128)
         return 0;
     const bool wide = type == B2W4_F32, two = !wide && dim == 64;
     const int tq = 128 / rep, per = wide || two ? 64 : 128;
     double keys = max_length;
     if (window > 0 && (double)window + sinks + tq < keys)
         keys = (double)window + sinks + tq;
+    if (!b2w4_paged_runs_takes(sm_count, dim, heads, kv_heads, rows, sequences, keys))
+        return 0;
     const double tiles = ((double)rows / tq + 0.5 * sequences) * kv_heads;
     const double waves = ceil(tiles / (sm_count * (two ? 2 : 1)));
     // (two blocks beside each other share the products' rate)
@@ -211,8 +213,10 @@ extern "C" int b2w4_paged_runs_wanted_by(int sm_count, int type, int dim, int he
 
 bool b2w4_paged_runs_wanted(int sm_count, const b2w4_paged_cache& c, const b2w4_paged_batch& b,
                             int heads, int window, int sinks) {
-    return b2w4_paged_runs_wanted_by(sm_count, c.type, c.dim, heads, c.kv_heads, b.rows,
-                                     b.sequences, b.max_length, window, sinks) != 0;
+    const double room = (double)b.table_len * c.page_size;  // a table's tokens
+    return b2w4_paged_runs_wanted_by(sm_count, c.type, c.dim, heads, c.kv_heads, b.rows, b.sequences,
+                                     room < b.max_length ? (int)room : b.max_length, window,
+                                     sinks) != 0;
 }
 
 // What a cache and a batch must be, whatever is done with them; the text of what is wrong, or

@@ -25,9 +25,8 @@ __device__ __forceinline__ bool odd_result(float x) {
 // Operands of 32 bits as sums of pieces of the cache's 16-bit type (bf16 beside an fp32 cache).
 // bf16 has fp32's exponents: three pieces are all 24 bits, whatever the number's size.  fp16 has
 // not: a second piece that is what the first one left falls among the numbers below 2^-14, whose
-// step does not shrink with them, from 2^-3 of the largest on.  So what is left is taken times
-// 2^kUp, about as large again as the first piece, and its products, in a sum of their own, times
-// 2^-kUp.  Two pieces are then 22 bits (off by 2^-23 of the number) down to 2^-14, and below that a
+// step does not shrink with them, from 2^-3 of the largest on.  So what is left is taken times kUp,
+// about as large again as the first piece, and the sum of its products times kDown.  Two pieces are then 22 bits (off by 2^-23 of the number) down to 2^-14, and below that a
 // multiple of 2^-36.  Largest numbers lie just below 2^15: what is left of them is below 2^3.
 template <typename T>
 constexpr bool kHalf = std::is_same_v<T, __half>;
@@ -84,7 +83,7 @@ __device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool there) 
 
 // Runs of rows (paged_runs.cu): heads of 64 or 128 numbers.  work: as the split kernel's.
 bool b2w4_paged_runs_takes(int sm_count, int dim, int heads, int kv_heads, int rows, int sequences,
-                           int max_length);
+                           double keys);
 int b2w4_launch_paged_runs(b2w4_ctx* ctx, int type, int dim, const paged::Args& a,
                            const paged::Attend& p, void* work);
 

@@ -1035,11 +1035,11 @@ int launch(b2w4_ctx* ctx, const Args& a, const Attend& p, void* work) {
 
 }  // namespace
 
-// Tiles are counted in 32 bits; the work area holds an entry of every block's lists for each, and a
+// keys: the most that a tile sees.  Tiles are counted in 32 bits; the work area holds an entry of every block's lists for each, and a
 // tile of 2^24 keys takes 0.7 s of a wait's 2.
 bool b2w4_paged_runs_takes(int sm_count, int dim, int heads, int kv_heads, int rows, int sequences,
-                           int max_length) {
-    if (dim > 128 || heads / kv_heads > kRows || max_length > 1 << 24)
+                           double keys) {
+    if (dim > 128 || heads / kv_heads > kRows || keys > 1 << 24)
         return false;
     const long tiles = tiles_of(rows, sequences, heads, kv_heads);
     return tiles < 0x3fffffff && 4 * sizeof(Again) * (tiles + (long)sm_count * kMostBlocks) <=

@@ -212,7 +212,7 @@ __device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint3
             : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
             : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-// What is left of a query or probability behind its first piece, in pieces' units (paged::kUp).
+// The next piece of two numbers; they keep what is left, times kUp beside an fp16 cache.
 template <typename T>
 __device__ __forceinline__ uint32_t take_piece(float& lo, float& hi) {
     uint64_t v = b2w4_pack2(lo, hi);

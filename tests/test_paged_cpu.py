@@ -332,3 +332,14 @@ def test_a_paged_decoder_that_no_step_could_run_is_refused(bad):
     cfg = pkg.decoder.DecoderConfig(1, 64, 1, 1, 64, 64, 64)
     with pytest.raises(ValueError, match="1 to 1024 slots"):
         pkg.decoder.PagedDecoder(None, cfg, None, **{**dict(slots=4, pages=4), **bad})
+
+
+def test_a_loose_bound_of_the_length_does_not_part_prompts_from_their_kernel():
+    """Under a window a tile sees few keys, however long the sequences may be."""
+    rule = capi.lib().b2w4_paged_runs_wanted_by
+    for kind in (capi.F32, capi.F16, capi.BF16):
+        for length in (8192, 1 << 24, (1 << 24) + 1, 2 ** 31 - 1):
+            assert rule(148, kind, 128, 32, 8, 2000, 1, length, 2048, 4) == 1
+        # beyond what a wait's limit leaves time for, and beyond the lists' room
+        assert rule(148, kind, 128, 32, 8, 2000, 1, (1 << 24) + 1, 0, 0) == 0
+        assert rule(148, kind, 64, 8, 8, 200000, 200000, 4000, 0, 0) == 0
